@@ -319,6 +319,72 @@ int p0_normadd(const p0_normadd_args_t* a);
 int p0_argmax(const float* mx, int64_t n, uint32_t* out);
 int p0_argmaxM(const float* mx, int64_t n, int64_t M, uint32_t* out);
 
+/* ---- keys and values in 4 bits: a cache in pages and its attention ----------------------------------------------- */
+/* These operators have no counterpart on the int4 path of the reference (its cache is one ring of fp16 rows per layer,
+ * engine/llm/gemma4.js:97-116); they are what a server of the same model needs beside it.
+ *
+ * A cache is a pool of pages of `page` tokens (32, 64, 128, 256, 512 or 1024), each with the keys and values of `heads`
+ * heads of `dim` channels (64, 128, 256 or 512) in mxfp4: 32 channels of a token share a power of two (a byte e: 2^(e - 127)),
+ * each value is 4 bits (sign, two bits of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6): 17/32 byte a value. A page is
+ * `heads` runs per 32 tokens of 34 dim bytes: key codes, key exponents, value codes, value exponents, in the orders that the
+ * attention's matrix instructions take them (p0pc0rn_amd/csrc/kv_common.hpp); p0_kv_put and p0_kv_get are the way in and out.
+ * Sequence b's token t is in page table[b * table_ld + t / page]; an entry outside [0, n_pages) is no page: its tokens are
+ * written nowhere, read as 0 and attended to by no row. len[b] is the number of tokens the sequence holds (more than cols *
+ * page count as that many). Tables and lengths are device memory: no call waits for the device.
+ * Several layers share one table: a pool of n_pages each, layer_bytes apart. */
+enum { P0_KV_F32 = 0, P0_KV_F16 = 1, P0_KV_BF16 = 2 };   /* type */
+typedef struct {
+  void* pages;             /* the pool, 16-byte aligned */
+  int64_t n_pages;         /* at most 2^30 */
+  int64_t page_bytes;      /* from a page to the next (a multiple of 16; 0 = p0_kv_page_bytes) */
+  int32_t page, heads, dim;
+  const int32_t* table;    /* [B][table_ld] (0 = cols), the first cols in use */
+  int64_t table_ld, cols;
+  const int32_t* len;      /* [B] */
+} p0_kv_t;
+int64_t p0_kv_page_bytes(int32_t page, int32_t heads, int32_t dim);   /* 0 where there is no such page */
+
+/* put: the keys and values of rows[b] (NULL: M; more than M count as M) rows of each sequence into its pages; get: back, in
+ * the same type (every value is exact in it). Row i of sequence b is token at[b] + i, or, where `at` is NULL, of its newest:
+ * len[b] - rows[b] + i. Tokens before the first or from len[b] on are left out (put) or 0 (get); a get clears rows past
+ * rows[b]. Element [b][i][h][c] is at b * ldb + i * ldm + h * ldh + c of k and v (0 = dim, heads * ldh, M * ldm).
+ * The exponent of 32 channels is the least e in [-23, 13] with max |x| <= 6 * 2^e, so nothing up to 49152 is cut; the codes are
+ * the nearest, ties to the even one. A head's token with a NaN or an infinity in its key or its value is held as a key of
+ * NaN and a value of 0, so that exactly the rows that see it become NaN. put: no two rows may name the same token. */
+typedef struct {
+  p0_kv_t kv;
+  int64_t B, M;
+  const int32_t* rows;
+  const int32_t* at;
+  int32_t type;
+  void* k;
+  void* v;
+  int64_t ldb, ldm, ldh;
+} p0_kv_rows_args_t;
+int p0_kv_put(const p0_kv_rows_args_t* a);
+int p0_kv_get(const p0_kv_rows_args_t* a);
+
+/* Attention of each sequence's newest rows[b] (NULL: M) rows over its pages. Row i is at position p = len[b] - rows[b] + i and
+ * sees token t if t <= p and, with a window, t > p - window or t < sinks. Query head q reads key head q / (heads / kv.heads).
+ * y = sum_t softmax_t(scale q . k_t) v_t (scale 0: 1 / sqrt(dim)); a row that sees nothing, and rows past rows[b], are 0.
+ * Element [b][i][q][c] of q is at b * q_ldb + i * q_ldm + q * q_ldh + c (0 = dim, heads * ldh, M * ldm), of y likewise.
+ * f32 queries and probabilities are taken as pairs of fp16 values (22 bits), f16 and bf16 queries exactly, sums in fp32.
+ * max_len: no sequence is longer (0 = cols * page): only the split of the work goes by it, longer ones are right too.
+ * Results are the same bit for bit from call to call with the same max_len. */
+typedef struct {
+  p0_kv_t kv;
+  int64_t B, M;
+  const int32_t* rows;
+  int64_t heads;
+  int32_t type;
+  const void* q; int64_t q_ldb, q_ldm, q_ldh;
+  void* y; int64_t y_ldb, y_ldm, y_ldh;
+  float scale;
+  int64_t window, sinks;   /* window 0: every token up to the row's own */
+  int64_t max_len;
+} p0_kv_attn_args_t;
+int p0_kv_attn(const p0_kv_attn_args_t* a);
+
 /* ---- the pack reader's I/O (engine/core/store.js:221-244) ---------------------------------------------------------- */
 /* bytes [offset, offset + bytes) of the file at path -> device memory dst + dst_off, streamed in 16 MB chunks through
  * two pinned host buffers (file reads overlap the host-to-device copies on the library's stream); returns when the

@@ -1,0 +1,138 @@
+"""CPU restatement, in numpy, of the 4-bit cache and its operators: what the tests hold the GPU's results against.
+
+mxfp4: 32 channels share 2^e, e the least integer in [-23, 13] with max |x| <= 6 * 2^e; a value is the nearest of 0, 0.5, 1,
+1.5, 2, 3, 4, 6 times it, ties to the even code. A token of a head with a NaN or an infinity in its key or value is held as a
+key of NaN and a value of 0. Arithmetic is float64 throughout.
+"""
+import numpy as np
+
+GRID = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+E_MIN, E_MAX = -23, 13
+
+
+def exponents(x):
+    """[..., 32] -> the exponent of each block"""
+    most = np.abs(x.astype(np.float64)).max(-1)
+    e = np.full(most.shape, E_MIN)
+    for i in range(E_MIN, E_MAX):      # one more while it does not hold the largest
+        e = np.where(most > 6.0 * 2.0 ** i, i + 1, e)
+    return e
+
+
+def codes(y):
+    """values / 2^e -> 4-bit codes"""
+    a = np.abs(y)
+    d = np.abs(a[..., None] - GRID)
+    near = d == d.min(-1, keepdims=True)
+    first = near.argmax(-1)
+    last = 7 - near[..., ::-1].argmax(-1)
+    c = np.where(first == last, first, np.where(first % 2 == 0, first, last))   # two as near: the even one
+    return np.where(np.signbit(y), c + 8, c)
+
+
+def quantise(x):
+    """rows [..., D] -> (codes [..., D], exponents [..., D / 32]), no NaN handling"""
+    b = x.astype(np.float64).reshape(*x.shape[:-1], -1, 32)
+    e = exponents(b)
+    return codes(b / 2.0 ** e[..., None]).reshape(x.shape), e
+
+
+def values(c, e):
+    v = np.where(c >= 8, -GRID[c & 7], GRID[c & 7]).reshape(*e.shape, 32)
+    return (v * 2.0 ** e[..., None].astype(np.float64)).reshape(c.shape)
+
+
+def held(k, v):
+    """what the cache gives back for keys and values [..., D]"""
+    bad = ~(np.isfinite(k).all(-1) & np.isfinite(v).all(-1))
+    out = []
+    for x, put in ((k, np.nan), (v, 0.0)):
+        y = values(*quantise(np.where(bad[..., None], 0.0, x)))
+        out.append(np.where(bad[..., None], put, y))
+    return out
+
+
+def offsets(D):
+    """byte offsets in a run of 32 tokens: key codes [32, D], key exponents [32, D / 32], value codes, value exponents"""
+    t, c = np.arange(32)[:, None], np.arange(D)[None]
+    g, u, i = t % 16 // 4, t // 16, t % 16
+    if D == 64:
+        kc = ((c // 16) * 16 + i) * 16 + u * 8 + c % 16 // 2
+    else:
+        kc = (u * (D // 128) + c // 128) * 1024 + (c % 128 // 32 * 16 + i) * 16 + c % 32 // 2
+    vc = 17 * D + c // 64 * 1024 + (g * 16 + c % 32 // 2) * 16 + c // 32 % 2 * 8 + u * 4 + i % 4
+    b = np.arange(D // 32)[None]
+    if D == 64:
+        ke = 16 * D + (b * 16 + i) * 2 + u
+    else:
+        ke = 16 * D + (((b % 4) * 16 + i) * 2 + u) * (D // 128) + b // 4
+    ve = 33 * D + (g * (D // 32) + b) * 8 + u * 4 + i % 4
+    return kc, ke, vc, ve
+
+
+class Cache:
+    """A pool of pages on the host, byte for byte as the device holds it."""
+
+    def __init__(self, n_pages, page, heads, dim, seed=None):
+        self.n_pages, self.page, self.heads, self.dim = n_pages, page, heads, dim
+        shape = (n_pages, heads, page // 32, 34 * dim)
+        self.pool = np.zeros(shape, np.uint8) if seed is None else np.random.default_rng(seed).integers(0, 256, shape, np.uint8)
+        self.at = offsets(dim)
+
+    def write(self, pg, t, h, k, v):
+        run = self.pool[pg, h, t // 32]
+        t %= 32
+        bad = not (np.isfinite(k).all() and np.isfinite(v).all())
+        for x, code_at, exp_at, e_bad in ((k, self.at[0], self.at[1], 255), (v, self.at[2], self.at[3], E_MIN + 127)):
+            c, e = quantise(np.where(bad, 0.0, x))
+            run[code_at[t, 0::2]] = c[0::2] | c[1::2] << 4
+            run[exp_at[t]] = e_bad if bad else e + 127
+
+    def read(self, pg, t, h):
+        run = self.pool[pg, h, t // 32]
+        t %= 32
+        out = []
+        for code_at, exp_at in (self.at[:2], self.at[2:]):
+            b = run[code_at[t]].astype(int)
+            c = np.where(np.arange(self.dim) % 2 == 0, b & 15, b >> 4)
+            e = run[exp_at[t]].astype(int)
+            with np.errstate(over="ignore", invalid="ignore"):
+                out.append(np.where(np.repeat(e, 32) == 255, np.nan, values(c, e - 127)))
+        return out
+
+    def tokens(self, table_row, n, h):
+        """keys, values [n, D] and which tokens have a page"""
+        k, v, ok = np.zeros((n, self.dim)), np.zeros((n, self.dim)), np.zeros(n, bool)
+        for t in range(n):
+            pg = table_row[t // self.page]
+            if 0 <= pg < self.n_pages:
+                k[t], v[t] = self.read(pg, t % self.page, h)
+                ok[t] = True
+        return k, v, ok
+
+
+def attention(cache, table, length, q, rows=None, scale=None, window=0, sinks=0):
+    """q [B, M, heads, D] -> [B, M, heads, D]"""
+    B, M, Hq, D = q.shape
+    G = Hq // cache.heads
+    scale = scale or 1.0 / np.sqrt(D)
+    out = np.zeros(q.shape)
+    for b in range(B):
+        n = int(np.clip(length[b], 0, table.shape[1] * cache.page))
+        m = M if rows is None else int(np.clip(rows[b], 0, M))
+        kv = [cache.tokens(table[b], n, h) for h in range(cache.heads)]
+        t = np.arange(n)
+        for i in range(m):
+            p = n - m + i
+            sees = t <= p
+            if window:
+                sees &= (t > p - window) | (t < sinks)
+            for hq in range(Hq):
+                k, v, ok = kv[hq // G]
+                use = sees & ok
+                if not use.any():
+                    continue
+                s = k[use] @ q[b, i, hq].astype(np.float64) * scale
+                w = np.exp(s - np.nanmax(s)) if not np.isnan(s).all() else s
+                out[b, i, hq] = w @ v[use] / w.sum()
+    return out

@@ -20,6 +20,7 @@ XMODE = {"f16": 0, "lnmod": 1, "rms": 2, "bf16": 3}
 GEPI = {"f16": 0, "f32": 1, "resadd": 2, "swiglu": 3, "bias": 4, "heads": 5}
 ROPE = {"inter": 0, "half": 1}
 ACT = {"silu": 0, "gelu": 1}
+KV_TYPE = {"f32": 0, "f16": 1, "bf16": 2}
 
 # every symbol the header declares (tests check the library exports each one)
 HEADER_SYMBOLS = [
@@ -31,6 +32,7 @@ HEADER_SYMBOLS = [
     "p0_record_begin", "p0_record_end", "p0_replay", "p0_record_info", "p0_record_free",
     "p0_chain_begin", "p0_chain_end", "p0_chain_run", "p0_chain_status", "p0_chain_info", "p0_chain_free",
     "p0_chain_tune", "p0_rowstats", "p0_normadd", "p0_argmax", "p0_argmaxM", "p0_upload_file",
+    "p0_kv_page_bytes", "p0_kv_put", "p0_kv_get", "p0_kv_attn",
 ]
 
 i64, i32, f32, vp = C.c_int64, C.c_int32, C.c_float, C.c_void_p
@@ -82,6 +84,23 @@ class NormaddArgs(C.Structure):
                 ("st_off", i64), ("D", i64), ("M", i64), ("eps", f32), ("scale", f32), ("mode", i32)]
 
 
+class Kv(C.Structure):
+    _fields_ = [("pages", vp), ("n_pages", i64), ("page_bytes", i64), ("page", i32), ("heads", i32), ("dim", i32),
+                ("table", vp), ("table_ld", i64), ("cols", i64), ("len", vp)]
+
+
+class KvRowsArgs(C.Structure):
+    _fields_ = [("kv", Kv), ("B", i64), ("M", i64), ("rows", vp), ("at", vp), ("type", i32), ("k", vp), ("v", vp),
+                ("ldb", i64), ("ldm", i64), ("ldh", i64)]
+
+
+class KvAttnArgs(C.Structure):
+    _fields_ = [("kv", Kv), ("B", i64), ("M", i64), ("rows", vp), ("heads", i64), ("type", i32),
+                ("q", vp), ("q_ldb", i64), ("q_ldm", i64), ("q_ldh", i64),
+                ("y", vp), ("y_ldb", i64), ("y_ldm", i64), ("y_ldh", i64),
+                ("scale", f32), ("window", i64), ("sinks", i64), ("max_len", i64)]
+
+
 class P0Error(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(msg)
@@ -122,11 +141,14 @@ def lib():
             "p0_rowstats": [C.POINTER(RowstatsArgs)], "p0_normadd": [C.POINTER(NormaddArgs)],
             "p0_argmax": [vp, i64, vp], "p0_argmaxM": [vp, i64, i64, vp],
             "p0_upload_file": [C.c_char_p, i64, i64, vp, i64],
+            "p0_kv_put": [C.POINTER(KvRowsArgs)], "p0_kv_get": [C.POINTER(KvRowsArgs)], "p0_kv_attn": [C.POINTER(KvAttnArgs)],
         }
         for name, args in sig.items():
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = C.c_int
+        L.p0_kv_page_bytes.argtypes = [i32, i32, i32]
+        L.p0_kv_page_bytes.restype = i64
         _lib = L
     return _lib
 
@@ -410,3 +432,38 @@ def argmaxM(mx, n, M, out):
 def upload_file(path, offset, nbytes, dst, dst_off=0):
     """bytes [offset, offset + nbytes) of a file -> device memory (the pack reader's I/O, engine/core/store.js:221-244)"""
     check(lib().p0_upload_file(os.fsencode(path), offset, nbytes, _ptr(dst), dst_off))
+
+
+# ------------------------------------------------------------------------------------------------ the 4-bit cache
+def _fields(cls, kw):
+    """cls from keyword fields; Buffer objects are accepted where the header takes a pointer"""
+    return cls(**{k: v.ptr if isinstance(v, Buffer) else v for k, v in kw.items()})
+
+
+def kv_page_bytes(page, heads, dim):
+    return lib().p0_kv_page_bytes(page, heads, dim)
+
+
+def kv(**kw):
+    """a cache descriptor (p0_kv_t)"""
+    return _fields(Kv, kw)
+
+
+def kv_rows_args(**kw):
+    return _fields(KvRowsArgs, kw)
+
+
+def kv_attn_args(**kw):
+    return _fields(KvAttnArgs, kw)
+
+
+def kv_put(args):
+    check(lib().p0_kv_put(C.byref(args)))
+
+
+def kv_get(args):
+    check(lib().p0_kv_get(C.byref(args)))
+
+
+def kv_attn(args):
+    check(lib().p0_kv_attn(C.byref(args)))

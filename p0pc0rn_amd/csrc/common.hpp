@@ -35,6 +35,7 @@ struct Ctx {
   // the GEMM's own, one per tile of a call with K slices: a chain whose wait gave up leaves counts behind in `counters`
   // until p0_chain_status clears them, and a GEMM enqueued in between must not take them for its own
   unsigned* gemm_counters = nullptr;
+  unsigned* kv_counters = nullptr;   // the cache's and the beam search's own, likewise (kKvCounters)
   // fp16 staging of GEMM activations that the MFMA kernel cannot stream as they are (bf16, the f32 prologues,
   // misaligned fp16): grown on demand, never inside a stream capture (ensure_xstage)
   void* xstage = nullptr;
@@ -46,6 +47,7 @@ struct Ctx {
   hipDeviceProp_t prop{};
 };
 Ctx& ctx();
+constexpr int64_t kKvCounters = 1 << 16;
 int ensure_xstage(size_t bytes, const char* op);   // P0_OK, or an error (no room while the stream is being captured)
 // per-file set-up at p0_open (kernel attributes; the no-allocation GEMM's scratch address)
 int gemm_init();

@@ -82,13 +82,14 @@ __global__ void copy4_kernel(const uint32_t* __restrict__ src, uint32_t* __restr
 
 using namespace p0;
 
-// Split-K workspace: 64 MiB of partial sums, 1 Mi arrival counters and the GEMM's 256 per device, in uncached device memory. The
+// Split-K workspace: 64 MiB of partial sums, 1 Mi arrival counters, the GEMM's 256 and the cache operators' 64 Ki per device, in uncached device memory. The
 // partials then reach memory when their stores are acknowledged and are read from memory, so the arrival protocol
 // needs no L2 write-back or invalidate (a device-scope fence costs a write-back of the XCD's whole L2). Uncached memory
 // that a kernel has read is never freed while the process runs (allocations made after such a free have been seen
 // holding wrong values), so each device's workspace is allocated once and kept across p0_close / p0_open.
 static constexpr size_t kPartBytes = 64ull << 20;
-static constexpr size_t kCounters = 1ull << 20, kGemmCounters = 256, kAllCounters = kCounters + kGemmCounters;
+static constexpr size_t kCounters = 1ull << 20, kGemmCounters = 256, 
+                        kAllCounters = kCounters + kGemmCounters + p0::kKvCounters;
 static constexpr int kWsDevices = 64;
 static float* g_ws_part[kWsDevices] = {};
 static unsigned* g_ws_cnt[kWsDevices] = {};
@@ -140,6 +141,7 @@ int p0_open(int device) {
   c.part_floats = kPartBytes / sizeof(float);
   c.n_counters = kCounters;
   c.gemm_counters = c.counters + kCounters;
+  c.kv_counters = c.gemm_counters + kGemmCounters;
   c.cur = c.own;
   c.cu_count = c.prop.multiProcessorCount;
   c.device = device;
