@@ -319,7 +319,7 @@ int p0_normadd(const p0_normadd_args_t* a);
 int p0_argmax(const float* mx, int64_t n, uint32_t* out);
 int p0_argmaxM(const float* mx, int64_t n, int64_t M, uint32_t* out);
 
-/* ---- keys and values in 4 bits: a cache in pages and its attention ----------------------------------------------- */
+/* ---- keys and values in 4 bits: a cache in pages, its attention, its pages ------------------------------------------ */
 /* These operators have no counterpart on the int4 path of the reference (its cache is one ring of fp16 rows per layer,
  * engine/llm/gemma4.js:97-116); they are what a server of the same model needs beside it.
  *
@@ -384,6 +384,46 @@ typedef struct {
   int64_t max_len;
 } p0_kv_attn_args_t;
 int p0_kv_attn(const p0_kv_attn_args_t* a);
+
+/* The sequences of the next step from those of the last: new sequence b holds the first keep[b] (NULL, or more than it has:
+ * all) tokens of sequence src[b] (NULL: b; outside [0, B): of none) and room for grow[b] (NULL: grow_n; below 0: 0) more;
+ * len_out[b] is their sum. Sequences share the pages of what they share. A page that a growing sequence ends in the middle of
+ * and that another one holds too is copied (in every layer), so that each writes its own: where all its holders grow in it,
+ * the first keeps the original. With a window, pages that no row from position keep on can see (p0_kv_attn's rule) are given
+ * up. A page that no new sequence holds is free. Free pages are taken in ascending order, for sequences and columns in
+ * ascending order. table_out ([Bo][out_ld], 0 = cols: no entry: -1), len_out, ref ([n_pages]: holders of each page; may be
+ * NULL) and status are written, table and len are read: they must not overlap. At most 2^21 pages here and in p0_kv_compact.
+ * status (device, 4 words): pages that were missing, free pages left, pages copied, sequences longer than cols * page. Where
+ * the first or last is not 0 nothing has been done: table_out and len_out are the old sequences (the first min(B, Bo);
+ * further ones are empty), ref is as it was, and the second word is the pages that there were to take. So this forks (several src alike), reorders (a beam search's
+ * parents), truncates (the rows a verify pass refused), extends and frees (src -1). */
+typedef struct {
+  p0_kv_t kv;
+  int64_t B, Bo;           /* sequences before, after (0 = B; src is needed where they differ) */
+  const int32_t* src;
+  const int32_t* keep;
+  const int32_t* grow; int64_t grow_n;
+  int64_t window, sinks;
+  int64_t layers, layer_bytes;   /* 0 = 1; 0 = n_pages * page_bytes */
+  int32_t* table_out; int64_t out_ld;
+  int32_t* len_out;
+  int32_t* ref;
+  int32_t* status;
+} p0_kv_update_args_t;
+int p0_kv_update(const p0_kv_update_args_t* a);
+
+/* Moves the live pages (held by a table row's first ceil(len / page) columns) to the front of the pool: with n of them, those
+ * at or above n go, in ascending order, to the free ones below n, in ascending order; table_out is the table with the moved
+ * ones' new places (columns past a sequence's tokens, and entries that are no page: -1). status (device, 2 words): n, pages
+ * moved. table_out must not overlap table. */
+typedef struct {
+  p0_kv_t kv;
+  int64_t B;
+  int64_t layers, layer_bytes;
+  int32_t* table_out; int64_t out_ld;
+  int32_t* status;
+} p0_kv_compact_args_t;
+int p0_kv_compact(const p0_kv_compact_args_t* a);
 
 /* ---- the pack reader's I/O (engine/core/store.js:221-244) ---------------------------------------------------------- */
 /* bytes [offset, offset + bytes) of the file at path -> device memory dst + dst_off, streamed in 16 MB chunks through

@@ -136,3 +136,69 @@ def attention(cache, table, length, q, rows=None, scale=None, window=0, sinks=0)
                 w = np.exp(s - np.nanmax(s)) if not np.isnan(s).all() else s
                 out[b, i, hq] = w @ v[use] / w.sum()
     return out
+
+
+def update(table, length, page, n_pages, Bo, src=None, keep=None, grow=None, grow_n=0, window=0, sinks=0):
+    """-> (table, length, holders of each page, status, [(from, to)]): one sequence, one column at a time"""
+    B, cols = table.shape
+    length = np.clip(length, 0, cols * page)
+    clean = lambda b, j: table[b, j] if 0 <= table[b, j] < n_pages else -1  # noqa: E731
+    new, kept, grown = np.full((Bo, cols), -1), np.zeros(Bo, int), np.zeros(Bo, int)
+    for b in range(Bo):
+        s = b if src is None else int(src[b])
+        if 0 <= s < B:
+            kept[b] = length[s] if keep is None else min(max(int(keep[b]), 0), length[s])
+            for j in range(-(-kept[b] // page)):
+                if window and (j + 1) * page <= kept[b] - window + 1 and j * page >= sinks:
+                    continue
+                new[b, j] = clean(s, j)
+        grown[b] = kept[b] + max(0, int(grow_n if grow is None else grow[b]))
+    too_long = grown > cols * page
+    opens = [new[b, kept[b] // page] if grown[b] > kept[b] and kept[b] % page else None for b in range(Bo)]
+    wants = []
+    for b in range(Bo):
+        o = opens[b]
+        copy = False
+        if o is not None and o >= 0:
+            holders = [x for x in range(Bo) if (new[x] == o).any()]
+            held = int((new == o).sum())
+            writers = [x for x in range(Bo) if opens[x] is not None and opens[x] == o]
+            copy = held > 1 and not (len(writers) == held and writers[0] == b)
+            assert holders
+        if grown[b] > kept[b] and not too_long[b]:
+            for j in range(kept[b] // page, -(-grown[b] // page)):
+                fresh = j * page >= kept[b]
+                if fresh or copy or o == -1:
+                    wants.append((b, j, o if copy and not fresh else None))
+    free = [pg for pg in range(n_pages) if not (new == pg).any()]
+    missing = max(0, len(wants) - len(free))
+    if missing or too_long.any():
+        old, oldlen = np.full((Bo, cols), -1), np.zeros(Bo, int)
+        for b in range(min(B, Bo)):
+            oldlen[b] = length[b]
+            for j in range(-(-int(length[b]) // page)):
+                old[b, j] = clean(b, j)
+        return old, oldlen, None, [missing, len(free), 0, int(too_long.sum())], []
+    moves = []
+    for (b, j, o), pg in zip(wants, free):
+        new[b, j] = pg
+        if o is not None:
+            moves.append((o, pg))
+    holders = np.array([(new == pg).sum() for pg in range(n_pages)])
+    return new, grown, holders, [0, len(free) - len(wants), len(moves), 0], moves
+
+
+def compact(table, length, page, n_pages):
+    """-> (table, status, [(from, to)])"""
+    B, cols = table.shape
+    out = np.full((B, cols), -1)
+    for b in range(B):
+        for j in range(-(-int(np.clip(length[b], 0, cols * page)) // page)):
+            if 0 <= table[b, j] < n_pages:
+                out[b, j] = table[b, j]
+    live = sorted(set(out[out >= 0].tolist()))
+    n = len(live)
+    moves = list(zip([x for x in live if x >= n], [x for x in range(n) if x not in set(live)]))
+    for a, b in moves:
+        out[out == a] = b
+    return out, [n, len(moves)], moves

@@ -32,7 +32,7 @@ HEADER_SYMBOLS = [
     "p0_record_begin", "p0_record_end", "p0_replay", "p0_record_info", "p0_record_free",
     "p0_chain_begin", "p0_chain_end", "p0_chain_run", "p0_chain_status", "p0_chain_info", "p0_chain_free",
     "p0_chain_tune", "p0_rowstats", "p0_normadd", "p0_argmax", "p0_argmaxM", "p0_upload_file",
-    "p0_kv_page_bytes", "p0_kv_put", "p0_kv_get", "p0_kv_attn",
+    "p0_kv_page_bytes", "p0_kv_put", "p0_kv_get", "p0_kv_attn", "p0_kv_update", "p0_kv_compact",
 ]
 
 i64, i32, f32, vp = C.c_int64, C.c_int32, C.c_float, C.c_void_p
@@ -101,6 +101,16 @@ class KvAttnArgs(C.Structure):
                 ("scale", f32), ("window", i64), ("sinks", i64), ("max_len", i64)]
 
 
+class KvUpdateArgs(C.Structure):
+    _fields_ = [("kv", Kv), ("B", i64), ("Bo", i64), ("src", vp), ("keep", vp), ("grow", vp), ("grow_n", i64),
+                ("window", i64), ("sinks", i64), ("layers", i64), ("layer_bytes", i64), ("table_out", vp), ("out_ld", i64),
+                ("len_out", vp), ("ref", vp), ("status", vp)]
+
+
+class KvCompactArgs(C.Structure):
+    _fields_ = [("kv", Kv), ("B", i64), ("layers", i64), ("layer_bytes", i64), ("table_out", vp), ("out_ld", i64), ("status", vp)]
+
+
 class P0Error(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(msg)
@@ -142,6 +152,7 @@ def lib():
             "p0_argmax": [vp, i64, vp], "p0_argmaxM": [vp, i64, i64, vp],
             "p0_upload_file": [C.c_char_p, i64, i64, vp, i64],
             "p0_kv_put": [C.POINTER(KvRowsArgs)], "p0_kv_get": [C.POINTER(KvRowsArgs)], "p0_kv_attn": [C.POINTER(KvAttnArgs)],
+            "p0_kv_update": [C.POINTER(KvUpdateArgs)], "p0_kv_compact": [C.POINTER(KvCompactArgs)],
         }
         for name, args in sig.items():
             fn = getattr(L, name)
@@ -467,3 +478,19 @@ def kv_get(args):
 
 def kv_attn(args):
     check(lib().p0_kv_attn(C.byref(args)))
+
+
+def kv_update_args(**kw):
+    return _fields(KvUpdateArgs, kw)
+
+
+def kv_update(args):
+    check(lib().p0_kv_update(C.byref(args)))
+
+
+def kv_compact_args(**kw):
+    return _fields(KvCompactArgs, kw)
+
+
+def kv_compact(args):
+    check(lib().p0_kv_compact(C.byref(args)))

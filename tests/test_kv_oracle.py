@@ -90,3 +90,35 @@ def test_attention_that_is_none_is_refused(kw, msg):
 def test_page_bytes():
     assert capi.kv_page_bytes(64, 2, 256) == 2 * 2 * 34 * 256
     assert capi.kv_page_bytes(33, 2, 256) == capi.kv_page_bytes(64, 2, 100) == 0
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(Bo=70000, src=16), "Bo 70000"), (dict(Bo=3), "3 sequences of 2 need src"),
+                                    (dict(window=-1), "window -1, sinks 0"), (dict(sinks=-1), "window 0, sinks -1"),
+                                    (dict(layers=-1), "-1 layers, 0 B apart"), (dict(layers=2, layer_bytes=64), "2 layers, 64 B apart"),
+                                    (dict(layer_bytes=8), "0 layers, 8 B apart"), (dict(table_out=None), "missing table_out or status buffer"),
+                                    (dict(status=None), "missing table_out or status buffer"), (dict(len_out=None), "missing len_out buffer"),
+                                    (dict(out_ld=3), "out_ld 3 of 4 columns"), (dict(table_out=40), "table_out or len_out overlaps what is read"),
+                                    (dict(len_out=1 << 20), "table_out or len_out overlaps what is read"),
+                                    (dict(kv=dict(n_pages=(1 << 21) + 1)), "2097153 pages (at most 2097152)"),
+                                    (dict(B=40000, kv=dict(cols=1 << 15)), "40000 sequences of 32768 columns")])
+def test_updates_that_are_none_are_refused(kw, msg):
+    base = dict(B=2, table_out=4096, len_out=8192, status=16, grow_n=1)
+    kv = dict(table=16, len=1 << 20)
+    base.update(kw)
+    kv.update(base.pop("kv", {}))
+    _refused(capi.kv_update, capi.kv_update_args(kv=_kv(**kv), **base), "kv_update: " + msg)
+    if kw.keys() <= {"layers", "layer_bytes", "table_out", "status", "out_ld", "kv", "B"} and "overlaps" not in msg:
+        for gone in ("len_out", "grow_n"):
+            base.pop(gone)
+        _refused(capi.kv_compact, capi.kv_compact_args(kv=_kv(**kv), **base), "kv_compact: " + msg)
+    if kw == dict(table_out=40):
+        _refused(capi.kv_compact, capi.kv_compact_args(kv=_kv(**kv), B=2, status=16, table_out=40), "kv_compact: table_out overlaps what is read")
+
+
+def test_an_update_by_hand():
+    """two beams of one parent in the middle of a page: the first writes on in it, the second in a copy"""
+    t, n, holders, status, moves = KV.update(np.array([[5, 3, -1], [1, 2, -1]]), np.array([40, 40]), 32, 6, 2, src=[0, 0], grow_n=1)
+    assert t.tolist() == [[5, 3, -1], [5, 0, -1]] and n.tolist() == [41, 41] and moves == [(3, 0)]
+    assert holders.tolist() == [1, 0, 0, 1, 0, 2] and status == [0, 3, 1, 0]
+    out, status, moves = KV.compact(t, n, 32, 6)
+    assert out.tolist() == [[2, 1, -1], [2, 0, -1]] and status == [3, 2] and moves == [(3, 1), (5, 2)]
