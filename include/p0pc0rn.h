@@ -319,7 +319,7 @@ int p0_normadd(const p0_normadd_args_t* a);
 int p0_argmax(const float* mx, int64_t n, uint32_t* out);
 int p0_argmaxM(const float* mx, int64_t n, int64_t M, uint32_t* out);
 
-/* ---- keys and values in 4 bits: a cache in pages, its attention, its pages ------------------------------------------ */
+/* ---- keys and values in 4 bits: a cache in pages, its attention, and a beam search over it ------------------------- */
 /* These operators have no counterpart on the int4 path of the reference (its cache is one ring of fp16 rows per layer,
  * engine/llm/gemma4.js:97-116); they are what a server of the same model needs beside it.
  *
@@ -424,6 +424,31 @@ typedef struct {
   int32_t* status;
 } p0_kv_compact_args_t;
 int p0_kv_compact(const p0_kv_compact_args_t* a);
+
+/* A beam search's step: n searches of W beams, one row of V logits (stride ld, 0 = V) and one score per beam. A beam's
+ * candidates are its k best logits (ties: the lower token) at score + (logit - log sum exp of the row); a beam with done[r] != 0
+ * (NULL: none) has one, itself, with token eos at its own score. Each search's k best (k <= 32, k <= V), by score, then
+ * beam, then the beam's own order, are written best first: token, parent (the row r the candidate continues, what
+ * p0_kv_update takes as src), score_out, done_out (parent's done, or the token is eos), each [n][k] (done_out may be
+ * NULL). eos < 0: no token ends a beam. NaN logits count as -infinity, and
+ * a sum that is not a number as a score of -infinity. Up to 65535 rows; the workspace holds 8 (k + 1) bytes per 8192 logits of them. hist (may
+ * be NULL): rows of hist_n tokens so far, hist_ld apart (0 = hist_n + 1); hist_out's row i is its parent's and the new
+ * token. Outputs must not overlap inputs. */
+typedef struct {
+  const float* logits; int64_t ld;
+  int64_t n, W, V, k;
+  const float* score;      /* [n][W] */
+  const int32_t* done;     /* [n][W] */
+  int32_t eos;
+  int32_t* token;
+  int32_t* parent;
+  float* score_out;
+  int32_t* done_out;
+  const int32_t* hist;
+  int32_t* hist_out;
+  int64_t hist_n, hist_ld;
+} p0_beam_args_t;
+int p0_beam(const p0_beam_args_t* a);
 
 /* ---- the pack reader's I/O (engine/core/store.js:221-244) ---------------------------------------------------------- */
 /* bytes [offset, offset + bytes) of the file at path -> device memory dst + dst_off, streamed in 16 MB chunks through

@@ -202,3 +202,32 @@ def compact(table, length, page, n_pages):
     for a, b in moves:
         out[out == a] = b
     return out, [n, len(moves)], moves
+
+
+def beam(logits, score, W, k, done=None, eos=-1):
+    """-> (token, parent, score, done) [n][k] and, per search, the least gap between neighbours of its first k + 1 candidates"""
+    x = np.where(np.isnan(logits), -np.inf, logits.astype(np.float64))
+    rows, V = x.shape
+    done = np.zeros(rows, bool) if done is None else np.asarray(done) != 0
+    out, gaps = [[], [], [], []], []
+    for g in range(rows // W):
+        cand = []
+        for w in range(W):
+            r = g * W + w
+            if done[r]:
+                cand += [(score[r] if i == 0 and score[r] == score[r] else -np.inf, w, i, eos) for i in range(k)]
+                continue
+            with np.errstate(invalid="ignore"):
+                m = x[r].max()
+                lse = m + np.log(np.exp(x[r] - m).sum())
+                order = np.argsort(-x[r], kind="stable")[:k]
+                for i, t in enumerate(order):
+                    s = float(score[r]) + (x[r, t] - lse)
+                    cand.append((-np.inf if s != s else s, w, i, int(t)))
+        cand.sort(key=lambda c: (-c[0], c[1], c[2]))
+        best = cand[:k]
+        gaps.append(min([a[0] - b[0] for a, b in zip(cand[:k], cand[1:k + 1]) if a[0] > b[0]] + [np.inf]))
+        for o, v in zip(out, ([c[3] for c in best], [g * W + c[1] for c in best], [c[0] for c in best],
+                              [bool(done[g * W + c[1]]) or (eos >= 0 and c[3] == eos) for c in best])):
+            o.append(v)
+    return [np.array(o) for o in out], min(gaps + [np.inf])

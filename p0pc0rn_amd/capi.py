@@ -32,7 +32,7 @@ HEADER_SYMBOLS = [
     "p0_record_begin", "p0_record_end", "p0_replay", "p0_record_info", "p0_record_free",
     "p0_chain_begin", "p0_chain_end", "p0_chain_run", "p0_chain_status", "p0_chain_info", "p0_chain_free",
     "p0_chain_tune", "p0_rowstats", "p0_normadd", "p0_argmax", "p0_argmaxM", "p0_upload_file",
-    "p0_kv_page_bytes", "p0_kv_put", "p0_kv_get", "p0_kv_attn", "p0_kv_update", "p0_kv_compact",
+    "p0_kv_page_bytes", "p0_kv_put", "p0_kv_get", "p0_kv_attn", "p0_kv_update", "p0_kv_compact", "p0_beam",
 ]
 
 i64, i32, f32, vp = C.c_int64, C.c_int32, C.c_float, C.c_void_p
@@ -111,6 +111,12 @@ class KvCompactArgs(C.Structure):
     _fields_ = [("kv", Kv), ("B", i64), ("layers", i64), ("layer_bytes", i64), ("table_out", vp), ("out_ld", i64), ("status", vp)]
 
 
+class BeamArgs(C.Structure):
+    _fields_ = [("logits", vp), ("ld", i64), ("n", i64), ("W", i64), ("V", i64), ("k", i64), ("score", vp), ("done", vp), ("eos", i32),
+                ("token", vp), ("parent", vp), ("score_out", vp), ("done_out", vp), ("hist", vp), ("hist_out", vp),
+                ("hist_n", i64), ("hist_ld", i64)]
+
+
 class P0Error(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(msg)
@@ -153,6 +159,7 @@ def lib():
             "p0_upload_file": [C.c_char_p, i64, i64, vp, i64],
             "p0_kv_put": [C.POINTER(KvRowsArgs)], "p0_kv_get": [C.POINTER(KvRowsArgs)], "p0_kv_attn": [C.POINTER(KvAttnArgs)],
             "p0_kv_update": [C.POINTER(KvUpdateArgs)], "p0_kv_compact": [C.POINTER(KvCompactArgs)],
+            "p0_beam": [C.POINTER(BeamArgs)],
         }
         for name, args in sig.items():
             fn = getattr(L, name)
@@ -494,3 +501,12 @@ def kv_compact_args(**kw):
 
 def kv_compact(args):
     check(lib().p0_kv_compact(C.byref(args)))
+
+
+def beam_args(**kw):
+    kw.setdefault("eos", -1)
+    return _fields(BeamArgs, kw)
+
+
+def beam(args):
+    check(lib().p0_beam(C.byref(args)))

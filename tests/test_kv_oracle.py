@@ -122,3 +122,28 @@ def test_an_update_by_hand():
     assert holders.tolist() == [1, 0, 0, 1, 0, 2] and status == [0, 3, 1, 0]
     out, status, moves = KV.compact(t, n, 32, 6)
     assert out.tolist() == [[2, 1, -1], [2, 0, -1]] and status == [3, 2] and moves == [(3, 1), (5, 2)]
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(n=-1), "-1 searches of 2 beams"), (dict(W=0), "1 searches of 0 beams"),
+                                    (dict(n=700, W=100), "700 searches of 100 beams"), (dict(V=0), "V 0, ld 0"), (dict(ld=99), "V 100, ld 99"),
+                                    (dict(k=0), "k 0 (1..32, at most V)"), (dict(k=33), "k 33 (1..32, at most V)"),
+                                    (dict(V=3), "k 4 (1..32, at most V)"), (dict(done=16), "done needs an eos token"),
+                                    (dict(hist=16), "hist and hist_out go together"), (dict(hist_out=16), "hist and hist_out go together"),
+                                    (dict(hist=16, hist_out=4096, hist_n=4, hist_ld=4), "hist of 4 tokens, stride 4"),
+                                    (dict(hist=16, hist_out=32, hist_n=4), "hist and hist_out overlap"),
+                                    (dict(n=60, W=1000, V=1 << 20), "60000 rows of 1048576 logits need 307200000 B of workspace")])
+def test_steps_that_are_none_are_refused(kw, msg):
+    base = dict(logits=16, n=1, W=2, V=100, k=4, score=16, token=16, parent=16, score_out=16)
+    base.update(kw)
+    _refused(capi.beam, capi.beam_args(**base), "beam: " + msg)
+    for gone in ("logits", "score", "token", "parent", "score_out"):
+        args = dict(base, **{k: v for k, v in dict(n=1, W=2, V=100, k=4, done=None, hist=None, hist_out=None, ld=0).items()})
+        args[gone] = None
+        _refused(capi.beam, capi.beam_args(**args), "beam: missing logits, score, token, parent or score_out buffer")
+
+
+def test_a_step_by_hand():
+    x = np.log(np.array([[0.5, 0.25, 0.25], [0.125, 0.75, 0.125]]))
+    (token, parent, score, done), _ = KV.beam(x, np.log([0.5, 0.5]), 2, 3, eos=1)
+    assert token.tolist() == [[1, 0, 1]] and parent.tolist() == [[1, 0, 0]] and done.tolist() == [[True, False, True]]
+    assert np.allclose(np.exp(score), [[0.375, 0.25, 0.125]])
