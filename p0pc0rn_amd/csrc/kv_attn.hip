@@ -22,15 +22,18 @@ struct AttnP {
   const void* q;
   void* y;
   int64_t q_ldb, q_ldm, q_ldh, y_ldb, y_ldm, y_ldh;
-  int64_t window;
-  int M, heads, group, R;   // R = M * group query rows of a key head
+  int window;               // 0 or at most 2^31 - 1 tokens: longer ones hide nothing
+  int M, group, R;          // R = M * group query rows of a key head
   int sinks;
-  int type, q_vec, y_vec;
+  int q_vec, y_vec;
   float scale2;             // scale * log2(e)
   int tiles, streams;       // row tiles of a workgroup, waves that share a row tile
-  int nsplit;               // workgroups that share their rows
-  float* part;
-  unsigned* cnt;
+  int groups, items;        // row groups of a key head; (sequence, key head, row group) triples
+  int shared;               // 1: long items are dealt to several workgroups, 0: a workgroup an item
+  int join;                 // 1: kv_join_kernel adds an item's parts, 0: the last workgroup to arrive does
+  int64_t slot;             // floats of a part
+  float* part;              // a part a workgroup
+  unsigned* cnt;            // per item
 };
 
 constexpr float kNone = -3.0e38f;    // the running maximum before any token
@@ -52,42 +55,49 @@ __device__ __forceinline__ float groups_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-__device__ __forceinline__ float load_one(const void* q, int64_t i, int type) {
-  if (type == P0_KV_F32) return ((const float*)q)[i];
-  if (type == P0_KV_F16) return (float)((const _Float16*)q)[i];
-  return __uint_as_float((uint32_t)((const uint16_t*)q)[i] << 16);
-}
 __device__ __forceinline__ uint16_t to_bf16(float v) {   // nearest even; NaN stays NaN
   const uint32_t u = __float_as_uint(v);
   if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)(u >> 16 | 0x40);
   return (uint16_t)((u + 0x7FFFu + (u >> 16 & 1)) >> 16);
 }
-__device__ __forceinline__ void load8(const void* q, int64_t i, int type, int vec, float (&v)[8]) {
-  if (vec) {
-    if (type == P0_KV_F32) {
-      const float4_t a = *(const float4_t*)((const float*)q + i), b = *(const float4_t*)((const float*)q + i + 4);
+// eight channels from element i on; vec: 16-byte aligned
+template <int TYPE> __device__ __forceinline__ void load8(const void* q, int64_t i, int vec, float (&v)[8]) {
+  if constexpr (TYPE == P0_KV_F32) {
+    const float* x = (const float*)q + i;
+    if (vec) {
+      const float4_t a = *(const float4_t*)x, b = *(const float4_t*)(x + 4);
 #pragma unroll
       for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
     } else {
-      const uint4_t a = *(const uint4_t*)((const uint16_t*)q + i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w = a[j];
-        if (type == P0_KV_F16) {
-          const half2_t h = __builtin_bit_cast(half2_t, w);
-          v[2 * j] = (float)h.x; v[2 * j + 1] = (float)h.y;
-        } else {
-          v[2 * j] = __uint_as_float(w << 16); v[2 * j + 1] = __uint_as_float(w & 0xFFFF0000u);
-        }
-      }
+      for (int j = 0; j < 8; ++j) v[j] = x[j];
     }
   } else {
+    const uint16_t* x = (const uint16_t*)q + i;
+    uint32_t w[4];
+    if (vec) {
+      const uint4_t a = *(const uint4_t*)x;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = load_one(q, i + j, type);
+      for (int j = 0; j < 4; ++j) w[j] = a[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = x[2 * j] | (uint32_t)x[2 * j + 1] << 16;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (TYPE == P0_KV_F16) {
+        const half2_t h = __builtin_bit_cast(half2_t, w[j]);
+        v[2 * j] = (float)h.x;
+        v[2 * j + 1] = (float)h.y;
+      } else {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+      }
+    }
   }
 }
-__device__ __forceinline__ void store8(void* y, int64_t i, int type, int vec, const float (&v)[8]) {
-  if (type == P0_KV_F32) {
+template <int TYPE> __device__ __forceinline__ void store8(void* y, int64_t i, int vec, const float (&v)[8]) {
+  if constexpr (TYPE == P0_KV_F32) {
     float* o = (float*)y + i;
     if (vec) {
       *(float4_t*)o = float4_t{v[0], v[1], v[2], v[3]};
@@ -96,21 +106,23 @@ __device__ __forceinline__ void store8(void* y, int64_t i, int type, int vec, co
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = v[j];
     }
-    return;
-  }
-  uint16_t h[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    h[j] = type == P0_KV_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[j]) : to_bf16(v[j]);
-  uint16_t* o = (uint16_t*)y + i;
-  if (vec) {
-    uint4_t w;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
-    *(uint4_t*)o = w;
   } else {
+    uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = h[j];
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (TYPE == P0_KV_F16) w[j] = __builtin_bit_cast(uint32_t, half2_t{(_Float16)v[2 * j], (_Float16)v[2 * j + 1]});
+      else w[j] = to_bf16(v[2 * j]) | (uint32_t)to_bf16(v[2 * j + 1]) << 16;
+    }
+    uint16_t* o = (uint16_t*)y + i;
+    if (vec) {
+      *(uint4_t*)o = uint4_t{w[0], w[1], w[2], w[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[2 * j] = (uint16_t)w[j];
+        o[2 * j + 1] = (uint16_t)(w[j] >> 16);
+      }
+    }
   }
 }
 
@@ -143,6 +155,13 @@ template <int D> struct KeyRegs {
     else if constexpr (D == 256) exp[0] = *(const uint32_t*)(e + lane * 4);
     else { const uint2_t w = *(const uint2_t*)(e + lane * 8); exp[0] = w.x; exp[1] = w.y; }
   }
+  // 16 tokens' operand of a step of 32 channels
+  __device__ __forceinline__ half8_t operand(int tt, int st) const {
+    const int x = D == 64 ? tt : tt * U + (st >> 2);
+    const uint32_t ew = exp[x >> 2];
+    const float e = (x & 3) == 0 ? exponent_of<0>(ew) : (x & 3) == 1 ? exponent_of<1>(ew) : (x & 3) == 2 ? exponent_of<2>(ew) : exponent_of<3>(ew);
+    return widen(D == 64 ? code[0][tt * 2 + st] : code[x % (2 * U)][st & 3], e);
+  }
 };
 template <int D> struct ValueRegs {
   uint4_t code[D / 64];      // [block / 2]: {block even: 8 tokens, block odd: 8 tokens}
@@ -152,6 +171,21 @@ template <int D> struct ValueRegs {
     for (int i = 0; i < D / 64; ++i) code[i] = *(const uint4_t*)(run + 17 * D + i * 1024 + lane * 16);
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) exp[i] = *(const uint4_t*)(run + 33 * D + ((lane >> 4) * (D / 64) + i) * 16);
+  }
+  // 32 tokens' operands of the even and the odd channels of a block
+  __device__ __forceinline__ void operands(int bl, half8_t (&a)[2]) const {
+    const uint4_t cw = code[bl >> 1], ew = exp[bl >> 1];
+    const uint32_t c0 = bl & 1 ? cw.z : cw.x, c1 = bl & 1 ? cw.w : cw.y, e0 = bl & 1 ? ew.z : ew.x, e1 = bl & 1 ? ew.w : ew.y;
+    const half2_t v[8] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c0, exponent_of<0>(e0), 0),
+                          __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c0, exponent_of<1>(e0), 1),
+                          __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c0, exponent_of<2>(e0), 2),
+                          __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c0, exponent_of<3>(e0), 3),
+                          __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c1, exponent_of<0>(e1), 0),
+                          __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c1, exponent_of<1>(e1), 1),
+                          __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c1, exponent_of<2>(e1), 2),
+                          __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c1, exponent_of<3>(e1), 3)};
+    a[0] = half8_t{v[0].x, v[1].x, v[2].x, v[3].x, v[4].x, v[5].x, v[6].x, v[7].x};
+    a[1] = half8_t{v[0].y, v[1].y, v[2].y, v[3].y, v[4].y, v[5].y, v[6].y, v[7].y};
   }
   // tokens from `left` on (of this run's 32) count as 0, whatever their bytes hold
   __device__ __forceinline__ void cut(int left, int lane) {
@@ -167,158 +201,288 @@ template <int D> struct ValueRegs {
   }
 };
 
-// the tokens a tile of rows can see: runs [0, ns) and [lo, hi)
+// the tokens that an item's rows can see: runs [0, ns) and [lo, ..), n in all
 struct Span {
-  int ns, lo, n;      // n runs in all
-  int p0, p1;         // positions of the tile's first and last row
+  int ns, lo, n;
+  int p0, p1;         // positions of the item's first and last row
   __device__ __forceinline__ int run(int i) const { return i < ns ? i : lo + (i - ns); }
 };
-__device__ __forceinline__ Span span_of(const AttnP& p, int len, int p0, int p1) {
-  Span s;
-  s.p0 = p0;
-  s.p1 = p1;
-  const int hi = (p1 + kKvRun) / kKvRun;
-  int64_t first = p.window ? (int64_t)p0 - p.window + 1 : 0;
+struct Item {
+  int b, h, rg, len, nrows;
+};
+__device__ __forceinline__ Span span_of(const AttnP& p, int rg, int len, int nrows) {
+  Span s{};
+  const int row0 = rg * p.tiles * 16, m0 = row0 / p.group, m1 = min((min(row0 + p.tiles * 16, p.R) - 1) / p.group, nrows - 1);
+  s.p0 = len - nrows + m0;
+  s.p1 = len - nrows + m1;
+  if (m0 > m1 || s.p1 < 0) return s;
+  const int64_t first = p.window ? (int64_t)s.p0 - p.window + 1 : 0;
   s.lo = first > 0 ? (int)(first / kKvRun) : 0;
-  const int ns = (int)(((int64_t)p.sinks + kKvRun - 1) / kKvRun);
+  const int ns = (int)(((int64_t)p.sinks + kKvRun - 1) / kKvRun), hi = (s.p1 + kKvRun) / kKvRun;
   s.ns = ns < s.lo ? ns : s.lo;
   s.n = s.ns + (hi > s.lo ? hi - s.lo : 0);
   return s;
 }
+// item i: sequence, then key head, then row group
+template <bool UNIFORM> __device__ __forceinline__ Item item_of(const AttnP& p, int i) {
+  Item it;
+  it.rg = i % p.groups;
+  it.h = i / p.groups % p.kv.heads;
+  it.b = i / p.groups / p.kv.heads;
+  if constexpr (UNIFORM) {
+    it.len = kv_len_uniform(p.kv, it.b);
+    const int n = p.rows ? kv_scalar(p.rows, it.b) : p.M;
+    it.nrows = n < 0 ? 0 : n < p.M ? n : p.M;
+  } else {
+    it.len = kv_len(p.kv, it.b);
+    it.nrows = kv_rows(p.rows, it.b, p.M);
+  }
+  return it;
+}
 
-// PARTS: fp16 values that a query's or a probability's f32 is taken as
-template <int D, int QPARTS, int PPARTS>
-__global__ __launch_bounds__(D == 512 ? 256 : 512) void kv_attn_kernel(const AttnP p) {
-  constexpr int NW = D == 512 ? 4 : 8;
-  constexpr int STEPS = D / 32, BLOCKS = D / 32;
-  __shared__ __attribute__((aligned(16))) float s_o[NW / 2][16 * D];
-  __shared__ float s_m[NW][16], s_l[NW][16];
+// Long items in parts, a workgroup a part: each item in as many equal parts as bring none over a common share, the least share
+// that leaves no more parts than workgroups, so that all of them run at once and end together however ragged the lengths are.
+// (Equal shares of all runs in a row, parts of two items to a workgroup where one ends, took 57 us where this takes 41: 64
+// sequences of up to 8192 tokens.) first[i]: the parts of the items before i.
+constexpr int kMostShared = 1024;   // items that are dealt so; more fill the chip an item each
+struct Deal {
+  int share, parts;
+};
+struct DealLds {
+  int first[kMostShared + 1], runs[kMostShared];
+  int sum[2][16];
+};
+// two sums over the workgroup and the exclusive prefix of the first, in thread order
+__device__ __forceinline__ int block_sums(int x, int y, int (&sum)[2][16], int* all_x, int* all_y) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6, own = x;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const int a = __shfl_up(x, s, 64), b = __shfl_up(y, s, 64);
+    if (lane >= s) { x += a; y += b; }
+  }
+  __syncthreads();   // the sums before have been read
+  if (lane == 63) { sum[0][wave] = x; sum[1][wave] = y; }
+  __syncthreads();
+  int under = 0;
+  *all_x = *all_y = 0;
+#pragma nounroll
+  for (int w = 0; w < nw; ++w) {
+    under += w < wave ? sum[0][w] : 0;
+    *all_x += sum[0][w];
+    *all_y += sum[1][w];
+  }
+  return under + x - own;
+}
+__device__ __forceinline__ Deal deal_of(const AttnP& p, int wgs, DealLds& l) {
+  const int tid = threadIdx.x;
+  int total = 0, some = 0;   // runs, items with runs
+#pragma nounroll
+  for (int i0 = 0; i0 < p.items; i0 += blockDim.x) {
+    const int i = i0 + tid;
+    int n = 0, a, b;
+    if (i < p.items) {
+      const Item it = item_of<false>(p, i);
+      l.runs[i] = n = span_of(p, it.rg, it.len, it.nrows).n;
+    }
+    block_sums(n, n > 0, l.sum, &a, &b);
+    total += a;
+    some += b;
+  }
+  // an item's last part wastes half a share on average: first as if so, then as if a whole one, which always fits
+  Deal d;
+  for (int k = 1; k <= 2; ++k) {
+    const int room = max(1, wgs - some * k / 2);
+    d.share = (max(1, (total + room - 1) / room) + p.streams - 1) / p.streams * p.streams;
+    d.parts = 0;
+#pragma nounroll
+    for (int i0 = 0; i0 < p.items; i0 += blockDim.x) {
+      const int i = i0 + tid;
+      int a, b;
+      const int c = i < p.items ? (l.runs[i] + d.share - 1) / d.share : 0, before = block_sums(c, 0, l.sum, &a, &b);
+      if (i < p.items) l.first[i] = d.parts + before;
+      d.parts += a;
+    }
+    if (tid == 0) l.first[p.items] = d.parts;
+    __syncthreads();
+    if (d.parts <= wgs) break;
+  }
+  return d;
+}
+
+// the place of eight channels of a row in y
+__device__ __forceinline__ int64_t out_at(const AttnP& p, const Item& it, int r) {
+  return (int64_t)it.b * p.y_ldb + (int64_t)(r / p.group) * p.y_ldm + (int64_t)(it.h * p.group + r % p.group) * p.y_ldh;
+}
+
+// fp16 values that a query's or a probability's f32 is taken as: 22 bits for f32; f16 and bf16 queries are exact in one. A
+// probability of one part is off by 2^-12 of itself: as much again as the rounding of an f16 output, next to nothing in bf16
+template <int TYPE> constexpr int kQParts = TYPE == P0_KV_F32 ? 2 : 1;
+template <int TYPE> constexpr int kPParts = TYPE == P0_KV_BF16 ? 1 : 2;
+
+constexpr int kRowWaves = 4, kRowThreads = 64 * kRowWaves;   // a workgroup of kv_attn_kernel
+
+// 1 / (sum of probabilities), 0 where a row has seen nothing
+__device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+
+template <int D, int TYPE>
+__global__ __launch_bounds__(kRowThreads, D <= 128 ? 4 : D == 256 ? 2 : 1) void kv_attn_kernel(const AttnP p) {
+  constexpr int NW = kRowWaves, STEPS = D / 32, BLOCKS = D / 32;
+  constexpr int QPARTS = kQParts<TYPE>, PPARTS = kPParts<TYPE>;
+  constexpr int TASKS = (D == 512 ? 1 : 2) * 16 * (D / 8), ROUNDS = (TASKS + kRowThreads - 1) / kRowThreads;
+  constexpr bool LOW_IN_LDS = D == 512 && QPARTS == 2;   // there the second parts stay in LDS: 64 registers
+  // the queries as operands [part][tile][step][lane], then the waves' sums
+  __shared__ __attribute__((aligned(16))) float s_o[NW][16 * D];
+  __shared__ float s_m[NW][16], s_l[NW][16], s_qs[2 * 16];
+  __shared__ DealLds s_deal;
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, col = lane & 15;
-  const int rg = blockIdx.y, h = blockIdx.z % p.kv.heads, b = blockIdx.z / p.kv.heads, split = blockIdx.x;
+  const int g = lane >> 4, col = lane & 15, wg = blockIdx.x;
   const int tile = wave % p.tiles, stream = wave / p.tiles;
   const bool works = stream < p.streams;
 
-  const int len = kv_len(p.kv, b), nrows = kv_rows(p.rows, b, p.M);
-  // the tile's rows, and their positions; rows past the sequence's own see nothing
-  const int row0 = (rg * p.tiles + tile) * 16, row = row0 + col, m = row / p.group;
-  const int pos = row < p.R && m < nrows ? len - nrows + m : -1;
-  const int mlast = min((row0 + 15) / p.group, nrows - 1), mfirst = row0 / p.group;
-  const bool whole = min(row0 + 15, p.R - 1) / p.group < nrows;   // every row of the tile that is one is the sequence's
-  Span sp{};
-  if (row0 < p.R && mfirst <= mlast) sp = span_of(p, len, len - nrows + mfirst, len - nrows + mlast);
-  // workgroups that have runs of any of their tiles: the last tile of the group sees the most
-  int nmax = 0;
-  for (int t = 0; t < p.tiles; ++t) {
-    const int r0 = (rg * p.tiles + t) * 16, ml = min((r0 + 15) / p.group, nrows - 1), mf = r0 / p.group;
-    if (r0 < p.R && mf <= ml) nmax = max(nmax, span_of(p, len, len - nrows + mf, len - nrows + ml).n);
+  int item = wg, part = 0, parts = 1;
+  if (p.shared) {
+    const Deal d = deal_of(p, gridDim.x, s_deal);
+    // rows that see nothing are some workgroup's too
+    for (int i = wg; i < p.items; i += gridDim.x) {
+      if (s_deal.runs[i] > 0) continue;
+      const Item it = item_of<false>(p, i);
+      const int rows = min(p.tiles * 16, p.R - it.rg * p.tiles * 16);
+      const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma nounroll
+      for (int t = tid; t < rows * (D / 8); t += kRowThreads)
+        store8<TYPE>(p.y, out_at(p, it, it.rg * p.tiles * 16 + t / (D / 8)) + t % (D / 8) * 8, p.y_vec, zero);
+    }
+    if (wg >= d.parts) return;
+    int lo = 0, hi = p.items - 1;   // the item of part wg: the last whose first part is at or before it
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_deal.first[mid] <= wg) lo = mid; else hi = mid - 1;
+    }
+    item = __builtin_amdgcn_readfirstlane(lo);
+    part = wg - __builtin_amdgcn_readfirstlane(s_deal.first[item]);
+    parts = __builtin_amdgcn_readfirstlane(s_deal.first[item + 1]) - (wg - part);
   }
-  const int active = max(1, min(p.nsplit, (nmax + p.streams - 1) / p.streams));
-  if (split >= active) return;
+  const Item it = item_of<true>(p, item);
+  const Span sp = span_of(p, it.rg, it.len, it.nrows);
+  const int each = ((sp.n + parts - 1) / parts + p.streams - 1) / p.streams * p.streams, off = part * each, end = min(sp.n, off + each);
+  const int row0 = (it.rg * p.tiles + tile) * 16, row = row0 + col, m = row / p.group;
+  const int pos = row < p.R && m < it.nrows ? it.len - it.nrows + m : -1;
+  const bool whole = min(row0 + 15, p.R - 1) / p.group < it.nrows;   // every row of the tile that is one is the sequence's
+  const int wgrow0 = it.rg * p.tiles * 16, wgrows = min(p.tiles * 16, p.R - wgrow0);
+  const int first = off + stream;
+  const bool active = works && first < end && row0 < p.R;
+
+  // ---- the loads of the queries, of the first run's page and of the run: two waits on memory, not four
+  float v[ROUNDS][8];
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int t = tid + k * kRowThreads, r = t / (D / 8), c = t % (D / 8) * 8, mm = (wgrow0 + r) / p.group;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[k][j] = 0.0f;
+    if (r < wgrows && mm < it.nrows)
+      load8<TYPE>(p.q, (int64_t)it.b * p.q_ldb + (int64_t)mm * p.q_ldm + (int64_t)(it.h * p.group + wgrow0 + r - mm * p.group) * p.q_ldh + c,
+                  p.q_vec, v[k]);
+  }
+  const int run_bytes = 34 * D, rlog = p.kv.page_log - 5, rmask = (1 << rlog) - 1;
+  const uint8_t* head = p.kv.pages + ((int64_t)it.h << rlog) * run_bytes;
+  // of run i of the span; past the last of these: the first again, so that the loads of the next run need no branch (with one
+  // the compiler waits for all of them at the loop's head, the values that are wanted last among them)
+  auto clamped = [&](int i) { return sp.run(i < end ? i : off); };
+  auto page_of = [&](int i) { return kv_page_uniform(p.kv, it.b, __builtin_amdgcn_readfirstlane(clamped(i) >> rlog)); };
+  auto run_at = [&](int i, int pg) {
+    return head + (int64_t)(pg < 0 ? 0 : pg) * p.kv.page_bytes + (int64_t)(clamped(i) & rmask) * run_bytes;
+  };
+  KeyRegs<D> kr;
+  ValueRegs<D> vr;
+  int pg = -1, pg_next = -1;
+  if (active) {
+    pg = page_of(first);
+    pg_next = page_of(first + p.streams);
+    kr.load(run_at(first, pg), lane);
+    vr.load(run_at(first, pg), lane);
+  }
+  // ---- the queries as operands, each row under a power of two that brings its largest value to [1, 2): D / 8 lanes a row
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    const int t = tid + k * kRowThreads, r = t / (D / 8), c = t % (D / 8) * 8;
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[k][j]));
+#pragma unroll
+    for (int s = 1; s < D / 8; s <<= 1) most = fmaxf(most, __shfl_xor(most, s, 64));
+    int e = (int)(__float_as_uint(most) >> 23) - 127;
+    e = most == 0.0f || e == 128 ? 0 : e < -120 ? -120 : e > 126 ? 126 : e;
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    half8_t hi, lo;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = v[k][j] * down;
+      hi[j] = (_Float16)x;
+      lo[j] = (_Float16)(x - (float)hi[j]);
+    }
+    if (r < p.tiles * 16) {
+      const int st = D == 64 ? c >> 3 & 1 : (c >> 7) * 4 + (c >> 3 & 3), gg = D == 64 ? c >> 4 : c >> 5 & 3;
+      half8_t* sq = (half8_t*)&s_o[0][0] + ((r >> 4) * STEPS + st) * 64 + gg * 16 + (r & 15);
+      *sq = hi;
+      if constexpr (QPARTS == 2) sq[p.tiles * STEPS * 64] = lo;
+      if (c == 0) s_qs[r] = ldexpf(p.scale2, e);
+    }
+  }
+  __syncthreads();
 
   float4_t o[2 * BLOCKS];
 #pragma unroll
   for (int i = 0; i < 2 * BLOCKS; ++i) o[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   float mrun = kNone, lrun = 0.0f;
-  const int first = split * p.streams + stream, stride = active * p.streams;
-
-  if (works && first < sp.n) {
-    // the queries, each row under a power of two that brings its largest value to [1, 2)
-    half8_t qh[STEPS], ql[QPARTS == 2 ? STEPS : 1];
-    float qs;
-    {
-      const bool in = pos >= 0;
-      const int64_t base = in ? (int64_t)b * p.q_ldb + (int64_t)m * p.q_ldm + (int64_t)(h * p.group + row % p.group) * p.q_ldh : 0;
-      auto channel = [&](int s) { return D == 64 ? g * 16 + 8 * s : (s >> 2) * 128 + g * 32 + 8 * (s & 3); };
-      auto get = [&](int s, float (&v)[8]) {
-        if (in) load8(p.q, base + channel(s), p.type, p.q_vec, v);
-        else
+  if (active) {
+    half8_t qh[STEPS], ql[QPARTS == 2 && !LOW_IN_LDS ? STEPS : 1];
+    const half8_t* sq = (const half8_t*)&s_o[0][0] + tile * STEPS * 64 + lane;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-      };
-      float most = 0.0f;
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        float v[8];
-        get(s, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
-      }
-      most = groups_max(most);
-      int e = (int)(__float_as_uint(most) >> 23) - 127;
-      e = most == 0.0f || e == 128 ? 0 : e < -120 ? -120 : e > 126 ? 126 : e;
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-      qs = ldexpf(p.scale2, e);
-#pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        float v[8];
-        get(s, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = v[j] * down;
-          qh[s][j] = (_Float16)x;
-          if constexpr (QPARTS == 2) ql[s][j] = (_Float16)(x - (float)qh[s][j]);
-        }
-      }
+    for (int st = 0; st < STEPS; ++st) {
+      qh[st] = sq[st * 64];
+      if constexpr (QPARTS == 2 && !LOW_IN_LDS) ql[st] = sq[(p.tiles * STEPS + st) * 64];
     }
-    const int run_bytes = 34 * D, rlog = p.kv.page_log - 5, rmask = (1 << rlog) - 1;
-    const uint8_t* head = p.kv.pages + ((int64_t)h << rlog) * run_bytes;
-    auto page_of = [&](int i) {   // of run i of the tile's; past the last: any
-      const int r = i < sp.n ? sp.run(i) : 0;
-      return __builtin_amdgcn_readfirstlane(kv_page(p.kv, b, r >> rlog));
-    };
-    auto run_at = [&](int i, int pg) {
-      const int r = i < sp.n ? sp.run(i) : 0;
-      return head + (int64_t)(pg < 0 ? 0 : pg) * p.kv.page_bytes + (int64_t)(r & rmask) * run_bytes;
-    };
-    KeyRegs<D> kr;
-    ValueRegs<D> vr;
-    int pg = page_of(first), pg_next = page_of(first + stride);
-    kr.load(run_at(first, pg), lane);
-    vr.load(run_at(first, pg), lane);
-    for (int i = first; i < sp.n; i += stride) {
+    const float qs = s_qs[tile * 16 + col];
+#pragma nounroll
+    for (int i = first; i < end; i += p.streams) {
       const int t0 = sp.run(i) * kKvRun;
       const bool dead = pg < 0;
-      // ---- scores: lane (g, col) gets tokens 16 tt + 4 g + r of row col
-      float4_t s[2];
+      // ---- scores: lane (g, col) gets tokens 16 tt + 4 g + r of row col. A chain of products per tile and part
+      float4_t s[2], sl[2];
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        s[tt] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int tt = 0; tt < 2; ++tt) s[tt] = sl[tt] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-          uint32_t w;
-          float e;
-          if constexpr (D == 64) {
-            w = kr.code[0][tt * 2 + st];
-            e = tt == 0 ? exponent_of<0>(kr.exp[0]) : exponent_of<1>(kr.exp[0]);
-          } else {
-            constexpr int U = D / 128;
-            const int u = st >> 2, x = tt * U + u;
-            w = kr.code[x][st & 3];
-            const uint32_t ew = kr.exp[x >> 2];
-            e = (x & 3) == 0 ? exponent_of<0>(ew) : (x & 3) == 1 ? exponent_of<1>(ew) : (x & 3) == 2 ? exponent_of<2>(ew) : exponent_of<3>(ew);
-          }
-          const half8_t a = widen(w, e);
+      for (int st = 0; st < STEPS; ++st) {
+        half8_t low;
+        if constexpr (LOW_IN_LDS) low = sq[(STEPS + st) * 64];
+        else if constexpr (QPARTS == 2) low = ql[st];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          const half8_t a = kr.operand(tt, st);
           s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[st], s[tt], 0, 0, 0);
-          if constexpr (QPARTS == 2) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[st], s[tt], 0, 0, 0);
+          if constexpr (QPARTS == 2) sl[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, low, sl[tt], 0, 0, 0);
         }
       }
-      const int pg_after = page_of(i + 2 * stride);
-      if (i + stride < sp.n) kr.load(run_at(i + stride, pg_next), lane);
+      if constexpr (QPARTS == 2) {
+        s[0] += sl[0];
+        s[1] += sl[1];
+      }
+      const int pg_after = page_of(i + 2 * p.streams);
+      kr.load(run_at(i + p.streams, pg_next), lane);
       // ---- what the rows do not see
       const bool all = !dead && t0 + kKvRun - 1 <= sp.p0 && whole &&
                        (!p.window || t0 > (int64_t)sp.p1 - p.window || t0 + kKvRun <= p.sinks);
       if (!all) {
+        const int last = dead ? -1 : pos, since = p.window ? pos - (int)p.window + 1 : 0;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int t = t0 + 16 * tt + 4 * g + r;
-            const bool sees = !dead && t <= pos && (!p.window || t > pos - p.window || t < p.sinks);
-            s[tt][r] = sees ? s[tt][r] : -INFINITY;
+            s[tt][r] = (t <= last) & ((t >= since) | (t < p.sinks)) ? s[tt][r] : -INFINITY;
           }
-        if (dead || t0 + kKvRun > len) vr.cut(dead ? 0 : len - t0, lane);
+        if (dead || t0 + kKvRun > it.len) vr.cut(dead ? 0 : it.len - t0, lane);
       }
       // ---- running maximum and sum
       float top = kNone;
@@ -348,129 +512,187 @@ __global__ __launch_bounds__(D == 512 ? 256 : 512) void kv_attn_kernel(const Att
       // ---- outputs: lane (g, col) gets channels 32 bl + 8 g + 2 r + u of row col
 #pragma unroll
       for (int bl = 0; bl < BLOCKS; ++bl) {
-        const uint4_t cw = vr.code[bl >> 1], ew = vr.exp[bl >> 1];
-        const uint32_t c0 = bl & 1 ? cw.z : cw.x, c1 = bl & 1 ? cw.w : cw.y, e0 = bl & 1 ? ew.z : ew.x, e1 = bl & 1 ? ew.w : ew.y;
-        const half2_t v[8] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c0, exponent_of<0>(e0), 0),
-                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c0, exponent_of<1>(e0), 1),
-                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c0, exponent_of<2>(e0), 2),
-                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c0, exponent_of<3>(e0), 3),
-                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c1, exponent_of<0>(e1), 0),
-                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c1, exponent_of<1>(e1), 1),
-                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c1, exponent_of<2>(e1), 2),
-                              __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c1, exponent_of<3>(e1), 3)};
-        const half8_t a0 = {v[0].x, v[1].x, v[2].x, v[3].x, v[4].x, v[5].x, v[6].x, v[7].x};
-        const half8_t a1 = {v[0].y, v[1].y, v[2].y, v[3].y, v[4].y, v[5].y, v[6].y, v[7].y};
-        o[2 * bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ph, o[2 * bl], 0, 0, 0);
-        o[2 * bl + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ph, o[2 * bl + 1], 0, 0, 0);
+        half8_t a[2];
+        vr.operands(bl, a);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) o[2 * bl + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[u], ph, o[2 * bl + u], 0, 0, 0);
         if constexpr (PPARTS == 2) {
-          o[2 * bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, pl, o[2 * bl], 0, 0, 0);
-          o[2 * bl + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pl, o[2 * bl + 1], 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) o[2 * bl + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[u], pl, o[2 * bl + u], 0, 0, 0);
         }
       }
-      if (i + stride < sp.n) vr.load(run_at(i + stride, pg_next), lane);
+      vr.load(run_at(i + p.streams, pg_next), lane);
       pg = pg_next;
       pg_next = pg_after;
     }
     lrun = groups_sum(lrun);
   }
 
-  // ---- waves with the same rows
+  // ---- waves with the same rows, through LDS: a thread adds eight channels of a row over the streams
+  __syncthreads();   // the queries there have been read
   if (g == 0) { s_m[wave][col] = mrun; s_l[wave][col] = lrun; }
+  if (works) {
+#pragma unroll
+    for (int k = 0; k < 2 * BLOCKS; ++k) *(float4_t*)(s_o[wave] + k * 256 + lane * 4) = o[k];
+  }
   __syncthreads();
-  float mall = kNone, lall = 0.0f;
-  for (int w = 0; w < p.streams; ++w) mall = fmaxf(mall, s_m[w * p.tiles + tile][col]);
-  for (int w = 0; w < p.streams; ++w) lall += s_l[w * p.tiles + tile][col] * exp2_fast(s_m[w * p.tiles + tile][col] - mall);
-  {
-    const float f = exp2_fast(mrun - mall);
+  float* mine = p.part + (int64_t)wg * p.slot;
+#pragma nounroll
+  for (int t = tid; t < p.tiles * BLOCKS * 64; t += kRowThreads) {
+    const int tl = t / (BLOCKS * 64), bl = t / 64 % BLOCKS, c = t & 15, gg = t >> 4 & 3, r = tl * 16 + c;
+    if (r >= wgrows) continue;
+    float mall = kNone, lall = 0.0f, f[NW];
 #pragma unroll
-    for (int k = 0; k < 2 * BLOCKS; ++k) o[k] *= f;
-  }
-  for (int half = p.streams >> 1; half > 0; half >>= 1) {
-    if (works && stream >= half && stream < 2 * half) {
-      float* d = s_o[(stream - half) * p.tiles + tile] + lane * 4;
-#pragma unroll
-      for (int k = 0; k < 2 * BLOCKS; ++k) *(float4_t*)(d + k * 256) = o[k];
+    for (int w = 0; w < NW; ++w) {   // past the last stream: the first again, at no weight
+      f[w] = w < p.streams ? s_m[w * p.tiles + tl][c] : kNone;
+      mall = fmaxf(mall, f[w]);
     }
-    __syncthreads();
-    if (stream < half) {
-      const float* d = s_o[stream * p.tiles + tile] + lane * 4;
+    float4_t x = {0.0f, 0.0f, 0.0f, 0.0f}, z = x;
 #pragma unroll
-      for (int k = 0; k < 2 * BLOCKS; ++k) o[k] += *(const float4_t*)(d + k * 256);
-    }
-    __syncthreads();
-  }
-  const bool writes = stream == 0 && row < p.R;
-  auto out_at = [&](int r) {
-    return (int64_t)b * p.y_ldb + (int64_t)(r / p.group) * p.y_ldm + (int64_t)(h * p.group + r % p.group) * p.y_ldh;
-  };
-  if (active == 1) {
-    if (writes) {
-      const float inv = lall > 0.0f || lall != lall ? 1.0f / lall : 0.0f;
-      const int64_t at = out_at(row);
+    for (int w = 0; w < NW; ++w) {
+      const int sw = (w < p.streams ? w : 0) * p.tiles + tl;
+      f[w] = w < p.streams ? exp2_fast(f[w] - mall) : 0.0f;
+      lall = w < p.streams ? fmaf(s_l[sw][c], f[w], lall) : lall;
+      const float* d = s_o[sw] + (t & 63) * 4;
+      const float4_t a = *(const float4_t*)(d + 2 * bl * 256), b = *(const float4_t*)(d + (2 * bl + 1) * 256);
+      if (w < p.streams) {
 #pragma unroll
-      for (int bl = 0; bl < BLOCKS; ++bl) {
-        float v[8];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) { v[2 * r] = o[2 * bl][r] * inv; v[2 * r + 1] = o[2 * bl + 1][r] * inv; }
-        store8(p.y, at + 32 * bl + 8 * g, p.type, p.y_vec, v);
+        for (int j = 0; j < 4; ++j) {
+          x[j] = fmaf(a[j], f[w], x[j]);
+          z[j] = fmaf(b[j], f[w], z[j]);
+        }
       }
     }
-    return;
-  }
-  // ---- workgroups with the same rows: sums to the workspace (uncached: a store is in memory once acknowledged), the last to
-  // arrive adds them in split order
-  const int item = (b * p.kv.heads + h) * gridDim.y + rg, wgrows = min(p.tiles * 16, p.R - rg * p.tiles * 16);
-  const int64_t step = wgrows * D + ((2 * wgrows + 3) & ~3);   // sums [wgrows][D], maxima, sums of probabilities
-  float* part = p.part + (int64_t)item * p.nsplit * (p.tiles * 16) * (D + 4);
-  float* mine = part + split * step;
-  if (writes) {
-    float* d = mine + (tile * 16 + col) * D + 8 * g;
-#pragma unroll
-    for (int bl = 0; bl < BLOCKS; ++bl) {
-      float4_t lo, hi;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) { lo[2 * r] = o[2 * bl][r]; lo[2 * r + 1] = o[2 * bl + 1][r]; hi[2 * r] = o[2 * bl][2 + r]; hi[2 * r + 1] = o[2 * bl + 1][2 + r]; }
-      *(float4_t*)(d + 32 * bl) = lo;
-      *(float4_t*)(d + 32 * bl + 4) = hi;
-    }
-    if (g == 0) {
-      mine[wgrows * D + tile * 16 + col] = mall;
-      mine[wgrows * D + wgrows + tile * 16 + col] = lall;
+    if (parts == 1) {
+      const float inv = inverse(lall);
+      const float y[8] = {x[0] * inv, z[0] * inv, x[1] * inv, z[1] * inv, x[2] * inv, z[2] * inv, x[3] * inv, z[3] * inv};
+      store8<TYPE>(p.y, out_at(p, it, wgrow0 + r) + 32 * bl + 8 * gg, p.y_vec, y);
+    } else {
+      float* d = mine + r * D + 32 * bl + 8 * gg;
+      *(float4_t*)d = float4_t{x[0], z[0], x[1], z[1]};
+      *(float4_t*)(d + 4) = float4_t{x[2], z[2], x[3], z[3]};
+      if (bl == 0 && gg == 0) {
+        mine[wgrows * D + 2 * r] = mall;
+        mine[wgrows * D + 2 * r + 1] = lall;
+      }
     }
   }
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (tid == 0) {
-    unsigned* c = p.cnt + item;
-    s_last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(active - 1);
-    if (s_last) __hip_atomic_exchange(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // leave it at zero
-  }
-  __syncthreads();
-  if (!s_last) return;
-  for (int t = tid; t < wgrows * (D / 8); t += blockDim.x) {
-    const int r = t / (D / 8), c = t % (D / 8) * 8;
-    float mm = kNone, ll = 0.0f;
-    for (int s = 0; s < active; ++s) mm = fmaxf(mm, __builtin_nontemporal_load(part + s * step + wgrows * D + r));
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < active; ++s) {
-      const float* x = part + s * step;
-      const float f = exp2_fast(__builtin_nontemporal_load(x + wgrows * D + r) - mm);
-      ll += f * __builtin_nontemporal_load(x + wgrows * D + wgrows + r);
-      const float4_t a = __builtin_nontemporal_load((const float4_t*)(x + r * D + c)), bb = __builtin_nontemporal_load((const float4_t*)(x + r * D + c + 4));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { v[j] = fmaf(a[j], f, v[j]); v[4 + j] = fmaf(bb[j], f, v[4 + j]); }
+  if (parts > 1 && !p.join) {
+    // ---- workgroups with the same rows: parts in the workspace (uncached: a store is in memory once acknowledged), the last
+    // to arrive adds them in order, four in flight
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+      unsigned* c = p.cnt + item;
+      s_last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(parts - 1);
+      if (s_last) __hip_atomic_exchange(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // leave it at zero
     }
-    const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f;
+    __syncthreads();
+    if (s_last) {
+      const float* all = p.part + (int64_t)(wg - part) * p.slot;
+#pragma nounroll
+      for (int t = tid; t < wgrows * (D / 8); t += kRowThreads) {
+        const int r = t / (D / 8), c = t % (D / 8) * 8;
+        float mm = kNone, ll = 0.0f, y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma nounroll
+        for (int w0 = 0; w0 < parts; w0 += 4) {   // past the last part: the last again, at no weight
+          float pm[4], pl[4];
+          float4_t a[4], b[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= inv;
-    store8(p.y, out_at(rg * p.tiles * 16 + r) + c, p.type, p.y_vec, v);
+          for (int u = 0; u < 4; ++u) {
+            const float* x = all + min(w0 + u, parts - 1) * p.slot;
+            pm[u] = __builtin_nontemporal_load(x + wgrows * D + 2 * r);
+            pl[u] = __builtin_nontemporal_load(x + wgrows * D + 2 * r + 1);
+            a[u] = __builtin_nontemporal_load((const float4_t*)(x + r * D + c));
+            b[u] = __builtin_nontemporal_load((const float4_t*)(x + r * D + c + 4));
+          }
+          const float was = mm;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mm = fmaxf(mm, pm[u]);
+          const float f0 = exp2_fast(was - mm);
+          ll *= f0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] *= f0;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (w0 + u >= parts) continue;
+            const float f = exp2_fast(pm[u] - mm);
+            ll = fmaf(f, pl[u], ll);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { y[j] = fmaf(a[u][j], f, y[j]); y[4 + j] = fmaf(b[u][j], f, y[4 + j]); }
+          }
+        }
+        const float inv = inverse(ll);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] *= inv;
+        store8<TYPE>(p.y, out_at(p, it, wgrow0 + r) + c, p.y_vec, y);
+      }
+    }
   }
 }
 
+// The parts of an item, where there may be many: a workgroup a row's 64 channels, 32 threads a channel of eight, LDS for the rest
+template <int D, int TYPE>
+__global__ __launch_bounds__(256) void kv_join_kernel(const AttnP p, int wgs) {
+  __shared__ DealLds s_deal;
+  __shared__ float s_f[4], s_w[256];
+  __shared__ __attribute__((aligned(16))) float s_v[32][64];
+  deal_of(p, wgs, s_deal);
+  const int tid = threadIdx.x, item = blockIdx.y, r = blockIdx.x / (D / 64), c = blockIdx.x % (D / 64) * 64 + (tid & 7) * 8;
+  const int wg0 = s_deal.first[item], parts = s_deal.first[item + 1] - wg0;
+  if (parts <= 1) return;
+  const Item it = item_of<true>(p, item);
+  const int wgrows = min(p.tiles * 16, p.R - it.rg * p.tiles * 16);
+  if (r >= wgrows) return;
+  const float* all = p.part + (int64_t)wg0 * p.slot;
+  float mm = kNone;
+  for (int w = tid; w < parts; w += 256) mm = fmaxf(mm, (all + w * p.slot)[wgrows * D + 2 * r]);
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) mm = fmaxf(mm, __shfl_xor(mm, s, 64));
+  if ((tid & 63) == 0) s_f[tid >> 6] = mm;
+  __syncthreads();
+  mm = fmaxf(fmaxf(s_f[0], s_f[1]), fmaxf(s_f[2], s_f[3]));
+  float ll = 0.0f, v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int w = tid >> 3; w < parts; w += 32) {
+    const float* x = all + w * p.slot;
+    const float f = exp2_fast(x[wgrows * D + 2 * r] - mm);
+    ll = fmaf(f, x[wgrows * D + 2 * r + 1], ll);
+    const float4_t a = *(const float4_t*)(x + r * D + c), b = *(const float4_t*)(x + r * D + c + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = fmaf(a[j], f, v[j]); v[4 + j] = fmaf(b[j], f, v[4 + j]); }
+  }
+  *(float4_t*)(s_v[tid >> 3] + (tid & 7) * 8) = float4_t{v[0], v[1], v[2], v[3]};
+  *(float4_t*)(s_v[tid >> 3] + (tid & 7) * 8 + 4) = float4_t{v[4], v[5], v[6], v[7]};
+  s_w[tid] = ll;
+  __syncthreads();
+  if (tid >= 8) return;
+  ll = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+  for (int w = 0; w < 32; ++w) {
+    ll += s_w[w * 8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += s_v[w][tid * 8 + j];
+  }
+  const float inv = inverse(ll);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] *= inv;
+  store8<TYPE>(p.y, out_at(p, it, it.rg * p.tiles * 16 + r) + c, p.y_vec, v);
+}
+
+template <int D, int TYPE>
+static void launch_typed(const AttnP& p, int wgs, hipStream_t s) {
+  hipLaunchKernelGGL((kv_attn_kernel<D, TYPE>), dim3((unsigned)wgs), dim3(kRowThreads), 0, s, p);
+  if (p.join)
+    hipLaunchKernelGGL((kv_join_kernel<D, TYPE>), dim3((unsigned)((p.R < p.tiles * 16 ? p.R : p.tiles * 16) * (D / 64)), (unsigned)p.items), dim3(256),
+                       0, s, p, wgs);
+}
 template <int D>
-static void launch_attn(const AttnP& p, dim3 grid, hipStream_t s) {
-  auto k = p.type == P0_KV_F32 ? kv_attn_kernel<D, 2, 2> : kv_attn_kernel<D, 1, 2>;
-  hipLaunchKernelGGL(k, grid, dim3(D == 512 ? 256 : 512), 0, s, p);
+static void launch_attn(const AttnP& p, int type, int wgs, hipStream_t s) {
+  if (type == P0_KV_F32) launch_typed<D, P0_KV_F32>(p, wgs, s);
+  else if (type == P0_KV_F16) launch_typed<D, P0_KV_F16>(p, wgs, s);
+  else launch_typed<D, P0_KV_BF16>(p, wgs, s);
 }
 
 }  // namespace p0
@@ -511,41 +733,41 @@ extern "C" int p0_kv_attn(const p0_kv_attn_args_t* a) {
   };
   p.q_vec = vec(a->q, p.q_ldh, p.q_ldm, p.q_ldb);
   p.y_vec = vec(a->y, p.y_ldh, p.y_ldm, p.y_ldb);
-  p.type = a->type;
   p.M = (int)a->M;
-  p.heads = (int)a->heads;
   p.group = (int)(a->heads / a->kv.heads);
   if (a->M * p.group > (1 << 28)) { set_error("kv_attn: M %lld of %d heads a key head", (long long)a->M, p.group); return P0_EINVAL; }
   p.R = p.M * p.group;
   const int64_t most = (int64_t)p.kv.cols << p.kv.page_log;
-  p.window = a->window >= most + a->M ? 0 : a->window;   // a window as long as the sequence hides nothing
+  p.window = a->window >= most ? 0 : (int)a->window;   // a window as long as the sequence hides nothing
   p.sinks = (int)(a->sinks < most ? a->sinks : most);
   const float scale = a->scale != 0.0f ? a->scale : 1.0f / sqrtf((float)D);
   p.scale2 = scale * 1.44269504088896340736f;
   // a workgroup's waves: row tiles first, then streams over the runs
-  const int NW = D == 512 ? 4 : 8, alltiles = (p.R + 15) / 16;
-  p.tiles = alltiles < NW ? alltiles : NW;
-  p.streams = 1;
-  while (2 * p.streams * p.tiles <= NW) p.streams *= 2;
-  const int groups = (alltiles + p.tiles - 1) / p.tiles;
-  const int64_t items = a->B * p.kv.heads * groups;
-  if (a->B * p.kv.heads > 65535 || groups > 65535) { set_error("kv_attn: %lld sequences of %d rows", (long long)a->B, p.R); return P0_EINVAL; }
-  const int64_t longest = a->max_len && a->max_len < most ? a->max_len : most;
-  const int64_t runs = (p.window && p.window + a->M + p.sinks + 2 * kKvRun < longest ? p.window + a->M + p.sinks + 2 * kKvRun : longest) / kKvRun + 1;
-  int64_t split = 512 / items;
-  if (split > runs / (2 * p.streams)) split = runs / (2 * p.streams);
-  const int64_t room = (int64_t)ctx().part_floats / (items * p.tiles * 16 * (D + 4));
-  if (split > room) split = room;
-  p.nsplit = split < 1 ? 1 : (int)split;
+  const int alltiles = (p.R + 15) / 16, most_tiles = D == 512 ? 1 : 2;
+  p.tiles = alltiles < most_tiles ? alltiles : most_tiles;
+  p.streams = kRowWaves / p.tiles;
+  p.groups = (alltiles + p.tiles - 1) / p.tiles;
+  const int64_t items = a->B * p.kv.heads * p.groups;
+  if (items > 0x7FFFFFFF) { set_error("kv_attn: %lld sequences of %d rows", (long long)a->B, p.R); return P0_EINVAL; }
+  p.items = (int)items;
+  const int64_t longest = a->max_len && a->max_len < most ? a->max_len : most, seen = p.window + a->M + p.sinks + 2 * kKvRun;
+  const int64_t runs = (p.window && seen < longest ? seen : longest) / kKvRun + 1;
+  const int64_t rows = p.R < p.tiles * 16 ? p.R : p.tiles * 16;
+  p.slot = rows * (D + 4);
   p.part = ctx().part;
   p.cnt = ctx().kv_counters;
-  if (p.nsplit > 1 && items > kKvCounters) p.nsplit = 1;
-  const dim3 grid((unsigned)p.nsplit, (unsigned)groups, (unsigned)(a->B * p.kv.heads));
+  int64_t wgs = 256 * (D <= 128 ? 4 : D == 256 ? 2 : 1);   // that run at once
+  const int64_t room = (int64_t)ctx().part_floats / p.slot, need = items * ((runs + 4 * p.streams - 1) / (4 * p.streams));
+  wgs = wgs < room ? wgs : room;
+  wgs = wgs < need ? wgs : need;
+  p.shared = items <= kMostShared && 2 * items <= wgs && runs > 8 * p.streams;
+  if (!p.shared) wgs = items;
+  p.join = p.shared && wgs > 16 * items;
   switch (D) {
-    case 64: launch_attn<64>(p, grid, ctx().cur); break;
-    case 128: launch_attn<128>(p, grid, ctx().cur); break;
-    case 256: launch_attn<256>(p, grid, ctx().cur); break;
-    default: launch_attn<512>(p, grid, ctx().cur); break;
+    case 64: launch_attn<64>(p, a->type, (int)wgs, ctx().cur); break;
+    case 128: launch_attn<128>(p, a->type, (int)wgs, ctx().cur); break;
+    case 256: launch_attn<256>(p, a->type, (int)wgs, ctx().cur); break;
+    default: launch_attn<512>(p, a->type, (int)wgs, ctx().cur); break;
   }
   P0_LAUNCHED("kv_attn");
   return P0_OK;

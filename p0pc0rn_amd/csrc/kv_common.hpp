@@ -55,6 +55,19 @@ __device__ __forceinline__ int kv_page(const KvP& p, int64_t b, int j) {
   const int pg = p.table[b * p.table_ld + j];
   return pg >= 0 && pg < p.n_pages ? pg : -1;
 }
+// the same where b and j are one for the wave: loads through the scalar cache, which no wait for vector loads holds up (the tables
+// are not written by the kernels that use these)
+typedef const __attribute__((address_space(4))) int32_t* KvConst;
+__device__ __forceinline__ int kv_scalar(const int32_t* a, int64_t i) { return ((KvConst)(uintptr_t)a)[i]; }
+__device__ __forceinline__ int kv_len_uniform(const KvP& p, int b) {
+  const int64_t most = (int64_t)p.cols << p.page_log;
+  const int n = kv_scalar(p.len, b);
+  return n < 0 ? 0 : n < most ? n : (int)most;
+}
+__device__ __forceinline__ int kv_page_uniform(const KvP& p, int b, int j) {
+  const int pg = kv_scalar(p.table, b * p.table_ld + j);
+  return pg >= 0 && pg < p.n_pages ? pg : -1;
+}
 // rows of sequence b: [0, M]
 __device__ __forceinline__ int kv_rows(const int32_t* rows, int64_t b, int M) {
   const int n = rows ? rows[b] : M;
