@@ -53,6 +53,7 @@ int ensure_xstage(size_t bytes, const char* op);   // P0_OK, or an error (no roo
 int gemm_init();
 int misc_init();
 int kv_pages_init();
+int kv_attn_init();
 
 // Thread-local message of the last failure (p0_last_error).
 void set_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
