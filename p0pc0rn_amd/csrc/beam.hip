@@ -1,10 +1,12 @@
 // beam.hip - a beam search's step: the best continuations of each search's beams, from the head's logits.
 //
 // One pass over the logits: a workgroup takes 8192 of a row, holds them in registers, and leaves their maximum, the sum of
-// their exponentials against it and their k best as 64-bit keys (the value's order, then the lower token). A second launch
-// joins a search's: the rows' sums of exponentials, each row's k best, then the k best of all beams.
-// A row's best need no full sort: at least k lanes of a wave have a maximum at or above the k-th of their sorted maxima, so
-// what lies below that is out, and what is left (a little over k values as a rule) is ranked by counting.
+// their exponentials against it and their k best as 64-bit keys (the value's order, then the lower token). The last workgroup of a
+// search to arrive joins them: the rows' sums of exponentials, each row's k best, then the k best of all beams.
+// A row's best need no sort: with the lanes in k groups, the least of the groups' best is at or below k values, so what lies
+// under it is out, and what is left (some 20 values as a rule) is ranked by counting. Where many are left, the lanes' best are
+// sorted for a closer bound: of a wave's lanes no more than k have anything at or above the k-th best of them.
+// Bound: HBM at many rows (32 searches of 8 beams, 262144 logits: 268 MB), launch and the join's round trips at few.
 #include "common.hpp"
 
 namespace p0 {
@@ -14,7 +16,7 @@ constexpr int kBmThreads = 256, kBmValues = 32, kBmChunk = kBmThreads * kBmValue
 struct BeamP {
   const float* logits;
   int64_t ld;
-  int V, W, k, chunks, vec, eos;
+  int V, W, k, chunks, eos;
   const float* score;
   const int32_t* done;
   int32_t *token, *parent;
@@ -23,8 +25,10 @@ struct BeamP {
   const int32_t* hist;
   int32_t* hist_out;
   int64_t hist_n, hist_ld;
+  // in the workspace (uncached: a store is in memory once acknowledged)
   uint64_t* keys;      // [rows][chunks][k]
   float* sums;         // [rows][chunks][2]: maximum, sum of exponentials
+  unsigned* cnt;       // per search
 };
 
 // floats in their order as unsigned: the larger float has the larger code
@@ -41,6 +45,34 @@ __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int l) {
   return (uint64_t)(uint32_t)__shfl((int)(v >> 32), l, 64) << 32 | (uint32_t)__shfl((int)(uint32_t)v, l, 64);
 }
+// lanes 8 .. 1 apart by rotations of a row of 16 (whose values then have that period), 16 and 32 apart by swaps of rows and halves
+template <int S, class F> __device__ __forceinline__ float with_lane(float v, F f) {
+  if constexpr (S == 32) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  } else if constexpr (S == 16) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  } else {
+    return f(v, __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x120 + S, 0xF, 0xF, true)));
+  }
+}
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ float added(float a, float b) { return a + b; }
+template <class F> __device__ __forceinline__ float wave_all(float v, F f) {
+  return with_lane<1>(with_lane<2>(with_lane<4>(with_lane<8>(with_lane<16>(with_lane<32>(v, f), f), f), f), f), f);
+}
+// the least of the largest of KM groups of lanes (the lanes with the same lane % KM): at most as large as KM of their values
+template <int KM> __device__ __forceinline__ float least_of_groups(float v) {
+  if constexpr (KM == 8) {
+    v = with_lane<8>(with_lane<16>(with_lane<32>(v, larger), larger), larger);
+    return with_lane<1>(with_lane<2>(with_lane<4>(v, smaller), smaller), smaller);
+  } else {
+    v = with_lane<32>(v, larger);
+    return with_lane<1>(with_lane<2>(with_lane<4>(with_lane<8>(with_lane<16>(v, smaller), smaller), smaller), smaller), smaller);
+  }
+}
 // the wave's values, largest in lane 0: a bitonic sort over its lanes
 __device__ __forceinline__ uint64_t wave_sort(uint64_t v) {
   const int lane = threadIdx.x & 63;
@@ -55,73 +87,228 @@ __device__ __forceinline__ uint64_t wave_sort(uint64_t v) {
   return v;
 }
 
-__global__ __launch_bounds__(kBmThreads) void beam_part_kernel(const BeamP p) {
-  __shared__ float s_f[4];
-  __shared__ uint64_t s_t[4];
-  __shared__ uint64_t s_list[4 * kBmMostK * kBmValues];
-  __shared__ int s_n;
+constexpr int kBmWaves = kBmThreads / 64, kBmBatch = 16;
+struct Cand {
+  uint64_t hi, lo;   // (score, beam), (logit, token)
+};
+__device__ __forceinline__ bool above(const Cand& a, const Cand& b) { return a.hi > b.hi || (a.hi == b.hi && a.lo > b.lo); }
+// KM: the most k. A chunk's list holds what the sorted bound leaves at the most
+template <int KM> struct PartLds {
+  uint64_t list[kBmWaves * KM * kBmValues];
+};
+template <int KM, int WAVES> struct JoinLds {
+  uint64_t list[WAVES][kBmBatch * KM], top[WAVES][KM];
+  Cand cand[WAVES * KM + KM];   // a round's rows and the best of the rounds before
+  Cand best[KM];
+  int row[KM], tok[KM];
+};
+constexpr float kLog2e = 1.44269504088896340736f;
+typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));   // a 16-byte load at 4-byte alignment
+
+// a row's k best of its chunks' keys and its sum of exponentials: lane r < k gets the r-th candidate of beam w
+template <int KM, int WAVES>
+__device__ __forceinline__ Cand row_best(const BeamP& p, JoinLds<KM, WAVES>& l, int64_t row, int w) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = p.k;
+  // what the row has left, all on its way before the first wait; an ended beam's too
+  const uint64_t* keys = p.keys + row * p.chunks * k;
+  const int total = p.chunks * k;
+  uint64_t q[kBmBatch], top = 0;
+  auto load = [&](int i0) {   // 15 keys a lane at a time beside the best of the batches before
+#pragma unroll
+    for (int u = 0; u < kBmBatch - 1; ++u) {
+      const int i = i0 + u * 64 + lane;
+      q[u] = i < total ? keys[i] : 0;
+    }
+  };
+  load(0);
+  const float score = p.score[row];
+  const bool ended = p.done && p.done[row];
+  float most = -INFINITY, sum = 0.0f;
+  for (int c = lane; c < p.chunks; c += 64) {
+    const float m = p.sums[(row * p.chunks + c) * 2], e = p.sums[(row * p.chunks + c) * 2 + 1], both = fmaxf(most, m);
+    sum = both == -INFINITY ? 0.0f : sum * exp2f((most - both) * kLog2e) + e * exp2f((m - both) * kLog2e);
+    most = both;
+  }
+  if (ended) {
+    const float s = lane == 0 && score == score ? score : -INFINITY;
+    return lane < k ? Cand{(uint64_t)order_of(s + 0.0f) << 32 | (uint32_t)~w, (uint64_t)(kBmMostK - lane) << 32 | (uint32_t)~p.eos} : Cand{0, 0};
+  }
+  const float own = most;
+  most = wave_all(most, larger);
+  sum = wave_all(own == -INFINITY ? 0.0f : sum * exp2f((own - most) * kLog2e), added);
+  const float lse = most + logf(sum);
+#pragma nounroll
+  for (int i0 = 0; i0 < total; i0 += 64 * (kBmBatch - 1)) {
+    if (i0) load(i0);
+    uint64_t best = top;
+#pragma unroll
+    for (int u = 0; u < kBmBatch - 1; ++u) best = q[u] > best ? q[u] : best;
+    q[kBmBatch - 1] = top;
+    uint64_t least = shfl64(wave_sort(best), k - 1);
+    if (least == 0) least = 1;
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < kBmBatch; ++u) {
+      const uint64_t in = __ballot(q[u] >= least);
+      if (q[u] >= least) l.list[wave][n + __popcll(in & ((1ull << lane) - 1))] = q[u];
+      n += __popcll(in);
+    }
+    l.top[wave][lane % KM] = 0;
+    __builtin_amdgcn_wave_barrier();
+    for (int i = lane; i < n; i += 64) {
+      const uint64_t key = l.list[wave][i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += l.list[wave][j] > key;
+      if (rank < k) l.top[wave][rank] = key;
+    }
+    __builtin_amdgcn_wave_barrier();
+    top = lane < k ? l.top[wave][lane] : 0;
+    __builtin_amdgcn_wave_barrier();
+  }
+  float s = score + (of_order((uint32_t)(top >> 32)) - lse);
+  if (s != s) s = -INFINITY;
+  return lane < k ? Cand{(uint64_t)order_of(s + 0.0f) << 32 | (uint32_t)~w, top} : Cand{0, 0};
+}
+// a search's k best, written out: a workgroup, a wave a row at a time
+template <int KM, int WAVES>
+__device__ __forceinline__ void search_best(const BeamP& p, JoinLds<KM, WAVES>& l, int64_t g) {
+  static_assert((WAVES + 1) * KM <= 64 * WAVES, "a candidate a thread");
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = p.k;
+  if (tid < k) l.best[tid] = Cand{0, 0};
+#pragma nounroll
+  for (int w0 = 0; w0 < p.W; w0 += WAVES) {
+    const int w = w0 + wave;
+    Cand mine{0, 0};
+    if (w < p.W) mine = row_best(p, l, g * p.W + w, w);
+    if (lane < k) l.cand[wave * k + lane] = mine;
+    if (tid < k) l.cand[WAVES * k + tid] = l.best[tid];
+    __syncthreads();
+    const int n = (WAVES + 1) * k;
+    if (tid < n) {
+      const Cand c = l.cand[tid];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += above(l.cand[j], c);
+      if (rank < k && c.hi) l.best[rank] = c;
+    }
+    __syncthreads();
+  }
+  if (tid < k) {
+    const Cand c = l.best[tid];
+    const int w = (int)~(uint32_t)c.hi, token = (int)~(uint32_t)c.lo, row = (int)(g * p.W + w);
+    p.token[g * k + tid] = token;
+    p.parent[g * k + tid] = row;
+    p.score_out[g * k + tid] = of_order((uint32_t)(c.hi >> 32));
+    if (p.done_out) p.done_out[g * k + tid] = (p.done && p.done[row]) || (p.eos >= 0 && token == p.eos);
+    l.row[tid] = row;
+    l.tok[tid] = token;
+  }
+  if (!p.hist) return;
+  __syncthreads();
+  for (int r = wave; r < k; r += WAVES)
+    for (int64_t c = lane; c <= p.hist_n; c += 64)
+      p.hist_out[(g * k + r) * p.hist_ld + c] = c < p.hist_n ? p.hist[l.row[r] * p.hist_ld + c] : l.tok[r];
+}
+
+// JOIN: the last of a search's workgroups to arrive joins them. It saves a launch where few are left idle by waiting for their
+// stores; many workgroups are through sooner without (us, one launch / two: 4 rows of 262144 logits 14.5 / 16.4, 256 rows 144 / 92)
+template <int KM, bool JOIN>
+__global__ __launch_bounds__(kBmThreads) void beam_kernel(const BeamP p) {
+  __shared__ union {
+    PartLds<KM> part;
+    JoinLds<JOIN ? KM : 1, kBmWaves> join;
+  } lds;
+  __shared__ float s_f[kBmWaves], s_b[kBmWaves];
+  __shared__ uint64_t s_t[kBmWaves];
+  __shared__ int s_n, s_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.y;
   const int c0 = blockIdx.x * kBmChunk;
   const float* x = p.logits + row * p.ld;
-  float v[kBmValues];
+  float v[kBmValues];   // of token c0 + (i / 4) * 1024 + tid * 4 + i % 4
+  if (c0 + kBmChunk <= p.V) {
 #pragma unroll
-  for (int i = 0; i < kBmValues / 4; ++i) {
-    const int c = c0 + i * 1024 + tid * 4;
-    if (p.vec && c + 4 <= p.V) {
-      const float4 q = *(const float4*)(x + c);
-      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
-    } else {
+    for (int i = 0; i < kBmValues / 4; ++i) {
+      const float4a4 q = *(const float4a4*)(x + c0 + i * 1024 + tid * 4);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * i + j] = c + j < p.V ? x[c + j] : -INFINITY;
+      for (int j = 0; j < 4; ++j) v[4 * i + j] = q[j];
+    }
+  } else {   // a row's end: four that are there, turned to where they belong
+    float few[3];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) few[j] = x[j < p.V ? j : 0];
+#pragma unroll
+    for (int i = 0; i < kBmValues / 4; ++i) {
+      const int c = c0 + i * 1024 + tid * 4, at = min(c, max(p.V - 4, 0)), d = c - at;
+      float4a4 q = {few[0], few[1], few[2], 0.0f};
+      if (p.V >= 4) q = *(const float4a4*)(x + at);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float y = q[j];
+#pragma unroll
+        for (int n = 1; n < 4 - j; ++n) y = d == n ? q[j + n] : y;
+        v[4 * i + j] = c + j < p.V ? y : -INFINITY;
+      }
     }
   }
   if (tid == 0) s_n = 0;
-  float most = -INFINITY;
+  // the lane's best: the first of its largest (its tokens ascend). NaN is -infinity: the maximum drops it
+  float bv = -INFINITY;
+  int bi = 0;
 #pragma unroll
   for (int i = 0; i < kBmValues; ++i) {
-    v[i] = v[i] == v[i] ? v[i] + 0.0f : -INFINITY;   // -0 is 0
-    most = fmaxf(most, v[i]);
+    v[i] = fmaxf(v[i], -INFINITY);
+    bi = v[i] > bv ? i : bi;
+    bv = fmaxf(v[i], bv);
   }
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor(most, s, 64));
-  if (lane == 0) s_f[wave] = most;
-  // the lane's best: the first of its largest (its tokens ascend)
-  uint64_t best = 0;
-#pragma unroll
-  for (int i = 0; i < kBmValues; ++i) {
-    const int c = c0 + (i >> 2) * 1024 + tid * 4 + (i & 3);
-    const uint64_t key = c < p.V ? key_of(v[i], c) : 0;
-    best = key > best ? key : best;
-  }
-  const uint64_t sorted = wave_sort(best);
-  const uint64_t kth = shfl64(sorted, p.k - 1);
-  if (lane == 0) s_t[wave] = kth;
+  const auto token = [&](int i) { return c0 + (i >> 2) * 1024 + tid * 4 + (i & 3); };
+  const uint64_t best = token(bi) < p.V ? key_of(bv + 0.0f, token(bi)) : 0;
+  float most = wave_all(bv, larger), bound = least_of_groups<KM>(bv);
+  if (lane == 0) { s_f[wave] = most; s_b[wave] = bound; }
   __syncthreads();
   most = fmaxf(fmaxf(s_f[0], s_f[1]), fmaxf(s_f[2], s_f[3]));
-  uint64_t least = s_t[0];
-#pragma unroll
-  for (int w = 1; w < 4; ++w) least = s_t[w] > least ? s_t[w] : least;
-  if (least == 0) least = 1;   // no key is 0: what lies past the row
+  bound = fmaxf(fmaxf(s_b[0], s_b[1]), fmaxf(s_b[2], s_b[3]));
+  // at or above `least` there are at least k keys: those of the bound's value and larger ones
+  uint64_t least = (uint64_t)order_of(bound + 0.0f) << 32;
   float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kBmValues; ++i) sum += most == -INFINITY ? 0.0f : exp2f((v[i] - most) * 1.44269504088896340736f);
+  for (int i = 0; i < kBmValues; ++i) sum += __builtin_amdgcn_exp2f((v[i] - most) * kLog2e);
+  if (most == -INFINITY) sum = 0.0f;
+  sum = wave_all(sum, added);
+  // the keys at or above `least`, in any order; past `most_n` they are counted only
+  auto collect = [&](int most_n) {
+    const float lv = of_order((uint32_t)(least >> 32));
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
+    for (int i = 0; i < kBmValues; ++i) {
+      if (!(v[i] >= lv)) continue;
+      const uint64_t key = key_of(v[i] + 0.0f, token(i));
+      if (key >= least && token(i) < p.V) {
+        const int at = atomicAdd(&s_n, 1);
+        if (at < most_n) lds.part.list[at] = key;
+      }
+    }
+    __syncthreads();
+    return s_n;
+  };
+  constexpr int kSmall = 256;
+  int n = collect(kSmall);
+  if (n > kSmall) {
+    const uint64_t kth = shfl64(wave_sort(best), p.k - 1);
+    __syncthreads();   // s_n has been read
+    if (lane == 0) s_t[wave] = kth;
+    if (tid == 0) s_n = 0;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kBmValues; ++i) {
-    const int c = c0 + (i >> 2) * 1024 + tid * 4 + (i & 3);
-    const uint64_t key = c < p.V ? key_of(v[i], c) : 0;
-    if (key >= least) s_list[atomicAdd(&s_n, 1)] = key;
+    for (int w = 0; w < kBmWaves; ++w) least = w == 0 || s_t[w] > least ? s_t[w] : least;
+    if (least == 0) least = (uint64_t)order_of(-INFINITY) << 32;   // fewer lanes than k have a token: all of theirs
+    n = collect(kBmWaves * KM * kBmValues);
   }
-  __syncthreads();   // s_f and the list
   if (lane == 0) s_f[wave] = sum;
-  const int n = s_n;
   uint64_t* out = p.keys + (row * p.chunks + blockIdx.x) * p.k;
   for (int i = tid; i < n; i += kBmThreads) {
-    const uint64_t key = s_list[i];
+    const uint64_t key = lds.part.list[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s_list[j] > key;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += lds.part.list[j] > key;
     if (rank < p.k) out[rank] = key;
   }
   if (tid >= n && tid < p.k) out[tid] = 0;   // a chunk of fewer than k
@@ -130,125 +317,34 @@ __global__ __launch_bounds__(kBmThreads) void beam_part_kernel(const BeamP p) {
     p.sums[(row * p.chunks + blockIdx.x) * 2] = most;
     p.sums[(row * p.chunks + blockIdx.x) * 2 + 1] = (s_f[0] + s_f[1]) + (s_f[2] + s_f[3]);
   }
-}
-
-struct Cand {
-  uint64_t hi, lo;   // (score, beam), (logit, token)
-};
-__device__ __forceinline__ bool above(const Cand& a, const Cand& b) { return a.hi > b.hi || (a.hi == b.hi && a.lo > b.lo); }
-
-// a workgroup a search: a wave a row at a time
-constexpr int kBmJoinThreads = 512, kBmJoinWaves = kBmJoinThreads / 64, kBmBatch = 16;
-__global__ __launch_bounds__(kBmJoinThreads) void beam_join_kernel(const BeamP p) {
-  __shared__ uint64_t s_list[kBmJoinWaves][kBmBatch * kBmMostK];
-  __shared__ Cand s_cand[kBmJoinWaves * kBmMostK + kBmMostK];   // a round's rows and the best of the rounds before
-  __shared__ Cand s_best[kBmMostK];
-  __shared__ int s_row[kBmMostK], s_tok[kBmMostK];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = p.k;
-  const int64_t g = blockIdx.x;
-  for (int i = tid; i < k; i += kBmJoinThreads) s_best[i] = Cand{0, 0};
-  for (int w0 = 0; w0 < p.W; w0 += kBmJoinWaves) {
-    const int w = w0 + wave;
-    Cand mine{0, 0};   // lane r < k: the row's r-th
-    if (w < p.W) {
-      const int64_t row = g * p.W + w;
-      const float score = p.score[row];
-      if (p.done && p.done[row]) {
-        if (lane < k) {
-          const float s = lane == 0 && score == score ? score : -INFINITY;
-          mine = Cand{(uint64_t)order_of(s + 0.0f) << 32 | (uint32_t)~w, (uint64_t)(kBmMostK - lane) << 32 | (uint32_t)~p.eos};
-        }
-      } else {
-        // the row's sum of exponentials
-        float most = -INFINITY;
-        for (int c = lane; c < p.chunks; c += 64) most = fmaxf(most, p.sums[(row * p.chunks + c) * 2]);
-#pragma unroll
-        for (int s = 32; s > 0; s >>= 1) most = fmaxf(most, __shfl_xor(most, s, 64));
-        float sum = 0.0f;
-        for (int c = lane; c < p.chunks; c += 64) {
-          const float m = p.sums[(row * p.chunks + c) * 2], e = p.sums[(row * p.chunks + c) * 2 + 1];
-          sum += m == -INFINITY ? 0.0f : e * exp2f((m - most) * 1.44269504088896340736f);
-        }
-#pragma unroll
-        for (int s = 32; s > 0; s >>= 1) sum += __shfl_xor(sum, s, 64);
-        const float lse = most + logf(sum);
-        // its k best, 15 keys a lane at a time beside those of the batches before
-        const uint64_t* keys = p.keys + row * p.chunks * k;
-        const int total = p.chunks * k;
-        uint64_t top = 0;
-        for (int i0 = 0; i0 < total; i0 += 64 * (kBmBatch - 1)) {
-          uint64_t q[kBmBatch], best = top;
-#pragma unroll
-          for (int u = 0; u < kBmBatch - 1; ++u) {
-            const int i = i0 + u * 64 + lane;
-            q[u] = i < total ? keys[i] : 0;
-            best = q[u] > best ? q[u] : best;
-          }
-          q[kBmBatch - 1] = top;
-          uint64_t least = shfl64(wave_sort(best), k - 1);
-          if (least == 0) least = 1;
-          int n = 0;
-#pragma unroll
-          for (int u = 0; u < kBmBatch; ++u) {
-            const uint64_t in = __ballot(q[u] >= least);
-            if (q[u] >= least) s_list[wave][n + __popcll(in & ((1ull << lane) - 1))] = q[u];
-            n += __popcll(in);
-          }
-          __builtin_amdgcn_wave_barrier();
-          top = 0;
-          uint64_t next = 0;
-          for (int i = lane; i < n + 63 - (n + 63) % 64; i += 64) {   // every lane the same number of times
-            const uint64_t key = i < n ? s_list[wave][i] : 0;
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += s_list[wave][j] > key;
-            const bool in = i < n && rank < k;
-            // lane `rank` takes it
-            uint64_t m = __ballot(in);
-            while (m) {
-              const int l = __ffsll((unsigned long long)m) - 1;
-              const uint64_t v = shfl64(key, l);
-              if (lane == __shfl(rank, l, 64)) next = v;
-              m &= m - 1;
-            }
-          }
-          top = next;
-          __builtin_amdgcn_wave_barrier();
-        }
-        if (lane < k) {
-          float s = score + (of_order((uint32_t)(top >> 32)) - lse);
-          if (s != s) s = -INFINITY;
-          mine = Cand{(uint64_t)order_of(s + 0.0f) << 32 | (uint32_t)~w, top};
-        }
-      }
-    }
-    if (lane < k) s_cand[wave * k + lane] = mine;
-    if (tid < k) s_cand[kBmJoinWaves * k + tid] = s_best[tid];
-    __syncthreads();
-    const int n = (kBmJoinWaves + 1) * k;
-    for (int i = tid; i < n; i += kBmJoinThreads) {
-      const Cand c = s_cand[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += above(s_cand[j], c);
-      if (rank < k && c.hi) s_best[rank] = c;
-    }
-    __syncthreads();
-  }
-  if (tid < k) {
-    const Cand c = s_best[tid];
-    const int w = (int)~(uint32_t)c.hi, token = (int)~(uint32_t)c.lo, row = (int)(g * p.W + w);
-    p.token[g * k + tid] = token;
-    p.parent[g * k + tid] = row;
-    p.score_out[g * k + tid] = of_order((uint32_t)(c.hi >> 32));
-    if (p.done_out) p.done_out[g * k + tid] = (p.done && p.done[row]) || (p.eos >= 0 && token == p.eos);
-    s_row[tid] = row;
-    s_tok[tid] = token;
-  }
-  if (!p.hist) return;
+  if constexpr (!JOIN) return;
+  const int64_t g = row / p.W;
+  __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  for (int64_t i = tid; i < k * (p.hist_n + 1); i += kBmJoinThreads) {
-    const int r = (int)(i / (p.hist_n + 1)), c = (int)(i % (p.hist_n + 1));
-    p.hist_out[(g * k + r) * p.hist_ld + c] = c < p.hist_n ? p.hist[s_row[r] * p.hist_ld + c] : s_tok[r];
+  if (tid == 0) {
+    unsigned* c = p.cnt + g;
+    s_last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(p.W * p.chunks - 1);
+    if (s_last) __hip_atomic_exchange(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // leave it at zero
   }
+  __syncthreads();
+  if constexpr (JOIN)
+    if (s_last) search_best(p, lds.join, g);
+}
+constexpr int kBmJoinWaves = 8;
+template <int KM>
+__global__ __launch_bounds__(64 * kBmJoinWaves) void beam_join_kernel(const BeamP p) {
+  __shared__ JoinLds<KM, kBmJoinWaves> lds;
+  search_best(p, lds, blockIdx.x);
+}
+template <int KM>
+static void launch_beam(const BeamP& p, int64_t n, hipStream_t s) {
+  const dim3 grid((unsigned)p.chunks, (unsigned)(n * p.W));
+  if (n * p.W * p.chunks <= 1024) {
+    hipLaunchKernelGGL((beam_kernel<KM, true>), grid, dim3(kBmThreads), 0, s, p);
+    return;
+  }
+  hipLaunchKernelGGL((beam_kernel<KM, false>), grid, dim3(kBmThreads), 0, s, p);
+  hipLaunchKernelGGL(beam_join_kernel<KM>, dim3((unsigned)n), dim3(64 * kBmJoinWaves), 0, s, p);
 }
 
 }  // namespace p0
@@ -290,7 +386,6 @@ extern "C" int p0_beam(const p0_beam_args_t* a) {
   p.W = (int)a->W;
   p.k = (int)a->k;
   p.chunks = (int)chunks;
-  p.vec = (uintptr_t)a->logits % 16 == 0 && p.ld % 4 == 0;
   p.eos = a->eos;
   p.score = a->score;
   p.done = a->done;
@@ -304,8 +399,9 @@ extern "C" int p0_beam(const p0_beam_args_t* a) {
   p.hist_ld = a->hist_ld ? a->hist_ld : a->hist_n + 1;
   p.keys = (uint64_t*)ctx().part;
   p.sums = (float*)(p.keys + rows * chunks * a->k);
-  hipLaunchKernelGGL(beam_part_kernel, dim3((unsigned)chunks, (unsigned)rows), dim3(kBmThreads), 0, ctx().cur, p);
-  hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)a->n), dim3(kBmJoinThreads), 0, ctx().cur, p);
+  p.cnt = ctx().kv_counters;
+  if (a->k <= 8) launch_beam<8>(p, a->n, ctx().cur);
+  else launch_beam<32>(p, a->n, ctx().cur);
   P0_LAUNCHED("beam");
   return P0_OK;
 }
