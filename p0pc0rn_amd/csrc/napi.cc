@@ -289,6 +289,84 @@ napi_value ArgmaxM(napi_env env, napi_callback_info info) {   // argmaxM(mx, n, 
   return undef(env);
 }
 
+// ---- the 4-bit cache: flat argument objects, the descriptor's fields prefixed kv_
+p0_kv_t kv_of(napi_env env, napi_value o) {
+  p0_kv_t c{};
+  c.pages = ptr<void>(env, o, "kv_pages"); c.n_pages = i64(env, o, "kv_n_pages"); c.page_bytes = i64(env, o, "kv_page_bytes");
+  c.page = i32(env, o, "kv_page"); c.heads = i32(env, o, "kv_heads"); c.dim = i32(env, o, "kv_dim");
+  c.table = ptr<const int32_t>(env, o, "kv_table"); c.table_ld = i64(env, o, "kv_table_ld"); c.cols = i64(env, o, "kv_cols");
+  c.len = ptr<const int32_t>(env, o, "kv_len");
+  return c;
+}
+napi_value KvPageBytes(napi_env env, napi_callback_info info) {   // kvPageBytes(page, heads, dim)
+  auto a = args(env, info, 3);
+  return make_num(env, (double)p0_kv_page_bytes((int32_t)num(env, a[0]), (int32_t)num(env, a[1]), (int32_t)num(env, a[2])));
+}
+napi_value kv_rows(napi_env env, napi_callback_info info, int (*fn)(const p0_kv_rows_args_t*)) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_kv_rows_args_t r{};
+  r.kv = kv_of(env, o); r.B = i64(env, o, "B"); r.M = i64(env, o, "M");
+  r.rows = ptr<const int32_t>(env, o, "rows"); r.at = ptr<const int32_t>(env, o, "at"); r.type = i32(env, o, "type");
+  r.k = ptr<void>(env, o, "k"); r.v = ptr<void>(env, o, "v");
+  r.ldb = i64(env, o, "ldb"); r.ldm = i64(env, o, "ldm"); r.ldh = i64(env, o, "ldh");
+  if (fail(env, fn(&r))) return nullptr;
+  return undef(env);
+}
+napi_value KvPut(napi_env env, napi_callback_info info) { return kv_rows(env, info, p0_kv_put); }
+napi_value KvGet(napi_env env, napi_callback_info info) { return kv_rows(env, info, p0_kv_get); }
+napi_value KvAttn(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_kv_attn_args_t r{};
+  r.kv = kv_of(env, o); r.B = i64(env, o, "B"); r.M = i64(env, o, "M");
+  r.rows = ptr<const int32_t>(env, o, "rows"); r.heads = i64(env, o, "heads"); r.type = i32(env, o, "type");
+  r.q = ptr<const void>(env, o, "q"); r.q_ldb = i64(env, o, "q_ldb"); r.q_ldm = i64(env, o, "q_ldm"); r.q_ldh = i64(env, o, "q_ldh");
+  r.y = ptr<void>(env, o, "y"); r.y_ldb = i64(env, o, "y_ldb"); r.y_ldm = i64(env, o, "y_ldm"); r.y_ldh = i64(env, o, "y_ldh");
+  r.scale = (float)field(env, o, "scale"); r.window = i64(env, o, "window"); r.sinks = i64(env, o, "sinks");
+  r.max_len = i64(env, o, "max_len");
+  if (fail(env, p0_kv_attn(&r))) return nullptr;
+  return undef(env);
+}
+napi_value KvUpdate(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_kv_update_args_t r{};
+  r.kv = kv_of(env, o); r.B = i64(env, o, "B"); r.Bo = i64(env, o, "Bo");
+  r.src = ptr<const int32_t>(env, o, "src"); r.keep = ptr<const int32_t>(env, o, "keep");
+  r.grow = ptr<const int32_t>(env, o, "grow"); r.grow_n = i64(env, o, "grow_n");
+  r.window = i64(env, o, "window"); r.sinks = i64(env, o, "sinks");
+  r.layers = i64(env, o, "layers"); r.layer_bytes = i64(env, o, "layer_bytes");
+  r.table_out = ptr<int32_t>(env, o, "table_out"); r.out_ld = i64(env, o, "out_ld"); r.len_out = ptr<int32_t>(env, o, "len_out");
+  r.ref = ptr<int32_t>(env, o, "ref"); r.status = ptr<int32_t>(env, o, "status");
+  if (fail(env, p0_kv_update(&r))) return nullptr;
+  return undef(env);
+}
+napi_value KvCompact(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_kv_compact_args_t r{};
+  r.kv = kv_of(env, o); r.B = i64(env, o, "B"); r.layers = i64(env, o, "layers"); r.layer_bytes = i64(env, o, "layer_bytes");
+  r.table_out = ptr<int32_t>(env, o, "table_out"); r.out_ld = i64(env, o, "out_ld"); r.status = ptr<int32_t>(env, o, "status");
+  if (fail(env, p0_kv_compact(&r))) return nullptr;
+  return undef(env);
+}
+napi_value Beam(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_beam_args_t r{};
+  r.logits = ptr<const float>(env, o, "logits"); r.ld = i64(env, o, "ld");
+  r.n = i64(env, o, "n"); r.W = i64(env, o, "W"); r.V = i64(env, o, "V"); r.k = i64(env, o, "k");
+  r.score = ptr<const float>(env, o, "score"); r.done = ptr<const int32_t>(env, o, "done");
+  r.eos = (int32_t)field(env, o, "eos", -1);
+  r.token = ptr<int32_t>(env, o, "token"); r.parent = ptr<int32_t>(env, o, "parent");
+  r.score_out = ptr<float>(env, o, "score_out"); r.done_out = ptr<int32_t>(env, o, "done_out");
+  r.hist = ptr<const int32_t>(env, o, "hist"); r.hist_out = ptr<int32_t>(env, o, "hist_out");
+  r.hist_n = i64(env, o, "hist_n"); r.hist_ld = i64(env, o, "hist_ld");
+  if (fail(env, p0_beam(&r))) return nullptr;
+  return undef(env);
+}
+
 napi_value UploadFile(napi_env env, napi_callback_info info) {   // uploadFile(path, offset, bytes, dst, dstOff)
   auto a = args(env, info, 5);
   size_t len = 0;
@@ -398,6 +476,8 @@ napi_value Init(napi_env env, napi_value exports) {
       {"replay", Replay}, {"recordInfo", RecordInfo}, {"recordFree", RecordFree}, {"chainInfo", ChainInfo}, {"chainBegin", ChainBegin}, {"chainEnd", ChainEnd},
       {"chainRun", ChainRun}, {"chainStatus", ChainStatus}, {"chainFree", ChainFree},
       {"rowstats", Rowstats}, {"normadd", Normadd}, {"argmaxM", ArgmaxM}, {"uploadFile", UploadFile},
+      {"kvPageBytes", KvPageBytes}, {"kvPut", KvPut}, {"kvGet", KvGet}, {"kvAttn", KvAttn}, {"kvUpdate", KvUpdate},
+      {"kvCompact", KvCompact}, {"beam", Beam},
   };
   for (auto& f : fns) {
     napi_value v;

@@ -641,3 +641,81 @@ console.log(JSON.stringify(res));
     assert res[7] == "gemm: epilogue onormgate is not part of this build"
     assert res[8] == "gemm: heads.rope needs 2048 B of a 2047 B buffer"
     assert res[9] == "gemm: heads ropeMode sideways"
+
+
+def test_js_cache_refusals(tmp_path):
+    """the library's own messages, and views against their buffers before the call"""
+    out = run_node(tmp_path, r"""
+const g = {}, B = { ptr: 4096 }, small = { ptr: 4096, _pf: 64 };
+const kv = (o) => Object.assign({ pages: { buf: B }, n: 4, page: 64, heads: 2, dim: 128, table: { buf: B }, cols: 4, len: { buf: B } }, o);
+const res = [];
+const t = (f) => { try { f(); res.push('no error'); } catch (e) { res.push(e.message); } };
+t(() => P.kvPut(g, { kv: kv({ page: 48 }), B: 1, M: 1, k: { buf: B }, v: { buf: B } }));
+t(() => P.kvGet(g, { kv: kv({}), B: 1, M: 1, k: { buf: small }, v: { buf: B } }));
+t(() => P.kvPut(g, { kv: kv({ pages: { buf: small } }), B: 1, M: 1, k: { buf: B }, v: { buf: B } }));
+t(() => P.kvAttn(g, { kv: kv({}), B: 1, M: 1, heads: 3, q: { buf: B }, y: { buf: B } }));
+t(() => P.kvAttn(g, { kv: kv({}), B: 2, M: 1, heads: 4, type: 'f8', q: { buf: B }, y: { buf: B } }));
+t(() => P.kvAttn(g, { kv: kv({}), B: 2, M: 3, heads: 4, type: 'f16', q: { buf: small }, y: { buf: B } }));
+t(() => P.kvUpdate(g, { kv: kv({}), B: 2, Bo: 3, grow: 1, out: { table: { buf: { ptr: 65536 } }, len: { buf: { ptr: 8192 } }, status: { buf: B } } }));
+t(() => P.kvUpdate(g, { kv: kv({}), B: 2, grow: 1, out: { table: { buf: B }, len: { buf: { ptr: 8192 } }, status: { buf: B } } }));
+t(() => P.kvCompact(g, { kv: kv({ len: { buf: small } }), B: 20, out: { table: { buf: { ptr: 65536 } }, status: { buf: B } } }));
+t(() => P.beam(g, { logits: { buf: B }, n: 1, W: 2, V: 100, k: 40, score: { buf: B }, out: { token: { buf: B }, parent: { buf: B }, score: { buf: B } } }));
+t(() => P.beam(g, { logits: { buf: small }, n: 1, W: 2, V: 100, k: 4, score: { buf: B }, out: { token: { buf: B }, parent: { buf: B }, score: { buf: B } } }));
+console.log(JSON.stringify(res));
+""")
+    assert json.loads(out.strip().splitlines()[-1]) == [
+        "kv_put: no pages of 48 tokens, 2 heads of 128", "kv_get: k needs 1024 B of a 64 B buffer", "kv_put: pages needs 69632 B of a 64 B buffer",
+        "kv_attn: 3 heads over 2 key heads", "kv_attn: type f8", "kv_attn: q needs 6144 B of a 64 B buffer",
+        "kv_update: 3 sequences of 2 need src", "kv_update: table_out or len_out overlaps what is read", "kv_compact: len needs 80 B of a 64 B buffer",
+        "beam: k 40 (1..32, at most V)", "beam: logits needs 800 B of a 64 B buffer"]
+
+
+@pytest.mark.gpu
+def test_js_cache_and_beam(tmp_path):
+    """a prompt's rows put and attended to, the sequence forked and compacted, a beam step: against the CPU restatement"""
+    from oracle import kvcache as KV
+    H, D, n, M, V = 2, 64, 70, 3, 500
+    rng = np.random.default_rng(1)
+    k, v = (rng.standard_normal((1, n, H, D)).astype(np.float32) for _ in "kv")
+    q = rng.standard_normal((1, M, 4, D)).astype(np.float32)
+    logits = (3 * rng.standard_normal((2, V))).astype(np.float32)
+    table = np.array([[6, 3, 5, -1]], np.int32)
+    _save(tmp_path, k=k, v=v, q=q, logits=logits, table=table, len=np.array([n], np.int32), src=np.zeros(2, np.int32),
+          score=np.array([-1, -1.5], np.float32))
+    run_node(tmp_path, r"""
+const g = await_gpu();
+const up = (name) => { const b = fs.readFileSync(name + '.bin'); return { buf: g.upload(new Uint8Array(b.buffer, b.byteOffset, b.length)) }; };
+const [k, v, q, logits, table, len, src, score] = ['k', 'v', 'q', 'logits', 'table', 'len', 'src', 'score'].map(up);
+const out = (bytes) => ({ buf: g.buffer(bytes) });
+const kv = { pages: out(8 * P.kvPageBytes(32, 2, 64)), n: 8, page: 32, heads: 2, dim: 64, table, cols: 4, len };
+const [y, k2, v2, t2, n2, ref, st, t3, st3, tok, par, sc] = [3072, 35840, 35840, 32, 8, 32, 16, 32, 8, 16, 16, 16].map(out);
+P.kvPut(g, { kv, B: 1, M: 70, k, v });
+P.kvGet(g, { kv, B: 1, M: 70, k: k2, v: v2 });
+P.kvAttn(g, { kv, B: 1, M: 3, heads: 4, q, y, window: 40, sinks: 4, maxLen: 70 });
+P.kvUpdate(g, { kv, B: 1, Bo: 2, src, grow: 1, out: { table: t2, len: n2, ref, status: st } });
+P.kvCompact(g, { kv: Object.assign({}, kv, { table: t2, len: n2 }), B: 2, out: { table: t3, status: st3 } });
+P.beam(g, { logits, n: 1, W: 2, V: 500, k: 4, score, out: { token: tok, parent: par, score: sc } });
+(async () => {
+  await g.done();
+  for (const [name, b] of Object.entries({ y, k2, v2, t2, n2, t3, st, st3, tok, par, sc }))
+    fs.writeFileSync(name + '.out', Buffer.from(await g.read(b.buf)));
+  g.freeAll(); g.device.destroy();
+})();
+""")
+    got = lambda name, dt: np.fromfile(str(tmp_path / (name + ".out")), dt)  # noqa: E731
+    hk, hv = KV.held(k, v)
+    assert np.array_equal(got("k2", np.float32), hk.ravel()) and np.array_equal(got("v2", np.float32), hv.ravel())
+    c = KV.Cache(8, 32, H, D)
+    for t in range(n):
+        for h in range(H):
+            c.write(table[0, t // 32], t % 32, h, k[0, t, h], v[0, t, h])
+    want = KV.attention(c, table, [n], q, window=40, sinks=4)
+    assert rel_l2(got("y", np.float32), want) <= 5e-6
+    t2, n2, _, st, moves = KV.update(table, np.array([n]), 32, 8, 2, src=[0, 0], grow_n=1)
+    assert np.array_equal(got("t2", np.int32), t2.ravel()) and got("n2", np.int32)[:2].tolist() == n2.tolist()
+    assert got("st", np.int32).tolist() == st
+    t3, st3, _ = KV.compact(t2, n2, 32, 8)
+    assert np.array_equal(got("t3", np.int32), t3.ravel()) and got("st3", np.int32)[:2].tolist() == st3
+    (token, parent, score, _), _ = KV.beam(logits, np.array([-1, -1.5], np.float32), 2, 4)
+    assert got("tok", np.int32).tolist() == token[0].tolist() and got("par", np.int32).tolist() == parent[0].tolist()
+    assert np.allclose(got("sc", np.float32), score[0], rtol=0, atol=1e-5)
