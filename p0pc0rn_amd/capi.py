@@ -455,7 +455,10 @@ def upload_file(path, offset, nbytes, dst, dst_off=0):
 # ------------------------------------------------------------------------------------------------ the 4-bit cache
 def _fields(cls, kw):
     """cls from keyword fields; Buffer objects are accepted where the header takes a pointer"""
-    return cls(**{k: v.ptr if isinstance(v, Buffer) else v for k, v in kw.items()})
+    try:
+        return cls(**kw)
+    except TypeError:   # a Buffer among them
+        return cls(**{k: v.ptr if isinstance(v, Buffer) else v for k, v in kw.items()})
 
 
 def kv_page_bytes(page, heads, dim):

@@ -224,12 +224,13 @@ __device__ __forceinline__ Span span_of(const AttnP& p, int rg, int len, int nro
   s.n = s.ns + (hi > s.lo ? hi - s.lo : 0);
   return s;
 }
-// item i: sequence, then key head, then row group
+// item i: sequence, then row group, then key head (so that an XCD, which gets every eighth workgroup, keeps to few heads)
 template <bool UNIFORM> __device__ __forceinline__ Item item_of(const AttnP& p, int i) {
   Item it;
-  it.rg = i % p.groups;
-  it.h = i / p.groups % p.kv.heads;
-  it.b = i / p.groups / p.kv.heads;
+  const int pair = i / p.kv.heads;
+  it.h = i - pair * p.kv.heads;
+  it.b = p.groups == 1 ? pair : pair / p.groups;
+  it.rg = pair - it.b * p.groups;
   if constexpr (UNIFORM) {
     it.len = kv_len_uniform(p.kv, it.b);
     const int n = p.rows ? kv_scalar(p.rows, it.b) : p.M;
@@ -243,71 +244,76 @@ template <bool UNIFORM> __device__ __forceinline__ Item item_of(const AttnP& p, 
 
 // Long items in parts, a workgroup a part: each item in as many equal parts as bring none over a common share, the least share
 // that leaves no more parts than workgroups, so that all of them run at once and end together however ragged the lengths are.
-// (Equal shares of all runs in a row, parts of two items to a workgroup where one ends, took 57 us where this takes 41: 64
-// sequences of up to 8192 tokens.) first[i]: the parts of the items before i.
-constexpr int kMostShared = 512;   // items that are dealt so; more fill the chip an item each
-struct Deal {
-  int share, parts;
-};
-struct DealLds {
-  int first[kMostShared + 1], runs[kMostShared];
-  int sum[2][16];
-};
-// two sums over the workgroup and the exclusive prefix of the first, in thread order
-__device__ __forceinline__ int block_sums(int x, int y, int (&sum)[2][16], int* all_x, int* all_y) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6, own = x;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const int a = __shfl_up(x, s, 64), b = __shfl_up(y, s, 64);
-    if (lane >= s) { x += a; y += b; }
-  }
-  __syncthreads();   // the sums before have been read
-  if (lane == 63) { sum[0][wave] = x; sum[1][wave] = y; }
-  __syncthreads();
-  int under = 0;
-  *all_x = *all_y = 0;
-#pragma nounroll
-  for (int w = 0; w < nw; ++w) {
-    under += w < wave ? sum[0][w] : 0;
-    *all_x += sum[0][w];
-    *all_y += sum[1][w];
-  }
-  return under + x - own;
+// (Equal shares of all runs in a row, parts of two items to a workgroup where one ends, took 57 us where this takes 38: 64
+// sequences of up to 8192 tokens.) A key head's items are alike, so a lane looks at (sequence, row group) pairs; every wave works
+// the deal out for itself, without LDS and barriers.
+constexpr int kMostItems = 512;   // 2 items <= workgroups <= 1024
+constexpr int kMostPairs = 512;   // that are dealt so; more fill the chip an item each
+__device__ __forceinline__ int wave_sum(int v) {
+  const auto a = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  v = (int)(a[0] + a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  v = (int)(b[0] + b[1]);
+  v += __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);
+  v += __builtin_amdgcn_mov_dpp(v, 0x124, 0xF, 0xF, true);
+  v += __builtin_amdgcn_mov_dpp(v, 0x122, 0xF, 0xF, true);
+  return v + __builtin_amdgcn_mov_dpp(v, 0x121, 0xF, 0xF, true);
 }
-__device__ __forceinline__ Deal deal_of(const AttnP& p, int wgs, DealLds& l) {
-  const int tid = threadIdx.x;
-  int total = 0, some = 0;   // runs, items with runs
-#pragma nounroll
-  for (int i0 = 0; i0 < p.items; i0 += blockDim.x) {
-    const int i = i0 + tid;
-    int n = 0, a, b;
-    if (i < p.items) {
-      const Item it = item_of<false>(p, i);
-      l.runs[i] = n = span_of(p, it.rg, it.len, it.nrows).n;
+struct Part {
+  int item, part, parts;   // item -1: this workgroup has none
+};
+// zeros(item): an item whose rows see nothing, one workgroup's
+template <class F> __device__ __forceinline__ Part part_of(const AttnP& p, int wg, int wgs, F zeros) {
+  const int lane = threadIdx.x & 63, H = p.kv.heads, pairs = p.items / H;
+  int n[kMostPairs / 64], total = 0, some = 0;   // runs of this lane's pairs; of all; pairs with runs
+#pragma unroll
+  for (int k = 0; k < kMostPairs / 64; ++k) {
+    n[k] = 0;
+    if (k * 64 >= pairs) continue;
+    const int i = k * 64 + lane;
+    if (i < pairs) {
+      const Item it = item_of<false>(p, i * H);
+      n[k] = span_of(p, it.rg, it.len, it.nrows).n;
     }
-    block_sums(n, n > 0, l.sum, &a, &b);
-    total += a;
-    some += b;
+    total += wave_sum(n[k]);
+    some += __popcll(__ballot(n[k] > 0));
+    for (uint64_t none = __ballot(i < pairs && n[k] == 0); none; none &= none - 1) {
+      const int z = (k * 64 + __ffsll((unsigned long long)none) - 1) * H;
+      for (int h = (wg + wgs - z % wgs) % wgs; h < H; h += wgs) zeros(z + h);
+    }
   }
+  total = __builtin_amdgcn_readfirstlane(total);
   // an item's last part wastes half a share on average: first as if so, then as if a whole one, which always fits
-  Deal d;
-  for (int k = 1; k <= 2; ++k) {
-    const int room = max(1, wgs - some * k / 2);
-    d.share = (max(1, (total + room - 1) / room) + p.streams - 1) / p.streams * p.streams;
-    d.parts = 0;
-#pragma nounroll
-    for (int i0 = 0; i0 < p.items; i0 += blockDim.x) {
-      const int i = i0 + tid;
-      int a, b;
-      const int c = i < p.items ? (l.runs[i] + d.share - 1) / d.share : 0, before = block_sums(c, 0, l.sum, &a, &b);
-      if (i < p.items) l.first[i] = d.parts + before;
-      d.parts += a;
+  Part r{-1, 0, 1};
+  for (int t = 1; t <= 2; ++t) {
+    const int room = max(1, wgs - some * H * t / 2);
+    int share = ((int64_t)total * H + room - 1) / room;
+    share = (max(share, 1) + p.streams - 1) / p.streams * p.streams;
+    int first = 0;   // parts before
+    r.item = -1;
+#pragma unroll
+    for (int k = 0; k < kMostPairs / 64; ++k) {
+      if (k * 64 >= pairs) continue;
+      const int c = (n[k] + share - 1) / share;
+      int x = c;
+#pragma unroll
+      for (int s = 1; s < 64; s <<= 1) {
+        const int y = __shfl_up(x, s, 64);
+        if (lane >= s) x += y;
+      }
+      const int under = first + (x - c) * H;
+      const uint64_t here = __ballot(c > 0 && under <= wg && wg < under + c * H);
+      if (here) {
+        const int l = __ffsll((unsigned long long)here) - 1, in = wg - __builtin_amdgcn_readlane(under, l);
+        r.parts = __builtin_amdgcn_readlane(c, l);
+        r.item = (k * 64 + l) * H + in / r.parts;
+        r.part = in % r.parts;
+      }
+      first += __builtin_amdgcn_readlane(x, 63) * H;
     }
-    if (tid == 0) l.first[p.items] = d.parts;
-    __syncthreads();
-    if (d.parts <= wgs) break;
+    if (first <= wgs) break;
   }
-  return d;
+  return r;
 }
 
 // the place of eight channels of a row in y
@@ -338,7 +344,6 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
   // the queries as operands [part][tile][step][lane], then the halves of the scores [round % 2][wave][tile][lane], then the waves' sums
   __shared__ __attribute__((aligned(16))) float s_o[NW * SPLIT][16 * D / SPLIT];
   __shared__ float s_m[NW][16], s_l[NW][16], s_qs[NW * 16];
-  __shared__ DealLds s_deal;
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15, wg = blockIdx.x;
@@ -347,27 +352,19 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
 
   int item = wg, part = 0, parts = 1;
   if (p.shared) {
-    const Deal d = deal_of(p, gridDim.x, s_deal);
-    // rows that see nothing are some workgroup's too
-    for (int i = wg; i < p.items; i += gridDim.x) {
-      if (s_deal.runs[i] > 0) continue;
+    const Part r = part_of(p, wg, gridDim.x, [&](int i) {   // rows that see nothing
       if (tid == 0) p.dealt[2 * i + 1] = 0;
-      const Item it = item_of<false>(p, i);
+      const Item it = item_of<true>(p, i);
       const int rows = min(p.tiles * 16, p.R - it.rg * p.tiles * 16);
       const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma nounroll
-      for (int t = tid; t < rows * (D / 8); t += kRowThreads<D, W>)
+      for (int t = tid; t < rows * (D / 8); t += blockDim.x)
         store8<TYPE>(p.y, out_at(p, it, it.rg * p.tiles * 16 + t / (D / 8)) + t % (D / 8) * 8, p.y_vec, zero);
-    }
-    if (wg >= d.parts) return;
-    int lo = 0, hi = p.items - 1;   // the item of part wg: the last whose first part is at or before it
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_deal.first[mid] <= wg) lo = mid; else hi = mid - 1;
-    }
-    item = __builtin_amdgcn_readfirstlane(lo);
-    part = wg - __builtin_amdgcn_readfirstlane(s_deal.first[item]);
-    parts = __builtin_amdgcn_readfirstlane(s_deal.first[item + 1]) - (wg - part);
+    });
+    if (r.item < 0) return;
+    item = r.item;
+    part = r.part;
+    parts = r.parts;
     if (part == 0 && tid == 0) {
       p.dealt[2 * item] = wg;
       p.dealt[2 * item + 1] = parts;
@@ -677,33 +674,25 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kerne
   constexpr int QPARTS = kQParts<TYPE>, PPARTS = TYPE == P0_KV_F32 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) uint8_t s_raw[];
   half8_t* buf = (half8_t*)s_raw;   // [2][RUNS][FRAGS][64]
-  __shared__ DealLds s_deal;
   __shared__ int s_dead[2][RUNS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15, wg = blockIdx.x;
 
   int item = wg, part = 0, parts = 1;
   if (p.shared) {
-    const Deal d = deal_of(p, gridDim.x, s_deal);
-    for (int i = wg; i < p.items; i += gridDim.x) {   // rows that see nothing
-      if (s_deal.runs[i] > 0) continue;
+    const Part r = part_of(p, wg, gridDim.x, [&](int i) {   // rows that see nothing
       if (tid == 0) p.dealt[2 * i + 1] = 0;
-      const Item it = item_of<false>(p, i);
+      const Item it = item_of<true>(p, i);
       const int rows = min(p.tiles * 16, p.R - it.rg * p.tiles * 16);
       const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma nounroll
-      for (int t = tid; t < rows * (D / 8); t += S::kThreads)
+      for (int t = tid; t < rows * (D / 8); t += blockDim.x)
         store8<TYPE>(p.y, out_at(p, it, it.rg * p.tiles * 16 + t / (D / 8)) + t % (D / 8) * 8, p.y_vec, zero);
-    }
-    if (wg >= d.parts) return;
-    int lo = 0, hi = p.items - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_deal.first[mid] <= wg) lo = mid; else hi = mid - 1;
-    }
-    item = __builtin_amdgcn_readfirstlane(lo);
-    part = wg - __builtin_amdgcn_readfirstlane(s_deal.first[item]);
-    parts = __builtin_amdgcn_readfirstlane(s_deal.first[item + 1]) - (wg - part);
+    });
+    if (r.item < 0) return;
+    item = r.item;
+    part = r.part;
+    parts = r.parts;
     if (part == 0 && tid == 0) {
       p.dealt[2 * item] = wg;
       p.dealt[2 * item + 1] = parts;
@@ -1112,13 +1101,13 @@ extern "C" int p0_kv_attn(const p0_kv_attn_args_t* a) {
   const int64_t rows = p.R < p.tiles * 16 ? p.R : p.tiles * 16;
   p.slot = rows * (D + 4);
   p.dealt = (int32_t*)ctx().part;
-  p.part = ctx().part + 2 * kMostShared;
+  p.part = ctx().part + 2 * kMostItems;
   p.cnt = ctx().kv_counters;
   int64_t wgs = 256 * (form == kTiles ? 2 : D == 64 ? kRowGroups<64> : D == 128 ? kRowGroups<128> : D == 256 ? kRowGroups<256> : kRowGroups<512>);
-  const int64_t room = ((int64_t)ctx().part_floats - 2 * kMostShared) / p.slot, need = items * ((runs + 4 * p.streams - 1) / (4 * p.streams));
+  const int64_t room = ((int64_t)ctx().part_floats - 2 * kMostItems) / p.slot, need = items * ((runs + 4 * p.streams - 1) / (4 * p.streams));
   wgs = wgs < room ? wgs : room;
   wgs = wgs < need ? wgs : need;
-  p.shared = items <= kMostShared && 2 * items <= wgs && runs > (D == 512 ? 4 : 10) * p.streams;
+  p.shared = items / p.kv.heads <= kMostPairs && 2 * items <= wgs && runs > (D == 512 ? 4 : 10) * p.streams;
   if (!p.shared) {
     wgs = items;
     if (form == kRows4 && D < 512 && items <= 256 && runs > p.streams) {   // CUs to spare: eight waves an item
