@@ -62,6 +62,21 @@ def test_the_best_continuations(dev, n, W, k, V):
         assert np.abs(s.reshape(n, k) - got[2]).max() <= 5e-5
 
 
+@pytest.mark.parametrize("n,W,k,V", [(300, 4, 4, 100), (300, 4, 20, 100), (40, 16, 16, 17000), (1100, 1, 1, 3)])
+def test_rows_enough_for_a_join_of_its_own(dev, n, W, k, V):
+    """among so many searches some scores lie within a rounding: each place's score, then that its token has it"""
+    rng = np.random.default_rng(n + k)
+    x = (3 * rng.standard_normal((n * W, V))).astype(np.float32)
+    score = (-20 * rng.random(n * W)).astype(np.float32)
+    want, _ = KV.beam(x, score, W, k)
+    got, _ = step(x, score, W, k)
+    assert np.abs(got[2] - want[2]).max() <= 2.0 ** -22 * 96
+    at = got[1].ravel(), got[0].ravel()
+    s = score[at[0]].astype(np.float64) + x[at] - np.log(np.exp(x.astype(np.float64)).sum(1))[at[0]]
+    assert np.abs(s.reshape(n, k) - got[2]).max() <= 2.0 ** -22 * 96
+    assert all(len(set(zip(t, p))) == k for t, p in zip(got[0].tolist(), got[1].tolist()))
+
+
 @pytest.mark.parametrize("ld,shift", [(501, 0), (512, 1), (504, 4), (600, 3)])
 def test_strides_and_alignments(dev, ld, shift):
     rng = np.random.default_rng(ld)

@@ -229,6 +229,75 @@ def test_windows_and_first_tokens(dev, window, sinks, D, M):
     c.free()
 
 
+@pytest.mark.parametrize("type_", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,M,G,H", [(64, 64, 4, 2), (64, 300, 1, 1), (128, 86, 3, 2), (128, 64, 8, 1), (128, 257, 1, 2)])
+def test_rows_that_share_converted_runs(dev, D, type_, M, G, H):
+    """256 rows of a key head and more, over lengths of which some are in parts"""
+    lens = [M, M + 333, M // 2, 0, 1500]
+    c = Held(lens, D, H, 64, seed=M + D)
+    rows = [M, M - 1, M, M, M]
+    q = np.random.default_rng(M).standard_normal((5, M, G * H, D))
+    got, exact = run_attn(c, q, type_, rows=rows)
+    again, _ = run_attn(c, q, type_, rows=rows)
+    assert np.array_equal(got, again)
+    want = KV.attention(c.c, c.table, c.len, exact, rows=rows)
+    assert not got[2, :M - M // 2].any() and not got[3].any() and not got[1, M - 1:].any()
+    check(got, want, type_)
+    c.free()
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (7, 3), (100, 200), (333, 4), (3, 100000)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_windows_of_rows_that_share_converted_runs(dev, D, window, sinks):
+    M = 130
+    c = Held([900, 140, 60], D, 1, 32, seed=window + D)
+    c.table[0, 3], c.table[0, 26] = -1, c.c.n_pages          # tokens 96-127 and 832-863 have no page
+    c.send()
+    q = np.random.default_rng(sinks % 1000).standard_normal((3, M, 2, D))
+    got, exact = run_attn(c, q, "f32", window=window, sinks=sinks, pad=(8, 3, 0), shift=2)
+    check(got, KV.attention(c.c, c.table, c.len, exact, window=window, sinks=sinks), "f32")
+    c.free()
+
+
+def test_a_token_that_is_no_number_among_shared_runs(dev):
+    M, n, D = 256, 420, 128
+
+    def special(b, h, k, v):
+        k[n - 40, 5] = np.inf                               # rows 216.. see it
+    c = Held([n], D, 1, 32, seed=5, special=special)
+    q = np.random.default_rng(5).standard_normal((1, M, 1, D))
+    got, exact = run_attn(c, q, "f32")
+    with np.errstate(invalid="ignore"):
+        want = KV.attention(c.c, c.table, c.len, exact)
+    assert np.isnan(got[0, M - 40:]).all() and not np.isnan(got[0, :M - 40]).any()
+    check(got[~np.isnan(got)], want[~np.isnan(want)], "f32")
+    c.free()
+
+
+@pytest.mark.parametrize("D,M,G,n,type_", [(64, 1, 4, 9000, "f32"), (128, 3, 8, 5000, "f16"), (256, 1, 16, 9000, "bf16"), (64, 256, 1, 3000, "f32"),
+                                           (128, 128, 2, 3000, "f16"), (512, 1, 8, 9000, "f32"), (512, 3, 8, 3000, "f16"), (512, 10, 8, 3000, "bf16")])
+def test_many_parts_of_one_item(dev, D, M, G, n, type_):
+    c = Held([n], D, 1, 128, seed=D + M)
+    q = np.random.default_rng(D + M).standard_normal((1, M, G, D))
+    got, exact = run_attn(c, q, type_)
+    check(got, KV.attention(c.c, c.table, c.len, exact), type_)
+    c.free()
+
+
+@pytest.mark.parametrize("B,H,D", [(150, 2, 64), (70, 3, 128), (33, 4, 256)])
+def test_many_sequences_of_very_different_lengths(dev, B, H, D):
+    """few long ones in parts beside short ones and empty ones"""
+    rng = np.random.default_rng(B)
+    lens = np.where(rng.random(B) < 0.5, 0, rng.integers(1, 40, B))
+    lens[[0, B // 2, B - 1]] = 1700, 900, 1333
+    c = Held(lens.tolist(), D, H, 64, seed=B)
+    q = rng.standard_normal((B, 1, 2 * H, D))
+    got, exact = run_attn(c, q, "f32")
+    assert not got[lens == 0].any()
+    check(got, KV.attention(c.c, c.table, c.len, exact), "f32")
+    c.free()
+
+
 def test_pages_outside_the_window_may_be_given_up(dev):
     D, window, sinks = 128, 50, 5
     c = Held([400, 333], D, 2, 32, seed=3)
