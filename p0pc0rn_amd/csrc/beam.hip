@@ -113,10 +113,13 @@ __device__ __forceinline__ Cand row_best(const BeamP& p, JoinLds<KM, WAVES>& l, 
   const uint64_t* keys = p.keys + row * p.chunks * k;
   const int total = p.chunks * k;
   uint64_t q[kBmBatch], top = 0;
-  auto load = [&](int i0) {   // 15 keys a lane at a time beside the best of the batches before
+  // 15 keys a lane at a time beside the best of the batches before. A chunk's keys descend, so the lanes turn from one 64 to the
+  // next: each gets keys of many ranks, and the k-th best of the lanes' best leaves few (32 of 262144 logits: 33 us the call, 92
+  // where a lane kept to a rank)
+  auto load = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < kBmBatch - 1; ++u) {
-      const int i = i0 + u * 64 + lane;
+      const int i = i0 + u * 64 + (lane + 13 * u) % 64;
       q[u] = i < total ? keys[i] : 0;
     }
   };
@@ -209,8 +212,10 @@ __device__ __forceinline__ void search_best(const BeamP& p, JoinLds<KM, WAVES>& 
       p.hist_out[(g * k + r) * p.hist_ld + c] = c < p.hist_n ? p.hist[l.row[r] * p.hist_ld + c] : l.tok[r];
 }
 
-// JOIN: the last of a search's workgroups to arrive joins them. It saves a launch where few are left idle by waiting for their
-// stores; many workgroups are through sooner without (us, one launch / two: 4 rows of 262144 logits 14.5 / 16.4, 256 rows 144 / 92)
+// The pass over the logits: 43 us for 256 rows of 262144 (6.2 TB/s, HBM); at few rows one memory round trip and the ranking.
+// JOIN: the last of a search's workgroups to arrive joins them. It saves a launch where its four waves have a row each and few
+// workgroups wait for their own stores before they count themselves in; else a join of eight waves a search is sooner. (us, one
+// launch / two: a search of 4 beams of 262144 logits 13.9 / 14.5, of 8 20.1 / 16.3; 4 searches of 4 18.0 / 16.2, 32 of 8 118 / 61.)
 template <int KM, bool JOIN>
 __global__ __launch_bounds__(kBmThreads) void beam_kernel(const BeamP p) {
   __shared__ union {
@@ -331,6 +336,7 @@ __global__ __launch_bounds__(kBmThreads) void beam_kernel(const BeamP p) {
     if (s_last) search_best(p, lds.join, g);
 }
 constexpr int kBmJoinWaves = 8;
+// bound: memory latency, one round trip a row, then the ranks from LDS (32 searches of 8 beams of 32 chunks: 10.6 us)
 template <int KM>
 __global__ __launch_bounds__(64 * kBmJoinWaves) void beam_join_kernel(const BeamP p) {
   __shared__ JoinLds<KM, kBmJoinWaves> lds;
@@ -339,7 +345,7 @@ __global__ __launch_bounds__(64 * kBmJoinWaves) void beam_join_kernel(const Beam
 template <int KM>
 static void launch_beam(const BeamP& p, int64_t n, hipStream_t s) {
   const dim3 grid((unsigned)p.chunks, (unsigned)(n * p.W));
-  if (n * p.W * p.chunks <= 1024) {
+  if (p.W <= kBmWaves && n * p.W * p.chunks <= 256) {
     hipLaunchKernelGGL((beam_kernel<KM, true>), grid, dim3(kBmThreads), 0, s, p);
     return;
   }
