@@ -244,7 +244,7 @@ template <bool UNIFORM> __device__ __forceinline__ Item item_of(const AttnP& p, 
 
 // Long items in parts, a workgroup a part: each item in as many equal parts as bring none over a common share, the least share
 // that leaves no more parts than workgroups, so that all of them run at once and end together however ragged the lengths are.
-// (Equal shares of all runs in a row, parts of two items to a workgroup where one ends, took 57 us where this takes 38: 64
+// (Equal shares of all runs in a row, parts of two items to a workgroup where one ends, took 57 us where this takes 37: 64
 // sequences of up to 8192 tokens.) A key head's items are alike, so a lane looks at (sequence, row group) pairs; every wave works
 // the deal out for itself, without LDS and barriers.
 constexpr int kMostItems = 512;   // 2 items <= workgroups <= 1024
@@ -329,6 +329,10 @@ template <int TYPE> constexpr int kPParts = TYPE == P0_KV_BF16 ? 1 : 2;
 // A workgroup of kv_attn_kernel: waves of 16 rows each, W of them or, at 512 channels, W pairs (the registers of one wave a
 // SIMD would hold them all, but a wave alone issues at half the rate): each of a pair has half of the channels' products and
 // outputs, and they exchange their halves of the scores through LDS
+// Bound: at few rows the vector instructions that turn 4-bit codes into fp16 operands and the softmax of 16 columns of which few
+// are rows (64 sequences of up to 8192 tokens, 128 channels, 4 heads a key head: 146 MB in 37 us, 4.0 TB/s of the 6.3 that a
+// read reaches; 5 rows of 8 heads, 512 channels, 131071 tokens: 70 us, of which the loop over the runs takes 40); of a short
+// sequence the chain from the page table to the first scores (one row over 517 tokens: 12.5 us)
 template <int D> constexpr int kRowSplit = D == 512 ? 2 : 1;
 template <int D, int W> constexpr int kRowThreads = 64 * W * kRowSplit<D>;
 template <int D> constexpr int kRowGroups = D == 64 ? 4 : D == 128 ? 3 : D == 256 ? 2 : 1;   // of them on a CU: what the registers allow
@@ -924,7 +928,8 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kerne
   }
 }
 
-// The parts of an item in a launch of their own: LANES threads for eight channels of a row, each its share of the parts, then LDS
+// The parts of an item in a launch of their own: LANES threads for eight channels of a row, each its share of the parts, then LDS.
+// Bound: memory latency, a few round trips (256 parts of 40 rows of 512 channels, 21 MB from the caches: 9 us)
 template <int D, int TYPE, int LANES>
 __global__ __launch_bounds__(256) void kv_join_kernel(const AttnP p) {
   constexpr int TASKS = 256 / LANES;
@@ -1082,9 +1087,15 @@ extern "C" int p0_kv_attn(const p0_kv_attn_args_t* a) {
   const float scale = a->scale != 0.0f ? a->scale : 1.0f / sqrtf((float)D);
   p.scale2 = scale * 1.44269504088896340736f;
   const int alltiles = (p.R + 15) / 16;
-  // rows that fill two workgroups of eight tiles share converted runs (f16, 128 channels, 2 x 64 rows of 4 heads a key head over
-  // 4096 tokens: 38.5 us, 40.0 without; f32 4 x 16 rows: 29.6, 23.7 without)
-  Form form = D <= 128 && p.R >= 256 ? kTiles : kRows4;
+  const int64_t longest = a->max_len && a->max_len < most ? a->max_len : most, seen = p.window + a->M + p.sinks + 2 * kKvRun;
+  const int64_t runs = (p.window && seen < longest ? seen : longest) / kKvRun + 1;
+  // Rows share converted runs where the chip's workgroups get enough runs each to outweigh a longer start and a barrier a round,
+  // fewer of 16-bit queries, whose products are cheaper beside the conversion. (us, shared / each wave for itself, 128 channels,
+  // 4 key heads of 4 heads over 4096 tokens: f16 32 x 32 rows 76 / 99, 2 x 1024 112 / 144, 4 x 128 52 / 56; over 2048, 8 key
+  // heads, 2 x 128 rows, 41 / 37; f32 2 x 1024 rows 152 / 159, 32 x 64 160 / 168, 4 x 128 65 / 58; 64 channels, f16, 8 x 256
+  // 77 / 105, 4 x 64 36 / 29.)
+  const int64_t work = a->B * p.kv.heads * ((p.R + 16 * TileShape<64>::TILES - 1) / (16 * TileShape<64>::TILES)) * runs;
+  Form form = D <= 128 && p.R >= 128 && work >= (a->type == P0_KV_F32 ? 48 : 12) * 512 ? kTiles : kRows4;
   if (form == kTiles) {
     p.tiles = TileShape<64>::TILES;
     p.streams = 2;
@@ -1096,8 +1107,6 @@ extern "C" int p0_kv_attn(const p0_kv_attn_args_t* a) {
   const int64_t items = a->B * p.kv.heads * p.groups;
   if (items > 0x7FFFFFFF) { set_error("kv_attn: %lld sequences of %d rows", (long long)a->B, p.R); return P0_EINVAL; }
   p.items = (int)items;
-  const int64_t longest = a->max_len && a->max_len < most ? a->max_len : most, seen = p.window + a->M + p.sinks + 2 * kKvRun;
-  const int64_t runs = (p.window && seen < longest ? seen : longest) / kKvRun + 1;
   const int64_t rows = p.R < p.tiles * 16 ? p.R : p.tiles * 16;
   p.slot = rows * (D + 4);
   p.dealt = (int32_t*)ctx().part;
@@ -1107,10 +1116,13 @@ extern "C" int p0_kv_attn(const p0_kv_attn_args_t* a) {
   const int64_t room = ((int64_t)ctx().part_floats - 2 * kMostItems) / p.slot, need = items * ((runs + 4 * p.streams - 1) / (4 * p.streams));
   wgs = wgs < room ? wgs : room;
   wgs = wgs < need ? wgs : need;
-  p.shared = items / p.kv.heads <= kMostPairs && 2 * items <= wgs && runs > (D == 512 ? 4 : 10) * p.streams;
+  // Few items in parts, where the runs that a part saves outweigh the join. (us, in parts / not: one row of 4 heads a key head,
+  // 256 channels, 800 tokens 16.2 / 14.9, 1200 16.5 / 18.5, 2500 18.0 / 29.0; 512 channels, one row of 8 heads, 600 tokens
+  // 20.3 / 21.5, five rows, 150 tokens 29.9 / 25.0, 300 33.4 / 37.3.)
+  p.shared = items / p.kv.heads <= kMostPairs && 2 * items <= wgs && runs > (D == 512 ? 3 * p.streams + 4 : 9 * p.streams);
   if (!p.shared) {
     wgs = items;
-    if (form == kRows4 && D < 512 && items <= 256 && runs > p.streams) {   // CUs to spare: eight waves an item
+    if (form == kRows4 && D < 512 && items <= 256 && runs > p.streams) {   // CUs to spare: eight waves an item (one row over 517 tokens 12.5 us, 14.3 in four)
       form = kRows8;
       p.streams = 8 / p.tiles;
     }
