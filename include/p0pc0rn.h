@@ -395,8 +395,9 @@ int p0_kv_attn(const p0_kv_attn_args_t* a);
  * NULL) and status are written, table and len are read: they must not overlap. At most 2^21 pages here and in p0_kv_compact.
  * status (device, 4 words): pages that were missing, free pages left, pages copied, sequences longer than cols * page. Where
  * the first or last is not 0 nothing has been done: table_out and len_out are the old sequences (the first min(B, Bo);
- * further ones are empty), ref is as it was, and the second word is the pages that there were to take. So this forks (several src alike), reorders (a beam search's
- * parents), truncates (the rows a verify pass refused), extends and frees (src -1). */
+ * further ones are empty), ref is as it was, and the second word is the pages that there were to take. So this forks
+ * (several src alike), reorders (a beam search's parents), truncates (the rows a verify pass refused), extends and frees
+ * (src -1). */
 typedef struct {
   p0_kv_t kv;
   int64_t B, Bo;           /* sequences before, after (0 = B; src is needed where they differ) */
@@ -430,10 +431,10 @@ int p0_kv_compact(const p0_kv_compact_args_t* a);
  * (NULL: none) has one, itself, with token eos at its own score. Each search's k best (k <= 32, k <= V), by score, then
  * beam, then the beam's own order, are written best first: token, parent (the row r the candidate continues, what
  * p0_kv_update takes as src), score_out, done_out (parent's done, or the token is eos), each [n][k] (done_out may be
- * NULL). eos < 0: no token ends a beam. NaN logits count as -infinity, and
- * a sum that is not a number as a score of -infinity. Up to 65535 rows; the workspace holds 8 (k + 1) bytes per 8192 logits of them. hist (may
- * be NULL): rows of hist_n tokens so far, hist_ld apart (0 = hist_n + 1); hist_out's row i is its parent's and the new
- * token. Outputs must not overlap inputs. */
+ * NULL). eos < 0: no token ends a beam. NaN logits count as -infinity, and a sum that is not a number as a score of
+ * -infinity. Up to 65535 rows; the workspace holds 8 (k + 1) bytes per 8192 logits of them. hist (may be NULL): rows of
+ * hist_n tokens so far, hist_ld apart (0 = hist_n + 1); hist_out's row i is its parent's and the new token. Outputs must not
+ * overlap inputs. */
 typedef struct {
   const float* logits; int64_t ld;
   int64_t n, W, V, k;

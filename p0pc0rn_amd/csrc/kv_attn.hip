@@ -330,7 +330,7 @@ template <int TYPE> constexpr int kPParts = TYPE == P0_KV_BF16 ? 1 : 2;
 // SIMD would hold them all, but a wave alone issues at half the rate): each of a pair has half of the channels' products and
 // outputs, and they exchange their halves of the scores through LDS
 // Bound: at few rows the vector instructions that turn 4-bit codes into fp16 operands and the softmax of 16 columns of which few
-// are rows (64 sequences of up to 8192 tokens, 128 channels, 4 heads a key head: 146 MB in 37 us, 4.0 TB/s of the 6.3 that a
+// are rows (64 sequences of up to 8192 tokens, 256 channels, 4 heads a key head: 146 MB in 37 us, 4.0 TB/s of the 6.3 that a
 // read reaches; 5 rows of 8 heads, 512 channels, 131071 tokens: 70 us, of which the loop over the runs takes 40); of a short
 // sequence the chain from the page table to the first scores (one row over 517 tokens: 12.5 us)
 template <int D> constexpr int kRowSplit = D == 512 ? 2 : 1;
