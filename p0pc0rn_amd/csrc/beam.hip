@@ -25,9 +25,10 @@ struct BeamP {
   const int32_t* hist;
   int32_t* hist_out;
   int64_t hist_n, hist_ld;
-  // in the workspace (uncached: a store is in memory once acknowledged)
+  // in the workspace (uncached), written and read with device-scope accesses: a store is in memory once acknowledged, and a join
+  // in the same launch gets no line that its CU's L1 took in before another workgroup's words of it were written
   uint64_t* keys;      // [rows][chunks][k]
-  float* sums;         // [rows][chunks][2]: maximum, sum of exponentials
+  uint64_t* sums;      // [rows][chunks]: maximum (low word), sum of exponentials
   unsigned* cnt;       // per search
 };
 
@@ -103,6 +104,8 @@ template <int KM, int WAVES> struct JoinLds {
   int row[KM], tok[KM];
 };
 constexpr float kLog2e = 1.44269504088896340736f;
+__device__ __forceinline__ uint64_t ws_load(const uint64_t* a) { return __hip_atomic_load(a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void ws_store(uint64_t* a, uint64_t v) { __hip_atomic_store(a, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));   // a 16-byte load at 4-byte alignment
 
 // a row's k best of its chunks' keys and its sum of exponentials: lane r < k gets the r-th candidate of beam w
@@ -120,7 +123,7 @@ __device__ __forceinline__ Cand row_best(const BeamP& p, JoinLds<KM, WAVES>& l, 
 #pragma unroll
     for (int u = 0; u < kBmBatch - 1; ++u) {
       const int i = i0 + u * 64 + (lane + 13 * u) % 64;
-      q[u] = i < total ? keys[i] : 0;
+      q[u] = i < total ? ws_load(keys + i) : 0;
     }
   };
   load(0);
@@ -128,7 +131,8 @@ __device__ __forceinline__ Cand row_best(const BeamP& p, JoinLds<KM, WAVES>& l, 
   const bool ended = p.done && p.done[row];
   float most = -INFINITY, sum = 0.0f;
   for (int c = lane; c < p.chunks; c += 64) {
-    const float m = p.sums[(row * p.chunks + c) * 2], e = p.sums[(row * p.chunks + c) * 2 + 1], both = fmaxf(most, m);
+    const uint64_t ms = ws_load(p.sums + row * p.chunks + c);
+    const float m = __uint_as_float((uint32_t)ms), e = __uint_as_float((uint32_t)(ms >> 32)), both = fmaxf(most, m);
     sum = both == -INFINITY ? 0.0f : sum * exp2f((most - both) * kLog2e) + e * exp2f((m - both) * kLog2e);
     most = both;
   }
@@ -314,14 +318,12 @@ __global__ __launch_bounds__(kBmThreads) void beam_kernel(const BeamP p) {
     int rank = 0;
 #pragma unroll 8
     for (int j = 0; j < n; ++j) rank += lds.part.list[j] > key;
-    if (rank < p.k) out[rank] = key;
+    if (rank < p.k) ws_store(out + rank, key);
   }
-  if (tid >= n && tid < p.k) out[tid] = 0;   // a chunk of fewer than k
+  if (tid >= n && tid < p.k) ws_store(out + tid, 0);   // a chunk of fewer than k
   __syncthreads();
-  if (tid == 0) {
-    p.sums[(row * p.chunks + blockIdx.x) * 2] = most;
-    p.sums[(row * p.chunks + blockIdx.x) * 2 + 1] = (s_f[0] + s_f[1]) + (s_f[2] + s_f[3]);
-  }
+  if (tid == 0)
+    ws_store(p.sums + row * p.chunks + blockIdx.x, (uint64_t)__float_as_uint((s_f[0] + s_f[1]) + (s_f[2] + s_f[3])) << 32 | __float_as_uint(most));
   if constexpr (!JOIN) return;
   const int64_t g = row / p.W;
   __builtin_amdgcn_s_waitcnt(0);
@@ -404,7 +406,7 @@ extern "C" int p0_beam(const p0_beam_args_t* a) {
   p.hist_n = a->hist_n;
   p.hist_ld = a->hist_ld ? a->hist_ld : a->hist_n + 1;
   p.keys = (uint64_t*)ctx().part;
-  p.sums = (float*)(p.keys + rows * chunks * a->k);
+  p.sums = p.keys + rows * chunks * a->k;
   p.cnt = ctx().kv_counters;
   if (a->k <= 8) launch_beam<8>(p, a->n, ctx().cur);
   else launch_beam<32>(p, a->n, ctx().cur);
