@@ -40,6 +40,16 @@ struct AttnP {
 constexpr float kNone = -3.0e38f;    // the running maximum before any token
 constexpr float kLift = 14.0f;       // probabilities are held times 2^14: fp16's normal range reaches 2^-28 of the largest
 
+// Parts go from workgroup to workgroup of one launch in device-scope accesses of 8 bytes: the workspace is uncached, so a store is
+// in memory once acknowledged, but parts are not padded to cache lines, and a plain load could be served by a line that this
+// CU's L1 took in for another item before this item's words in it were written
+__device__ __forceinline__ float2 part_load(const float* a) {
+  return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void part_store(float* a, float x, float y) {
+  __hip_atomic_store((uint64_t*)a, __builtin_bit_cast(uint64_t, float2{x, y}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // the maximum / sum over the four lane groups of 16 lanes (lane ^ 16, lane ^ 32)
@@ -594,17 +604,18 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
       store8<TYPE>(p.y, out_at(p, it, wgrow0 + r) + 32 * bl + 8 * gg, p.y_vec, y);
     } else {
       float* d = mine + r * D + 32 * bl + 8 * gg;
-      *(float4_t*)d = float4_t{x[0], z[0], x[1], z[1]};
-      *(float4_t*)(d + 4) = float4_t{x[2], z[2], x[3], z[3]};
-      if (bl == 0 && gg == 0) {
-        mine[wgrows * D + 2 * r] = mall;
-        mine[wgrows * D + 2 * r + 1] = lall;
+      if (p.join) {   // for the next launch
+        *(float4_t*)d = float4_t{x[0], z[0], x[1], z[1]};
+        *(float4_t*)(d + 4) = float4_t{x[2], z[2], x[3], z[3]};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part_store(d + 2 * j, x[j], z[j]);
       }
+      if (bl == 0 && gg == 0) part_store(mine + wgrows * D + 2 * r, mall, lall);
     }
   }
   if (parts > 1 && !p.join) {
-    // ---- workgroups with the same rows: parts in the workspace (uncached: a store is in memory once acknowledged), the last
-    // to arrive adds them in order, four in flight
+    // ---- workgroups with the same rows: parts in the workspace, the last to arrive adds them in order, four in flight
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (tid == 0) {
@@ -621,19 +632,17 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
         float mm = kNone, ll = 0.0f, y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma nounroll
         for (int w0 = 0; w0 < parts; w0 += 4) {   // past the last part: the last again, at no weight
-          float pm[4], pl[4];
-          float4_t a[4], b[4];
+          float2 ml[4], a[4][4];   // maximum and sum; eight channels
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const float* x = all + min(w0 + u, parts - 1) * p.slot;
-            pm[u] = __builtin_nontemporal_load(x + wgrows * D + 2 * r);
-            pl[u] = __builtin_nontemporal_load(x + wgrows * D + 2 * r + 1);
-            a[u] = __builtin_nontemporal_load((const float4_t*)(x + r * D + c));
-            b[u] = __builtin_nontemporal_load((const float4_t*)(x + r * D + c + 4));
+            ml[u] = part_load(x + wgrows * D + 2 * r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[u][j] = part_load(x + r * D + c + 2 * j);
           }
           const float was = mm;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mm = fmaxf(mm, pm[u]);
+          for (int u = 0; u < 4; ++u) mm = fmaxf(mm, ml[u].x);
           const float f0 = exp2_fast(was - mm);
           ll *= f0;
 #pragma unroll
@@ -641,10 +650,10 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             if (w0 + u >= parts) continue;
-            const float f = exp2_fast(pm[u] - mm);
-            ll = fmaf(f, pl[u], ll);
+            const float f = exp2_fast(ml[u].x - mm);
+            ll = fmaf(f, ml[u].y, ll);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { y[j] = fmaf(a[u][j], f, y[j]); y[4 + j] = fmaf(b[u][j], f, y[4 + j]); }
+            for (int j = 0; j < 4; ++j) { y[2 * j] = fmaf(a[u][j].x, f, y[2 * j]); y[2 * j + 1] = fmaf(a[u][j].y, f, y[2 * j + 1]); }
           }
         }
         const float inv = inverse(ll);

@@ -55,3 +55,15 @@ def test_a_beam_search_is_joined_over_device_scope_accesses():
     for name, code in kernels.items():
         words = [x for x in code if re.match(r"(global|flat)_(load|store)_dwordx2 ", x)]
         assert words and all(" sc1" in x for x in words), (name, [x for x in words if " sc1" not in x][:3])
+
+
+def test_parts_of_an_item_are_joined_over_device_scope_accesses():
+    """kv_attn_kernel's last workgroup of an item has 20 words of 8 bytes in flight; none of its loads go by `nt`, which passes by
+    no cache"""
+    kernels = _code("kv_attn_kernel")
+    assert len(kernels) == 21
+    for name, code in kernels.items():
+        words = [x for x in code if re.match(r"(global|flat)_load_dwordx2 ", x) and " sc1" in x]
+        stores = [x for x in code if re.match(r"(global|flat)_store_dwordx2 ", x) and " sc1" in x]
+        assert len(words) >= 20 and len(stores) >= 5, (name, len(words), len(stores))
+        assert not [x for x in code if re.match(r"(global|flat)_load", x) and re.search(r"\bnt\b", x)], name
