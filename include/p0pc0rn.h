@@ -391,10 +391,12 @@ int p0_kv_attn(const p0_kv_attn_args_t* a);
  * and that another one holds too is copied (in every layer), so that each writes its own: where all its holders grow in it,
  * the first keeps the original. With a window, pages that no row from position keep on can see (p0_kv_attn's rule) are given
  * up. A page that no new sequence holds is free. Free pages are taken in ascending order, for sequences and columns in
- * ascending order. table_out ([Bo][out_ld], 0 = cols: no entry: -1), len_out, ref ([n_pages]: holders of each page; may be
+ * ascending order. A sequence whose new tokens would begin in the middle of a page that is none cannot grow: where it is cut
+ * back into pages that a window has given up, which do not come back, keep has to be a multiple of page (its rows then miss
+ * those tokens). table_out ([Bo][out_ld], 0 = cols: no entry: -1), len_out, ref ([n_pages]: holders of each page; may be
  * NULL) and status are written, table and len are read: they must not overlap. At most 2^21 pages here and in p0_kv_compact.
- * status (device, 4 words): pages that were missing, free pages left, pages copied, sequences longer than cols * page. Where
- * the first or last is not 0 nothing has been done: table_out and len_out are the old sequences (the first min(B, Bo);
+ * status (device, 4 words): pages that were missing, free pages left, pages copied, sequences that cannot grow (so, or past
+ * cols * page). Where the first or last is not 0 nothing has been done: table_out and len_out are the old sequences (the first min(B, Bo);
  * further ones are empty), ref is as it was, and the second word is the pages that there were to take. So this forks
  * (several src alike), reorders (a beam search's parents), truncates (the rows a verify pass refused), extends and frees
  * (src -1). */

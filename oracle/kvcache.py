@@ -153,8 +153,8 @@ def update(table, length, page, n_pages, Bo, src=None, keep=None, grow=None, gro
                     continue
                 new[b, j] = clean(s, j)
         grown[b] = kept[b] + max(0, int(grow_n if grow is None else grow[b]))
-    too_long = grown > cols * page
     opens = [new[b, kept[b] // page] if grown[b] > kept[b] and kept[b] % page else None for b in range(Bo)]
+    stuck = (grown > cols * page) | np.array([o == -1 for o in opens], bool)   # too long, or to go on in a page that is none
     wants = []
     for b in range(Bo):
         o = opens[b]
@@ -165,20 +165,20 @@ def update(table, length, page, n_pages, Bo, src=None, keep=None, grow=None, gro
             writers = [x for x in range(Bo) if opens[x] is not None and opens[x] == o]
             copy = held > 1 and not (len(writers) == held and writers[0] == b)
             assert holders
-        if grown[b] > kept[b] and not too_long[b]:
+        if grown[b] > kept[b] and not stuck[b]:
             for j in range(kept[b] // page, -(-grown[b] // page)):
                 fresh = j * page >= kept[b]
-                if fresh or copy or o == -1:
+                if fresh or copy:
                     wants.append((b, j, o if copy and not fresh else None))
     free = [pg for pg in range(n_pages) if not (new == pg).any()]
     missing = max(0, len(wants) - len(free))
-    if missing or too_long.any():
+    if missing or stuck.any():
         old, oldlen = np.full((Bo, cols), -1), np.zeros(Bo, int)
         for b in range(min(B, Bo)):
             oldlen[b] = length[b]
             for j in range(-(-int(length[b]) // page)):
                 old[b, j] = clean(b, j)
-        return old, oldlen, None, [missing, len(free), 0, int(too_long.sum())], []
+        return old, oldlen, None, [missing, len(free), 0, int(stuck.sum())], []
     moves = []
     for (b, j, o), pg in zip(wants, free):
         new[b, j] = pg

@@ -70,9 +70,9 @@ class Search:
         capi.kv_update(capi.kv_update_args(kv=self._cache(), B=self.rows, Bo=rows, src=src, keep=keep, grow_n=1, window=self.window,
                                            sinks=self.sinks, layers=self.m.layers, table_out=self.tables[1], len_out=self.lens[1],
                                            ref=self.ref, status=self.status))
-        missing, _, _, long_ = self.status.read(np.int32, 4)
-        if missing or long_:
-            raise RuntimeError("beam_search: %d pages missing, %d sequences too long" % (missing, long_))
+        missing, _, _, stuck = self.status.read(np.int32, 4)
+        if missing or stuck:
+            raise RuntimeError("beam_search: %d pages missing, %d sequences that cannot grow" % (missing, stuck))
         self.tables.reverse()
         self.lens.reverse()
         self.rows, self.length = rows, self.length + 1

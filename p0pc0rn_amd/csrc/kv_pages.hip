@@ -19,7 +19,7 @@ constexpr int kPgSmallRows = 1024, kPgSmallEntries = 1 << 15, kPgSmallPages = 81
 
 // the workspace: a few words, per sequence, per page
 struct PgWs {
-  int32_t* head;      // [0] pages wanted, [1] free pages, [2] sequences too long, [3] copies
+  int32_t* head;      // [0] pages wanted, [1] free pages, [2] sequences that cannot grow, [3] copies
   int32_t *src, *kept, *grown, *open, *first_free, *copy_to;   // per sequence
   int32_t *from, *to;                                          // the copies
   int32_t *ref, *writers, *leader, *list;                      // per page
@@ -64,8 +64,13 @@ __device__ __forceinline__ int open_column(const KvP& kv, const Seq& s) {
   return s.grown > s.kept && (s.kept & ((1 << kv.page_log) - 1)) ? s.kept >> kv.page_log : -1;
 }
 __device__ __forceinline__ bool too_long(const KvP& kv, const Seq& s) { return s.grown > ((int64_t)kv.cols << kv.page_log); }
-__device__ __forceinline__ int wanted_by(const KvP& kv, const Seq& s, bool opened_anew) {
-  return s.grown > s.kept && !too_long(kv, s) ? pages_of(kv, s.grown) - pages_of(kv, s.kept) + (opened_anew ? 1 : 0) : 0;
+// whether it cannot grow: past the columns, or on in a column begun already whose page is none (open < 0). A free page there would
+// show its old bytes as the column's earlier tokens
+__device__ __forceinline__ bool stuck(const KvP& kv, const Seq& s, int open) {
+  return too_long(kv, s) || (open < 0 && open_column(kv, s) >= 0);
+}
+__device__ __forceinline__ int wanted_by(const KvP& kv, const Seq& s, int open, bool copy) {
+  return s.grown > s.kept && !stuck(kv, s, open) ? pages_of(kv, s.grown) - pages_of(kv, s.kept) + (copy ? 1 : 0) : 0;
 }
 
 // the exclusive prefix of one value a thread over the workgroup, in thread order; *all: the sum
@@ -104,10 +109,10 @@ __global__ __launch_bounds__(kPgThreads) void kv_update_small_kernel(const UpdP 
   int* s_open = s_grown + p.Bo;
   int* s_first = s_open + p.Bo;
   int* s_copy = s_first + p.Bo;
-  __shared__ int s_long, s_copies;
+  __shared__ int s_stuck, s_copies;
   const int tid = threadIdx.x, P = p.kv.n_pages, cols = p.kv.cols;
   for (int i = tid; i < P; i += kPgThreads) ref[i] = 0;
-  if (tid == 0) s_long = s_copies = 0;
+  if (tid == 0) s_stuck = s_copies = 0;
   Seq mine{-1, 0, 0};
   if (tid < p.Bo) {
     mine = seq_of(p, tid);
@@ -141,8 +146,8 @@ __global__ __launch_bounds__(kPgThreads) void kv_update_small_kernel(const UpdP 
         }
       copy = !(writers == ref[open] && leader == tid);
     }
-    want = wanted_by(p.kv, mine, copy || (open < 0 && open_column(p.kv, mine) >= 0));
-    if (too_long(p.kv, mine)) atomicAdd(&s_long, 1);
+    want = wanted_by(p.kv, mine, open, copy);
+    if (stuck(p.kv, mine, open)) atomicAdd(&s_stuck, 1);
   }
   int total, nfree = 0;
   const int before = block_prefix(want, &total);
@@ -158,7 +163,7 @@ __global__ __launch_bounds__(kPgThreads) void kv_update_small_kernel(const UpdP 
     nfree += all;
   }
   __syncthreads();
-  const bool fail = total > nfree || s_long > 0;
+  const bool fail = total > nfree || s_stuck > 0;
   if (!fail) {
     if (copy) {
       s_copy[tid] = atomicAdd(&s_copies, 1);
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(kPgThreads) void kv_update_small_kernel(const UpdP 
     p.status[0] = total > nfree ? total - nfree : 0;
     p.status[1] = fail ? nfree : nfree - total;
     p.status[2] = s_copies;
-    p.status[3] = s_long;
+    p.status[3] = s_stuck;
     p.ws.head[3] = s_copies;
   }
 }
@@ -217,7 +222,6 @@ __global__ __launch_bounds__(256) void kv_keep_kernel(const UpdP p) {   // grid:
     p.ws.grown[b] = s.grown;
     p.ws.copy_to[b] = -1;
     if (oc < 0) p.ws.open[b] = -1;
-    if (too_long(p.kv, s)) atomicAdd(&p.ws.head[2], 1);
   }
   if (j >= p.kv.cols) return;
   const int pg = kept_page(p, s, j);
@@ -244,7 +248,8 @@ __global__ __launch_bounds__(kPgThreads) void kv_decide_kernel(const UpdP p) {  
       const int open = p.ws.open[b];
       const bool copy = copies(p, b, open);
       if (copy) p.ws.copy_to[b] = atomicAdd(&p.ws.head[3], 1);
-      want = wanted_by(p.kv, s, copy || (open < 0 && open_column(p.kv, s) >= 0));
+      want = wanted_by(p.kv, s, open, copy);
+      if (stuck(p.kv, s, open)) atomicAdd(&p.ws.head[2], 1);
     }
     const int at = base + block_prefix(want, &all);
     if (b < p.Bo) p.ws.first_free[b] = at;
@@ -271,8 +276,8 @@ __global__ __launch_bounds__(kPgThreads) void kv_free_kernel(const int32_t* ref,
 }
 __global__ __launch_bounds__(256) void kv_assign_kernel(const UpdP p) {   // grid: max(columns, pages / sequences) / 256, sequences
   const int b = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
-  const int total = p.ws.head[0], nfree = p.ws.head[1], longer = p.ws.head[2];
-  const bool fail = total > nfree || longer > 0;
+  const int total = p.ws.head[0], nfree = p.ws.head[1], held_up = p.ws.head[2];
+  const bool fail = total > nfree || held_up > 0;
   if (j < p.kv.cols) {
     if (fail) {
       p.table_out[b * p.out_ld + j] = b < p.B && j < pages_of(p.kv, kv_len(p.kv, b)) ? kv_page(p.kv, b, j) : -1;
@@ -294,7 +299,7 @@ __global__ __launch_bounds__(256) void kv_assign_kernel(const UpdP p) {   // gri
     p.status[0] = total > nfree ? total - nfree : 0;
     p.status[1] = fail ? nfree : nfree - total;
     p.status[2] = fail ? 0 : p.ws.head[3];
-    p.status[3] = longer;
+    p.status[3] = held_up;
   }
 }
 // the counts of the new tables: a kept page's holders less those that took a copy of it, 1 for one taken from the free list
@@ -313,8 +318,8 @@ __global__ __launch_bounds__(256) void kv_count_kernel(const UpdP p) {
 constexpr int kPgPiece = 16384;   // four 16-byte loads of each of 256 threads
 __global__ __launch_bounds__(256) void kv_move_kernel(uint8_t* pages, int64_t page_bytes, int64_t bytes, int64_t layer_bytes, int layers,
                                                       const int32_t* count, const int32_t* from, const int32_t* to,
-                                                      const int32_t* wanted, const int32_t* nfree, const int32_t* longer) {
-  if (wanted && (*wanted > *nfree || *longer > 0)) return;
+                                                      const int32_t* wanted, const int32_t* nfree, const int32_t* held_up) {
+  if (wanted && (*wanted > *nfree || *held_up > 0)) return;
   const int pieces = (int)((bytes + kPgPiece - 1) / kPgPiece);
   const int64_t n = (int64_t)*count * layers * pieces;
   for (int64_t u = blockIdx.x; u < n; u += gridDim.x) {

@@ -124,6 +124,17 @@ def test_an_update_by_hand():
     assert out.tolist() == [[2, 1, -1], [2, 0, -1]] and status == [3, 2] and moves == [(3, 1), (5, 2)]
 
 
+def test_a_sequence_does_not_go_on_in_a_page_that_is_gone():
+    """cut back to 50 tokens of a window's 100, the page of tokens 32-63 has been given up: a fresh one would show tokens that nobody put"""
+    table = np.array([[-1, -1, 7, 8]])
+    t, n, holders, status, moves = KV.update(table, np.array([100]), 32, 12, 1, keep=[50], grow_n=1, window=16)
+    assert status == [0, 12, 0, 1] and t.tolist() == table.tolist() and n.tolist() == [100] and holders is None and not moves
+    t, n, _, status, _ = KV.update(table, np.array([100]), 32, 12, 1, keep=[64], grow_n=1, window=16)   # where a page ends it can
+    assert status == [0, 11, 0, 0] and t.tolist() == [[-1, -1, 0, -1]] and n.tolist() == [65]
+    t, n, _, status, _ = KV.update(table, np.array([100]), 32, 12, 1, keep=[50], window=16)             # nor does one that does not grow
+    assert status == [0, 12, 0, 0] and t.tolist() == [[-1, -1, -1, -1]] and n.tolist() == [50]
+
+
 @pytest.mark.parametrize("kw,msg", [(dict(n=-1), "-1 searches of 2 beams"), (dict(W=0), "1 searches of 0 beams"),
                                     (dict(n=700, W=100), "700 searches of 100 beams"), (dict(V=0), "V 0, ld 0"), (dict(ld=99), "V 100, ld 99"),
                                     (dict(k=0), "k 0 (1..32, at most V)"), (dict(k=33), "k 33 (1..32, at most V)"),

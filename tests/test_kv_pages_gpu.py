@@ -249,3 +249,36 @@ def test_recorded_updates_replay(dev):
     rec.free()
     src.free()
     pool.free()
+
+
+@pytest.mark.parametrize("big", [False, True])
+def test_a_sequence_does_not_go_on_in_a_page_that_is_gone(dev, big):
+    """a window's sequence cut back into pages that it has given up: refused as a whole, also beside one that could go on; a cut
+    where a page ends goes on, and its new row sees what has been put alone, in a pool of random bytes"""
+    H, D, page, P = 1, 64, 32, 12400 if big else 12
+    table = [[-1, -1, 7, 8], [1, 2, -1, -1]]
+    pool = Pool(table, [100, 40], page, P, H=H, D=D, seed=2)
+    ws, moves = check_update(pool, 2, keep=[50, 40], grow=[1, 1], window=16)
+    assert ws == [0, P - 2, 0, 1] and not moves
+    ws, _ = check_update(pool, 2, keep=[50, 40], grow=[300, 1], window=16)   # too long and gone: one sequence
+    assert ws == [0, P - 2, 0, 1]
+    ws, _ = check_update(pool, 2, keep=[50, 40], grow=[0, 1], window=16)
+    assert ws == [0, P - 2, 0, 0]
+    ws, _ = check_update(pool, 2, keep=[64, 40], grow=[1, 1], window=16)
+    assert ws == [0, P - 3, 0, 0]
+    t, n, _, _ = pool.outs
+    kv = capi.kv(pages=pool.bufs[0], n_pages=P, page_bytes=pool.size, page=page, heads=H, dim=D, table=t, cols=4, len=n)
+    rng = np.random.default_rng(1)
+    k, v = (rng.standard_normal((2, 1, H, D)).astype(np.float32) for _ in "kv")
+    bufs = [capi.to_device(x) for x in (k, v)]
+    capi.kv_put(capi.kv_rows_args(kv=kv, B=2, M=1, k=bufs[0], v=bufs[1]))
+
+    class C:
+        pass
+    C.kv = staticmethod(lambda: kv)
+    got, _ = run_attn(C, rng.standard_normal((2, 1, 2, D)), "f32", window=16)
+    want = KV.held(k, v)[1]
+    assert np.allclose(got[0], want[0], rtol=1e-6, atol=0)   # its window's other tokens are on no page
+    for b in bufs:
+        b.free()
+    pool.free()
