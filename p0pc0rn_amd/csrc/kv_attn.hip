@@ -331,10 +331,32 @@ __device__ __forceinline__ int64_t out_at(const AttnP& p, const Item& it, int r)
   return (int64_t)it.b * p.y_ldb + (int64_t)(r / p.group) * p.y_ldm + (int64_t)(it.h * p.group + r % p.group) * p.y_ldh;
 }
 
-// fp16 values that a query's or a probability's f32 is taken as: 22 bits for f32; f16 and bf16 queries are exact in one. A
-// probability of one part is off by 2^-12 of itself: as much again as the rounding of an f16 output, next to nothing in bf16
+// fp16 values that a query's or a probability's f32 is taken as. A probability of one part is off by 2^-12 of itself: as much again
+// as the rounding of an f16 output, next to nothing in bf16
 template <int TYPE> constexpr int kQParts = TYPE == P0_KV_F32 ? 2 : 1;
 template <int TYPE> constexpr int kPParts = TYPE == P0_KV_BF16 ? 1 : 2;
+
+// Queries as fp16 operands: f16 as it is. Else a row is taken under the power of two that brings its largest value to [2^14, 2^15),
+// the top of fp16's range, as keys may be 0 where the query is large and large where it is small. bf16's 8 bits are whole down to
+// 2^-17, that is 2^-31 of the largest, and off by 2^-39 of it at the most below. f32's second part is the rest times 2^12, with an
+// accumulator of its own: 22 bits down to 2^-29 of the largest, off by 2^-51 of it below.
+constexpr int kQTop = 14;
+constexpr float kQRest = 4096.0f;
+// the exponent of that power of two for a row whose largest magnitude is `most`. 0 for rows of nothing, and of an infinity
+template <int TYPE> __device__ __forceinline__ int query_exponent(float most) {
+  if constexpr (TYPE == P0_KV_F16) return 0;
+  const int e = (int)(__float_as_uint(most) >> 23) - 127 - kQTop;
+  return most == 0.0f || most == INFINITY ? 0 : e < -127 ? -127 : e;
+}
+template <int TYPE> __device__ __forceinline__ void query_operand(const float (&v)[8], int e, half8_t& hi, half8_t& lo) {
+  const float down = __uint_as_float((uint32_t)(127 - e) << 23);   // e is -127 .. 113
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = TYPE == P0_KV_F16 ? v[j] : v[j] * down;
+    hi[j] = (_Float16)x;
+    if constexpr (kQParts<TYPE> == 2) lo[j] = (_Float16)((x - (float)hi[j]) * kQRest);
+  }
+}
 
 // A workgroup of kv_attn_kernel: waves of 16 rows each, W of them or, at 512 channels, W pairs (the registers of one wave a
 // SIMD would hold them all, but a wave alone issues at half the rate): each of a pair has half of the channels' products and
@@ -423,25 +445,20 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
     kr.load(run_at(first, pg), lane, half);
     vr.load(run_at(first, pg), lane, half);
   }
-  // ---- the queries as operands, each row under a power of two that brings its largest value to [1, 2): D / 8 lanes a row
+  // ---- the queries as operands, each row under its power of two: D / 8 lanes a row
 #pragma unroll
   for (int k = 0; k < ROUNDS; ++k) {
     const int t = tid + k * kRowThreads<D, W>, r = t / (D / 8), c = t % (D / 8) * 8;
     float most = 0.0f;
+    if constexpr (TYPE != P0_KV_F16) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[k][j]));
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[k][j]));
 #pragma unroll
-    for (int s = 1; s < D / 8; s <<= 1) most = fmaxf(most, __shfl_xor(most, s, 64));
-    int e = (int)(__float_as_uint(most) >> 23) - 127;
-    e = most == 0.0f || e == 128 ? 0 : e < -120 ? -120 : e > 126 ? 126 : e;
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-    half8_t hi, lo;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = v[k][j] * down;
-      hi[j] = (_Float16)x;
-      lo[j] = (_Float16)(x - (float)hi[j]);
+      for (int s = 1; s < D / 8; s <<= 1) most = fmaxf(most, __shfl_xor(most, s, 64));
     }
+    const int e = query_exponent<TYPE>(most);
+    half8_t hi, lo;
+    query_operand<TYPE>(v[k], e, hi, lo);
     if (r < p.tiles * 16) {
       const int st = D == 64 ? c >> 3 & 1 : (c >> 7) * 4 + (c >> 3 & 3), gg = D == 64 ? c >> 4 : c >> 5 & 3;
       // (a row's lanes are one bank apart in `st` and `gg`: the column is turned by them)
@@ -489,8 +506,8 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
           }
       }
       if constexpr (QPARTS == 2) {
-        s[0] += sl[0];
-        s[1] += sl[1];
+        s[0] += sl[0] * (1.0f / kQRest);
+        s[1] += sl[1] * (1.0f / kQRest);
       }
       const int pg_after = page_of(i + 2 * p.streams);
       if constexpr (SPLIT == 2) {
@@ -802,28 +819,23 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kerne
       if (in) load8<TYPE>(p.q, base + (D == 64 ? g * 16 + 8 * st : (st >> 2) * 128 + g * 32 + 8 * (st & 3)), p.q_vec, v);
     };
     float most = 0.0f;
+    if constexpr (TYPE != P0_KV_F16) {
 #pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-      float v[8];
-      query(st, v);
+      for (int st = 0; st < STEPS; ++st) {
+        float v[8];
+        query(st, v);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+      }
+      most = groups_max(most);
     }
-    most = groups_max(most);
-    int e = (int)(__float_as_uint(most) >> 23) - 127;
-    e = most == 0.0f || e == 128 ? 0 : e < -120 ? -120 : e > 126 ? 126 : e;
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const int e = query_exponent<TYPE>(most);
     qs = ldexpf(p.scale2, e);
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
       float v[8];
       query(st, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = v[j] * down;
-        qh[st][j] = (_Float16)x;
-        if constexpr (QPARTS == 2) ql[st][j] = (_Float16)(x - (float)qh[st][j]);
-      }
+      query_operand<TYPE>(v, e, qh[st], ql[QPARTS == 2 ? st : 0]);
     }
   }
 
@@ -861,8 +873,8 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kerne
             if constexpr (QPARTS == 2) sl[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[st], sl[tt], 0, 0, 0);
           }
         if constexpr (QPARTS == 2) {
-          s[0] += sl[0];
-          s[1] += sl[1];
+          s[0] += sl[0] * (1.0f / kQRest);
+          s[1] += sl[1] * (1.0f / kQRest);
         }
         const bool all = t0 + kKvRun - 1 <= pos0 && whole && (!p.window || t0 > pos1 - p.window || t0 + kKvRun <= p.sinks);
         if (!all) {

@@ -493,3 +493,20 @@ def test_a_chain_being_built_refuses_them(dev):
         if h.value:
             capi.lib().p0_chain_free(h)
     c.free()
+
+
+@pytest.mark.parametrize("type_,most,rest,sigma", [("f32", 1e3, 1, 1), ("f32", 1e6, 1, 1), ("f32", 100, 0.01, 100), ("f16", 1000, 0.01, 100),
+                                                   ("f16", 60000, 0.01, 100), ("f16", 60000, 3e-5, 1e4), ("bf16", 1e4, 1, 1), ("bf16", 1e7, 1, 1)])
+@pytest.mark.parametrize("D,M,G,cols", [(64, 2, 2, None), (128, 3, 1, None), (256, 2, 2, None), (512, 2, 1, None), (64, 256, 1, 13000), (128, 256, 1, 13000)])
+def test_a_channel_far_above_the_rest_of_its_row(dev, D, M, G, cols, type_, most, rest, sigma):
+    """the keys are 0 in the large channel, so the scores are the small ones' alone, each of which has to be held to its own bits;
+    256 rows are those that share converted runs"""
+    def special(b, h, k, v):
+        k *= sigma
+        k[:, 5] = 0.0
+    c = Held([90], D, 1, 32, seed=D, special=special, cols=cols)
+    q = rest * np.random.default_rng(D + M).standard_normal((1, M, G, D))
+    q[..., 5] = most
+    got, exact = run_attn(c, q, type_)
+    check(got, KV.attention(c.c, c.table, c.len, exact), type_)
+    c.free()
