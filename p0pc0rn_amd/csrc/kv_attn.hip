@@ -348,6 +348,8 @@ template <int TYPE> __device__ __forceinline__ int query_exponent(float most) {
   const int e = (int)(__float_as_uint(most) >> 23) - 127 - kQTop;
   return most == 0.0f || most == INFINITY ? 0 : e < -127 ? -127 : e;
 }
+// the factor of such a row's scores: neither 0 nor infinite, so that it leaves the scores of -infinity of what is not seen, and those of 0
+__device__ __forceinline__ float score_factor(float scale2, int e) { return fminf(fmaxf(ldexpf(scale2, e), 0x1p-126f), 0x1.fffffep127f); }
 template <int TYPE> __device__ __forceinline__ void query_operand(const float (&v)[8], int e, half8_t& hi, half8_t& lo) {
   const float down = __uint_as_float((uint32_t)(127 - e) << 23);   // e is -127 .. 113
 #pragma unroll
@@ -465,7 +467,7 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
       half8_t* sq = (half8_t*)&s_o[0][0] + ((r >> 4) * (D / 32) + st) * 64 + gg * 16 + ((r ^ (4 * st + gg)) & 15);
       *sq = hi;
       if constexpr (QPARTS == 2) sq[p.tiles * (D / 32) * 64] = lo;
-      if (c == 0) s_qs[r] = ldexpf(p.scale2, e);
+      if (c == 0) s_qs[r] = score_factor(p.scale2, e);
     }
   }
   __syncthreads();
@@ -830,7 +832,7 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kerne
       most = groups_max(most);
     }
     const int e = query_exponent<TYPE>(most);
-    qs = ldexpf(p.scale2, e);
+    qs = score_factor(p.scale2, e);
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
       float v[8];

@@ -510,3 +510,20 @@ def test_a_channel_far_above_the_rest_of_its_row(dev, D, M, G, cols, type_, most
     got, exact = run_attn(c, q, type_)
     check(got, KV.attention(c.c, c.table, c.len, exact), type_)
     c.free()
+
+
+@pytest.mark.parametrize("scale,size", [(1e-10, 1e-35), (1e-44, 1.0), (1e30, 1e30), (3e38, 1.0)])
+@pytest.mark.parametrize("D,M,cols", [(128, 3, None), (512, 2, None), (64, 256, 13000)])
+def test_scales_past_what_fp32_holds(dev, scale, size, D, M, cols):
+    """scale times a query's power of two may be under the least fp32 number, or over the largest: rows whose scores are all next to
+    nothing are means of what they see, and a score of exactly 0 stays one (the rows of zeros)"""
+    c = Held([90], D, 1, 32, seed=D, cols=cols)
+    q = size * np.random.default_rng(D).standard_normal((1, M, 2 if M < 9 else 1, D))
+    if scale > 1:
+        q[0, 0] = 0.0
+    got, exact = run_attn(c, q, "f32", scale=scale)
+    want = KV.attention(c.c, c.table, c.len, exact, scale=scale)
+    if scale > 1:
+        got, want = got[0, 0], want[0, 0]
+    check(got, want, "f32")
+    c.free()
