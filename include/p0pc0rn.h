@@ -369,7 +369,8 @@ int p0_kv_get(const p0_kv_rows_args_t* a);
  * y = sum_t softmax_t(scale q . k_t) v_t (scale 0: 1 / sqrt(dim)); a row that sees nothing, and rows past rows[b], are 0.
  * Element [b][i][q][c] of q is at b * q_ldb + i * q_ldm + q * q_ldh + c (0 = dim, heads * ldh, M * ldm), of y likewise.
  * f32 queries are taken as pairs of fp16 values (22 bits of each, down to 2^-29 of its row's largest), f16 queries exactly, bf16
- * queries exactly down to 2^-31 of the row's largest and to within 2^-39 of it below, f32 probabilities as pairs of fp16 values, sums in fp32.
+ * queries exactly down to 2^-31 of the row's largest and to within 2^-39 of it below; f32's and f16's probabilities as pairs of fp16
+ * values, bf16's as one (11 bits); maxima and sums are fp32.
  * max_len: no sequence is longer (0 = cols * page): only the split of the work goes by it, longer ones are right too.
  * Results are the same bit for bit from call to call with the same max_len. */
 typedef struct {

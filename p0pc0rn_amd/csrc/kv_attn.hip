@@ -331,8 +331,10 @@ __device__ __forceinline__ int64_t out_at(const AttnP& p, const Item& it, int r)
   return (int64_t)it.b * p.y_ldb + (int64_t)(r / p.group) * p.y_ldm + (int64_t)(it.h * p.group + r % p.group) * p.y_ldh;
 }
 
-// fp16 values that a query's or a probability's f32 is taken as. A probability of one part is off by 2^-12 of itself: as much again
-// as the rounding of an f16 output, next to nothing in bf16
+// fp16 values that a query's or a probability's f32 is taken as. A probability of one part is off by up to 2^-12 of itself. In f16
+// that shows (one row of 16 heads over 700 tokens, relative L2: 2.14e-4 in two parts, the rounding of the output, 2.69e-4 in one), in
+// bf16 it does not (1.54e-3 either way; 3% of the outputs round to the neighbour), and it spares a third of the products (2 x 1024
+// rows of 16 heads over 4096 tokens: f16 130 us, 110 in one part; bf16 113, 134 in two)
 template <int TYPE> constexpr int kQParts = TYPE == P0_KV_F32 ? 2 : 1;
 template <int TYPE> constexpr int kPParts = TYPE == P0_KV_BF16 ? 1 : 2;
 
@@ -689,7 +691,7 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
 // (whose bytes it loaded two rounds before) into the other; one barrier a round.
 // Bound: at 16 KB of operands a wave and run, LDS (half the time at 128 channels), then the vector instructions of the softmax;
 // two workgroups a CU hide each other's barriers (one of 16 waves: 114 us where two of 8 take 95, 2 x 1024 rows under a window of
-// 4096). 8 x 1024 rows of 16 heads over 4096 tokens: 370 us, 650 TFLOP/s. Wider heads leave too few waves for that, and run
+// 4096). 8 x 1024 rows of 16 heads over 4096 tokens: bf16 355 us, 678 TFLOP/s, f16 424, f32 497. Wider heads leave too few waves for that, and run
 // faster where each wave converts for itself (256 channels, 2 x 1024 rows over 4096: 467 us here, 237 there).
 template <int D> struct TileShape {
   static constexpr int TILES = 8, RUNS = 2, kWaves = TILES, kThreads = 64 * kWaves;
@@ -703,7 +705,7 @@ template <int D, int TYPE>
 __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kernel(const AttnP p) {
   using S = TileShape<D>;
   constexpr int RUNS = S::RUNS, PER = S::PER, DEPTH = S::DEPTH, STEPS = D / 32, BLOCKS = D / 32;
-  constexpr int QPARTS = kQParts<TYPE>, PPARTS = TYPE == P0_KV_F32 ? 2 : 1;
+  constexpr int QPARTS = kQParts<TYPE>, PPARTS = kPParts<TYPE>;
   extern __shared__ __attribute__((aligned(16))) uint8_t s_raw[];
   half8_t* buf = (half8_t*)s_raw;   // [2][RUNS][FRAGS][64]
   __shared__ int s_dead[2][RUNS];
@@ -1114,9 +1116,9 @@ extern "C" int p0_kv_attn(const p0_kv_attn_args_t* a) {
   const int64_t runs = (p.window && seen < longest ? seen : longest) / kKvRun + 1;
   // Rows share converted runs where the chip's workgroups get enough runs each to outweigh a longer start and a barrier a round,
   // fewer of 16-bit queries, whose products are cheaper beside the conversion. (us, shared / each wave for itself, 128 channels,
-  // 4 key heads of 4 heads over 4096 tokens: f16 32 x 32 rows 76 / 99, 2 x 1024 112 / 144, 4 x 128 52 / 56; over 2048, 8 key
-  // heads, 2 x 128 rows, 41 / 37; f32 2 x 1024 rows 152 / 159, 32 x 64 160 / 168, 4 x 128 65 / 58; 64 channels, f16, 8 x 256
-  // 77 / 105, 4 x 64 36 / 29.)
+  // 4 key heads of 4 heads over 4096 tokens: f16 32 x 32 rows 88 / 95, 2 x 1024 130 / 142, 4 x 128 54 / 58; over 2048, 8 key
+  // heads, 2 x 128 rows, 42 / 39; bf16 2 x 1024 113 / 127, 4 x 128 52 / 55; f32 2 x 1024 152 / 159, 32 x 64 160 / 168, 4 x 128
+  // 65 / 61; 64 channels, f16, 8 x 256 92 / 104, 4 x 64 37 / 33.)
   const int64_t work = a->B * p.kv.heads * ((p.R + 16 * TileShape<64>::TILES - 1) / (16 * TileShape<64>::TILES)) * runs;
   Form form = D <= 128 && p.R >= 128 && work >= (a->type == P0_KV_F32 ? 48 : 12) * 512 ? kTiles : kRows4;
   if (form == kTiles) {

@@ -527,3 +527,16 @@ def test_scales_past_what_fp32_holds(dev, scale, size, D, M, cols):
         got, want = got[0, 0], want[0, 0]
     check(got, want, "f32")
     c.free()
+
+
+@pytest.mark.parametrize("D,M,cols", [(64, 2, None), (128, 2, None), (256, 2, None), (512, 2, None), (64, 256, 13000), (128, 256, 13000)])
+def test_f16_outputs_are_off_by_their_own_rounding(dev, D, M, cols):
+    """whichever kernel takes the rows. An output is the rounding of a value off by d, |d| <= 5e-6 as f32's are: where that rounds as
+    the exact value does the error is the exact value's own, else the exact value lies within d of the middle and the error is over
+    its own by 2 d at the most"""
+    c = Held([700], D, 1, 32, seed=D, cols=cols)
+    q = 0.1 * np.random.default_rng(D + M).standard_normal((1, M, 16 if M < 9 else 1, D))
+    got, exact = run_attn(c, q, "f16")
+    want = KV.attention(c.c, c.table, c.len, exact)
+    assert rel_l2(got, want) <= rel_l2(want.astype(np.float16), want) + 2 * BOUND["f32"]
+    c.free()
