@@ -14,12 +14,12 @@ int kv_check(const char* op, const p0_kv_t& kv, int64_t B, KvP* out) {
     return P0_EINVAL;
   }
   if (kv.n_pages < 1 || kv.n_pages > (1 << 30)) { set_error("%s: %lld pages", op, (long long)kv.n_pages); return P0_EINVAL; }
-  if (kv.page_bytes && (kv.page_bytes < bytes || kv.page_bytes % 16)) {
+  if (kv.page_bytes && (kv.page_bytes < bytes || kv.page_bytes % 16 || kv.page_bytes > (1ll << 62) / kv.n_pages)) {
     set_error("%s: page_bytes %lld (a page is %lld)", op, (long long)kv.page_bytes, (long long)bytes); return P0_EINVAL;
   }
   if (!kv.pages || !kv.table || !kv.len) { set_error("%s: missing pages, table or len buffer", op); return P0_EINVAL; }
   if ((uintptr_t)kv.pages % 16) { set_error("%s: pages must be 16-byte aligned", op); return P0_EINVAL; }
-  if (kv.cols < 1 || kv.cols * kv.page > (1ll << 31) - 64 || (kv.table_ld && kv.table_ld < kv.cols)) {
+  if (kv.cols < 1 || kv.cols > ((1ll << 31) - 64) / kv.page || (kv.table_ld && kv.table_ld < kv.cols)) {
     set_error("%s: table of %lld columns, stride %lld", op, (long long)kv.cols, (long long)kv.table_ld); return P0_EINVAL;
   }
   if (B < 0 || B > 65535) { set_error("%s: B %lld", op, (long long)B); return P0_EINVAL; }

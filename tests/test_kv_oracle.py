@@ -158,3 +158,15 @@ def test_a_step_by_hand():
     (token, parent, score, done), _ = KV.beam(x, np.log([0.5, 0.5]), 2, 3, eos=1)
     assert token.tolist() == [[1, 0, 1]] and parent.tolist() == [[1, 0, 0]] and done.tolist() == [[True, False, True]]
     assert np.allclose(np.exp(score), [[0.375, 0.25, 0.125]])
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(cols=1 << 58), "table of 288230376151711744 columns, stride 0"),
+                                    (dict(cols=(1 << 25) + 1), "table of 33554433 columns, stride 0"),
+                                    (dict(page_bytes=1 << 62), "page_bytes 4611686018427387904 (a page is 17408)")])
+def test_a_cache_whose_size_passes_64_bits_is_refused(kw, msg):
+    """cols * page and n_pages * page_bytes of these are small again in 64 bits"""
+    _refused(capi.kv_put, capi.kv_rows_args(kv=_kv(**kw), B=1, M=1, k=16, v=16), "kv_put: " + msg)
+    _refused(capi.kv_attn, capi.kv_attn_args(kv=_kv(**kw), B=1, M=1, heads=2, q=16, y=16), "kv_attn: " + msg)
+    args = dict(B=1, layers=2, layer_bytes=16, table_out=4096, status=16)
+    _refused(capi.kv_update, capi.kv_update_args(kv=_kv(**kw), len_out=8192, **args), "kv_update: " + msg)
+    _refused(capi.kv_compact, capi.kv_compact_args(kv=_kv(**kw), **args), "kv_compact: " + msg)
