@@ -396,7 +396,8 @@ int p0_kv_attn(const p0_kv_attn_args_t* a);
  * ascending order. A sequence whose new tokens would begin in the middle of a page that is none cannot grow: where it is cut
  * back into pages that a window has given up, which do not come back, keep has to be a multiple of page (its rows then miss
  * those tokens). table_out ([Bo][out_ld], 0 = cols: no entry: -1), len_out, ref ([n_pages]: holders of each page; may be
- * NULL) and status are written, table and len are read: they must not overlap. At most 2^21 pages here and in p0_kv_compact.
+ * NULL) and status are written, table and len are read: they must not overlap (two tables of one stride may lie in each other's
+ * gaps), nor table_out src, keep and grow. At most 2^21 pages here and in p0_kv_compact.
  * status (device, 4 words): pages that were missing, free pages left, pages copied, sequences that cannot grow (so, or past
  * cols * page). Where the first or last is not 0 nothing has been done: table_out and len_out are the old sequences (the first min(B, Bo);
  * further ones are empty), ref is as it was, and the second word is the pages that there were to take. So this forks
@@ -420,7 +421,7 @@ int p0_kv_update(const p0_kv_update_args_t* a);
 /* Moves the live pages (held by a table row's first ceil(len / page) columns) to the front of the pool: with n of them, those
  * at or above n go, in ascending order, to the free ones below n, in ascending order; table_out is the table with the moved
  * ones' new places (columns past a sequence's tokens, and entries that are no page: -1). status (device, 2 words): n, pages
- * moved. table_out must not overlap table. */
+ * moved. table_out and status must not overlap table and len. */
 typedef struct {
   p0_kv_t kv;
   int64_t B;

@@ -375,8 +375,9 @@ extern "C" int p0_beam(const p0_beam_args_t* a) {
   }
   if (a->hist) {
     const int64_t ld = a->hist_ld ? a->hist_ld : a->hist_n + 1;
-    const uintptr_t in = (uintptr_t)a->hist, out = (uintptr_t)a->hist_out;
-    if (in < out + a->n * a->k * ld * 4 && out < in + a->n * a->W * ld * 4) { set_error("beam: hist and hist_out overlap"); return P0_EINVAL; }
+    if (overlap({a->hist, a->n * a->W, a->hist_n, ld}, {a->hist_out, a->n * a->k, a->hist_n + 1, ld})) {
+      set_error("beam: hist and hist_out overlap"); return P0_EINVAL;
+    }
   }
   if (a->done && a->eos < 0) { set_error("beam: done needs an eos token"); return P0_EINVAL; }
   BeamP p{};

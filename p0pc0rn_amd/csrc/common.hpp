@@ -55,6 +55,22 @@ int misc_init();
 int kv_pages_init();
 int kv_attn_init();
 
+// `rows` rows of `width` 4-byte words, `ld` words apart, as arguments are checked. Rows of one stride may lie in each other's gaps;
+// of two strides the whole extents have to be apart
+struct Words {
+  const void* at;
+  int64_t rows, width, ld;
+};
+inline bool overlap(const Words& a, const Words& b) {
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  const auto end = [](const Words& w) { return (__int128)(uintptr_t)w.at + ((__int128)(w.rows - 1) * w.ld + w.width) * 4; };
+  if ((__int128)(uintptr_t)a.at >= end(b) || (__int128)(uintptr_t)b.at >= end(a)) return false;
+  const int64_t ld = a.rows > 1 ? a.ld : b.ld;
+  if ((a.rows > 1 && b.rows > 1 && a.ld != b.ld) || (a.rows == 1 && b.rows == 1)) return true;
+  const __int128 step = (__int128)ld * 4, d = (__int128)(uintptr_t)b.at - (__int128)(uintptr_t)a.at, in = (d % step + step) % step;
+  return in < (__int128)a.width * 4 || in + (__int128)b.width * 4 > step;
+}
+
 // Thread-local message of the last failure (p0_last_error).
 void set_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
 

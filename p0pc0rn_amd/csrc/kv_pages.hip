@@ -461,9 +461,6 @@ static int layers_check(const char* op, const p0_kv_t& kv, int64_t rows, int64_t
   if (out_ld && out_ld < kv.cols) { set_error("%s: out_ld %lld of %lld columns", op, (long long)out_ld, (long long)kv.cols); return P0_EINVAL; }
   return P0_OK;
 }
-static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
-  return (uintptr_t)a < (uintptr_t)b + nb * 4 && (uintptr_t)b < (uintptr_t)a + na * 4;
-}
 static void launch_moves(const p0_kv_t& kv, int64_t layers, int64_t layer_bytes, const PgWs& w, bool update, int64_t most) {
   const int64_t page = kv_page_bytes(kv), bytes = p0_kv_page_bytes(kv.page, kv.heads, kv.dim);
   layers = layers ? layers : 1;
@@ -495,8 +492,16 @@ extern "C" int p0_kv_update(const p0_kv_update_args_t* a) {
   if (int r = layers_check("kv_update", a->kv, a->B > Bo ? a->B : Bo, a->layers, a->layer_bytes, a->out_ld, a->table_out, a->status)) return r;
   if (!a->len_out) { set_error("kv_update: missing len_out buffer"); return P0_EINVAL; }
   const int64_t cols = a->kv.cols, ld = a->out_ld ? a->out_ld : cols;
-  if (overlap(a->kv.table, a->B * p.kv.table_ld, a->table_out, Bo * ld) || overlap(a->kv.len, a->B, a->len_out, Bo)) {
-    set_error("kv_update: table_out or len_out overlaps what is read"); return P0_EINVAL;
+  const Words table{a->kv.table, a->B, cols, p.kv.table_ld}, len{a->kv.len, 1, a->B, 0}, status{a->status, 1, 4, 0},
+      table_out{a->table_out, Bo, cols, ld}, len_out{a->len_out, 1, Bo, 0}, ref{a->ref, 1, a->kv.n_pages, 0};
+  bool over = overlap(table_out, table) || overlap(table_out, len) || overlap(len_out, table) || overlap(len_out, len);
+  for (const int32_t* q : {a->src, a->keep, a->grow}) over = over || overlap(table_out, {q, 1, Bo, 0});
+  if (over) { set_error("kv_update: table_out or len_out overlaps what is read"); return P0_EINVAL; }
+  for (const Words& w : {ref, status})
+    if (overlap(w, table) || overlap(w, len)) { set_error("kv_update: ref or status overlaps what is read"); return P0_EINVAL; }
+  if (overlap(table_out, len_out) || overlap(table_out, ref) || overlap(table_out, status) || overlap(len_out, ref) || overlap(len_out, status) ||
+      overlap(ref, status)) {
+    set_error("kv_update: two of table_out, len_out, ref and status overlap"); return P0_EINVAL;
   }
   if (int r = refuse_in_chain("kv_update")) return r;
   if (int r = require_open("kv_update")) return r;
@@ -541,8 +546,11 @@ extern "C" int p0_kv_compact(const p0_kv_compact_args_t* a) {
   if (int r = kv_check("kv_compact", a->kv, a->B, &p.kv)) return r;
   if (int r = layers_check("kv_compact", a->kv, a->B, a->layers, a->layer_bytes, a->out_ld, a->table_out, a->status)) return r;
   const int64_t cols = a->kv.cols, ld = a->out_ld ? a->out_ld : cols, P = a->kv.n_pages;
-  if (overlap(a->kv.table, a->B * p.kv.table_ld, a->table_out, a->B * ld)) {
-    set_error("kv_compact: table_out overlaps what is read"); return P0_EINVAL;
+  const Words table{a->kv.table, a->B, cols, p.kv.table_ld}, len{a->kv.len, 1, a->B, 0}, table_out{a->table_out, a->B, cols, ld},
+      status{a->status, 1, 2, 0};
+  if (overlap(table_out, table)) { set_error("kv_compact: table_out overlaps what is read"); return P0_EINVAL; }
+  if (overlap(table_out, len) || overlap(status, table) || overlap(status, len) || overlap(status, table_out)) {
+    set_error("kv_compact: table_out or status overlaps what is read"); return P0_EINVAL;
   }
   if (int r = refuse_in_chain("kv_compact")) return r;
   if (int r = require_open("kv_compact")) return r;

@@ -1,9 +1,14 @@
 """The CPU restatement of the 4-bit cache (oracle/kvcache.py), and what the kv_* calls refuse before they touch a device."""
+import json
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
 from oracle import kvcache as KV
 from p0pc0rn_amd import capi
+from tests.conftest import ROOT
 
 DIMS = [64, 128, 256, 512]
 
@@ -170,3 +175,54 @@ def test_a_cache_whose_size_passes_64_bits_is_refused(kw, msg):
     args = dict(B=1, layers=2, layer_bytes=16, table_out=4096, status=16)
     _refused(capi.kv_update, capi.kv_update_args(kv=_kv(**kw), len_out=8192, **args), "kv_update: " + msg)
     _refused(capi.kv_compact, capi.kv_compact_args(kv=_kv(**kw), **args), "kv_compact: " + msg)
+
+
+def _in_a_process_of_its_own(body):
+    """`body` in a process that never opens a device, where a call whose arguments are taken ends with P0_ENODEV (3)"""
+    code = "from p0pc0rn_amd import capi\nfrom tests.test_kv_oracle import _kv\n" + """
+def says(fn, args):
+    try:
+        fn(args)
+    except capi.P0Error as e:
+        return "taken" if e.code == 3 else str(e)
+""" + body
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    return json.loads(r.stdout)
+
+
+def test_rows_that_lie_between_each_other_do_not_overlap():
+    """two tables, two histories of one stride, the one's rows in the other's gaps; and up to the last word of a last row"""
+    got = _in_a_process_of_its_own("""
+import json
+out = []
+for at in (4096 + 16, 4096 + 12, 4096 + 20, 4096 + 80, 4096 + 76, 4096 - 80, 4096 - 76):
+    kv = _kv(table=4096, table_ld=8, cols=4, len=1 << 20)
+    out.append([says(capi.kv_update, capi.kv_update_args(kv=kv, B=3, table_out=at, out_ld=8, len_out=1 << 21, status=1 << 22)),
+                says(capi.kv_compact, capi.kv_compact_args(kv=kv, B=3, table_out=at, out_ld=8, status=1 << 22))])
+for at in (4096 + 20, 4096 + 16, 4096 + 12, 4096 + 24, 4096 + 20 + 40, 4096 + 56, 4096 - 140, 4096 - 136):
+    out.append(says(capi.beam, capi.beam_args(logits=16, n=1, W=2, V=100, k=4, score=16, token=16, parent=16, score_out=16,
+                                              hist=4096, hist_out=at, hist_n=4, hist_ld=10)))
+print(json.dumps(out))""")
+    over = ["kv_update: table_out or len_out overlaps what is read", "kv_compact: table_out overlaps what is read"]
+    assert got[:7] == [["taken"] * 2 if fine else over for fine in (True, False, False, True, False, True, False)]
+    # rows of 4 words at 10, 5 at 10 into them
+    assert got[7:] == ["taken" if fine else "beam: hist and hist_out overlap" for fine in (True, True, False, False, True, True, True, False)]
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(table_out=(1 << 20) - 4), "table_out or len_out overlaps what is read"),
+                                    (dict(len_out=4096 + 28), "table_out or len_out overlaps what is read"),
+                                    (dict(src=8192, table_out=8196), "table_out or len_out overlaps what is read"),
+                                    (dict(keep=8192, table_out=8196), "table_out or len_out overlaps what is read"),
+                                    (dict(grow=8192, table_out=8196), "table_out or len_out overlaps what is read"),
+                                    (dict(status=4096 + 16), "ref or status overlaps what is read"), (dict(status=1 << 20), "ref or status overlaps what is read"),
+                                    (dict(ref=4096 - 12), "ref or status overlaps what is read"),
+                                    (dict(status=(1 << 21) + 4), "two of table_out, len_out, ref and status overlap"),
+                                    (dict(ref=(1 << 23) + 8), "two of table_out, len_out, ref and status overlap"),
+                                    (dict(table_out=(1 << 22) - 8), "two of table_out, len_out, ref and status overlap")])
+def test_outputs_of_an_update_that_overlap_are_refused(kw, msg):
+    base = dict(kv=_kv(table=4096, len=1 << 20), B=2, table_out=1 << 23, len_out=1 << 21, status=1 << 22, grow_n=1)
+    base.update(kw)
+    _refused(capi.kv_update, capi.kv_update_args(**base), "kv_update: " + msg)
+    if kw.keys() == {"status"} and "read" in msg:
+        _refused(capi.kv_compact, capi.kv_compact_args(kv=base["kv"], B=2, table_out=1 << 23, **kw), "kv_compact: table_out or status overlaps what is read")

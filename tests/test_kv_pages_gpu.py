@@ -282,3 +282,30 @@ def test_a_sequence_does_not_go_on_in_a_page_that_is_gone(dev, big):
     for b in bufs:
         b.free()
     pool.free()
+
+
+@pytest.mark.parametrize("P", [90, 12400])
+def test_two_tables_in_each_others_gaps(dev, P):
+    """one array with a row of the old table and a row of the new one in turn, which then change places"""
+    rng = np.random.default_rng(P)
+    table, length = beams(rng, 3, 3, 32, 7, P, 150)
+    pool = Pool(table, length, 32, P, seed=4)
+    both = np.full((9, 2, 7), FRESH, np.int32)
+    both[:, 0] = table
+    t, s, n = capi.to_device(both), capi.Buffer(16), [pool.bufs[2], capi.Buffer(48)]
+    for turn in range(2):
+        src = (rng.integers(0, 3, (3, 3)) + np.arange(3)[:, None] * 3).ravel()
+        sb = capi.to_device(src.astype(np.int32))
+        kv = capi.kv(pages=pool.bufs[0], n_pages=P, page_bytes=pool.size, page=32, heads=1, dim=64, table=t.ptr + 28 * turn, table_ld=14, cols=7,
+                     len=n[turn])
+        capi.kv_update(capi.kv_update_args(kv=kv, B=9, src=sb, grow_n=1, table_out=t.ptr + 28 * (1 - turn), out_ld=14, len_out=n[1 - turn], status=s))
+        want, length, _, ws, _ = KV.update(table, length, 32, P, 9, src=src, grow_n=1)
+        got = t.read(np.int32).reshape(9, 2, 7)
+        assert s.read(np.int32, 4).tolist() == ws and np.array_equal(got[:, 1 - turn], want) and np.array_equal(got[:, turn], table)
+        assert np.array_equal(n[1 - turn].read(np.int32, 9), length)
+        table = want
+        sb.free()
+    for b in (t, s, n[1]):
+        b.free()
+    pool.outs = []
+    pool.free()
