@@ -1144,7 +1144,9 @@ extern "C" int p0_kv_attn(const p0_kv_attn_args_t* a) {
   // Few items in parts, where the runs that a part saves outweigh the join. (us, in parts / not: one row of 4 heads a key head,
   // 256 channels, 800 tokens 16.2 / 14.9, 1200 16.5 / 18.5, 2500 18.0 / 29.0; 512 channels, one row of 8 heads, 600 tokens
   // 20.3 / 21.5, five rows, 150 tokens 29.9 / 25.0, 300 33.4 / 37.3.)
-  p.shared = items / p.kv.heads <= kMostPairs && 2 * items <= wgs && runs > (D == 512 ? 3 * p.streams + 4 : 9 * p.streams);
+  // (The deal counts the runs of all pairs in 32 bits: where the table holds more, whatever max_len says, there are no parts.)
+  const int64_t pairs = items / p.kv.heads;
+  p.shared = pairs <= kMostPairs && pairs * (most / kKvRun + 1) <= 0x7FFFFFFF && 2 * items <= wgs && runs > (D == 512 ? 3 * p.streams + 4 : 9 * p.streams);
   if (!p.shared) {
     wgs = items;
     if (form == kRows4 && D < 512 && items <= 256 && runs > p.streams) {   // CUs to spare: eight waves an item (one row over 517 tokens 12.5 us, 14.3 in four)

@@ -540,3 +540,13 @@ def test_f16_outputs_are_off_by_their_own_rounding(dev, D, M, cols):
     want = KV.attention(c.c, c.table, c.len, exact)
     assert rel_l2(got, want) <= rel_l2(want.astype(np.float16), want) + 2 * BOUND["f32"]
     c.free()
+
+
+def test_tables_of_more_runs_than_32_bits_count(dev):
+    """34 groups of rows over a table of 2^31 tokens, of which 1300 are there: no parts, whose deal would count past 32 bits if they all were"""
+    D, M, n = 256, 1060, 1300
+    c = Held([n], D, 1, 1024, seed=3, cols=(1 << 21) - 1)
+    q = np.random.default_rng(3).standard_normal((1, M, 1, D))
+    got, exact = run_attn(c, q, "f32")
+    check(got, KV.attention(c.c, c.table, c.len, exact), "f32")
+    c.free()
