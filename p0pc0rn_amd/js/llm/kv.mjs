@@ -100,8 +100,9 @@ export function beam(g, a) {
   need(op, 'done', a.done, R * 4);
   for (const n of ['token', 'parent', 'score', 'done']) need(op, n, o[n], k * 4);
   if (h) {
-    need(op, 'hist', h, R * (h.ld || h.n + 1) * 4);
-    need(op, 'hist_out', h.out, k * (h.ld || h.n + 1) * 4);
+    const ld = h.ld || h.n + 1;
+    need(op, 'hist', h, R > 0 ? ((R - 1) * ld + h.n) * 4 : 0);
+    need(op, 'hist_out', h.out, k > 0 ? ((k - 1) * ld + h.n + 1) * 4 : 0);
   }
   native().beam({
     logits: at(a.logits), ld: a.logits.ld || 0, n: a.n, W: a.W, V: a.V, k: a.k, score: at(a.score), done: at(a.done),

@@ -719,3 +719,19 @@ P.beam(g, { logits, n: 1, W: 2, V: 500, k: 4, score, out: { token: tok, parent: 
     (token, parent, score, _), _ = KV.beam(logits, np.array([-1, -1.5], np.float32), 2, 4)
     assert got("tok", np.int32).tolist() == token[0].tolist() and got("par", np.int32).tolist() == parent[0].tolist()
     assert np.allclose(got("sc", np.float32), score[0], rtol=0, atol=1e-5)
+
+
+def test_js_beam_takes_histories_that_end_with_their_last_word(tmp_path):
+    """rows 10 words apart of which 4 are read and 5 written: the last row's gap need not be there"""
+    out = run_node(tmp_path, r"""
+const B = (n) => ({ ptr: 4096, _pf: n }), C = { ptr: 1 << 20 }, res = [];
+for (const [r, w] of [[56, 140], [55, 140], [56, 139]]) {
+  try {
+    P.beam({}, { logits: { buf: C }, n: 1, W: 2, V: 100, k: 4, score: { buf: C }, out: { token: { buf: C }, parent: { buf: C }, score: { buf: C } },
+                 hist: { buf: B(r), n: 4, ld: 10, out: { buf: Object.assign(B(w), { ptr: 8192 }) } } });
+  } catch (e) { res.push(e.message); }
+}
+console.log(JSON.stringify(res));
+""")
+    assert json.loads(out.strip().splitlines()[-1]) == ["beam: no device (p0_open was not called)", "beam: hist needs 56 B of a 55 B buffer",
+                                                        "beam: hist_out needs 140 B of a 139 B buffer"]
