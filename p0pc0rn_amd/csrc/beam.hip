@@ -106,6 +106,11 @@ template <int KM, int WAVES> struct JoinLds {
 constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ uint64_t ws_load(const uint64_t* a) { return __hip_atomic_load(a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void ws_store(uint64_t* a, uint64_t v) { __hip_atomic_store(a, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// a wave's LDS writes before its lanes' reads of them. (The LDS takes a wave's accesses in order; the fence keeps the compiler to it)
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));   // a 16-byte load at 4-byte alignment
 
 // a row's k best of its chunks' keys and its sum of exponentials: lane r < k gets the r-th candidate of beam w
@@ -161,16 +166,16 @@ __device__ __forceinline__ Cand row_best(const BeamP& p, JoinLds<KM, WAVES>& l, 
       n += __popcll(in);
     }
     l.top[wave][lane % KM] = 0;
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     for (int i = lane; i < n; i += 64) {
       const uint64_t key = l.list[wave][i];
       int rank = 0;
       for (int j = 0; j < n; ++j) rank += l.list[wave][j] > key;
       if (rank < k) l.top[wave][rank] = key;
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
     top = lane < k ? l.top[wave][lane] : 0;
-    __builtin_amdgcn_wave_barrier();
+    wave_sync();
   }
   float s = score + (of_order((uint32_t)(top >> 32)) - lse);
   if (s != s) s = -INFINITY;
