@@ -67,3 +67,17 @@ def test_parts_of_an_item_are_joined_over_device_scope_accesses():
         stores = [x for x in code if re.match(r"(global|flat)_store_dwordx2 ", x) and " sc1" in x]
         assert len(words) >= 20 and len(stores) >= 5, (name, len(words), len(stores))
         assert not [x for x in code if re.match(r"(global|flat)_load", x) and re.search(r"\bnt\b", x)], name
+
+
+def test_the_kernels_spill_no_registers():
+    """not one of them does: each keeps its tile, its loads on their way and its sums in the registers that its launch bounds leave"""
+    readelf = shutil.which("llvm-readelf") or "/opt/rocm/llvm/bin/llvm-readelf"
+    spills = {}
+    with tempfile.TemporaryDirectory() as d:
+        f = os.path.join(d, "code.elf")
+        for elf in _objects():
+            open(f, "wb").write(elf)
+            notes = subprocess.run([readelf, "--notes", f], capture_output=True, text=True, check=True).stdout
+            for name, n in re.findall(r"\.name: +(_ZN2p0\d+(?:kv|beam)_\S+).*?\.vgpr_spill_count: +(\d+)", notes, re.S):
+                spills[name] = int(n)
+    assert len(spills) >= 21 + 24 + 6 + 8 + 12 + 6 and not any(spills.values()), {k: v for k, v in spills.items() if v}

@@ -309,3 +309,46 @@ def test_two_tables_in_each_others_gaps(dev, P):
         b.free()
     pool.outs = []
     pool.free()
+
+
+@pytest.mark.parametrize("groups,W,cols,P", [(6, 4, 9, 8192), (6, 4, 9, 8193), (256, 4, 32, 3000), (1, 1025, 5, 3000), (205, 5, 31, 3000), (256, 4, 33, 3000)])
+def test_updates_on_both_sides_of_one_workgroups_reach(dev, groups, W, cols, P):
+    """8192 pages, 1024 sequences, 32768 entries are one workgroup's; one more of any is the chip's"""
+    rng = np.random.default_rng(cols + P)
+    table, length = beams(rng, groups, W, 32, cols, P, 60 if groups * W > 100 else 200)
+    src = (rng.integers(0, W, (groups, W)) + np.arange(groups)[:, None] * W).ravel()
+    pool = Pool(table, length, 32, P, seed=cols)
+    ws, _ = check_update(pool, groups * W, src=src, grow_n=1)
+    assert ws[0] == ws[3] == 0
+    pool.free()
+
+
+@pytest.mark.parametrize("B,longest,P", [(40, 3000, 8192), (40, 3000, 8193), (1024, 1000, 8000), (1024, 1030, 8000)])
+def test_compact_on_both_sides_of_one_workgroups_reach(dev, B, longest, P):
+    rng = np.random.default_rng(B + P)
+    cols = -(-longest // 32)
+    length = rng.integers(0, longest // (8 if B > 100 else 1), B)
+    need = -(-length // 32)
+    order = rng.permutation(P)
+    table = np.full((B, cols), -1, np.int32)
+    at = 0
+    for b in range(B):
+        table[b, :need[b]] = order[np.arange(at, at + need[b]) % P]
+        at += need[b]
+    pool = Pool(table, length, 32, P, seed=B)
+    t, _, _, s = pool.out(B)
+    capi.kv_compact(capi.kv_compact_args(kv=pool.kv(), B=B, table_out=t, status=s))
+    wt, ws, moves = KV.compact(table, length, 32, P)
+    assert s.read(np.int32, 2).tolist() == ws and ws[1] > 100
+    assert np.array_equal(t.read(np.int32, B * cols).reshape(B, cols), wt)
+    pool.moved(moves)
+    pool.free()
+
+
+@pytest.mark.parametrize("length", [64, 40])
+def test_too_few_pages_over_the_chip_change_nothing(dev, length):
+    """1030 sequences on two pages want one each, or a copy of the second each but the first's"""
+    pool = Pool(np.tile(np.array([[3, 1, -1, -1]]), (1030, 1)), np.full(1030, length), 32, 6, seed=length)
+    ws, moves = check_update(pool, 1030, grow_n=1)
+    assert ws == [1030 - 4 if length == 64 else 1029 - 4, 4, 0, 0] and not moves
+    pool.free()
