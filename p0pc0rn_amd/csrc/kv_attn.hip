@@ -37,7 +37,10 @@ struct AttnP {
   unsigned* cnt;            // per item
 };
 
-constexpr float kNone = -3.0e38f;    // the running maximum before any token
+// A row's running maximum m is one of its scores, before their factor qs, and a probability 2^((s - m) qs + kLift): the largest
+// score's is exactly 1 (lifted) however large the scores are. (2^(s qs - (m qs - kLift)), a rounded product under the fma's exact
+// one, saves a subtraction a score, 1% of a call; past 2^24 it leaves whole powers of two, and infinities among them)
+constexpr float kNone = -3.0e38f;    // before any token
 constexpr float kLift = 14.0f;       // probabilities are held times 2^14: fp16's normal range reaches 2^-28 of the largest
 
 // Parts go from workgroup to workgroup of one launch in device-scope accesses of 8 bytes: the workspace is uncached, so a store is
@@ -362,6 +365,13 @@ template <int TYPE> __device__ __forceinline__ void query_operand(const float (&
   }
 }
 
+// a part's maximum with its factor, as a row's parts are joined by it; *f: what makes up for the product's rounding
+__device__ __forceinline__ float part_maximum(float m, float qs, float* f) {
+  const float r = m * qs;
+  *f = fabsf(r) < 0x1p20f ? exp2_fast(fmaf(m, qs, -r)) : 1.0f;
+  return m == kNone ? kNone : r;
+}
+
 // A workgroup of kv_attn_kernel: waves of 16 rows each, W of them or, at 512 channels, W pairs (the registers of one wave a
 // SIMD would hold them all, but a wave alone issues at half the rate): each of a pair has half of the channels' products and
 // outputs, and they exchange their halves of the scores through LDS
@@ -546,21 +556,20 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, s[tt][r]);
-      top = fmaxf(groups_max(top) * qs, mrun);
+      top = fmaxf(groups_max(top), mrun);
       if (__any(top > mrun)) {
-        const float f = exp2_fast(mrun - top);
+        const float f = exp2_fast((mrun - top) * qs);
         lrun *= f;
 #pragma unroll
         for (int k = 0; k < 2 * BLOCKS; ++k) o[k] *= f;
         mrun = top;
       }
-      const float shift = kLift - mrun;
       half8_t ph, pl;
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float x = exp2_fast(fmaf(s[tt][r], qs, shift));
+          const float x = exp2_fast(fmaf(s[tt][r] - mrun, qs, kLift));
           lrun += x;
           ph[tt * 4 + r] = (_Float16)x;
           if constexpr (PPARTS == 2) pl[tt * 4 + r] = (_Float16)(x - (float)ph[tt * 4 + r]);
@@ -597,17 +606,19 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
   for (int t = tid; t < p.tiles * (D / 32) * 64; t += kRowThreads<D, W>) {
     const int tl = t / (D / 32 * 64), bl = t / 64 % (D / 32), c = t & 15, gg = t >> 4 & 3, r = tl * 16 + c;
     if (r >= wgrows) continue;
-    float mall = kNone, lall = 0.0f, f[NW];
+    const float rqs = s_qs[r];
+    float mall = kNone, lall = 0.0f, f[NW], made_up = 1.0f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {   // past the last stream: the first again, at no weight
       f[w] = w < p.streams ? s_m[w * p.tiles + tl][c] : kNone;
       mall = fmaxf(mall, f[w]);
     }
+    const float mpart = parts == 1 ? 0.0f : part_maximum(mall, rqs, &made_up);
     float4_t x = {0.0f, 0.0f, 0.0f, 0.0f}, z = x;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const int sw = (w < p.streams ? w : 0) * p.tiles + tl;
-      f[w] = w < p.streams ? exp2_fast(f[w] - mall) : 0.0f;
+      f[w] = w < p.streams ? exp2_fast((f[w] - mall) * rqs) * made_up : 0.0f;
       lall = w < p.streams ? fmaf(s_l[sw][c], f[w], lall) : lall;
       const float* d = s_o[sw * SPLIT + bl / BLOCKS] + bl % BLOCKS * 512 + (t & 63) * 4;
       const float4_t a = *(const float4_t*)d, b = *(const float4_t*)(d + 256);
@@ -632,7 +643,7 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
 #pragma unroll
         for (int j = 0; j < 4; ++j) part_store(d + 2 * j, x[j], z[j]);
       }
-      if (bl == 0 && gg == 0) part_store(mine + wgrows * D + 2 * r, mall, lall);
+      if (bl == 0 && gg == 0) part_store(mine + wgrows * D + 2 * r, mpart, lall);
     }
   }
   if (parts > 1 && !p.join) {
@@ -896,21 +907,20 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kerne
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) top = fmaxf(top, s[tt][r]);
-        top = fmaxf(groups_max(top) * qs, mrun);
+        top = fmaxf(groups_max(top), mrun);
         if (__any(top > mrun)) {
-          const float f = exp2_fast(mrun - top);
+          const float f = exp2_fast((mrun - top) * qs);
           lrun *= f;
 #pragma unroll
           for (int k = 0; k < 2 * BLOCKS; ++k) o[k] *= f;
           mrun = top;
         }
-        const float shift = kLift - mrun;
         half8_t ph, pl;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float x = exp2_fast(fmaf(s[tt][r], qs, shift));
+            const float x = exp2_fast(fmaf(s[tt][r] - mrun, qs, kLift));
             lrun += x;
             ph[tt * 4 + r] = (_Float16)x;
             if constexpr (PPARTS == 2) pl[tt * 4 + r] = (_Float16)(x - (float)ph[tt * 4 + r]);
@@ -937,7 +947,8 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kerne
   lrun = groups_sum(lrun);
   const int r = wave * 16 + col;
   if (r >= wgrows) return;
-  const float inv = parts == 1 ? inverse(lrun) : 1.0f;
+  float made_up;
+  const float mpart = part_maximum(mrun, qs, &made_up), inv = parts == 1 ? inverse(lrun) : made_up;
   float* mine = p.part + (int64_t)wg * p.slot;
   const int64_t at = out_at(p, it, wgrow0 + r);
 #pragma unroll
@@ -948,8 +959,8 @@ __global__ __launch_bounds__(TileShape<D>::kThreads, 4) void kv_attn_tiles_kerne
     else store8<P0_KV_F32>(mine, (int64_t)r * D + 32 * k + 8 * g, 1, y);
   }
   if (parts > 1 && g == 0) {
-    mine[wgrows * D + 2 * r] = mrun;
-    mine[wgrows * D + 2 * r + 1] = lrun;
+    mine[wgrows * D + 2 * r] = mpart;
+    mine[wgrows * D + 2 * r + 1] = lrun * made_up;
   }
 }
 

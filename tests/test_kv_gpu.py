@@ -550,3 +550,17 @@ def test_tables_of_more_runs_than_32_bits_count(dev):
     got, exact = run_attn(c, q, "f32")
     check(got, KV.attention(c.c, c.table, c.len, exact), "f32")
     c.free()
+
+
+@pytest.mark.parametrize("type_,size", [("f32", 1e4), ("f32", 1e6), ("f32", 1e8), ("f32", 1e15), ("f32", -1e30), ("f16", 6e4), ("bf16", 1e20)])
+@pytest.mark.parametrize("D,M,cols", [(128, 3, None), (512, 2, None), (64, 256, 13000)])
+def test_scores_of_any_magnitude(dev, D, M, cols, type_, size):
+    """past 2^24 an fp32 score's neighbours are whole powers of two apart: a row is then its best token's value, and no NaN"""
+    def special(b, h, k, v):
+        k *= 1e3
+    c = Held([90], D, 1, 32, seed=D + 1, cols=cols, special=special)
+    q = size * np.random.default_rng(D).uniform(0.5, 1.0, (1, M, 2 if M < 9 else 1, D))
+    got, exact = run_attn(c, q, type_)
+    want = KV.attention(c.c, c.table, c.len, exact)
+    check(got, want, type_)
+    c.free()
