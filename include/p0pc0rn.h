@@ -350,7 +350,8 @@ int64_t p0_kv_page_bytes(int32_t page, int32_t heads, int32_t dim);   /* 0 where
  * rows[b]. Element [b][i][h][c] is at b * ldb + i * ldm + h * ldh + c of k and v (0 = dim, heads * ldh, M * ldm).
  * The exponent of 32 channels is the least e in [-23, 13] with max |x| <= 6 * 2^e, so nothing up to 49152 is cut; the codes are
  * the nearest, ties to the even one. A head's token with a NaN or an infinity in its key or its value is held as a key of
- * NaN and a value of 0, so that exactly the rows that see it become NaN. put: no two rows may name the same token. */
+ * NaN and a value of 0, so that exactly the rows that see it become NaN. put: no two rows may name the same token. B * heads is at
+ * most 65535. */
 typedef struct {
   p0_kv_t kv;
   int64_t B, M;
@@ -437,7 +438,7 @@ int p0_kv_compact(const p0_kv_compact_args_t* a);
  * beam, then the beam's own order, are written best first: token, parent (the row r the candidate continues, what
  * p0_kv_update takes as src), score_out, done_out (parent's done, or the token is eos), each [n][k] (done_out may be
  * NULL). eos < 0: no token ends a beam. NaN logits count as -infinity, and a sum that is not a number as a score of
- * -infinity. Up to 65535 rows; the workspace holds 8 (k + 1) bytes per 8192 logits of them. hist (may be NULL): rows of
+ * -infinity. Where fewer than k candidates are left the other places have a score of -infinity. Up to 65535 rows; the workspace holds 8 (k + 1) bytes per 8192 logits of them. hist (may be NULL): rows of
  * hist_n tokens so far, hist_ld apart (0 = hist_n + 1); hist_out's row i is its parent's and the new token. Outputs must not
  * overlap inputs. */
 typedef struct {

@@ -4,9 +4,11 @@
 // their exponentials against it and their k best as 64-bit keys (the value's order, then the lower token). The last workgroup of a
 // search to arrive joins them: the rows' sums of exponentials, each row's k best, then the k best of all beams.
 // A row's best need no sort: with the lanes in k groups, the least of the groups' best is at or below k values, so what lies
-// under it is out, and what is left (some 20 values as a rule) is ranked by counting. Where many are left, the lanes' best are
-// sorted for a closer bound: of a wave's lanes no more than k have anything at or above the k-th best of them.
-// Bound: HBM at many rows (32 searches of 8 beams, 262144 logits: 268 MB), launch and the join's round trips at few.
+// under it is out, and what is left is ranked by counting (of 8192 logits some 50 for k up to 8). Where many are left, the lanes'
+// best are sorted for a closer bound: of a wave's lanes no more than k have anything at or above the k-th best of them. (For k over
+// 8 the first bound leaves some 370 of 8192, more than is ranked, so nearly every workgroup takes the second.)
+// Bound: HBM at many rows and k up to 8 (32 searches of 8 beams, 262144 logits: 268 MB), the VALU for k over 8 (k = 32: 135 us and a join
+// of 26, busy in 71% of the cycles), launch and the join's round trips at few.
 #include "common.hpp"
 
 namespace p0 {

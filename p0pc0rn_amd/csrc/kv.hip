@@ -151,7 +151,9 @@ __device__ __forceinline__ int block_exp(float most) {
 // A wave takes one row at a time: lanes 0-31 its key, 32-63 its value, D / 32 consecutive channels each. A whole run is put
 // together in LDS and leaves in 16-byte stores (a token's value codes are single bytes 16 apart: 19.5 us for 16336 rows of 256
 // f16 channels without, 10.4 with); of a part of one each byte is stored by itself, as its other tokens stay.
-// Bound: the rows' bytes at many rows (16336 rows: 42 MB, 4.0 TB/s), launch and three memory round trips at one (2.8 us).
+// Bound: launch and three memory round trips at one row (3.2 us). At many neither HBM nor a unit is full (16336 rows: 21.2 MB read and
+// written in 10.4 us, 2.0 TB/s; VALU busy in 33% of the cycles, LDS in 19, three quarters of that bank conflicts of single bytes):
+// two rounds of loads one after the other, then the run's way through LDS, in workgroups of one run.
 constexpr int kRunThreads = 256, kRunWaves = kRunThreads / 64;
 template <int D>
 __global__ __launch_bounds__(kRunThreads) void kv_put_kernel(const RowsP p) {
@@ -200,7 +202,7 @@ __global__ __launch_bounds__(kRunThreads) void kv_put_kernel(const RowsP p) {
 }
 
 // The way back: several rows of a run from a copy of it in LDS, few straight from the page. Bound as above (16336 rows of 256
-// f16 channels 7.8 to 9.6 us)
+// f16 channels 8.5 to 9.4 us, 2.3 to 2.5 TB/s; LDS busy in 21% of the cycles, four fifths of that conflicts)
 template <int D>
 __global__ __launch_bounds__(kRunThreads) void kv_get_kernel(const RowsP p) {
   constexpr int E = D / 32;

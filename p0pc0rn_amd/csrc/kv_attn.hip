@@ -375,10 +375,12 @@ __device__ __forceinline__ float part_maximum(float m, float qs, float* f) {
 // A workgroup of kv_attn_kernel: waves of 16 rows each, W of them or, at 512 channels, W pairs (the registers of one wave a
 // SIMD would hold them all, but a wave alone issues at half the rate): each of a pair has half of the channels' products and
 // outputs, and they exchange their halves of the scores through LDS
-// Bound: at few rows the vector instructions that turn 4-bit codes into fp16 operands and the softmax of 16 columns of which few
-// are rows (64 sequences of up to 8192 tokens, 256 channels, 4 heads a key head: 146 MB in 37 us, 4.0 TB/s of the 6.3 that a
-// read reaches; 5 rows of 8 heads, 512 channels, 131071 tokens: 70 us, of which the loop over the runs takes 40); of a short
-// sequence the chain from the page table to the first scores (one row over 517 tokens: 12.5 us)
+// Bound: latency. The registers leave two waves a SIMD at 256 and 512 channels, and a run is a chain of loads, conversions,
+// products, maximum and exponentials. Of the cycles of 64 sequences of up to 8192 tokens (256 channels, 4 heads a key head, 136 MB
+// in 36 us, 3.8 TB/s of the 6.3 that a read reaches) the VALU is busy in 42%, most of it turning 4-bit codes into fp16 operands,
+// the MFMA in 17%, LDS in 4%; of 5 rows of 8 heads of 512 channels over 131071 tokens (67 us and a join of 9.5) 40, 15 and 5%. Of a
+// short sequence it is the chain from the page table to the first scores, then two or three runs a wave one after the other (one row over 517
+// tokens: 12.5 us)
 template <int D> constexpr int kRowSplit = D == 512 ? 2 : 1;
 template <int D, int W> constexpr int kRowThreads = 64 * W * kRowSplit<D>;
 template <int D> constexpr int kRowGroups = D == 64 ? 4 : D == 128 ? 3 : D == 256 ? 2 : 1;   // of them on a CU: what the registers allow
@@ -700,9 +702,9 @@ __global__ __launch_bounds__((kRowThreads<D, W>), D == 512 || W == 8 ? 2 : kRowG
 // ---- many rows of at most 128 channels: the runs are converted once for a workgroup, into LDS as operands, and each of eight
 // waves reads them for its 16 rows. Two buffers of two runs: while the waves work on one, each converts its share of the next
 // (whose bytes it loaded two rounds before) into the other; one barrier a round.
-// Bound: at 16 KB of operands a wave and run, LDS (half the time at 128 channels), then the vector instructions of the softmax;
-// two workgroups a CU hide each other's barriers (one of 16 waves: 114 us where two of 8 take 95, 2 x 1024 rows under a window of
-// 4096). 8 x 1024 rows of 16 heads over 4096 tokens: bf16 355 us, 678 TFLOP/s, f16 424, f32 497. Wider heads leave too few waves for that, and run
+// Bound: latency between the barriers, at 16 KB of operands from LDS a wave and run. 2 x 1024 bf16 rows of 16 heads of 128 channels
+// under a window of 4096, 96 us and a join of 7: VALU busy in 34% of the cycles, LDS in 19, MFMA in 14; two workgroups a CU hide each
+// other's barriers (one of 16 waves: 114 us where two of 8 take 95). 8 x 1024 rows of 16 heads over 4096 tokens: bf16 355 us, 678 TFLOP/s, f16 424, f32 497. Wider heads leave too few waves for that, and run
 // faster where each wave converts for itself (256 channels, 2 x 1024 rows over 4096: 467 us here, 237 there).
 template <int D> struct TileShape {
   static constexpr int TILES = 8, RUNS = 2, kWaves = TILES, kThreads = 64 * kWaves;
