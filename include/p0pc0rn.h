@@ -457,6 +457,102 @@ typedef struct {
 } p0_beam_args_t;
 int p0_beam(const p0_beam_args_t* a);
 
+/* ---- a layer's linears in 8-bit floating point, and the rotation of its heads ---------------------------------------- */
+/* These operators have no counterpart in the reference (its linears read 4-bit weights and 16-bit activations); they are the
+ * large-M product at the 8-bit matrix rate, what makes its operands, and the heads' rotation, which here only the q4 GEMM's
+ * heads epilogue had.
+ *
+ * Values are e4m3 codes (a sign, 4 bits of exponent, 3 of mantissa; largest 448; no infinities) with one fp32 scale per 128
+ * consecutive channels of a row of activations, and per 128 x 128 block of a weight: a value is code * scale. The scale of a
+ * block is s = max(amax / 448, 2^-126), amax its largest finite magnitude; a code is x * (1 / s), each operation rounded to
+ * fp32, rounded to the nearest e4m3, ties to the even one. NaN and infinities become the code NaN: exactly the rows (of
+ * activations, or of a weight) that hold one become NaN. Rows hold whole blocks: channels past the last are written as 0.
+ *   activations  [M][K] codes, ld bytes from row to row (a multiple of 16), scales s[kb * lds + m] (K / 128 runs of M)
+ *   weights      [N][K] codes likewise, scales s[nb * lds + kb] (nb = n / 128)
+ * K is the channels rounded up to 128. Codes are 16-byte aligned. Outputs must not overlap inputs. */
+enum { P0_F32 = 0, P0_F16 = 1, P0_BF16 = 2 };                    /* type */
+enum { P0_GLU_NONE = 0, P0_GLU_SILU = 1, P0_GLU_GELU = 2 };      /* f8_rows glu */
+
+/* a weight of N rows, K channels (x, ldx elements from row to row, 0 = K) into codes (ldw 0 = K rounded up) and scales (lds 0 =
+ * ceil(K / 128)) */
+typedef struct {
+  const void* x; int64_t ldx; int32_t type;
+  int64_t N, K;
+  void* w; int64_t ldw;
+  float* s; int64_t lds;
+} p0_f8_pack_args_t;
+int p0_f8_pack(const p0_f8_pack_args_t* a);
+
+/* The residual stream's update and its norm, into codes. For each of M rows of D channels (D <= 32768):
+ *   r = x + t, or, with tw, x + t / sqrt(mean(t^2) + eps) * tw, or, without t, x; times scale (0: 1); rounded to x's type
+ *   x_out = r (NULL: x itself, in place; not written where there is neither t nor a scale nor x_out)
+ *   mode 1: y = r / sqrt(mean(r^2) + eps) * g + b;  mode 0: y = (r - mean(r)) / sqrt(var(r) + eps) * g + b
+ *   g = w, or 1 + w with w_one (an lnmod's scale), or 1 without w; b 0 without b
+ * Sums and statistics are fp32. eps 0 = 1e-6. ldx, ldt, ldo 0 = D, ldy 0 = D rounded up, lds 0 = M. x_out has x's type. */
+typedef struct {
+  void* x; int64_t ldx; int32_t type;
+  const void* t; int64_t ldt; int32_t t_type;
+  const float* tw;
+  void* x_out; int64_t ldo;
+  float scale, eps;
+  int32_t mode, w_one;
+  const float* w;
+  const float* b;
+  int64_t M, D;
+  void* y; int64_t ldy;
+  float* s; int64_t lds;
+} p0_f8_norm_args_t;
+int p0_f8_norm(const p0_f8_norm_args_t* a);
+
+/* M rows of D activations into codes: x[m][c], or act(x[m][c]) * x[m][up + c] (up 0 = D; gelu: 0.5 g (1 + tanh(sqrt(2 / pi) (g +
+ * 0.044715 g^3)))). ldx 0 = D, with a glu up + D; ldy 0 = D rounded up, lds 0 = M. */
+typedef struct {
+  const void* x; int64_t ldx; int32_t type;
+  int64_t up; int32_t glu;
+  int64_t M, D;
+  void* y; int64_t ldy;
+  float* s; int64_t lds;
+} p0_f8_rows_args_t;
+int p0_f8_rows(const p0_f8_rows_args_t* a);
+
+/* y[m][n] = sum_kb xs[kb][m] ws[n / 128][kb] sum_{k in kb} x[m][k] w[n][k], sums in fp32, rounded once to y's type. K is a
+ * multiple of 128 (the rounded one), at most 2^20, ldx and ldw at most 2^22. 0: ldx = ldw = K, ldxs = M, ldws = K / 128, ldy = N.
+ * Results are the same bit for bit from call to call. */
+typedef struct {
+  const void* x; int64_t ldx;
+  const float* xs; int64_t ldxs;
+  const void* w; int64_t ldw;
+  const float* ws; int64_t ldws;
+  int64_t M, N, K;
+  int32_t type;
+  void* y; int64_t ldy;
+} p0_f8_gemm_args_t;
+int p0_f8_gemm(const p0_f8_gemm_args_t* a);
+
+/* Rotates the heads of each row by its positions on 1 .. 4 axes (text: one; images, clips: time, height, width ...). A row has hq
+ * query and hk key heads of dim channels (even, at most 512), ldh elements from head to head (0 = dim), ldr from row to row (0 =
+ * (hq + hk) ldh); y likewise, and may be x with the same strides. With qw (query heads) or kw (key heads), a head is first
+ * h / sqrt(mean(h^2) + eps) * w (eps 0 = 1e-6). Axis a takes axis_dim[a] channels (even), R in all (R <= dim; the channels from R
+ * on are not rotated): pair i < R / 2 is channels (2 i, 2 i + 1) (P0_ROPE_INTER) or (i, i + R / 2) (P0_ROPE_HALF), its axis the
+ * one that holds channel 2 i when the axes lie one after the other, its angle pos[a][row] theta^-e with e = 2 j / axis_dim[a], j
+ * the pair's place within its axis (freq 0), or e = 2 i / R (freq 1): (u, v) -> (u cos - v sin, v cos + u sin). Positions are
+ * int32, pos[a * pos_ld + row] (pos_ld 0 = rows); angles are held in 64 bits, so far positions lose nothing. axes 0 counts as
+ * 1, an axis_dim[0] of 0 with one axis as dim, theta 0 as 10000. */
+typedef struct {
+  const void* x; int64_t ldr, ldh;
+  void* y; int64_t y_ldr, y_ldh;
+  int32_t type;
+  int64_t rows;
+  int32_t hq, hk, dim;
+  int32_t mode, axes, axis_dim[4], freq;
+  const int32_t* pos; int64_t pos_ld;
+  double theta;
+  const float* qw;
+  const float* kw;
+  float eps;
+} p0_rope_args_t;
+int p0_rope(const p0_rope_args_t* a);
+
 /* ---- the pack reader's I/O (engine/core/store.js:221-244) ---------------------------------------------------------- */
 /* bytes [offset, offset + bytes) of the file at path -> device memory dst + dst_off, streamed in 16 MB chunks through
  * two pinned host buffers (file reads overlap the host-to-device copies on the library's stream); returns when the

@@ -21,6 +21,9 @@ GEPI = {"f16": 0, "f32": 1, "resadd": 2, "swiglu": 3, "bias": 4, "heads": 5}
 ROPE = {"inter": 0, "half": 1}
 ACT = {"silu": 0, "gelu": 1}
 KV_TYPE = {"f32": 0, "f16": 1, "bf16": 2}
+TYPE = KV_TYPE
+GLU = {"none": 0, "silu": 1, "gelu": 2}
+FREQ = {"own": 0, "shared": 1}
 
 # every symbol the header declares (tests check the library exports each one)
 HEADER_SYMBOLS = [
@@ -33,6 +36,7 @@ HEADER_SYMBOLS = [
     "p0_chain_begin", "p0_chain_end", "p0_chain_run", "p0_chain_status", "p0_chain_info", "p0_chain_free",
     "p0_chain_tune", "p0_rowstats", "p0_normadd", "p0_argmax", "p0_argmaxM", "p0_upload_file",
     "p0_kv_page_bytes", "p0_kv_put", "p0_kv_get", "p0_kv_attn", "p0_kv_update", "p0_kv_compact", "p0_beam",
+    "p0_f8_pack", "p0_f8_norm", "p0_f8_rows", "p0_f8_gemm", "p0_rope",
 ]
 
 i64, i32, f32, vp = C.c_int64, C.c_int32, C.c_float, C.c_void_p
@@ -117,6 +121,32 @@ class BeamArgs(C.Structure):
                 ("hist_n", i64), ("hist_ld", i64)]
 
 
+class F8PackArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldx", i64), ("type", i32), ("N", i64), ("K", i64), ("w", vp), ("ldw", i64), ("s", vp), ("lds", i64)]
+
+
+class F8NormArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldx", i64), ("type", i32), ("t", vp), ("ldt", i64), ("t_type", i32), ("tw", vp), ("x_out", vp), ("ldo", i64),
+                ("scale", f32), ("eps", f32), ("mode", i32), ("w_one", i32), ("w", vp), ("b", vp), ("M", i64), ("D", i64),
+                ("y", vp), ("ldy", i64), ("s", vp), ("lds", i64)]
+
+
+class F8RowsArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldx", i64), ("type", i32), ("up", i64), ("glu", i32), ("M", i64), ("D", i64),
+                ("y", vp), ("ldy", i64), ("s", vp), ("lds", i64)]
+
+
+class F8GemmArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldx", i64), ("xs", vp), ("ldxs", i64), ("w", vp), ("ldw", i64), ("ws", vp), ("ldws", i64),
+                ("M", i64), ("N", i64), ("K", i64), ("type", i32), ("y", vp), ("ldy", i64)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [("x", vp), ("ldr", i64), ("ldh", i64), ("y", vp), ("y_ldr", i64), ("y_ldh", i64), ("type", i32), ("rows", i64),
+                ("hq", i32), ("hk", i32), ("dim", i32), ("mode", i32), ("axes", i32), ("axis_dim", i32 * 4), ("freq", i32),
+                ("pos", vp), ("pos_ld", i64), ("theta", C.c_double), ("qw", vp), ("kw", vp), ("eps", f32)]
+
+
 class P0Error(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(msg)
@@ -160,6 +190,8 @@ def lib():
             "p0_kv_put": [C.POINTER(KvRowsArgs)], "p0_kv_get": [C.POINTER(KvRowsArgs)], "p0_kv_attn": [C.POINTER(KvAttnArgs)],
             "p0_kv_update": [C.POINTER(KvUpdateArgs)], "p0_kv_compact": [C.POINTER(KvCompactArgs)],
             "p0_beam": [C.POINTER(BeamArgs)],
+            "p0_f8_pack": [C.POINTER(F8PackArgs)], "p0_f8_norm": [C.POINTER(F8NormArgs)], "p0_f8_rows": [C.POINTER(F8RowsArgs)],
+            "p0_f8_gemm": [C.POINTER(F8GemmArgs)], "p0_rope": [C.POINTER(RopeArgs)],
         }
         for name, args in sig.items():
             fn = getattr(L, name)
@@ -513,3 +545,51 @@ def beam_args(**kw):
 
 def beam(args):
     check(lib().p0_beam(C.byref(args)))
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit linears, rotation
+def f8_pack_args(**kw):
+    return _fields(F8PackArgs, kw)
+
+
+def f8_pack(args):
+    check(lib().p0_f8_pack(C.byref(args)))
+
+
+def f8_norm_args(**kw):
+    """mode is 1 (rms) unless given"""
+    kw.setdefault("mode", 1)
+    return _fields(F8NormArgs, kw)
+
+
+def f8_norm(args):
+    check(lib().p0_f8_norm(C.byref(args)))
+
+
+def f8_rows_args(**kw):
+    return _fields(F8RowsArgs, kw)
+
+
+def f8_rows(args):
+    check(lib().p0_f8_rows(C.byref(args)))
+
+
+def f8_gemm_args(**kw):
+    return _fields(F8GemmArgs, kw)
+
+
+def f8_gemm(args):
+    check(lib().p0_f8_gemm(C.byref(args)))
+
+
+def rope_args(**kw):
+    """axis_dim is a sequence of 1 .. 4 channel counts, one per axis"""
+    dims = kw.get("axis_dim")
+    if dims is not None:
+        kw["axis_dim"] = (i32 * 4)(*dims)
+        kw.setdefault("axes", len(dims))
+    return _fields(RopeArgs, kw)
+
+
+def rope(args):
+    check(lib().p0_rope(C.byref(args)))

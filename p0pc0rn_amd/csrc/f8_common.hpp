@@ -1,0 +1,140 @@
+// f8_common.hpp - what the 8-bit operators and the rotation share (f8_rows.hip, f8_gemm.hip, rope.hip): e4m3 codes with a scale
+// per block of 128 (include/p0pc0rn.h has the format), loads and stores of 8 values of a type, checks of arguments.
+#pragma once
+#include "common.hpp"
+
+namespace p0 {
+
+constexpr int kF8Block = 128;
+constexpr int64_t kF8MaxRows = (1ll << 31) - 1;
+
+// ---- arguments: `rows` rows of `width` bytes, `ld` bytes apart
+struct Span {
+  const void* at;
+  int64_t rows, width, ld;
+};
+// of elements; a stride that no buffer has (negative, past 2^56) becomes one that f8_check refuses
+inline Span f8_span(const void* at, int64_t rows, int64_t width, int64_t ld, int size) {
+  return Span{at, rows, width * size, ld < 0 || ld > (1ll << 56) ? -size : ld * size};
+}
+// rows of one stride may lie in each other's gaps; of two strides the whole extents have to be apart
+inline bool overlap(const Span& a, const Span& b) {
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+  const auto end = [](const Span& w) { return (__int128)(uintptr_t)w.at + (__int128)(w.rows - 1) * w.ld + w.width; };
+  if ((__int128)(uintptr_t)a.at >= end(b) || (__int128)(uintptr_t)b.at >= end(a)) return false;
+  if ((a.rows > 1 && b.rows > 1 && a.ld != b.ld) || (a.rows == 1 && b.rows == 1)) return true;
+  const __int128 step = a.rows > 1 ? a.ld : b.ld, d = (__int128)(uintptr_t)b.at - (__int128)(uintptr_t)a.at, in = (d % step + step) % step;
+  return in < (__int128)a.width || in + (__int128)b.width > step;
+}
+// a matrix argument: there, aligned, its rows apart and its extent within 2^62 bytes
+inline int f8_check(const char* op, const char* name, const Span& s, int align) {
+  if (!s.at) { set_error("%s: missing %s buffer", op, name); return P0_EINVAL; }
+  if ((uintptr_t)s.at % align || s.ld % align) { set_error("%s: %s must be %d-byte aligned, its rows too", op, name, align); return P0_EINVAL; }
+  if (s.ld < s.width || (__int128)s.rows * s.ld > ((__int128)1 << 62)) {
+    set_error("%s: %s has rows of %lld B, %lld B apart", op, name, (long long)s.width, (long long)s.ld); return P0_EINVAL;
+  }
+  return P0_OK;
+}
+inline bool f8_type(int t) { return t >= P0_F32 && t <= P0_BF16; }
+inline int f8_size(int t) { return t == P0_F32 ? 4 : 2; }
+inline int64_t f8_blocks(int64_t n) { return (n + kF8Block - 1) / kF8Block; }
+
+// ---- values
+template <int TYPE> __device__ __forceinline__ float f8_value(uint32_t h) {   // a 16-bit value's low half
+  return TYPE == P0_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
+}
+// n of 8 consecutive elements from element i on (vec: all 8, 16-byte aligned); the others are 0
+template <int TYPE> __device__ __forceinline__ void f8_load8(const void* x, int64_t i, bool vec, int n, float (&f)[8]) {
+  if constexpr (TYPE == P0_F32) {
+    const float* a = (const float*)x + i;
+    if (vec) {
+      const float4 u = *(const float4*)a, v = *(const float4*)(a + 4);
+      f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = j < n ? a[j] : 0.0f;
+    }
+  } else {
+    const uint16_t* a = (const uint16_t*)x + i;
+    if (vec) {
+      const uint4 u = *(const uint4*)a;
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[2 * j] = f8_value<TYPE>(w[j] & 0xFFFFu);
+        f[2 * j + 1] = TYPE == P0_F16 ? f8_value<TYPE>(w[j] >> 16) : __uint_as_float(w[j] & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = j < n ? f8_value<TYPE>(a[j]) : 0.0f;
+    }
+  }
+}
+// to the nearest value of a 16-bit type, ties to the even one
+template <int TYPE> __device__ __forceinline__ uint32_t f8_half(float v) {
+  if constexpr (TYPE == P0_F16) return __builtin_bit_cast(uint16_t, (_Float16)v);
+  else return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+template <int TYPE> __device__ __forceinline__ float f8_rounded(float v) {
+  if constexpr (TYPE == P0_F32) return v;
+  else return f8_value<TYPE>(f8_half<TYPE>(v));
+}
+template <int TYPE> __device__ __forceinline__ void f8_store8(void* x, int64_t i, bool vec, int n, const float (&f)[8]) {
+  if constexpr (TYPE == P0_F32) {
+    float* a = (float*)x + i;
+    if (vec) {
+      *(float4*)a = float4{f[0], f[1], f[2], f[3]};
+      *(float4*)(a + 4) = float4{f[4], f[5], f[6], f[7]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) a[j] = f[j];
+    }
+  } else {
+    uint16_t* a = (uint16_t*)x + i;
+    if (vec) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = f8_half<TYPE>(f[2 * j]) | f8_half<TYPE>(f[2 * j + 1]) << 16;
+      *(uint4*)a = uint4{w[0], w[1], w[2], w[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) a[j] = (uint16_t)f8_half<TYPE>(f[j]);
+    }
+  }
+}
+
+// ---- codes
+template <int CTRL> __device__ __forceinline__ float f8_dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float f8_max16(float v) {   // of the lane's 16: rotations within a row of lanes
+  v = fmaxf(v, f8_dpp<0x128>(v));
+  v = fmaxf(v, f8_dpp<0x124>(v));
+  v = fmaxf(v, f8_dpp<0x122>(v));
+  return fmaxf(v, f8_dpp<0x121>(v));
+}
+// the largest finite magnitude of 8 values
+__device__ __forceinline__ float f8_most(const float (&f)[8]) {
+  float most = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float a = fabsf(f[j]);
+    most = fmaxf(most, a < INFINITY ? a : 0.0f);
+  }
+  return most;
+}
+__device__ __forceinline__ float f8_scale(float most) { return fmaxf(most / 448.0f, 0x1p-126f); }
+// x * inv rounded to e4m3, ties to the even code; |x * inv| of a finite x is below 448.001 and so never past the largest
+__device__ __forceinline__ uint2 f8_codes(const float (&f)[8], float inv) {
+  uint32_t w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j] * inv, f[4 * j + 1] * inv, 0, false);
+    w[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j + 2] * inv, f[4 * j + 3] * inv, r, true);
+  }
+  return uint2{w[0], w[1]};
+}
+
+}  // namespace p0

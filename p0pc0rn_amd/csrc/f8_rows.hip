@@ -1,0 +1,350 @@
+// f8_rows.hip - values into e4m3 codes with a scale per block of 128: weights (f8_pack), the residual stream's update and norm
+// (f8_norm), activations and gated ones (f8_rows).
+//
+// A lane holds 8 consecutive channels, 16 lanes a block: its largest magnitude is 4 lane moves away. All three read their
+// input once into registers and write codes from there.
+#include "f8_common.hpp"
+
+namespace p0 {
+
+// ------------------------------------------------------------------------------------------------ weights
+struct PackP {
+  const void* x;
+  uint8_t* w;
+  float* s;
+  int64_t ldx, ldw, lds;
+  int64_t N, K;
+  int blocks;   // of 128 channels in a row
+  int vec;
+};
+// A workgroup takes a block of 128 x 128, a thread 8 rows of 8 channels.
+template <int TYPE>
+__global__ __launch_bounds__(256) void f8_pack_kernel(const PackP p) {
+  __shared__ float red[4];
+  const int64_t nb = blockIdx.x / (unsigned)p.blocks;
+  const int kb = (int)(blockIdx.x - nb * p.blocks), c = kb * 128 + (threadIdx.x & 15) * 8, lane = threadIdx.x & 63;
+  const int64_t n0 = nb * 128 + (threadIdx.x >> 4);
+  const int n = (int)(p.K - c < 8 ? (p.K - c < 0 ? 0 : p.K - c) : 8);
+  float f[8][8], most = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int64_t r = n0 + 16 * j;
+    if (r < p.N) f8_load8<TYPE>(p.x, r * p.ldx + c, p.vec && n == 8, n, f[j]);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[j][i] = 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) most = fmaxf(most, f8_most(f[j]));
+  most = f8_max16(most);
+  most = fmaxf(most, __shfl_xor(most, 16, 64));
+  most = fmaxf(most, __shfl_xor(most, 32, 64));
+  if (lane == 0) red[threadIdx.x >> 6] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float s = f8_scale(most), inv = 1.0f / s;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int64_t r = n0 + 16 * j;
+    if (r < p.N) *(uint2*)(p.w + r * p.ldw + c) = f8_codes(f[j], inv);
+  }
+  if (threadIdx.x == 0) p.s[nb * p.lds + kb] = s;
+}
+
+// ------------------------------------------------------------------------------------------------ activations
+__device__ __forceinline__ float gated(int glu, float g, float u) {
+  // g * sigmoid(z), z = g, or 2 sqrt(2 / pi) (g + 0.044715 g^3) (= 0.5 g (1 + tanh(z / 2)))
+  const float z = glu == P0_GLU_SILU ? g : 1.5957691216f * (g + 0.044715f * g * g * g);
+  return g / (1.0f + __expf(-z)) * u;
+}
+struct RowsF8P {
+  const void* x;
+  uint8_t* y;
+  float* s;
+  int64_t ldx, up, ldy, lds;
+  int64_t M, D;
+  int strips, ls;   // 1 << ls lanes side by side take a strip of 8 << ls channels of a row
+  int vec, glu;
+};
+// A workgroup takes a strip of 256 >> ls rows, U times.
+template <int TYPE, bool GLU, int U>
+__global__ __launch_bounds__(256) void f8_rows_kernel(const RowsF8P p) {
+  const int64_t rblk = blockIdx.x / (unsigned)p.strips;
+  const int side = 256 >> p.ls, c = (((int)(blockIdx.x - rblk * p.strips) << p.ls) + (threadIdx.x & ((1 << p.ls) - 1))) * 8;
+  const int64_t m0 = rblk * side * U + (threadIdx.x >> p.ls);
+  if (c >= (int)((p.D + 127) / 128 * 128)) return;   // whole blocks of lanes
+  const int n = (int)(p.D - c < 8 ? (p.D - c < 0 ? 0 : p.D - c) : 8);
+  const bool vec = p.vec && n == 8;
+  float f[U][8], g[GLU ? U : 1][8];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t m = m0 + (int64_t)u * side < p.M ? m0 + (int64_t)u * side : p.M - 1;   // past the last row: it again (not stored)
+    f8_load8<TYPE>(p.x, m * p.ldx + c, vec, n, f[u]);
+    if constexpr (GLU) f8_load8<TYPE>(p.x, m * p.ldx + p.up + c, vec, n, g[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t m = m0 + (int64_t)u * side;
+    if constexpr (GLU) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[u][j] = gated(p.glu, f[u][j], g[u][j]);
+    }
+    const float s = f8_scale(f8_max16(f8_most(f[u])));
+    const uint2 w = f8_codes(f[u], 1.0f / s);
+    if (m >= p.M) continue;
+    *(uint2*)(p.y + m * p.ldy + c) = w;
+    if ((threadIdx.x & 15) == 0) p.s[(int64_t)(c >> 7) * p.lds + m] = s;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the stream's norm
+struct NormP {
+  const void* x;
+  const void* t;
+  void* xo;          // null: the sum is not stored
+  const float* tw;
+  const float* w;
+  const float* b;
+  uint8_t* y;
+  float* s;
+  int64_t ldx, ldt, ldo, ldy, lds;
+  int64_t M;
+  int D, xvec, tvec, mode, one;
+  float scale, eps;
+};
+__device__ __forceinline__ float sum64(float v) {
+  v += f8_dpp<0x128>(v);
+  v += f8_dpp<0x124>(v);
+  v += f8_dpp<0x122>(v);
+  v += f8_dpp<0x121>(v);
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+// W waves take a row (W = 1: a workgroup has four rows), a lane 8 channels of NC steps of 512 W. The row stays in registers.
+template <int XT, int TT, int W, int NC>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void f8_norm_kernel(const NormP p) {
+  __shared__ float red[3][W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t m = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+  if (m >= p.M) return;
+  const int c0 = ((W == 1 ? 0 : wave) * 64 + lane) * 8;
+  auto total = [&](float v, int slot) {
+    v = sum64(v);
+    if constexpr (W > 1) {
+      if (lane == 0) red[slot][wave] = v;
+      __syncthreads();
+      v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v += red[slot][i];
+    }
+    return v;
+  };
+  float f[NC][8];
+  const float over = 1.0f / (float)p.D;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = c0 + i * 512 * W, n = p.D - c < 8 ? (p.D - c < 0 ? 0 : p.D - c) : 8;
+    f8_load8<XT>(p.x, m * p.ldx + c, p.xvec && n == 8, n, f[i]);
+  }
+  if (p.t) {
+    float t[NC][8], ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = c0 + i * 512 * W, n = p.D - c < 8 ? (p.D - c < 0 ? 0 : p.D - c) : 8;
+      f8_load8<TT>(p.t, m * p.ldt + c, p.tvec && n == 8, n, t[i]);
+    }
+    if (p.tw) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(t[i][j], t[i][j], ss);
+      const float r = 1.0f / sqrtf(total(ss, 0) * over + p.eps);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = c0 + i * 512 * W + j;
+          t[i][j] *= r * (c < p.D ? p.tw[c] : 0.0f);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[i][j] += t[i][j];
+  }
+  float sum = 0.0f, sq = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[i][j] = f8_rounded<XT>(f[i][j] * p.scale);
+      sum += f[i][j];
+    }
+    const int c = c0 + i * 512 * W, n = p.D - c < 8 ? (p.D - c < 0 ? 0 : p.D - c) : 8;
+    if (p.xo && n > 0) f8_store8<XT>(p.xo, m * p.ldo + c, p.xvec && n == 8, n, f[i]);
+  }
+  float mean = 0.0f;
+  if (p.mode == 0) mean = total(sum, 1) * over;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[i][j] = c0 + i * 512 * W + j < p.D ? f[i][j] - mean : 0.0f;
+      sq = __builtin_fmaf(f[i][j], f[i][j], sq);
+    }
+  const float rstd = 1.0f / sqrtf(total(sq, 2) * over + p.eps);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = c0 + i * 512 * W;
+    if (c >= (p.D + 127) / 128 * 128) break;   // whole blocks of lanes
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (c + j >= p.D) continue;
+      const float g = (p.w ? p.w[c + j] : p.one ? 0.0f : 1.0f) + (p.one ? 1.0f : 0.0f);
+      f[i][j] = f[i][j] * rstd * g + (p.b ? p.b[c + j] : 0.0f);
+    }
+    const float s = f8_scale(f8_max16(f8_most(f[i])));
+    *(uint2*)(p.y + m * p.ldy + c) = f8_codes(f[i], 1.0f / s);
+    if ((lane & 15) == 0) p.s[(int64_t)(c >> 7) * p.lds + m] = s;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the calls
+static int refuse(const char* op) {
+  if (int r = refuse_in_chain(op)) return r;
+  return require_open(op);
+}
+static int rows_count(const char* op, const char* name, int64_t M) {
+  if (M < 0 || M > kF8MaxRows) { set_error("%s: %s %lld", op, name, (long long)M); return P0_EINVAL; }
+  return P0_OK;
+}
+
+static int pack_call(const p0_f8_pack_args_t* a) {
+  const char* op = "f8_pack";
+  if (!a) { set_error("%s: no arguments", op); return P0_EINVAL; }
+  if (!f8_type(a->type)) { set_error("%s: type %d", op, (int)a->type); return P0_EINVAL; }
+  if (int r = rows_count(op, "N", a->N)) return r;
+  if (a->K < 1 || a->K > (1 << 20)) { set_error("%s: K %lld", op, (long long)a->K); return P0_EINVAL; }
+  if (a->N == 0) return refuse(op);
+  const int size = f8_size(a->type);
+  const int64_t blocks = f8_blocks(a->K), K8 = blocks * 128, ldx = a->ldx ? a->ldx : a->K, ldw = a->ldw ? a->ldw : K8,
+                lds = a->lds ? a->lds : blocks;
+  const Span x = f8_span(a->x, a->N, a->K, ldx, size), w = f8_span(a->w, a->N, K8, ldw, 1), s = f8_span(a->s, f8_blocks(a->N), blocks, lds, 4);
+  if (int r = f8_check(op, "x", x, size)) return r;
+  if (int r = f8_check(op, "w", w, 16)) return r;
+  if (int r = f8_check(op, "s", s, 4)) return r;
+  if (overlap(x, w) || overlap(x, s) || overlap(w, s)) { set_error("%s: outputs overlap", op); return P0_EINVAL; }
+  if (f8_blocks(a->N) * blocks >= (1ll << 31)) { set_error("%s: %lld x %lld values", op, (long long)a->N, (long long)a->K); return P0_EINVAL; }
+  if (int r = refuse(op)) return r;
+  PackP p{a->x, (uint8_t*)a->w, a->s, ldx, ldw, lds, a->N, a->K, (int)blocks, ((uintptr_t)a->x | (uintptr_t)(ldx * size)) % 16 == 0};
+  auto k = a->type == P0_F32 ? f8_pack_kernel<P0_F32> : a->type == P0_F16 ? f8_pack_kernel<P0_F16> : f8_pack_kernel<P0_BF16>;
+  hipLaunchKernelGGL(k, dim3((unsigned)(f8_blocks(a->N) * blocks)), dim3(256), 0, ctx().cur, p);
+  P0_LAUNCHED(op);
+  return P0_OK;
+}
+
+template <int U> static auto rows_kernel(int type, bool glu) {
+  return type == P0_F32 ? (glu ? f8_rows_kernel<P0_F32, true, U> : f8_rows_kernel<P0_F32, false, U>)
+       : type == P0_F16 ? (glu ? f8_rows_kernel<P0_F16, true, U> : f8_rows_kernel<P0_F16, false, U>)
+                        : (glu ? f8_rows_kernel<P0_BF16, true, U> : f8_rows_kernel<P0_BF16, false, U>);
+}
+
+static int rows_f8_call(const p0_f8_rows_args_t* a) {
+  const char* op = "f8_rows";
+  if (!a) { set_error("%s: no arguments", op); return P0_EINVAL; }
+  if (!f8_type(a->type)) { set_error("%s: type %d", op, (int)a->type); return P0_EINVAL; }
+  if (a->glu < P0_GLU_NONE || a->glu > P0_GLU_GELU) { set_error("%s: glu %d", op, (int)a->glu); return P0_EINVAL; }
+  if (int r = rows_count(op, "M", a->M)) return r;
+  if (a->D < 1 || a->D > (1 << 20)) { set_error("%s: D %lld", op, (long long)a->D); return P0_EINVAL; }
+  const bool glu = a->glu != P0_GLU_NONE;
+  const int size = f8_size(a->type);
+  const int64_t up = !glu ? 0 : a->up ? a->up : a->D;
+  if (up < 0 || up > (1ll << 31)) { set_error("%s: up %lld", op, (long long)a->up); return P0_EINVAL; }
+  if (a->M == 0) return refuse(op);
+  const int64_t blocks = f8_blocks(a->D), K8 = blocks * 128, ldx = a->ldx ? a->ldx : up + a->D, ldy = a->ldy ? a->ldy : K8,
+                lds = a->lds ? a->lds : a->M;
+  const Span x = f8_span(a->x, a->M, up + a->D, ldx, size), y = f8_span(a->y, a->M, K8, ldy, 1), s = f8_span(a->s, blocks, a->M, lds, 4);
+  if (int r = f8_check(op, "x", x, size)) return r;
+  if (int r = f8_check(op, "y", y, 16)) return r;
+  if (int r = f8_check(op, "s", s, 4)) return r;
+  if (overlap(x, y) || overlap(x, s) || overlap(y, s)) { set_error("%s: outputs overlap", op); return P0_EINVAL; }
+  if (int r = refuse(op)) return r;
+  RowsF8P p{a->x, (uint8_t*)a->y, a->s, ldx, up, ldy, lds, a->M, a->D, 0, 8, 0, a->glu};
+  p.vec = ((uintptr_t)a->x | (uintptr_t)(ldx * size) | (uintptr_t)(up * size)) % 16 == 0;
+  const int64_t chunks = K8 / 8;
+  while (p.ls > 4 && ((chunks + (1 << p.ls) - 1) >> p.ls << p.ls) - chunks > chunks / 8) --p.ls;
+  p.strips = (int)((chunks + (1 << p.ls) - 1) >> p.ls);
+  const int side = 256 >> p.ls;
+  const int64_t steps = (a->M + side - 1) / side;
+  const int U = steps * p.strips > 2048 ? 2 : 1;
+  const int64_t grid = (steps + U - 1) / U * p.strips;
+  if (grid >= (1ll << 31)) { set_error("%s: %lld rows of %lld", op, (long long)a->M, (long long)a->D); return P0_EINVAL; }
+  hipLaunchKernelGGL((U == 2 ? rows_kernel<2>(a->type, glu) : rows_kernel<1>(a->type, glu)), dim3((unsigned)grid), dim3(256), 0,
+                     ctx().cur, p);
+  P0_LAUNCHED(op);
+  return P0_OK;
+}
+
+typedef void (*NormKernel)(NormP);
+template <int XT, int TT> static NormKernel norm_kernel(int W, int NC) {
+  if (W == 1) return NC == 1 ? f8_norm_kernel<XT, TT, 1, 1> : NC == 2 ? f8_norm_kernel<XT, TT, 1, 2> : f8_norm_kernel<XT, TT, 1, 5>;
+  if (W == 4) return NC == 1 ? f8_norm_kernel<XT, TT, 4, 1> : NC == 2 ? f8_norm_kernel<XT, TT, 4, 2> : f8_norm_kernel<XT, TT, 4, 4>;
+  return NC == 2 ? f8_norm_kernel<XT, TT, 16, 2> : f8_norm_kernel<XT, TT, 16, 4>;
+}
+
+static int norm_call(const p0_f8_norm_args_t* a) {
+  const char* op = "f8_norm";
+  if (!a) { set_error("%s: no arguments", op); return P0_EINVAL; }
+  if (!f8_type(a->type) || (a->t && !f8_type(a->t_type))) { set_error("%s: type %d, t_type %d", op, (int)a->type, (int)a->t_type); return P0_EINVAL; }
+  if (a->mode != 0 && a->mode != 1) { set_error("%s: mode %d", op, (int)a->mode); return P0_EINVAL; }
+  if (int r = rows_count(op, "M", a->M)) return r;
+  if (a->D < 1 || a->D > 32768) { set_error("%s: D %lld (1 .. 32768)", op, (long long)a->D); return P0_EINVAL; }
+  if (a->tw && !a->t) { set_error("%s: tw needs t", op); return P0_EINVAL; }
+  if (a->M == 0) return refuse(op);
+  const int xsize = f8_size(a->type), tsize = a->t ? f8_size(a->t_type) : 4;
+  const int64_t M = a->M, D = a->D, blocks = f8_blocks(D), K8 = blocks * 128, ldx = a->ldx ? a->ldx : D, ldt = a->ldt ? a->ldt : D,
+                ldo = a->x_out ? (a->ldo ? a->ldo : D) : ldx, ldy = a->ldy ? a->ldy : K8, lds = a->lds ? a->lds : M;
+  const float scale = a->scale != 0.0f ? a->scale : 1.0f;
+  void* xo = a->x_out ? a->x_out : a->t || scale != 1.0f ? a->x : nullptr;
+  const Span x = f8_span(a->x, M, D, ldx, xsize), t = f8_span(a->t, M, D, ldt, tsize), o = f8_span(xo, M, D, ldo, xsize),
+             y = f8_span(a->y, M, K8, ldy, 1), s = f8_span(a->s, blocks, M, lds, 4), tw{a->tw, 1, D * 4, D * 4}, w{a->w, 1, D * 4, D * 4},
+             b{a->b, 1, D * 4, D * 4};
+  if (int r = f8_check(op, "x", x, xsize)) return r;
+  if (a->t) { if (int r = f8_check(op, "t", t, tsize)) return r; }
+  if (xo) { if (int r = f8_check(op, "x_out", o, xsize)) return r; }
+  if (int r = f8_check(op, "y", y, 16)) return r;
+  if (int r = f8_check(op, "s", s, 4)) return r;
+  if (((uintptr_t)a->tw | (uintptr_t)a->w | (uintptr_t)a->b) % 4) { set_error("%s: tw, w and b must be 4-byte aligned", op); return P0_EINVAL; }
+  const bool same = xo == a->x && ldo == ldx;
+  const Span* in[] = {&x, &t, &tw, &w, &b};
+  for (const Span* i : in)
+    if (overlap(*i, y) || overlap(*i, s) || (overlap(*i, o) && !(i == &x && same))) { set_error("%s: outputs overlap", op); return P0_EINVAL; }
+  if (overlap(y, s) || overlap(o, y) || overlap(o, s)) { set_error("%s: outputs overlap", op); return P0_EINVAL; }
+  if (int r = refuse(op)) return r;
+  NormP p{};
+  p.x = a->x; p.t = a->t; p.xo = xo; p.tw = a->tw; p.w = a->w; p.b = a->b; p.y = (uint8_t*)a->y; p.s = a->s;
+  p.ldx = ldx; p.ldt = ldt; p.ldo = ldo; p.ldy = ldy; p.lds = lds; p.M = M; p.D = (int)D;
+  p.xvec = ((uintptr_t)a->x | (uintptr_t)(ldx * xsize) | (uintptr_t)xo | (uintptr_t)(ldo * xsize)) % 16 == 0;
+  p.tvec = ((uintptr_t)a->t | (uintptr_t)(ldt * tsize)) % 16 == 0;
+  p.mode = a->mode; p.one = a->w_one ? 1 : 0; p.scale = scale; p.eps = a->eps != 0.0f ? a->eps : 1e-6f;
+  const int W = D <= 2560 && M >= 256 ? 1 : D <= 8192 ? 4 : 16, steps = (int)((K8 + 512 * W - 1) / (512 * W));
+  const int NC = W == 1 ? (steps <= 2 ? steps : 5) : W == 4 ? (steps <= 2 ? steps : 4) : (steps <= 2 ? 2 : 4);
+  const int tt = a->t ? a->t_type : a->type;
+  NormKernel k = nullptr;
+#define P0_NORM(XT, TT) if (a->type == XT && tt == TT) k = norm_kernel<XT, TT>(W, NC)
+  P0_NORM(P0_F32, P0_F32); P0_NORM(P0_F32, P0_F16); P0_NORM(P0_F32, P0_BF16);
+  P0_NORM(P0_F16, P0_F32); P0_NORM(P0_F16, P0_F16); P0_NORM(P0_F16, P0_BF16);
+  P0_NORM(P0_BF16, P0_F32); P0_NORM(P0_BF16, P0_F16); P0_NORM(P0_BF16, P0_BF16);
+#undef P0_NORM
+  hipLaunchKernelGGL(k, dim3((unsigned)(W == 1 ? (M + 3) / 4 : M)), dim3(W == 1 ? 256 : 64 * W), 0, ctx().cur, p);
+  P0_LAUNCHED(op);
+  return P0_OK;
+}
+
+}  // namespace p0
+
+using namespace p0;
+
+extern "C" int p0_f8_pack(const p0_f8_pack_args_t* a) { return pack_call(a); }
+extern "C" int p0_f8_norm(const p0_f8_norm_args_t* a) { return norm_call(a); }
+extern "C" int p0_f8_rows(const p0_f8_rows_args_t* a) { return rows_f8_call(a); }

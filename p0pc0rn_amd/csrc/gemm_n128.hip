@@ -1,9 +1,8 @@
 // gemm_n128.hip - the q4g32a.t64 dequant-GEMM in tiles of 128 x 128 outputs (engine/ops/gemm.js:255-322, as gemm.hip),
 // for calls whose 256 x 256 tiles would leave most CUs idle: prompt chunks, text streams, small images.
 //
-//  * K runs in steps of 64 (two q4 groups). X' rows and the raw weight records go to LDS by LDS-DMA, S - 1 steps ahead,
-//    written in asm: the compiler, which takes an LDS-DMA load for a pending write of all LDS, would wait for every one in
-//    flight before each LDS read. The loads are waited for by count; one barrier a step.
+//  * K runs in steps of 64 (two q4 groups). X' rows and the raw weight records go to LDS by LDS-DMA (dma.hpp), S - 1 steps
+//    ahead. The loads are waited for by count; one barrier a step.
 //  * While a step's MFMAs run, the workgroup dequantises the next step's weights from the raw records in LDS into the other
 //    of two fp16 tiles, each weight once per workgroup.
 //  * When the tiles alone do not fill the chip, K is cut into slices over workgroups: fp32 partial tiles in the uncached
@@ -16,23 +15,10 @@
 // which bounds it from M = 512 on; M = 256, 16384 x 2048 41 against 36); tiles of 256 x 128 (28, 84) and 256 x 256 (44, 76)
 // in this form; whole GEMMs at M = 4608 with 256 x 256 tiles in this form (800-890 TFLOP/s) and over a W dequantised
 // once (750-960 against 800-990 of gemm.hip, with X' and W by LDS-DMA and two wave groups taking turns).
+#include "dma.hpp"
 #include "gemm_common.hpp"
 
 namespace p0 {
-
-// 64 lanes x 16 bytes, buffer resource + lane offset + scalar offset -> LDS at dst + 16 lane
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void dma16(uint32_t dst, int voff, i32x4 rsrc, int soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :: "s"(dst), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
-}
-__device__ __forceinline__ i32x4 resource(const void* b) {   // raw, no bounds of its own
-  const uint64_t a = (uint64_t)(uintptr_t)b;
-  return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)), -1,
-               0x00020000};
-}
-template <int N>
-__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
 constexpr int kBand = 4;
 struct N128P {

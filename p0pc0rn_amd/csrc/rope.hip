@@ -1,0 +1,239 @@
+// rope.hip - the rotation of query and key heads by positions on one to four axes, after an optional norm of each head.
+//
+// Pair i of a head, (u, v) -> (u cos - v sin, v cos + u sin), has angle pos theta^-e: the same for every head of a row. A workgroup
+// takes a few rows, works their cosines and sines out once (in LDS), and streams the rows' heads through. An angle of a far position
+// is many turns: it is held in 64 bits, in turns, and only the fraction of a turn goes on in 32.
+#include "f8_common.hpp"
+
+namespace p0 {
+
+constexpr int kRopeThreads = 256, kRopePairs = 256, kRopeTable = 2048;   // pairs of a head at most; angles of a workgroup's rows
+struct RopeP {
+  const void* x;
+  void* y;
+  const int32_t* pos;
+  const float* qw;
+  const float* kw;
+  int64_t ldr, ldh, yldr, yldh, pos_ld, rows;
+  double log2_theta;
+  int heads, hq, dim, R;      // R: channels that turn
+  int first[4], size[4];      // an axis's first pair, its channels
+  int axes, shared, inter, vec;
+  int rb, hb, hblocks;        // rows, heads of a workgroup, workgroups a row block
+  uint32_t magic;             // item / hb = item * magic >> 20
+  int ls;                     // 1 << ls lanes take a head
+  float eps;
+};
+
+// the two channels of pair i; past the turning ones neighbours go together, unturned
+__device__ __forceinline__ int rope_first(const RopeP& p, int i) { return p.inter || i >= p.R / 2 ? 2 * i : i; }
+__device__ __forceinline__ int rope_second(const RopeP& p, int i) { return p.inter || i >= p.R / 2 ? 2 * i + 1 : i + p.R / 2; }
+
+__device__ __forceinline__ float2 rope_turn(const RopeP& p, int64_t row, int i) {
+  if (i >= p.R / 2) return float2{1.0f, 0.0f};
+  int a = 0;
+  for (int k = 1; k < p.axes; ++k) a = i >= p.first[k] ? k : a;
+  const double e = p.shared ? 2.0 * i / p.R : 2.0 * (i - p.first[a]) / p.size[a];
+  const double turns = (double)p.pos[a * p.pos_ld + row] * (exp2(-e * p.log2_theta) * 0.15915494309189535);
+  float s, c;
+  sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+  return float2{c, s};
+}
+
+// V pairs a lane
+template <int TYPE, int V> __device__ __forceinline__ void rope_load(const RopeP& p, int64_t at, int i0, int n, float (&u)[V], float (&v)[V]) {
+  if constexpr (V > 1) {   // vec: whole runs, all of one kind of pair
+    if (p.inter) {
+      float f[2 * V];
+#pragma unroll
+      for (int h = 0; h < 2 * V; h += 8) {
+        float g[8];
+        f8_load8<TYPE>(p.x, at + 2 * i0 + h, true, 8, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[h + j] = g[j];
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) { u[j] = f[2 * j]; v[j] = f[2 * j + 1]; }
+    } else {
+      f8_load8<TYPE>(p.x, at + i0, true, 8, u);
+      f8_load8<TYPE>(p.x, at + i0 + p.R / 2, true, 8, v);
+    }
+  } else {
+    float g[8];
+    f8_load8<TYPE>(p.x, at + rope_first(p, i0), false, n, g);
+    u[0] = g[0];
+    f8_load8<TYPE>(p.x, at + rope_second(p, i0), false, n, g);
+    v[0] = g[0];
+  }
+}
+template <int TYPE, int V> __device__ __forceinline__ void rope_store(const RopeP& p, int64_t at, int i0, const float (&u)[V], const float (&v)[V]) {
+  if constexpr (V > 1) {
+    if (p.inter) {
+#pragma unroll
+      for (int h = 0; h < V; h += 4) {
+        float g[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { g[2 * j] = u[h + j]; g[2 * j + 1] = v[h + j]; }
+        f8_store8<TYPE>(p.y, at + 2 * (i0 + h), true, 8, g);
+      }
+    } else {
+      f8_store8<TYPE>(p.y, at + i0, true, 8, u);
+      f8_store8<TYPE>(p.y, at + i0 + p.R / 2, true, 8, v);
+    }
+  } else {
+    const float a[8] = {u[0]}, b[8] = {v[0]};
+    f8_store8<TYPE>(p.y, at + rope_first(p, i0), false, 1, a);
+    f8_store8<TYPE>(p.y, at + rope_second(p, i0), false, 1, b);
+  }
+}
+
+// V = 8: 8 pairs a lane, dim / 16 lanes a head (rounded up to a power of two); V = 1: one pair a lane at a time, 16 lanes a head
+template <int TYPE, int V>
+__global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeP p) {
+  __shared__ float2 turn[kRopeTable];
+  const int64_t blk = blockIdx.x / (unsigned)p.hblocks, row0 = blk * p.rb;
+  const int h0 = (int)(blockIdx.x - blk * p.hblocks) * p.hb, pairs = p.dim / 2;
+  const int rows = (int)(p.rows - row0 < p.rb ? p.rows - row0 : p.rb), hb = p.heads - h0 < p.hb ? p.heads - h0 : p.hb;
+  for (int r = 0; r < rows; ++r)
+    for (int i = threadIdx.x; i < pairs; i += kRopeThreads) turn[r * pairs + i] = rope_turn(p, row0 + r, i);
+  __syncthreads();
+  const int lane = threadIdx.x & ((1 << p.ls) - 1), items = rows * p.hb;
+  for (int it = threadIdx.x >> p.ls; it < items; it += kRopeThreads >> p.ls) {
+    const int r = (int)((uint32_t)it * p.magic >> 20), hl = it - r * p.hb, h = h0 + hl;
+    if (hl >= hb) continue;   // the last block of heads may be shorter (whole groups of lanes)
+    const int64_t from = (row0 + r) * p.ldr + h * p.ldh, to = (row0 + r) * p.yldr + h * p.yldh;
+    const float* w = h < p.hq ? p.qw : p.kw;
+    if constexpr (V > 1) {
+      const int i0 = lane * V;
+      const bool on = i0 < pairs;
+      float u[V], v[V];
+      if (on) rope_load<TYPE, V>(p, from, i0, 1, u, v);
+      if (w) {
+        float ss = 0.0f;
+        if (on) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) ss += u[j] * u[j] + v[j] * v[j];
+        }
+        for (int o = 1 << p.ls >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        const float rstd = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
+        if (on) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            u[j] = u[j] * rstd * w[rope_first(p, i0 + j)];
+            v[j] = v[j] * rstd * w[rope_second(p, i0 + j)];
+          }
+        }
+      }
+      if (on) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float2 t = turn[r * pairs + i0 + j];
+          const float a = u[j] * t.x - v[j] * t.y, b = v[j] * t.x + u[j] * t.y;
+          u[j] = a;
+          v[j] = b;
+        }
+        rope_store<TYPE, V>(p, to, i0, u, v);
+      }
+    } else {
+      float rstd = 1.0f;
+      if (w) {
+        float ss = 0.0f, u[1], v[1];
+        for (int i = lane; i < pairs; i += 16) {
+          rope_load<TYPE, 1>(p, from, i, 1, u, v);
+          ss += u[0] * u[0] + v[0] * v[0];
+        }
+        for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        rstd = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
+      }
+      for (int i = lane; i < pairs; i += 16) {
+        float u[1], v[1];
+        rope_load<TYPE, 1>(p, from, i, 1, u, v);
+        if (w) {
+          u[0] = u[0] * rstd * w[rope_first(p, i)];
+          v[0] = v[0] * rstd * w[rope_second(p, i)];
+        }
+        const float2 t = turn[r * pairs + i];
+        const float a[1] = {u[0] * t.x - v[0] * t.y}, b[1] = {v[0] * t.x + u[0] * t.y};
+        rope_store<TYPE, 1>(p, to, i, a, b);
+      }
+    }
+  }
+}
+
+static int rope_call(const p0_rope_args_t* a) {
+  const char* op = "rope";
+  if (!a) { set_error("%s: no arguments", op); return P0_EINVAL; }
+  if (!f8_type(a->type)) { set_error("%s: type %d", op, (int)a->type); return P0_EINVAL; }
+  if (a->mode != P0_ROPE_INTER && a->mode != P0_ROPE_HALF) { set_error("%s: mode %d", op, (int)a->mode); return P0_EINVAL; }
+  if (a->freq != 0 && a->freq != 1) { set_error("%s: freq %d", op, (int)a->freq); return P0_EINVAL; }
+  if (a->rows < 0 || a->rows > kF8MaxRows) { set_error("%s: rows %lld", op, (long long)a->rows); return P0_EINVAL; }
+  if (a->dim < 2 || a->dim > 2 * kRopePairs || a->dim % 2) { set_error("%s: heads of %d channels", op, (int)a->dim); return P0_EINVAL; }
+  const int64_t heads = (int64_t)a->hq + a->hk;
+  if (a->hq < 0 || a->hk < 0 || heads < 1 || heads > 65535) { set_error("%s: %d and %d heads", op, (int)a->hq, (int)a->hk); return P0_EINVAL; }
+  RopeP p{};
+  p.axes = a->axes ? a->axes : 1;
+  if (p.axes < 1 || p.axes > 4) { set_error("%s: %d axes", op, (int)a->axes); return P0_EINVAL; }
+  for (int k = 0; k < p.axes; ++k) {
+    const int d = a->axis_dim[k] || p.axes > 1 ? a->axis_dim[k] : a->dim;
+    if (d < 2 || d % 2 || d > a->dim - p.R) { set_error("%s: axis %d of %d channels (heads of %d)", op, k, d, (int)a->dim); return P0_EINVAL; }
+    p.first[k] = p.R / 2;
+    p.size[k] = d;
+    p.R += d;
+  }
+  const double theta = a->theta != 0.0 ? a->theta : 10000.0;
+  if (!(theta > 0.0 && theta < 1e300)) { set_error("%s: theta %g", op, a->theta); return P0_EINVAL; }
+  if (a->rows == 0) { if (int r = refuse_in_chain(op)) return r; return require_open(op); }
+  const int size = f8_size(a->type);
+  const int64_t wide = 1ll << 40;
+  p.ldh = a->ldh ? a->ldh : a->dim;
+  p.yldh = a->y_ldh ? a->y_ldh : a->dim;
+  if (p.ldh < a->dim || p.yldh < a->dim || p.ldh > wide || p.yldh > wide) {
+    set_error("%s: heads %lld and %lld apart", op, (long long)p.ldh, (long long)p.yldh); return P0_EINVAL;
+  }
+  const int64_t xw = (heads - 1) * p.ldh + a->dim, yw = (heads - 1) * p.yldh + a->dim;
+  p.ldr = a->ldr ? a->ldr : heads * p.ldh;
+  p.yldr = a->y_ldr ? a->y_ldr : heads * p.yldh;
+  p.pos_ld = a->pos_ld ? a->pos_ld : a->rows;
+  const Span x = f8_span(a->x, a->rows, xw, p.ldr, size), y = f8_span(a->y, a->rows, yw, p.yldr, size),
+             pos = f8_span(a->pos, p.axes, a->rows, p.pos_ld, 4), qw{a->qw, 1, a->dim * 4, a->dim * 4}, kw{a->kw, 1, a->dim * 4, a->dim * 4};
+  if (int r = f8_check(op, "x", x, size)) return r;
+  if (int r = f8_check(op, "y", y, size)) return r;
+  if (int r = f8_check(op, "pos", pos, 4)) return r;
+  if (((uintptr_t)a->qw | (uintptr_t)a->kw) % 4) { set_error("%s: qw and kw must be 4-byte aligned", op); return P0_EINVAL; }
+  const bool same = a->x == a->y && p.ldr == p.yldr && p.ldh == p.yldh;
+  if ((overlap(x, y) && !same) || overlap(pos, y) || overlap(qw, y) || overlap(kw, y)) { set_error("%s: y overlaps an input", op); return P0_EINVAL; }
+  if (int r = refuse_in_chain(op)) return r;
+  if (int r = require_open(op)) return r;
+  p.x = a->x; p.y = a->y; p.pos = a->pos; p.qw = a->qw; p.kw = a->kw; p.rows = a->rows;
+  p.log2_theta = log2(theta);
+  p.heads = (int)heads; p.hq = a->hq; p.dim = a->dim; p.shared = a->freq; p.inter = a->mode == P0_ROPE_INTER;
+  p.eps = a->eps != 0.0f ? a->eps : 1e-6f;
+  // 8 pairs a lane where every lane's are whole 16-byte runs of one kind
+  const bool rows16 = ((uintptr_t)a->x | (uintptr_t)a->y | (uintptr_t)(p.ldr * size) | (uintptr_t)(p.ldh * size) | (uintptr_t)(p.yldr * size) |
+                       (uintptr_t)(p.yldh * size)) % 16 == 0;
+  p.vec = rows16 && a->dim % 16 == 0 && (p.inter || p.R == a->dim);
+  const int lanes = p.vec ? a->dim / 16 : 16;
+  while (1 << p.ls < lanes) ++p.ls;
+  const int side = kRopeThreads >> p.ls, pairs = a->dim / 2;
+  // A workgroup's work is four rounds of its groups of lanes where that leaves work for every CU: several rows, or a part of a row's
+  // heads; one round where it does not
+  const int rounds = a->rows * heads >= (int64_t)side * 4 * 1024 ? 4 : 1;
+  p.hb = (int)(heads < side * rounds ? heads : side * rounds);
+  p.rb = side * rounds / p.hb;
+  if (p.rb > kRopeTable / pairs) p.rb = kRopeTable / pairs;
+  p.hblocks = (int)((heads + p.hb - 1) / p.hb);
+  p.magic = (1u << 20) / (uint32_t)p.hb + 1;   // exact below 2^20 / hb: items are at most side * rounds <= 256 * 4... of hb <= 1024
+  const int64_t grid = (a->rows + p.rb - 1) / p.rb * p.hblocks;
+  if (grid >= (1ll << 31)) { set_error("%s: %lld rows of %lld heads", op, (long long)a->rows, (long long)heads); return P0_EINVAL; }
+#define P0_ROPE(T) if (a->type == T) hipLaunchKernelGGL((p.vec ? rope_kernel<T, 8> : rope_kernel<T, 1>), dim3((unsigned)grid), dim3(kRopeThreads), 0, ctx().cur, p)
+  P0_ROPE(P0_F32);
+  P0_ROPE(P0_F16);
+  P0_ROPE(P0_BF16);
+#undef P0_ROPE
+  P0_LAUNCHED(op);
+  return P0_OK;
+}
+
+}  // namespace p0
+
+extern "C" int p0_rope(const p0_rope_args_t* a) { return p0::rope_call(a); }

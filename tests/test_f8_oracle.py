@@ -1,0 +1,175 @@
+"""The CPU restatement of the 8-bit operators and the rotation (oracle/f8.py) against torch's e4m3 and the definitions, and the
+calls' refusals: arguments are checked before any device work, so these run without a GPU."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import f8
+from p0pc0rn_amd import capi
+
+P = 1 << 20   # an address: nothing is read there
+
+
+def test_codes_are_the_nearest_values():
+    rng = np.random.default_rng(1)
+    v = np.concatenate([rng.standard_normal(50000) * np.exp(3 * rng.standard_normal(50000)), (f8.VALUES[:126] + f8.VALUES[1:127]) / 2,
+                        -(f8.VALUES[:126] + f8.VALUES[1:127]) / 2, [0.0, -0.0, 448.0, 2.0 ** -10, 2.0 ** -11]]).astype(np.float32)
+    v = np.clip(v, -448, 448)
+    want = torch.from_numpy(v).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(f8.encode(v), want)
+    assert np.array_equal(f8.encode(np.float64([np.nan, np.inf, -np.inf])) & 127, [127] * 3)
+    finite = (np.arange(256) & 127) != 127
+    assert np.array_equal(f8.encode(f8.VALUES[finite]), np.arange(256)[finite])
+
+
+def test_scales_leave_no_value_out():
+    """the largest of a block is at 448, up to the rounding of 1 / s"""
+    rng = np.random.default_rng(2)
+    x = (rng.standard_normal((64, 300)) * np.exp(20 * rng.standard_normal((64, 1)))).astype(np.float32)
+    c, s = f8.quantise(x)
+    back = f8.values(c, s)[:, :300]
+    assert np.abs(back - x).max() <= 2.0 ** -4 * np.abs(x).max() * 1.001
+    assert (f8.VALUES[c[:, :128]].__abs__().max(1) == 448).all() and not c[:, 300:].any()
+    w, ws = f8.pack(x)
+    assert w.shape == (64, 384) and ws.shape == (1, 3)
+    assert np.isclose(ws[0], s.max(1), rtol=0).all()
+
+
+def test_a_value_that_is_not_finite_stays_by_itself():
+    x = np.ones((3, 256), np.float32)
+    x[1, 5], x[2, 200] = np.inf, np.nan
+    c, s = f8.quantise(x)
+    assert np.isnan(f8.values(c, s)).sum() == 2 and (s == np.float32(1) / np.float32(448)).all()
+
+
+def test_zeros_and_the_smallest_values():
+    c, s = f8.quantise(np.zeros((2, 128), np.float32))
+    assert not c.any() and (s == 2.0 ** -126).all()
+    c, s = f8.quantise(np.full((1, 128), 2.0 ** -140, np.float32))
+    assert (f8.values(c, s) == 0).all() or np.allclose(f8.values(c, s), 2.0 ** -140, atol=2.0 ** -136)
+
+
+def test_rotation_keeps_lengths_and_depends_on_distance_alone():
+    rng = np.random.default_rng(3)
+    q, k = rng.standard_normal((2, 1, 1, 32))
+    for mode in ("inter", "half"):
+        for freq in ("own", "shared"):
+            kw = dict(axis_dim=[12, 8, 8], theta=1e4, mode=mode, freq=freq)
+            turn = lambda x, at: f8.rope(x, np.array(at).reshape(3, 1), **kw)[0, 0]  # noqa: E731
+            a = turn(q, [5, 9, 100]) @ turn(k, [2, 3, 40])
+            b = turn(q, [1005, 59, 60]) @ turn(k, [1002, 53, 0])
+            assert abs(a - b) < 1e-10 and abs(turn(q, [5, 9, 100]) @ turn(q, [5, 9, 100]) - (q * q).sum()) < 1e-10
+            assert np.array_equal(turn(q, [7, 7, 7])[28:], q[0, 0, 28:])
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def refused(call, args):
+    rc = getattr(capi.lib(), "p0_" + call)(ctypes.byref(args))
+    return rc, capi.last_error()
+
+
+BIG = 1 << 24
+PACK = dict(x=P, type=1, N=256, K=256, w=P + BIG, s=P + 2 * BIG)
+NORM = dict(x=P, type=1, t=P + BIG, t_type=1, M=4, D=256, y=P + 2 * BIG, s=P + 3 * BIG)
+ROWS = dict(x=P, type=1, M=4, D=256, y=P + BIG, s=P + 2 * BIG)
+GEMM = dict(x=P, xs=P + BIG, w=P + 2 * BIG, ws=P + 3 * BIG, M=4, N=256, K=256, type=2, y=P + 4 * BIG)
+ROPE = dict(x=P, y=P + BIG, type=1, rows=4, hq=2, hk=1, dim=64, pos=P + 2 * BIG)
+
+
+@pytest.mark.parametrize("base,call,kw,msg", [
+    (PACK, "f8_pack", dict(type=3), "f8_pack: type 3"),
+    (PACK, "f8_pack", dict(K=0), "f8_pack: K 0"),
+    (PACK, "f8_pack", dict(N=-1), "f8_pack: N -1"),
+    (PACK, "f8_pack", dict(x=None), "f8_pack: missing x buffer"),
+    (PACK, "f8_pack", dict(x=P + 1), "f8_pack: x must be 2-byte aligned, its rows too"),
+    (PACK, "f8_pack", dict(w=P + BIG + 8), "f8_pack: w must be 16-byte aligned, its rows too"),
+    (PACK, "f8_pack", dict(ldw=264), "f8_pack: w must be 16-byte aligned, its rows too"),
+    (PACK, "f8_pack", dict(ldw=240), "f8_pack: w has rows of 256 B, 240 B apart"),
+    (PACK, "f8_pack", dict(ldx=255), "f8_pack: x has rows of 512 B, 510 B apart"),
+    (PACK, "f8_pack", dict(ldx=-256), "f8_pack: x has rows of 512 B, -2 B apart"),
+    (PACK, "f8_pack", dict(ldx=(1 << 62) + 256), "f8_pack: x has rows of 512 B, -2 B apart"),
+    (PACK, "f8_pack", dict(lds=1), "f8_pack: s has rows of 8 B, 4 B apart"),
+    (PACK, "f8_pack", dict(w=P + 256), "f8_pack: outputs overlap"),
+    (PACK, "f8_pack", dict(s=P + BIG + 16), "f8_pack: outputs overlap"),
+    (NORM, "f8_norm", dict(type=-1), "f8_norm: type -1, t_type 1"),
+    (NORM, "f8_norm", dict(t_type=9), "f8_norm: type 1, t_type 9"),
+    (NORM, "f8_norm", dict(mode=2), "f8_norm: mode 2"),
+    (NORM, "f8_norm", dict(D=32769), "f8_norm: D 32769 (1 .. 32768)"),
+    (NORM, "f8_norm", dict(M=1 << 31), "f8_norm: M 2147483648"),
+    (NORM, "f8_norm", dict(t=None, tw=P), "f8_norm: tw needs t"),
+    (NORM, "f8_norm", dict(w=P + 2), "f8_norm: tw, w and b must be 4-byte aligned"),
+    (NORM, "f8_norm", dict(y=None), "f8_norm: missing y buffer"),
+    (NORM, "f8_norm", dict(s=None), "f8_norm: missing s buffer"),
+    (NORM, "f8_norm", dict(lds=3), "f8_norm: s has rows of 16 B, 12 B apart"),
+    (NORM, "f8_norm", dict(x_out=P + BIG), "f8_norm: outputs overlap"),
+    (NORM, "f8_norm", dict(x_out=P, ldo=512), "f8_norm: outputs overlap"),
+    (NORM, "f8_norm", dict(x_out=P + 2), "f8_norm: outputs overlap"),
+    (NORM, "f8_norm", dict(y=P), "f8_norm: outputs overlap"),
+    (NORM, "f8_norm", dict(b=P + 3 * BIG), "f8_norm: outputs overlap"),
+    (ROWS, "f8_rows", dict(glu=3), "f8_rows: glu 3"),
+    (ROWS, "f8_rows", dict(D=0), "f8_rows: D 0"),
+    (ROWS, "f8_rows", dict(glu=1, up=-256), "f8_rows: up -256"),
+    (ROWS, "f8_rows", dict(glu=1, ldx=500), "f8_rows: x has rows of 1024 B, 1000 B apart"),
+    (ROWS, "f8_rows", dict(y=P + 16), "f8_rows: outputs overlap"),
+    (GEMM, "f8_gemm", dict(K=0), "f8_gemm: K 0 must be a multiple of 128"),
+    (GEMM, "f8_gemm", dict(K=192), "f8_gemm: K 192 must be a multiple of 128"),
+    (GEMM, "f8_gemm", dict(M=-1), "f8_gemm: M -1"),
+    (GEMM, "f8_gemm", dict(type=4), "f8_gemm: type 4"),
+    (GEMM, "f8_gemm", dict(ldx=1 << 23), "f8_gemm: rows 8388608 and 256 B apart"),
+    (GEMM, "f8_gemm", dict(ldw=264), "f8_gemm: w must be 16-byte aligned, its rows too"),
+    (GEMM, "f8_gemm", dict(ldws=1), "f8_gemm: ws has rows of 8 B, 4 B apart"),
+    (GEMM, "f8_gemm", dict(ldy=255), "f8_gemm: y has rows of 512 B, 510 B apart"),
+    (GEMM, "f8_gemm", dict(xs=None), "f8_gemm: missing xs buffer"),
+    (GEMM, "f8_gemm", dict(y=P + 2 * BIG + 64), "f8_gemm: y overlaps an input"),
+    (ROPE, "rope", dict(type=3), "rope: type 3"),
+    (ROPE, "rope", dict(mode=2), "rope: mode 2"),
+    (ROPE, "rope", dict(freq=2), "rope: freq 2"),
+    (ROPE, "rope", dict(dim=63), "rope: heads of 63 channels"),
+    (ROPE, "rope", dict(dim=514), "rope: heads of 514 channels"),
+    (ROPE, "rope", dict(hq=0, hk=0), "rope: 0 and 0 heads"),
+    (ROPE, "rope", dict(axes=5, axis_dim=[2]), "rope: 5 axes"),
+    (ROPE, "rope", dict(axis_dim=[32, 34]), "rope: axis 1 of 34 channels (heads of 64)"),
+    (ROPE, "rope", dict(axis_dim=[32, 15]), "rope: axis 1 of 15 channels (heads of 64)"),
+    (ROPE, "rope", dict(axis_dim=[32, 0]), "rope: axis 1 of 0 channels (heads of 64)"),
+    (ROPE, "rope", dict(theta=-1.0), "rope: theta -1"),
+    (ROPE, "rope", dict(ldh=62), "rope: heads 62 and 64 apart"),
+    (ROPE, "rope", dict(ldr=128), "rope: x has rows of 384 B, 256 B apart"),
+    (ROPE, "rope", dict(pos=None), "rope: missing pos buffer"),
+    (ROPE, "rope", dict(pos_ld=3, axis_dim=[32, 32]), "rope: pos has rows of 16 B, 12 B apart"),
+    (ROPE, "rope", dict(y=P + 64), "rope: y overlaps an input"),
+    (ROPE, "rope", dict(y=P, y_ldr=256), "rope: y overlaps an input"),
+    (ROPE, "rope", dict(y=P + 2 * BIG), "rope: y overlaps an input"),
+])
+def test_refusals(base, call, kw, msg):
+    make = getattr(capi, call + "_args")
+    rc, err = refused(call, make(**{**base, **kw}))
+    assert (rc, err) == (capi.P0_EINVAL, msg)
+
+
+def no_device():
+    d = capi.DeviceInfo()
+    if capi.lib().p0_device_info(ctypes.byref(d)) == capi.P0_OK:
+        pytest.skip("a device is open: these calls would run")
+
+
+@pytest.mark.parametrize("base,call", [(PACK, "f8_pack"), (NORM, "f8_norm"), (ROWS, "f8_rows"), (GEMM, "f8_gemm"), (ROPE, "rope")])
+def test_good_arguments_need_a_device(base, call):
+    """what passes every check gets as far as the missing device; no call takes a null pointer"""
+    no_device()
+    rc, err = refused(call, getattr(capi, call + "_args")(**base))
+    assert rc == capi.P0_ENODEV and err == call + ": no device (p0_open was not called)"
+    rows = "N" if call == "f8_pack" else "rows" if call == "rope" else "M"
+    rc, err = refused(call, getattr(capi, call + "_args")(**{**base, rows: 0}))
+    assert rc == capi.P0_ENODEV
+    assert getattr(capi.lib(), "p0_" + call)(None) == capi.P0_EINVAL and capi.last_error() == call + ": no arguments"
+
+
+def test_outputs_may_lie_in_the_gaps_of_inputs():
+    """a norm that writes beside the rows it reads, in the gaps of one stride; a rotation in place"""
+    no_device()
+    a = capi.f8_norm_args(x=P, type=0, ldx=512, M=4, D=128, x_out=P + 512, ldo=512, t=P + BIG, y=P + 2 * BIG, s=P + 3 * BIG)
+    assert refused("f8_norm", a)[0] == capi.P0_ENODEV
+    a = capi.rope_args(**{**ROPE, "y": P, "ldr": 320, "y_ldr": 320})
+    assert refused("rope", a)[0] == capi.P0_ENODEV
