@@ -54,6 +54,7 @@ int gemm_init();
 int misc_init();
 int kv_pages_init();
 int kv_attn_init();
+int f8_gemm_init();
 
 // `rows` rows of `width` 4-byte words, `ld` words apart, as arguments are checked. Rows of one stride may lie in each other's gaps;
 // of two strides the whole extents have to be apart

@@ -33,18 +33,19 @@ struct F8GemmP {
   int yvec;            // 4 consecutive outputs from a multiple of 4 on are aligned together
 };
 
+// a lane's 32 codes of a block: 16 bytes from two places
+__device__ __forceinline__ i32x8 codes32(const i32x4& lo, const i32x4& hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 
 // a lane's 32 codes of a block -> 32 fp16 values, exactly
-__device__ __forceinline__ void to_half(const uint4& c0, const uint4& c1, half8v (&h)[4]) {
-  const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+__device__ __forceinline__ void to_half(const i32x8& w, half8v (&h)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const half2v lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[2 * i + j], 1.0f, false);
-      const half2v hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w[2 * i + j], 1.0f, true);
+      const half2v lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[2 * i + j], 1.0f, false);
+      const half2v hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[2 * i + j], 1.0f, true);
       h[i][4 * j] = lo.x; h[i][4 * j + 1] = lo.y; h[i][4 * j + 2] = hi.x; h[i][4 * j + 3] = hi.y;
     }
 }
@@ -54,9 +55,7 @@ __device__ __forceinline__ f32x4 mfma_half(const half8v (&a)[4], const half8v (&
   for (int i = 0; i < 4; ++i) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[i], b[i], d, 0, 0, 0);
   return d;
 }
-__device__ __forceinline__ f32x4 mfma_block(const uint4& w0, const uint4& w1, const uint4& x0, const uint4& x1) {
-  const i32x8 a = {(int)w0.x, (int)w0.y, (int)w0.z, (int)w0.w, (int)w1.x, (int)w1.y, (int)w1.z, (int)w1.w};
-  const i32x8 b = {(int)x0.x, (int)x0.y, (int)x0.z, (int)x0.w, (int)x1.x, (int)x1.y, (int)x1.z, (int)x1.w};
+__device__ __forceinline__ f32x4 mfma_block(const i32x8& a, const i32x8& b) {
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, zero, 0, 0, 0, 0, 0, 0);   // e4m3 both, no block scales of its own
 }
@@ -99,23 +98,21 @@ __global__ __launch_bounds__(64 * kThinWaves) void f8_thin_kernel(const F8GemmP 
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int U = 4;
   for (int kb = wave; kb < p.blocks; kb += U * kThinWaves) {
-    uint4 a[U][2], b[U][2];
+    i32x8 a[U], b[U];
     float s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {   // past the last block: it again, times 0
       const int k = min(kb + u * kThinWaves, p.blocks - 1);
-      a[u][0] = *(const uint4*)(w + (int64_t)k * 128);
-      a[u][1] = *(const uint4*)(w + (int64_t)k * 128 + 64);
-      b[u][0] = *(const uint4*)(x + (int64_t)k * 128);
-      b[u][1] = *(const uint4*)(x + (int64_t)k * 128 + 64);
+      a[u] = codes32(*(const i32x4*)(w + (int64_t)k * 128), *(const i32x4*)(w + (int64_t)k * 128 + 64));
+      b[u] = codes32(*(const i32x4*)(x + (int64_t)k * 128), *(const i32x4*)(x + (int64_t)k * 128 + 64));
       s[u] = xs[k * p.ldxs] * ws[k];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (kb + u * kThinWaves >= p.blocks) break;
       half8v ah[4], bh[4];
-      to_half(a[u][0], a[u][1], ah);
-      to_half(b[u][0], b[u][1], bh);
+      to_half(a[u], ah);
+      to_half(b[u], bh);
       const f32x4 d = mfma_half(ah, bh);
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s[u], acc[i]);
@@ -129,6 +126,199 @@ __global__ __launch_bounds__(64 * kThinWaves) void f8_thin_kernel(const F8GemmP 
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] += part[k][lane][i];
   if (m0 + (lane & 15) < p.M) store4<TYPE>(p, m0 + (lane & 15), n0 + 4 * g, acc);
+}
+
+// Many rows: a workgroup takes BN outputs (weight rows) of BM activation rows, its WN x WM waves 16 AN x 16 AM of them each. A stage in LDS is
+// a block of k of every row: BN + BM rows of 128 codes and BM scales, S stages in all, filled by loads that go straight to LDS,
+// S - 1 steps ahead and dealt out over a step. The 16-byte chunk c of row r lies at position c ^ key(r): of 16 consecutive rows one chunk is in
+// 16 different (row parity, position) pairs, of 8 in 8 positions: no bank conflicts.
+// One barrier a step, ahead of the step's last matrix instructions: every wave then holds the rest of its step in registers, the
+// next step's first fragments are read while those run, and the stage just left is free for loads.
+__device__ __forceinline__ int f8_key(int r) { return (r ^ (r >> 3 & 1)) & 7; }
+
+template <int WN_, int WM_, int AN_, int AM_, int S_>
+struct F8Tile {
+  static constexpr int WN = WN_, WM = WM_, AN = AN_, AM = AM_, S = S_;
+  static constexpr int Waves = WN * WM, Threads = 64 * Waves, BN = 16 * AN * WN, BM = 16 * AM * WM;
+  static constexpr int Rows = BN + BM, Loads = Rows / 8 / Waves;   // loads of 8 rows, per wave
+  static constexpr int Codes = Rows * 128, Stage = Codes + 4 * (BM < 64 ? 64 : BM), Lds = S * Stage;
+  static_assert(Rows % (8 * Waves) == 0 && 128 % (16 * AN) == 0 && BM <= 64 * Waves, "tile");
+};
+
+struct F8TileP {
+  F8GemmP g;
+  int nbx, nby;   // tiles of N, of M
+};
+
+template <int TYPE, class T>
+__global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr bool Exact = TYPE == P0_F32;
+  const F8GemmP& p = a.g;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wv % T::WN, wm = wv / T::WN, l16 = lane & 15, g = lane >> 4;
+  // consecutive workgroups go to the 8 XCDs in turn: each XCD takes a contiguous run of tiles, which goes down a band of 4 row tiles, then
+  // on to the next column tile
+  constexpr int kBand = 4;
+  const int tiles = a.nbx * a.nby;
+  int t = blockIdx.x;
+  if (tiles % 8 == 0) t = (blockIdx.x % 8) * (tiles / 8) + blockIdx.x / 8;
+  const int per = a.nbx * kBand, band = t / per, brows = min(kBand, a.nby - band * kBand), in = t - band * per;
+  const int m0 = (band * kBand + in % brows) * T::BM, n0 = in / brows * T::BN;
+
+  const uint32_t lbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  const i32x4 rw = resource(p.w + (int64_t)n0 * p.ldw), rx = resource(p.x + (int64_t)m0 * p.ldx);
+  // load i of a wave fills rows (i Waves + wv) 8 .. + 7 of the stage: weights first; rows past the last are it again
+  int off[T::Loads];
+#pragma unroll
+  for (int i = 0; i < T::Loads; ++i) {
+    const int r = (i * T::Waves + wv) * 8 + (lane >> 3), c = ((lane & 7) ^ f8_key(r)) * 16;
+    const bool isw = (i * T::Waves + wv) * 8 < T::BN;
+    off[i] = isw ? min(r, p.N - 1 - n0) * (int)p.ldw + c : min(r - T::BN, p.M - 1 - m0) * (int)p.ldx + c;
+  }
+  const int soff = min(tid % T::BM, p.M - 1 - m0) * 4;   // scales: wave wv takes those of rows 64 wv on (mod BM)
+  // block kb into the stage at LDS offset `st`; past the last block it is that again, never read: every step's loads count alike
+  const int nk = p.blocks;
+  auto load = [&](int kb, int st, int i) {
+    const bool isw = (i * T::Waves + wv) * 8 < T::BN;
+    dma16(lbase + st + (i * T::Waves + wv) * 1024, off[i], isw ? rw : rx, min(kb, nk - 1) * 128);
+  };
+  auto load_scales = [&](int kb, int st) {
+    dma4(lbase + st + T::Codes + (wv * 64 % T::BM) * 4, soff, resource(p.xs + m0 + (int64_t)min(kb, nk - 1) * p.ldxs), 0);
+  };
+
+  f32x4 acc[T::AN][T::AM];
+#pragma unroll
+  for (int i = 0; i < T::AN; ++i)
+#pragma unroll
+    for (int j = 0; j < T::AM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // fragments: row 16 i + l16 of the wave's, chunks g and g + 4
+  const int chunk = (g ^ f8_key(l16)) << 4, wrow = (wn * 16 * T::AN + l16) * 128, xrow = (T::BN + wm * 16 * T::AM + l16) * 128;
+  const int w0 = wrow + chunk, w1 = wrow + (chunk ^ 64), x0 = xrow + chunk, x1 = xrow + (chunk ^ 64);
+  const int srow = T::Codes + (wm * 16 * T::AM + l16) * 4;
+  // the weight's scales of this wave's rows: 64 steps' in a lane each
+  const float* ws = p.ws + (int64_t)(min(n0 + wn * 16 * T::AN, p.N - 1) >> 7) * p.ldws;
+  float wsv = 0.0f;
+
+  i32x8 wf[2], xf[T::AM];
+  half8v xh[Exact ? T::AM : 1][4], wh[4];
+  float sf[T::AM], s[T::AM];   // the activations' scales as read, times the weight's
+  f32x4 d[4];                  // the last blocks' sums, on their way into acc
+  auto read_w = [&](const uint8_t* st, int i) { wf[i & 1] = codes32(*(const i32x4*)(st + w0 + i * 2048), *(const i32x4*)(st + w1 + i * 2048)); };
+  auto read_x = [&](const uint8_t* st, int j) {
+    xf[j] = codes32(*(const i32x4*)(st + x0 + j * 2048), *(const i32x4*)(st + x1 + j * 2048));
+    sf[j] = *(const float*)(st + srow + j * 64);
+  };
+#pragma unroll
+  for (int q = 0; q < 4; ++q) d[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < T::AM; ++j) s[j] = 0.0f;
+
+  // A step is AN AM cells of one block product each: its matrix instruction, and the fmas of the product two cells before, which is done
+  // by then. The next weight fragment is read an AM ahead; the next step's first ones follow the barrier in the last AM cells.
+  constexpr int Q = T::AN * T::AM, Each = (T::Loads + T::AN - 2) / (T::AN - 1);
+  static_assert(T::AM == 4 && T::AN % 2 == 0, "cells");
+  auto fold = [&](int q) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[q / T::AM][q % T::AM][e] = __builtin_fmaf(d[q & 3][e], s[q % T::AM], acc[q / T::AM][q % T::AM][e]);
+  };
+  auto step = [&](int kb, const uint8_t* st, const uint8_t* st_next, int st_load) {
+    if ((kb & 63) == 0) {
+      wsv = ws[min(kb + lane, nk - 1)];
+      asm volatile("" : "+v"(wsv));   // waited for here: no other step has a wait of its own for it
+    }
+    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wsv), kb & 63));
+    if constexpr (Exact) {
+#pragma unroll
+      for (int j = 0; j < T::AM; ++j) to_half(xf[j], xh[j]);
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int i = q / T::AM, j = q % T::AM;
+      if (q == Q - T::AM) {
+        // this wave's loads of the next stage have come (those of later ones need not have), and its reads of this one
+        wait_dma<(T::S - 2) * (T::Loads + 1)>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read_w(st_next, 0);
+      }
+      if constexpr (Exact) {
+        if (j == 0) to_half(wf[i & 1], wh);
+        d[q & 3] = mfma_half(wh, xh[j]);
+      } else {
+        d[q & 3] = mfma_block(wf[i & 1], xf[j]);
+      }
+      if (i == T::AN - 1) {
+        read_x(st_next, j);
+      } else {
+        if (j == 0) read_w(st, i + 1);
+        if (j == 1 && i * Each < T::Loads) load(kb + T::S - 1, st_load, i * Each);
+        if (j == 2 && Each > 1 && i * Each + 1 < T::Loads) load(kb + T::S - 1, st_load, i * Each + 1);
+        if (j == 3 && Each > 2 && i * Each + 2 < T::Loads) load(kb + T::S - 1, st_load, i * Each + 2);
+        if (j == 3 && i == 0) load_scales(kb + T::S - 1, st_load);
+      }
+      fold((q + Q - 2) % Q);
+      if (q == 1) {
+#pragma unroll
+        for (int k = 0; k < T::AM; ++k) s[k] = sf[k] * w;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  static_assert(Each <= 3, "loads dealt out over a step");
+#pragma unroll
+  for (int kb = 0; kb < T::S - 1; ++kb) {
+#pragma unroll
+    for (int l = 0; l < T::Loads; ++l) load(kb, kb * T::Stage, l);
+    load_scales(kb, kb * T::Stage);
+  }
+  wait_dma<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < T::AM; ++j) read_x(lds, j);
+  read_w(lds, 0);
+  int at = 0, to = (T::S - 1) * T::Stage;
+  for (int kb = 0; kb < nk; ++kb) {
+    const int next = at + T::Stage == T::Lds ? 0 : at + T::Stage;
+    step(kb, lds + at, lds + next, to);
+    to = at;
+    at = next;
+  }
+  fold(Q - 2);
+  fold(Q - 1);
+  wait_dma<0>();   // loads that nothing reads must not land in another workgroup's LDS
+
+#pragma unroll
+  for (int j = 0; j < T::AM; ++j) {
+    const int m = m0 + (wm * T::AM + j) * 16 + l16;
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int i = 0; i < T::AN; ++i) {
+      const int n = n0 + (wn * T::AN + i) * 16 + 4 * g;
+      if (n < p.N) store4<TYPE>(p, m, n, acc[i][j]);
+    }
+  }
+}
+
+using TileBig = F8Tile<2, 4, 8, 4, 2>;     // 256 x 256, 8 waves of 128 x 64
+using TileHalf = F8Tile<2, 2, 4, 4, 4>;    // 128 x 128, 4 waves of 64 x 64
+
+template <class T> static void f8_tile_launch(const F8GemmP& g, int type, hipStream_t s) {
+  F8TileP a{g, (g.N + T::BN - 1) / T::BN, (g.M + T::BM - 1) / T::BM};
+  auto k = type == P0_F32 ? f8_tile_kernel<P0_F32, T> : type == P0_F16 ? f8_tile_kernel<P0_F16, T> : f8_tile_kernel<P0_BF16, T>;
+  hipLaunchKernelGGL(k, dim3((unsigned)(a.nbx * a.nby)), dim3(T::Threads), T::Lds, s, a);
+}
+template <class T> static int f8_tile_init() {
+  const void* k[] = {(const void*)f8_tile_kernel<P0_F32, T>, (const void*)f8_tile_kernel<P0_F16, T>, (const void*)f8_tile_kernel<P0_BF16, T>};
+  for (const void* f : k) P0_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, T::Lds), "p0_open: f8_gemm");
+  return P0_OK;
+}
+int f8_gemm_init() {
+  if (int r = f8_tile_init<TileBig>()) return r;
+  return f8_tile_init<TileHalf>();
 }
 
 static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
@@ -157,8 +347,15 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   if (int r = refuse_in_chain(op)) return r;
   if (int r = require_open(op)) return r;
   F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks};
-  p.nt = (int)((N + 15) / 16);
   p.yvec = ((uintptr_t)a->y | (uintptr_t)(ldy * size)) % (4 * size) == 0;
+  if (M > 16) {
+    const int64_t big = (N + 255) / 256 * ((M + 255) / 256);
+    if (big >= 192 && a->type != P0_F32) f8_tile_launch<TileBig>(p, a->type, ctx().cur);
+    else f8_tile_launch<TileHalf>(p, a->type, ctx().cur);
+    P0_LAUNCHED(op);
+    return P0_OK;
+  }
+  p.nt = (int)((N + 15) / 16);
   auto k = a->type == P0_F32 ? f8_thin_kernel<P0_F32> : a->type == P0_F16 ? f8_thin_kernel<P0_F16> : f8_thin_kernel<P0_BF16>;
   hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(64 * kThinWaves), 0, ctx().cur, p);
   P0_LAUNCHED(op);

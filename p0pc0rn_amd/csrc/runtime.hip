@@ -140,6 +140,7 @@ int p0_open(int device) {
   if (int r = misc_init()) return r;
   if (int r = kv_pages_init()) return r;
   if (int r = kv_attn_init()) return r;
+  if (int r = f8_gemm_init()) return r;
   c.part_floats = kPartBytes / sizeof(float);
   c.n_counters = kCounters;
   c.gemm_counters = c.counters + kCounters;
