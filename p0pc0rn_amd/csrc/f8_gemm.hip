@@ -84,10 +84,9 @@ template <int TYPE> __device__ __forceinline__ void store4(const F8GemmP& p, int
 }
 
 // Few rows: a workgroup takes 16 outputs of 16 rows, its waves the blocks of k in turn; their sums meet in LDS.
-constexpr int kThinWaves = 4;
-template <int TYPE>
-__global__ __launch_bounds__(64 * kThinWaves) void f8_thin_kernel(const F8GemmP p) {
-  __shared__ f32x4 part[kThinWaves][64];
+template <int TYPE, int W>
+__global__ __launch_bounds__(64 * W) void f8_thin_kernel(const F8GemmP p) {
+  __shared__ f32x4 part[W][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
   const int mt = blockIdx.x / (unsigned)p.nt, n0 = (blockIdx.x - mt * p.nt) * 16, m0 = mt * 16;
   const int n = min(n0 + (lane & 15), p.N - 1), m = min(m0 + (lane & 15), p.M - 1);   // rows past the last: it again
@@ -97,19 +96,18 @@ __global__ __launch_bounds__(64 * kThinWaves) void f8_thin_kernel(const F8GemmP 
   const float* xs = p.xs + m;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int U = 4;
-  for (int kb = wave; kb < p.blocks; kb += U * kThinWaves) {
+  for (int kb = wave; kb < p.blocks; kb += U * W) {
     i32x8 a[U], b[U];
     float s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {   // past the last block: it again, times 0
-      const int k = min(kb + u * kThinWaves, p.blocks - 1);
+      const int k = min(kb + u * W, p.blocks - 1);
       a[u] = codes32(*(const i32x4*)(w + (int64_t)k * 128), *(const i32x4*)(w + (int64_t)k * 128 + 64));
       b[u] = codes32(*(const i32x4*)(x + (int64_t)k * 128), *(const i32x4*)(x + (int64_t)k * 128 + 64));
-      s[u] = xs[k * p.ldxs] * ws[k];
+      s[u] = kb + u * W < p.blocks ? xs[k * p.ldxs] * ws[k] : 0.0f;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (kb + u * kThinWaves >= p.blocks) break;
       half8v ah[4], bh[4];
       to_half(a[u], ah);
       to_half(b[u], bh);
@@ -122,9 +120,7 @@ __global__ __launch_bounds__(64 * kThinWaves) void f8_thin_kernel(const F8GemmP 
   __syncthreads();
   if (wave) return;
 #pragma unroll
-  for (int k = 1; k < kThinWaves; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += part[k][lane][i];
+  for (int k = 1; k < W; ++k) acc += part[k][lane];
   if (m0 + (lane & 15) < p.M) store4<TYPE>(p, m0 + (lane & 15), n0 + 4 * g, acc);
 }
 
@@ -148,11 +144,15 @@ struct F8Tile {
 struct F8TileP {
   F8GemmP g;
   int nbx, nby;   // tiles of N, of M
+  int nks, spk;   // slices of K, blocks of one
+  float* part;    // the slices' sums: [tile][slice][wave][cell][lane]
+  unsigned* cnt;
 };
 
 template <int TYPE, class T>
 __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ int s_last;
   constexpr bool Exact = TYPE == P0_F32;
   const F8GemmP& p = a.g;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -160,11 +160,13 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   // consecutive workgroups go to the 8 XCDs in turn: each XCD takes a contiguous run of tiles, which goes down a band of 4 row tiles, then
   // on to the next column tile
   constexpr int kBand = 4;
-  const int tiles = a.nbx * a.nby;
+  const int groups = a.nbx * a.nby * a.nks;
   int t = blockIdx.x;
-  if (tiles % 8 == 0) t = (blockIdx.x % 8) * (tiles / 8) + blockIdx.x / 8;
-  const int per = a.nbx * kBand, band = t / per, brows = min(kBand, a.nby - band * kBand), in = t - band * per;
-  const int m0 = (band * kBand + in % brows) * T::BM, n0 = in / brows * T::BN;
+  if (groups % 8 == 0) t = (blockIdx.x % 8) * (groups / 8) + blockIdx.x / 8;
+  const int per = a.nbx * a.nks * kBand, band = t / per, brows = min(kBand, a.nby - band * kBand), in = t - band * per;
+  const int mb = band * kBand + in % brows, cs = in / brows, ks = cs % a.nks, nb = cs / a.nks;
+  const int m0 = mb * T::BM, n0 = nb * T::BN;
+  const int kb0 = ks * a.spk, nk = min(p.blocks, kb0 + a.spk);
 
   const uint32_t lbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   const i32x4 rw = resource(p.w + (int64_t)n0 * p.ldw), rx = resource(p.x + (int64_t)m0 * p.ldx);
@@ -178,7 +180,6 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   }
   const int soff = min(tid % T::BM, p.M - 1 - m0) * 4;   // scales: wave wv takes those of rows 64 wv on (mod BM)
   // block kb into the stage at LDS offset `st`; past the last block it is that again, never read: every step's loads count alike
-  const int nk = p.blocks;
   auto load = [&](int kb, int st, int i) {
     const bool isw = (i * T::Waves + wv) * 8 < T::BN;
     dma16(lbase + st + (i * T::Waves + wv) * 1024, off[i], isw ? rw : rx, min(kb, nk - 1) * 128);
@@ -217,18 +218,18 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
 
   // A step is AN AM cells of one block product each: its matrix instruction, and the fmas of the product two cells before, which is done
   // by then. The next weight fragment is read an AM ahead; the next step's first ones follow the barrier in the last AM cells.
-  constexpr int Q = T::AN * T::AM, Each = (T::Loads + T::AN - 2) / (T::AN - 1);
+  constexpr int Q = T::AN * T::AM, Each = (T::Loads + Q - T::AM - 2) / (Q - T::AM - 1);   // loads a cell before the barrier; the last: scales
   static_assert(T::AM == 4 && T::AN % 2 == 0, "cells");
   auto fold = [&](int q) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[q / T::AM][q % T::AM][e] = __builtin_fmaf(d[q & 3][e], s[q % T::AM], acc[q / T::AM][q % T::AM][e]);
   };
   auto step = [&](int kb, const uint8_t* st, const uint8_t* st_next, int st_load) {
-    if ((kb & 63) == 0) {
+    if (((kb - kb0) & 63) == 0) {
       wsv = ws[min(kb + lane, nk - 1)];
       asm volatile("" : "+v"(wsv));   // waited for here: no other step has a wait of its own for it
     }
-    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wsv), kb & 63));
+    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wsv), (kb - kb0) & 63));
     if constexpr (Exact) {
 #pragma unroll
       for (int j = 0; j < T::AM; ++j) to_half(xf[j], xh[j]);
@@ -254,10 +255,9 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
         read_x(st_next, j);
       } else {
         if (j == 0) read_w(st, i + 1);
-        if (j == 1 && i * Each < T::Loads) load(kb + T::S - 1, st_load, i * Each);
-        if (j == 2 && Each > 1 && i * Each + 1 < T::Loads) load(kb + T::S - 1, st_load, i * Each + 1);
-        if (j == 3 && Each > 2 && i * Each + 2 < T::Loads) load(kb + T::S - 1, st_load, i * Each + 2);
-        if (j == 3 && i == 0) load_scales(kb + T::S - 1, st_load);
+#pragma unroll
+        for (int l = q * Each; l < (q + 1) * Each && l < T::Loads; ++l) load(kb + T::S - 1, st_load, l);
+        if (q == Q - T::AM - 1) load_scales(kb + T::S - 1, st_load);
       }
       fold((q + Q - 2) % Q);
       if (q == 1) {
@@ -267,12 +267,11 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  static_assert(Each <= 3, "loads dealt out over a step");
 #pragma unroll
   for (int kb = 0; kb < T::S - 1; ++kb) {
 #pragma unroll
-    for (int l = 0; l < T::Loads; ++l) load(kb, kb * T::Stage, l);
-    load_scales(kb, kb * T::Stage);
+    for (int l = 0; l < T::Loads; ++l) load(kb0 + kb, kb * T::Stage, l);
+    load_scales(kb0 + kb, kb * T::Stage);
   }
   wait_dma<0>();
   __builtin_amdgcn_s_barrier();
@@ -281,7 +280,7 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   for (int j = 0; j < T::AM; ++j) read_x(lds, j);
   read_w(lds, 0);
   int at = 0, to = (T::S - 1) * T::Stage;
-  for (int kb = 0; kb < nk; ++kb) {
+  for (int kb = kb0; kb < nk; ++kb) {
     const int next = at + T::Stage == T::Lds ? 0 : at + T::Stage;
     step(kb, lds + at, lds + next, to);
     to = at;
@@ -290,6 +289,57 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   fold(Q - 2);
   fold(Q - 1);
   wait_dma<0>();   // loads that nothing reads must not land in another workgroup's LDS
+
+  if (a.nks > 1) {
+    // The slices' sums meet in the workspace: it is uncached, a store is in memory once acknowledged and device-scope loads read memory,
+    // so the arrival count needs no fence. The last workgroup to arrive adds the slices in order and leaves the count at zero.
+    typedef unsigned long long u64;
+    const int64_t tile = (int64_t)nb * a.nby + mb, slice = (int64_t)T::BM * T::BN / 2;   // in pairs of values
+    u64* mine = (u64*)a.part + (tile * a.nks + ks) * slice + wv * (Q * 128) + lane;
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4& v = acc[q / T::AM][q % T::AM];
+        __hip_atomic_store(mine + (q * 2 + h) * 64, (u64)__float_as_uint(v[2 * h]) | (u64)__float_as_uint(v[2 * h + 1]) << 32, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+      }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+      const unsigned prev = __hip_atomic_fetch_add(a.cnt + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int last_in = prev == (unsigned)(a.nks - 1);
+      if (last_in) __hip_atomic_exchange(a.cnt + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last = last_in;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    const u64* all = (const u64*)a.part + tile * a.nks * slice + wv * (Q * 128) + lane;
+    constexpr int QB = 8;   // cells whose words are on their way together
+#pragma unroll
+    for (int q0 = 0; q0 < Q; q0 += QB) {
+      f32x4 v[QB];
+#pragma unroll
+      for (int q = 0; q < QB; ++q) v[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int k = 0; k < a.nks; ++k) {
+        u64 w[QB][2];
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            w[q][h] = __hip_atomic_load(all + k * slice + ((q0 + q) * 2 + h) * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            v[q][2 * h] += __uint_as_float((uint32_t)w[q][h]);
+            v[q][2 * h + 1] += __uint_as_float((uint32_t)(w[q][h] >> 32));
+          }
+      }
+#pragma unroll
+      for (int q = 0; q < QB; ++q) acc[(q0 + q) / T::AM][(q0 + q) % T::AM] = v[q];
+    }
+  }
 
 #pragma unroll
   for (int j = 0; j < T::AM; ++j) {
@@ -305,11 +355,29 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
 
 using TileBig = F8Tile<2, 4, 8, 4, 2>;     // 256 x 256, 8 waves of 128 x 64
 using TileHalf = F8Tile<2, 2, 4, 4, 4>;    // 128 x 128, 4 waves of 64 x 64
+using TileLow = F8Tile<4, 1, 2, 4, 6>;     // 128 outputs of 64 rows, 4 waves of 32 x 64
 
-template <class T> static void f8_tile_launch(const F8GemmP& g, int type, hipStream_t s) {
+template <int W> static void f8_thin_launch(const F8GemmP& p, int type, int64_t tiles, hipStream_t s) {
+  auto k = type == P0_F32 ? f8_thin_kernel<P0_F32, W> : type == P0_F16 ? f8_thin_kernel<P0_F16, W> : f8_thin_kernel<P0_BF16, W>;
+  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(64 * W), 0, s, p);
+}
+template <class T> static int64_t f8_tiles(const F8GemmP& g) { return ((int64_t)g.N + T::BN - 1) / T::BN * (((int64_t)g.M + T::BM - 1) / T::BM); }
+// slices of K: as many as leave a workgroup per CU, each of at least `least` blocks, partials within the workspace
+template <class T> static int f8_slices(const F8GemmP& g, int least) {
+  const int64_t tiles = f8_tiles<T>(g);
+  int64_t n = tiles >= 256 ? 1 : 256 / tiles;
+  if (n > g.blocks / least) n = g.blocks / least;
+  while (n > 1 && (size_t)tiles * n * T::BM * T::BN > ctx().part_floats) --n;
+  return n < 1 ? 1 : (int)n;
+}
+template <class T> static void f8_tile_launch(const F8GemmP& g, int type, int nks, hipStream_t s) {
   F8TileP a{g, (g.N + T::BN - 1) / T::BN, (g.M + T::BM - 1) / T::BM};
+  a.spk = (g.blocks + nks - 1) / nks;
+  a.nks = (g.blocks + a.spk - 1) / a.spk;
+  a.part = ctx().part;
+  a.cnt = ctx().kv_counters;   // one per tile where there are slices: at most 128 tiles
   auto k = type == P0_F32 ? f8_tile_kernel<P0_F32, T> : type == P0_F16 ? f8_tile_kernel<P0_F16, T> : f8_tile_kernel<P0_BF16, T>;
-  hipLaunchKernelGGL(k, dim3((unsigned)(a.nbx * a.nby)), dim3(T::Threads), T::Lds, s, a);
+  hipLaunchKernelGGL(k, dim3((unsigned)(a.nbx * a.nby * a.nks)), dim3(T::Threads), T::Lds, s, a);
 }
 template <class T> static int f8_tile_init() {
   const void* k[] = {(const void*)f8_tile_kernel<P0_F32, T>, (const void*)f8_tile_kernel<P0_F16, T>, (const void*)f8_tile_kernel<P0_BF16, T>};
@@ -318,6 +386,7 @@ template <class T> static int f8_tile_init() {
 }
 int f8_gemm_init() {
   if (int r = f8_tile_init<TileBig>()) return r;
+  if (int r = f8_tile_init<TileLow>()) return r;
   return f8_tile_init<TileHalf>();
 }
 
@@ -349,15 +418,19 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks};
   p.yvec = ((uintptr_t)a->y | (uintptr_t)(ldy * size)) % (4 * size) == 0;
   if (M > 16) {
-    const int64_t big = (N + 255) / 256 * ((M + 255) / 256);
-    if (big >= 192 && a->type != P0_F32) f8_tile_launch<TileBig>(p, a->type, ctx().cur);
-    else f8_tile_launch<TileHalf>(p, a->type, ctx().cur);
+    const int force = getenv("F8T") ? atoi(getenv("F8T")) : 0, fs = getenv("F8S") ? atoi(getenv("F8S")) : 0;
+    const int kind = force ? force : f8_tiles<TileBig>(p) >= 192 ? 1 : M > 64 ? 2 : 3;
+    if (kind == 1) f8_tile_launch<TileBig>(p, a->type, fs ? fs : f8_slices<TileBig>(p, 8), ctx().cur);
+    else if (kind == 2) f8_tile_launch<TileHalf>(p, a->type, fs ? fs : f8_slices<TileHalf>(p, 8), ctx().cur);
+    else f8_tile_launch<TileLow>(p, a->type, fs ? fs : f8_slices<TileLow>(p, 8), ctx().cur);
     P0_LAUNCHED(op);
     return P0_OK;
   }
   p.nt = (int)((N + 15) / 16);
-  auto k = a->type == P0_F32 ? f8_thin_kernel<P0_F32> : a->type == P0_F16 ? f8_thin_kernel<P0_F16> : f8_thin_kernel<P0_BF16>;
-  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(64 * kThinWaves), 0, ctx().cur, p);
+  // four blocks a wave at once
+  if (blocks <= 16) f8_thin_launch<4>(p, a->type, tiles, ctx().cur);
+  else if (blocks <= 32) f8_thin_launch<8>(p, a->type, tiles, ctx().cur);
+  else f8_thin_launch<16>(p, a->type, tiles, ctx().cur);
   P0_LAUNCHED(op);
   return P0_OK;
 }

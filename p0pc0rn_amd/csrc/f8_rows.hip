@@ -109,7 +109,7 @@ struct NormP {
   float* s;
   int64_t ldx, ldt, ldo, ldy, lds;
   int64_t M;
-  int D, xvec, tvec, mode, one;
+  int D, mode, one;
   float scale, eps;
 };
 __device__ __forceinline__ float sum64(float v) {
@@ -121,7 +121,8 @@ __device__ __forceinline__ float sum64(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 // W waves take a row (W = 1: a workgroup has four rows), a lane 8 channels of NC steps of 512 W. The row stays in registers.
-template <int XT, int TT, int W, int NC>
+// VEC: every run of 8 channels is there whole or not at all, and 16-byte aligned everywhere.
+template <int XT, int TT, int W, int NC, bool VEC>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void f8_norm_kernel(const NormP p) {
   __shared__ float red[3][W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -139,19 +140,26 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void f8_norm_kernel(const No
     }
     return v;
   };
+  auto count = [&](int c) { return VEC ? 8 : p.D - c < 8 ? p.D - c : 8; };   // of the 8 channels from c < D on
+  auto fill = [&](float (&v)[8], float x) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = x;
+  };
   float f[NC][8];
   const float over = 1.0f / (float)p.D;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int c = c0 + i * 512 * W, n = p.D - c < 8 ? (p.D - c < 0 ? 0 : p.D - c) : 8;
-    f8_load8<XT>(p.x, m * p.ldx + c, p.xvec && n == 8, n, f[i]);
+    const int c = c0 + i * 512 * W;
+    fill(f[i], 0.0f);
+    if (c < p.D) f8_load8<XT>(p.x, m * p.ldx + c, VEC, count(c), f[i]);
   }
   if (p.t) {
     float t[NC][8], ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = c0 + i * 512 * W, n = p.D - c < 8 ? (p.D - c < 0 ? 0 : p.D - c) : 8;
-      f8_load8<TT>(p.t, m * p.ldt + c, p.tvec && n == 8, n, t[i]);
+      const int c = c0 + i * 512 * W;
+      fill(t[i], 0.0f);
+      if (c < p.D) f8_load8<TT>(p.t, m * p.ldt + c, VEC, count(c), t[i]);
     }
     if (p.tw) {
 #pragma unroll
@@ -160,12 +168,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void f8_norm_kernel(const No
         for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(t[i][j], t[i][j], ss);
       const float r = 1.0f / sqrtf(total(ss, 0) * over + p.eps);
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
+      for (int i = 0; i < NC; ++i) {
+        const int c = c0 + i * 512 * W;
+        if (c >= p.D) continue;
+        float g[8];
+        f8_load8<P0_F32>(p.tw, c, VEC, count(c), g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = c0 + i * 512 * W + j;
-          t[i][j] *= r * (c < p.D ? p.tw[c] : 0.0f);
-        }
+        for (int j = 0; j < 8; ++j) t[i][j] *= r * g[j];
+      }
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -180,28 +190,33 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void f8_norm_kernel(const No
       f[i][j] = f8_rounded<XT>(f[i][j] * p.scale);
       sum += f[i][j];
     }
-    const int c = c0 + i * 512 * W, n = p.D - c < 8 ? (p.D - c < 0 ? 0 : p.D - c) : 8;
-    if (p.xo && n > 0) f8_store8<XT>(p.xo, m * p.ldo + c, p.xvec && n == 8, n, f[i]);
+    const int c = c0 + i * 512 * W;
+    if (p.xo && c < p.D) f8_store8<XT>(p.xo, m * p.ldo + c, VEC, count(c), f[i]);
   }
-  float mean = 0.0f;
-  if (p.mode == 0) mean = total(sum, 1) * over;
+  const float mean = p.mode == 0 ? total(sum, 1) * over : 0.0f;
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
+  for (int i = 0; i < NC; ++i) {
+    const int c = c0 + i * 512 * W;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      f[i][j] = c0 + i * 512 * W + j < p.D ? f[i][j] - mean : 0.0f;
+      f[i][j] = (VEC ? c : c + j) < p.D ? f[i][j] - mean : 0.0f;
       sq = __builtin_fmaf(f[i][j], f[i][j], sq);
     }
+  }
   const float rstd = 1.0f / sqrtf(total(sq, 2) * over + p.eps);
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = c0 + i * 512 * W;
     if (c >= (p.D + 127) / 128 * 128) break;   // whole blocks of lanes
+    if (c < p.D) {
+      float g[8], b[8];
+      if (p.w) f8_load8<P0_F32>(p.w, c, VEC, count(c), g);
+      else fill(g, p.one ? 0.0f : 1.0f);
+      if (p.b) f8_load8<P0_F32>(p.b, c, VEC, count(c), b);
+      else fill(b, 0.0f);
+      const float one = p.one ? 1.0f : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (c + j >= p.D) continue;
-      const float g = (p.w ? p.w[c + j] : p.one ? 0.0f : 1.0f) + (p.one ? 1.0f : 0.0f);
-      f[i][j] = f[i][j] * rstd * g + (p.b ? p.b[c + j] : 0.0f);
+      for (int j = 0; j < 8; ++j) f[i][j] = VEC || c + j < p.D ? f[i][j] * rstd * (g[j] + one) + b[j] : 0.0f;
     }
     const float s = f8_scale(f8_max16(f8_most(f[i])));
     *(uint2*)(p.y + m * p.ldy + c) = f8_codes(f[i], 1.0f / s);
@@ -286,10 +301,11 @@ static int rows_f8_call(const p0_f8_rows_args_t* a) {
 }
 
 typedef void (*NormKernel)(NormP);
-template <int XT, int TT> static NormKernel norm_kernel(int W, int NC) {
-  if (W == 1) return NC == 1 ? f8_norm_kernel<XT, TT, 1, 1> : NC == 2 ? f8_norm_kernel<XT, TT, 1, 2> : f8_norm_kernel<XT, TT, 1, 5>;
-  if (W == 4) return NC == 1 ? f8_norm_kernel<XT, TT, 4, 1> : NC == 2 ? f8_norm_kernel<XT, TT, 4, 2> : f8_norm_kernel<XT, TT, 4, 4>;
-  return NC == 2 ? f8_norm_kernel<XT, TT, 16, 2> : f8_norm_kernel<XT, TT, 16, 4>;
+template <int XT, int TT> static NormKernel norm_kernel(bool vec, int W, int steps) {
+  if (!vec) return W == 4 ? f8_norm_kernel<XT, TT, 4, 4, false> : f8_norm_kernel<XT, TT, 16, 4, false>;
+  if (W == 1) return steps == 1 ? f8_norm_kernel<XT, TT, 1, 1, true> : steps == 2 ? f8_norm_kernel<XT, TT, 1, 2, true> : f8_norm_kernel<XT, TT, 1, 5, true>;
+  if (W == 4) return steps == 1 ? f8_norm_kernel<XT, TT, 4, 1, true> : steps == 2 ? f8_norm_kernel<XT, TT, 4, 2, true> : f8_norm_kernel<XT, TT, 4, 4, true>;
+  return steps <= 2 ? f8_norm_kernel<XT, TT, 16, 2, true> : f8_norm_kernel<XT, TT, 16, 4, true>;
 }
 
 static int norm_call(const p0_f8_norm_args_t* a) {
@@ -324,14 +340,13 @@ static int norm_call(const p0_f8_norm_args_t* a) {
   NormP p{};
   p.x = a->x; p.t = a->t; p.xo = xo; p.tw = a->tw; p.w = a->w; p.b = a->b; p.y = (uint8_t*)a->y; p.s = a->s;
   p.ldx = ldx; p.ldt = ldt; p.ldo = ldo; p.ldy = ldy; p.lds = lds; p.M = M; p.D = (int)D;
-  p.xvec = ((uintptr_t)a->x | (uintptr_t)(ldx * xsize) | (uintptr_t)xo | (uintptr_t)(ldo * xsize)) % 16 == 0;
-  p.tvec = ((uintptr_t)a->t | (uintptr_t)(ldt * tsize)) % 16 == 0;
+  const bool vec = D % 8 == 0 && ((uintptr_t)a->x | (uintptr_t)(ldx * xsize) | (uintptr_t)xo | (uintptr_t)(ldo * xsize) | (uintptr_t)a->t |
+                                  (uintptr_t)(ldt * tsize) | (uintptr_t)a->tw | (uintptr_t)a->w | (uintptr_t)a->b) % 16 == 0;
   p.mode = a->mode; p.one = a->w_one ? 1 : 0; p.scale = scale; p.eps = a->eps != 0.0f ? a->eps : 1e-6f;
-  const int W = D <= 2560 && M >= 256 ? 1 : D <= 8192 ? 4 : 16, steps = (int)((K8 + 512 * W - 1) / (512 * W));
-  const int NC = W == 1 ? (steps <= 2 ? steps : 5) : W == 4 ? (steps <= 2 ? steps : 4) : (steps <= 2 ? 2 : 4);
+  const int W = vec && D <= 2560 && M >= 256 ? 1 : D <= 8192 ? 4 : 16, steps = (int)((K8 + 512 * W - 1) / (512 * W));
   const int tt = a->t ? a->t_type : a->type;
   NormKernel k = nullptr;
-#define P0_NORM(XT, TT) if (a->type == XT && tt == TT) k = norm_kernel<XT, TT>(W, NC)
+#define P0_NORM(XT, TT) if (a->type == XT && tt == TT) k = norm_kernel<XT, TT>(vec, W, steps)
   P0_NORM(P0_F32, P0_F32); P0_NORM(P0_F32, P0_F16); P0_NORM(P0_F32, P0_BF16);
   P0_NORM(P0_F16, P0_F32); P0_NORM(P0_F16, P0_F16); P0_NORM(P0_F16, P0_BF16);
   P0_NORM(P0_BF16, P0_F32); P0_NORM(P0_BF16, P0_F16); P0_NORM(P0_BF16, P0_BF16);
