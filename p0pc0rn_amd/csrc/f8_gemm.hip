@@ -30,7 +30,7 @@ struct F8GemmP {
   int64_t ldx, ldxs, ldw, ldws, ldy;
   int M, N, blocks;    // blocks of 128 k
   int nt;              // tiles of N
-  int yvec;            // 4 consecutive outputs from a multiple of 4 on are aligned together
+  int yvec;            // 1: 4 consecutive outputs from a multiple of 4 on are aligned together; 2: rows are 16-byte aligned
 };
 
 // a lane's 32 codes of a block: 16 bytes from two places
@@ -83,54 +83,115 @@ template <int TYPE> __device__ __forceinline__ void store4(const F8GemmP& p, int
   }
 }
 
-// Few rows: a workgroup takes 16 outputs of 16 rows, its waves the blocks of k in turn; their sums meet in LDS.
-template <int TYPE, int W>
+// Few rows: a workgroup takes 16 NT outputs of 16 MT rows, its W waves the blocks of k in turn, U at a time; their sums meet in LDS.
+template <int TYPE, int W, int U, int MT, int NT>
 __global__ __launch_bounds__(64 * W) void f8_thin_kernel(const F8GemmP p) {
-  __shared__ f32x4 part[W][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-  const int mt = blockIdx.x / (unsigned)p.nt, n0 = (blockIdx.x - mt * p.nt) * 16, m0 = mt * 16;
-  const int n = min(n0 + (lane & 15), p.N - 1), m = min(m0 + (lane & 15), p.M - 1);   // rows past the last: it again
-  const uint8_t* w = p.w + n * p.ldw + g * 16;
-  const uint8_t* x = p.x + m * p.ldx + g * 16;
+  __shared__ f32x4 part[W][MT * NT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+  const int mt = blockIdx.x / (unsigned)p.nt, n0 = (blockIdx.x - mt * p.nt) * 16 * NT, m0 = mt * 16 * MT;
+  const uint8_t* w[NT];
+  const uint8_t* x[MT];
+  const float* xs[MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) w[i] = p.w + min(n0 + 16 * i + l16, p.N - 1) * p.ldw + g * 16;   // rows past the last: it again
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int m = min(m0 + 16 * j + l16, p.M - 1);
+    x[j] = p.x + m * p.ldx + g * 16;
+    xs[j] = p.xs + m;
+  }
   const float* ws = p.ws + (int64_t)(n0 >> 7) * p.ldws;
-  const float* xs = p.xs + m;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int U = 4;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   for (int kb = wave; kb < p.blocks; kb += U * W) {
-    i32x8 a[U], b[U];
-    float s[U];
+    i32x8 a[U][NT], b[U][MT];
+    float s[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {   // past the last block: it again, times 0
       const int k = min(kb + u * W, p.blocks - 1);
-      a[u] = codes32(*(const i32x4*)(w + (int64_t)k * 128), *(const i32x4*)(w + (int64_t)k * 128 + 64));
-      b[u] = codes32(*(const i32x4*)(x + (int64_t)k * 128), *(const i32x4*)(x + (int64_t)k * 128 + 64));
-      s[u] = kb + u * W < p.blocks ? xs[k * p.ldxs] * ws[k] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) a[u][i] = codes32(*(const i32x4*)(w[i] + (int64_t)k * 128), *(const i32x4*)(w[i] + (int64_t)k * 128 + 64));
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        b[u][j] = codes32(*(const i32x4*)(x[j] + (int64_t)k * 128), *(const i32x4*)(x[j] + (int64_t)k * 128 + 64));
+        s[u][j] = kb + u * W < p.blocks ? xs[j][k * p.ldxs] * ws[k] : 0.0f;
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      half8v ah[4], bh[4];
-      to_half(a[u], ah);
-      to_half(b[u], bh);
-      const f32x4 d = mfma_half(ah, bh);
+      half8v ah[NT][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(d[i], s[u], acc[i]);
+      for (int i = 0; i < NT; ++i) to_half(a[u][i], ah[i]);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        half8v bh[4];
+        to_half(b[u][j], bh);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const f32x4 d = mfma_half(ah[i], bh);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][i][e] = __builtin_fmaf(d[e], s[u][j], acc[j][i][e]);
+        }
+      }
     }
   }
-  part[wave][lane] = acc;
-  __syncthreads();
-  if (wave) return;
 #pragma unroll
-  for (int k = 1; k < W; ++k) acc += part[k][lane];
-  if (m0 + (lane & 15) < p.M) store4<TYPE>(p, m0 + (lane & 15), n0 + 4 * g, acc);
+  for (int j = 0; j < MT; ++j)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) part[wave][j * NT + i][lane] = acc[j][i];
+  __syncthreads();
+  for (int c = wave; c < MT * NT; c += W) {
+    f32x4 v = part[0][c][lane];
+#pragma unroll
+    for (int k = 1; k < W; ++k) v += part[k][c][lane];
+    const int m = m0 + c / NT * 16 + l16, n = n0 + c % NT * 16 + 4 * g;
+    if (m < p.M && n < p.N) store4<TYPE>(p, m, n, v);
+  }
+}
+
+// The sums of a wave's 16 AM rows from row m on, of 16 AN outputs from output n on
+template <int TYPE, int AM, int AN>
+__device__ __forceinline__ void tile_out(const F8GemmP& p, const f32x4 (&acc)[AM][AN], int m, int n, int lane) {
+  const int l16 = lane & 15, g = lane >> 4;
+  const bool whole = m + 16 * AM <= p.M && n + 16 * AN <= p.N && p.yvec > 1;
+#pragma unroll
+  for (int j = 0; j < AM; ++j) {
+    const int mr = m + 16 * j + l16;
+    if (whole && TYPE != P0_F32) {
+      // two cells' outputs change places between neighbouring groups of 16 lanes: 8 consecutive ones a lane, 64 bytes a row and store
+#pragma unroll
+      for (int i = 0; i < AN; i += 2) {
+        uint32_t a[2], b[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const auto x = __builtin_amdgcn_permlane16_swap(f8_half<TYPE>(acc[j][i][2 * h]) | f8_half<TYPE>(acc[j][i][2 * h + 1]) << 16,
+                                                          f8_half<TYPE>(acc[j][i + 1][2 * h]) | f8_half<TYPE>(acc[j][i + 1][2 * h + 1]) << 16, false, false);
+          a[h] = x[0];
+          b[h] = x[1];
+        }
+        *(uint4*)((uint16_t*)p.y + (int64_t)mr * p.ldy + n + 16 * (i + (g & 1)) + 8 * (g >> 1)) = uint4{a[0], a[1], b[0], b[1]};
+      }
+    } else if (mr < p.M) {
+#pragma unroll
+      for (int i = 0; i < AN; ++i)
+        if (n + 16 * i + 4 * g < p.N) store4<TYPE>(p, mr, n + 16 * i + 4 * g, acc[j][i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);   // one row of cells at a time: the registers of more are not there
+  }
 }
 
 // Many rows: a workgroup takes BN outputs (weight rows) of BM activation rows, its WN x WM waves 16 AN x 16 AM of them each. A stage in LDS is
 // a block of k of every row: BN + BM rows of 128 codes and BM scales, S stages in all, filled by loads that go straight to LDS,
-// S - 1 steps ahead and dealt out over a step. The 16-byte chunk c of row r lies at position c ^ key(r): of 16 consecutive rows one chunk is in
-// 16 different (row parity, position) pairs, of 8 in 8 positions: no bank conflicts.
+// S - 1 steps ahead and dealt out over a step. The 16-byte chunk c of row r lies at position c ^ key(r): a fragment's read takes chunk g
+// (and g ^ 4) of rows 0 .. 15 for the lane groups g = 0 .. 3, and LDS serves lanes 0-3, 12-15 of one group with 4-11 of the next; under key = r & 6 those
+// 16 lie in 16 different (row parity, position) pairs, so no bank conflicts (the counter reads 0; a key that suits 16 lanes of one
+// group each, (r ^ r / 8) & 7, read 48%).
 // One barrier a step, ahead of the step's last matrix instructions: every wave then holds the rest of its step in registers, the
 // next step's first fragments are read while those run, and the stage just left is free for loads.
-__device__ __forceinline__ int f8_key(int r) { return (r ^ (r >> 3 & 1)) & 7; }
+__device__ __forceinline__ int f8_key(int r) { return r & 6; }
 
 template <int WN_, int WM_, int AN_, int AM_, int S_>
 struct F8Tile {
@@ -188,11 +249,11 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
     dma4(lbase + st + T::Codes + (wv * 64 % T::BM) * 4, soff, resource(p.xs + m0 + (int64_t)min(kb, nk - 1) * p.ldxs), 0);
   };
 
-  f32x4 acc[T::AN][T::AM];
+  f32x4 acc[T::AM][T::AN];
 #pragma unroll
-  for (int i = 0; i < T::AN; ++i)
+  for (int j = 0; j < T::AM; ++j)
 #pragma unroll
-    for (int j = 0; j < T::AM; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < T::AN; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   // fragments: row 16 i + l16 of the wave's, chunks g and g + 4
   const int chunk = (g ^ f8_key(l16)) << 4, wrow = (wn * 16 * T::AN + l16) * 128, xrow = (T::BN + wm * 16 * T::AM + l16) * 128;
@@ -219,10 +280,12 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   // A step is AN AM cells of one block product each: its matrix instruction, and the fmas of the product two cells before, which is done
   // by then. The next weight fragment is read an AM ahead; the next step's first ones follow the barrier in the last AM cells.
   constexpr int Q = T::AN * T::AM, Each = (T::Loads + Q - T::AM - 2) / (Q - T::AM - 1);   // loads a cell before the barrier; the last: scales
-  static_assert(T::AM == 4 && T::AN % 2 == 0, "cells");
+  static_assert((T::AM == 2 || T::AM == 4) && T::AN % 2 == 0, "cells");
   auto fold = [&](int q) {
+    f32x4& v = acc[q % T::AM][q / T::AM];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[q / T::AM][q % T::AM][e] = __builtin_fmaf(d[q & 3][e], s[q % T::AM], acc[q / T::AM][q % T::AM][e]);
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(d[q & 3][e], s[q % T::AM], v[e]);
+    asm volatile("" : "+v"(v));   // here and below: keeps the cell's order
   };
   auto step = [&](int kb, const uint8_t* st, const uint8_t* st_next, int st_load) {
     if (((kb - kb0) & 63) == 0) {
@@ -251,6 +314,7 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
       } else {
         d[q & 3] = mfma_block(wf[i & 1], xf[j]);
       }
+      asm volatile("" : "+v"(d[q & 3]));
       if (i == T::AN - 1) {
         read_x(st_next, j);
       } else {
@@ -300,7 +364,7 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
     for (int q = 0; q < Q; ++q)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const f32x4& v = acc[q / T::AM][q % T::AM];
+        const f32x4& v = acc[q % T::AM][q / T::AM];
         __hip_atomic_store(mine + (q * 2 + h) * 64, (u64)__float_as_uint(v[2 * h]) | (u64)__float_as_uint(v[2 * h + 1]) << 32, __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
       }
@@ -315,7 +379,7 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
     __syncthreads();
     if (!s_last) return;
     const u64* all = (const u64*)a.part + tile * a.nks * slice + wv * (Q * 128) + lane;
-    constexpr int QB = 8;   // cells whose words are on their way together
+    constexpr int QB = Q < 8 ? Q : 8;   // cells whose words are on their way together
 #pragma unroll
     for (int q0 = 0; q0 < Q; q0 += QB) {
       f32x4 v[QB];
@@ -337,45 +401,183 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
           }
       }
 #pragma unroll
-      for (int q = 0; q < QB; ++q) acc[(q0 + q) / T::AM][(q0 + q) % T::AM] = v[q];
+      for (int q = 0; q < QB; ++q) acc[(q0 + q) % T::AM][(q0 + q) / T::AM] = v[q];
     }
   }
 
+  tile_out<TYPE, T::AM, T::AN>(p, acc, m0 + wm * 16 * T::AM, n0 + wn * 16 * T::AN, lane);
+}
+
+// Many rows of many outputs: tiles of 256 outputs by 32 SX rows on one workgroup per CU, 8 waves of 64 outputs by 16 SX rows, the tiles of a
+// workgroup one after the other in one unbroken run of steps: the next tile's first block is on its way while the last one's last block is
+// multiplied, and its sums leave from registers.
+template <int SX_>
+struct Wide {
+  static constexpr int SX = SX_, WN = 4, WM = 2, AN = 4, Waves = 8, Threads = 512, BN = 256, BM = 32 * SX;
+  static constexpr int Loads = (BN + BM + 63) / 64, Codes = (BN + BM) * 128, Stage = Codes + BM * 4, Lds = 2 * Stage, Q = AN * SX;
+};
+struct F8WideP {
+  F8GemmP g;
+  int nbx, nby;      // tiles of N, of M
+};
+
+template <int TYPE, class T>
+__global__ __launch_bounds__(T::Threads, 2) void f8_wide_kernel(const F8WideP a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const F8GemmP& p = a.g;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wv % T::WN, wm = wv / T::WN, l16 = lane & 15, g = lane >> 4, nk = p.blocks;
+  // consecutive workgroups go to the 8 XCDs in turn: each XCD takes neighbours in the order of tiles, which goes down a band of 4 row
+  // tiles, then on to the next column tile: what an XCD works on at one time is 4 x 8 tiles
+  const int G = gridDim.x, tiles = a.nbx * a.nby;
+  const int xcd = blockIdx.x % 8, cu = blockIdx.x / 8, rounds = tiles / G, rest = tiles - rounds * G;
+  // tile of round r, or -1: a last round that is not full is spread over the XCDs too
+  auto tile_of = [&](int r) {
+    if (G % 8) return r * G + (int)blockIdx.x < tiles ? r * G + (int)blockIdx.x : -1;
+    if (r < rounds) return r * G + xcd * (G / 8) + cu;
+    const int first = rest * xcd / 8;
+    return r == rounds && first + cu < rest * (xcd + 1) / 8 ? r * G + first + cu : -1;
+  };
+  constexpr int kBand = 4;
+  const int per = a.nbx * kBand;
+
+  // ---- loads: a wave's load i fills rows (8 i + wv) 8 .. + 7 of a stage, weights first; rows past the last are it again
+  const uint32_t lbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  i32x4 rw, rx;
+  const int sbase = min((wv & 3) * 64, T::BM - 64);   // the 64 scales that a wave loads
+  int off[T::Loads], soff, m0 = 0, n0 = 0, lk = 0;    // where loads are aimed
+  auto aim = [&](int t) {
+    const int band = t / per, rows = min(kBand, a.nby - band * kBand), in = t - band * per;
+    m0 = (band * kBand + in % rows) * T::BM;
+    n0 = in / rows * T::BN;
+    rw = resource(p.w + (int64_t)n0 * p.ldw);
+    rx = resource(p.x + (int64_t)m0 * p.ldx);
 #pragma unroll
-  for (int j = 0; j < T::AM; ++j) {
-    const int m = m0 + (wm * T::AM + j) * 16 + l16;
-    if (m >= p.M) continue;
-#pragma unroll
-    for (int i = 0; i < T::AN; ++i) {
-      const int n = n0 + (wn * T::AN + i) * 16 + 4 * g;
-      if (n < p.N) store4<TYPE>(p, m, n, acc[i][j]);
+    for (int i = 0; i < T::Loads; ++i) {
+      const int r = (i * T::Waves + wv) * 8 + (lane >> 3), c = ((lane & 7) ^ f8_key(r)) * 16;
+      off[i] = i < 4 ? min(r, p.N - 1 - n0) * (int)p.ldw + c : min(r - T::BN, p.M - 1 - m0) * (int)p.ldx + c;
     }
+    soff = min(sbase + lane, p.M - 1 - m0) * 4;
+    lk = 0;
+  };
+  // the last load of BM = 224, 160 has work for half the waves: the others repeat the one before
+  constexpr int Rows = (T::BN + T::BM) / 8;
+  auto load = [&](int st, int i) {
+    const bool spare = (i + 1) * T::Waves > Rows && i * T::Waves + wv >= Rows;
+    dma16(lbase + st + ((spare ? i - 1 : i) * T::Waves + wv) * 1024, spare ? off[i - (i > 0)] : off[i], i < 4 ? rw : rx, lk * 128);
+  };
+  auto load_scales = [&](int st) {
+    dma4(lbase + st + T::Codes + sbase * 4, soff, resource(p.xs + m0 + (int64_t)lk * p.ldxs), 0);
+  };
+
+  f32x4 acc[T::SX][T::AN];
+  const int chunk = (g ^ f8_key(l16)) << 4, wrow = (wn * 16 * T::AN + l16) * 128, xrow = (T::BN + wm * 16 * T::SX + l16) * 128;
+  const int w0 = wrow + chunk, w1 = wrow + (chunk ^ 64), x0 = xrow + chunk, x1 = xrow + (chunk ^ 64);
+  const int srow = T::Codes + (wm * 16 * T::SX + l16) * 4;
+  float wsv = 0.0f, s = 0.0f, sf[3];
+  i32x8 wf[T::AN], xf[3];
+  f32x4 d[4];   // the last cells' products, on their way into acc
+  // the activations' fragments take turns; an odd number's last has a place of its own
+  constexpr auto turn = [](int j) { return (T::SX & 1) && j == T::SX - 1 ? 2 : j & 1; };
+  auto read_w = [&](const uint8_t* st, int i) { wf[i] = codes32(*(const i32x4*)(st + w0 + i * 2048), *(const i32x4*)(st + w1 + i * 2048)); };
+  auto read_x = [&](const uint8_t* st, int j) {
+    xf[turn(j)] = codes32(*(const i32x4*)(st + x0 + j * 2048), *(const i32x4*)(st + x1 + j * 2048));
+    sf[turn(j)] = *(const float*)(st + srow + j * 64);
+  };
+  auto fold = [&](int q) {
+    f32x4& v = acc[q / T::AN][q % T::AN];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(d[q & 3][e], s, v[e]);
+    asm volatile("" : "+v"(v));   // here and below: keeps the cell's order
+  };
+  // A step is a block of k: SX rows of 4 cells, a cell one block product: its matrix instruction, and the fmas of the product two cells
+  // before, which is done by then. One barrier, ahead of the last row: every wave then holds the rest of its step in registers.
+  auto step = [&](const uint8_t* st, const uint8_t* st_next, int st_load, float wk) {
+#pragma unroll
+    for (int q = 0; q < T::Q; ++q) {
+      const int j = q / T::AN, i = q % T::AN;
+      if (q == T::Q - T::AN) {
+        wait_dma<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read_x(st_next, 0);
+      }
+      d[q & 3] = mfma_block(wf[i], xf[turn(j)]);
+      asm volatile("" : "+v"(d[q & 3]));
+      if (j == T::SX - 1) {
+        read_w(st_next, i);
+      } else {
+        if (i == 0) read_x(st, j + 1);
+        if (q < T::Loads) load(st_load, q);
+        if (q == T::Loads) load_scales(st_load);
+      }
+      fold((q + T::Q - 2) % T::Q);
+      if (i == 1) s = sf[turn(j)] * wk;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  int tile = tile_of(0);
+  if (tile < 0) return;   // whole workgroups
+  aim(tile);
+#pragma unroll
+  for (int i = 0; i < T::Loads; ++i) load(0, i);
+  load_scales(0);
+  wait_dma<0>();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < T::AN; ++i) read_w(lds, i);
+  read_x(lds, 0);
+  int at = 0, to = T::Stage;
+  for (int round = 0; tile >= 0;) {
+    const int m = m0 + wm * 16 * T::SX, n = n0 + wn * 16 * T::AN;
+    tile = tile_of(++round);
+    const float* ws = p.ws + (int64_t)(min(n, p.N - 1) >> 7) * p.ldws;   // of this wave's outputs: 64 steps' in a lane each
+#pragma unroll
+    for (int j = 0; j < T::SX; ++j)
+#pragma unroll
+      for (int i = 0; i < T::AN; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) d[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    s = 0.0f;
+    for (int kb = 0; kb < nk; ++kb) {
+      if ((kb & 63) == 0) {
+        wsv = ws[min(kb + lane, nk - 1)];
+        asm volatile("" : "+v"(wsv));   // waited for here: no other step has a wait of its own for it
+      }
+      if (kb + 1 < nk) ++lk;
+      else if (tile >= 0) aim(tile);   // else: the last block again, never read
+      step(lds + at, lds + to, to, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wsv), kb & 63)));
+      const int x = at;
+      at = to;
+      to = x;
+    }
+    fold(T::Q - 2);
+    fold(T::Q - 1);
+    tile_out<TYPE, T::SX, T::AN>(p, acc, m, n, lane);
   }
+  wait_dma<0>();   // loads that nothing reads must not land in another workgroup's LDS
 }
 
-using TileBig = F8Tile<2, 4, 8, 4, 2>;     // 256 x 256, 8 waves of 128 x 64
-using TileHalf = F8Tile<2, 2, 4, 4, 4>;    // 128 x 128, 4 waves of 64 x 64
-using TileLow = F8Tile<4, 1, 2, 4, 6>;     // 128 outputs of 64 rows, 4 waves of 32 x 64
+using TileSmall = F8Tile<2, 2, 2, 2, 9>;   // 64 outputs of 64 rows, 4 waves of 32 x 32
+using TileLow = F8Tile<4, 1, 2, 4, 6>;     // 128 of 64, 4 waves of 32 x 64
+using TileHalf = F8Tile<2, 4, 4, 2, 4>;    // 128 of 128, 8 waves of 64 x 32
+using TileLong = F8Tile<2, 4, 4, 4, 3>;    // 128 of 256, 8 waves of 64 x 64
+using TileWide = Wide<8>;
 
-template <int W> static void f8_thin_launch(const F8GemmP& p, int type, int64_t tiles, hipStream_t s) {
-  auto k = type == P0_F32 ? f8_thin_kernel<P0_F32, W> : type == P0_F16 ? f8_thin_kernel<P0_F16, W> : f8_thin_kernel<P0_BF16, W>;
-  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(64 * W), 0, s, p);
-}
-template <class T> static int64_t f8_tiles(const F8GemmP& g) { return ((int64_t)g.N + T::BN - 1) / T::BN * (((int64_t)g.M + T::BM - 1) / T::BM); }
-// slices of K: as many as leave a workgroup per CU, each of at least `least` blocks, partials within the workspace
-template <class T> static int f8_slices(const F8GemmP& g, int least) {
-  const int64_t tiles = f8_tiles<T>(g);
-  int64_t n = tiles >= 256 ? 1 : 256 / tiles;
-  if (n > g.blocks / least) n = g.blocks / least;
-  while (n > 1 && (size_t)tiles * n * T::BM * T::BN > ctx().part_floats) --n;
-  return n < 1 ? 1 : (int)n;
+template <int W, int U, int MT, int NT> static void f8_thin_launch(F8GemmP p, int type, hipStream_t s) {
+  p.nt = (p.N + 16 * NT - 1) / (16 * NT);
+  auto k = type == P0_F32 ? f8_thin_kernel<P0_F32, W, U, MT, NT> : type == P0_F16 ? f8_thin_kernel<P0_F16, W, U, MT, NT> : f8_thin_kernel<P0_BF16, W, U, MT, NT>;
+  hipLaunchKernelGGL(k, dim3((unsigned)(p.nt * ((p.M + 16 * MT - 1) / (16 * MT)))), dim3(64 * W), 0, s, p);
 }
 template <class T> static void f8_tile_launch(const F8GemmP& g, int type, int nks, hipStream_t s) {
   F8TileP a{g, (g.N + T::BN - 1) / T::BN, (g.M + T::BM - 1) / T::BM};
   a.spk = (g.blocks + nks - 1) / nks;
   a.nks = (g.blocks + a.spk - 1) / a.spk;
   a.part = ctx().part;
-  a.cnt = ctx().kv_counters;   // one per tile where there are slices: at most 128 tiles
+  a.cnt = ctx().kv_counters;   // one per tile where there are slices: at most half as many as CUs
   auto k = type == P0_F32 ? f8_tile_kernel<P0_F32, T> : type == P0_F16 ? f8_tile_kernel<P0_F16, T> : f8_tile_kernel<P0_BF16, T>;
   hipLaunchKernelGGL(k, dim3((unsigned)(a.nbx * a.nby * a.nks)), dim3(T::Threads), T::Lds, s, a);
 }
@@ -384,10 +586,59 @@ template <class T> static int f8_tile_init() {
   for (const void* f : k) P0_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, T::Lds), "p0_open: f8_gemm");
   return P0_OK;
 }
+template <class T> static void f8_wide_launch(const F8GemmP& g, int type, hipStream_t s) {
+  F8WideP a{g, (g.N + T::BN - 1) / T::BN, (g.M + T::BM - 1) / T::BM};
+  const int64_t tiles = (int64_t)a.nbx * a.nby, cus = ctx().cu_count;
+  auto k = type == P0_F16 ? f8_wide_kernel<P0_F16, T> : f8_wide_kernel<P0_BF16, T>;
+  hipLaunchKernelGGL(k, dim3((unsigned)(tiles < cus ? tiles : cus)), dim3(T::Threads), T::Lds, s, a);
+}
 int f8_gemm_init() {
-  if (int r = f8_tile_init<TileBig>()) return r;
+  if (int r = f8_tile_init<TileSmall>()) return r;
   if (int r = f8_tile_init<TileLow>()) return r;
-  return f8_tile_init<TileHalf>();
+  if (int r = f8_tile_init<TileHalf>()) return r;
+  if (int r = f8_tile_init<TileLong>()) return r;
+  for (const void* k : {(const void*)f8_wide_kernel<P0_F16, TileWide>, (const void*)f8_wide_kernel<P0_BF16, TileWide>})
+    P0_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, TileWide::Lds), "p0_open: f8_gemm");
+  return P0_OK;
+}
+
+// Which tile, and how many slices of K, by time: a round of workgroups takes its blocks of k, one after the other, and then its outputs; a
+// slice's sums go through memory. The figures (us a block and a round) are fitted to 67 shapes of 17 to 2048 rows, 512 to 16384 outputs, 16 to 72
+// blocks, each tile and slicing measured on its own: the fastest by them is on average within 1% of the fastest measured, 13%
+// at the worst (2048 rows, 2048 outputs, 64 blocks: 43.8 for 38.6). Measured (us; 16-bit results, small / low / half / long / wide):
+// 64 rows, 16384 x 2048: 11.0 / 12.9 / 14.1 / 20 / 30; 256 rows 34 / 23 / 16.1 / 22 / 38; 1021 rows - / 88 / 57 / 44 / 38.7.
+struct F8Shape {
+  int bn, bm;
+  float block, round;       // 16-bit results
+  float block32, round32;   // fp32 results: half the matrix rate, conversions
+};
+constexpr F8Shape kF8Shapes[] = {{64, 64, 0.32f, 2.4f, 0.51f, 3.6f},       // TileSmall
+                                 {128, 64, 0.47f, 2.2f, 0.72f, 4.5f},      // TileLow
+                                 {128, 128, 0.61f, 2.4f, 0.94f, 7.1f},     // TileHalf
+                                 {128, 256, 1.01f, 3.3f, 1.54f, 9.8f},     // TileLong
+                                 {256, 256, 1.73f, 8.0f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
+static void f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
+  const bool f32 = type == P0_F32;
+  const int cus = ctx().cu_count;
+  float least = 0.0f;
+  int kind = -1, nks = 1;
+  for (int k = 0; k < (f32 ? 4 : 5); ++k) {
+    const F8Shape& c = kF8Shapes[k];
+    const int64_t tiles = ((int64_t)p.N + c.bn - 1) / c.bn * (((int64_t)p.M + c.bm - 1) / c.bm);
+    for (int n = 1; n <= 16; n *= 2) {
+      if (n > 1 && (k == 4 || p.blocks / n < 4 || tiles * n > cus || (size_t)tiles * n * c.bn * c.bm > ctx().part_floats)) break;
+      const int64_t groups = tiles * n, rounds = (groups + cus - 1) / cus;
+      const float fill = groups < cus ? (float)groups / cus : 1.0f, alone = f32 ? 0.8f : 0.67f;   // a chip that is not full runs a little faster
+      const float t = rounds * ((p.blocks + n - 1) / n * (f32 ? c.block32 : c.block) * (alone + (1.0f - alone) * fill) + (f32 ? c.round32 : c.round)) +
+                      (n > 1 ? 1.5f + 0.265f * n * (c.bn * c.bm / 4096) : 0.0f);
+      if (kind < 0 || t < least) { least = t; kind = k; nks = n; }
+    }
+  }
+  if (kind == 0) f8_tile_launch<TileSmall>(p, type, nks, s);
+  else if (kind == 1) f8_tile_launch<TileLow>(p, type, nks, s);
+  else if (kind == 2) f8_tile_launch<TileHalf>(p, type, nks, s);
+  else if (kind == 3) f8_tile_launch<TileLong>(p, type, nks, s);
+  else f8_wide_launch<TileWide>(p, type, s);
 }
 
 static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
@@ -416,21 +667,16 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   if (int r = refuse_in_chain(op)) return r;
   if (int r = require_open(op)) return r;
   F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks};
-  p.yvec = ((uintptr_t)a->y | (uintptr_t)(ldy * size)) % (4 * size) == 0;
-  if (M > 16) {
-    const int force = getenv("F8T") ? atoi(getenv("F8T")) : 0, fs = getenv("F8S") ? atoi(getenv("F8S")) : 0;
-    const int kind = force ? force : f8_tiles<TileBig>(p) >= 192 ? 1 : M > 64 ? 2 : 3;
-    if (kind == 1) f8_tile_launch<TileBig>(p, a->type, fs ? fs : f8_slices<TileBig>(p, 8), ctx().cur);
-    else if (kind == 2) f8_tile_launch<TileHalf>(p, a->type, fs ? fs : f8_slices<TileHalf>(p, 8), ctx().cur);
-    else f8_tile_launch<TileLow>(p, a->type, fs ? fs : f8_slices<TileLow>(p, 8), ctx().cur);
-    P0_LAUNCHED(op);
-    return P0_OK;
+  const uintptr_t ya = (uintptr_t)a->y | (uintptr_t)(ldy * size);
+  p.yvec = ya % 16 == 0 ? 2 : ya % (4 * size) == 0;
+  if (M <= 16) {
+    // the blocks of k in turns over the waves, one block a wave and turn: 4 waves while that is at most 4 turns, more for longer k.
+    // Enough outputs for two workgroups a CU, and rows that are worth it: 32 outputs a workgroup, which halves its reads of the rows
+    if (N >= 16384 && M > 8) f8_thin_launch<4, 1, 1, 2>(p, a->type, ctx().cur);
+    else f8_thin_launch<8, 1, 1, 1>(p, a->type, ctx().cur);
+  } else {
+    f8_tile_choice(p, a->type, ctx().cur);
   }
-  p.nt = (int)((N + 15) / 16);
-  // four blocks a wave at once
-  if (blocks <= 16) f8_thin_launch<4>(p, a->type, tiles, ctx().cur);
-  else if (blocks <= 32) f8_thin_launch<8>(p, a->type, tiles, ctx().cur);
-  else f8_thin_launch<16>(p, a->type, tiles, ctx().cur);
   P0_LAUNCHED(op);
   return P0_OK;
 }
