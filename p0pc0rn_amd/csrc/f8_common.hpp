@@ -125,7 +125,17 @@ __device__ __forceinline__ float f8_most(const float (&f)[8]) {
   }
   return most;
 }
-__device__ __forceinline__ float f8_scale(float most) { return fmaxf(most / 448.0f, 0x1p-126f); }
+// max(most / 448, 2^-126) and 1 / s, each rounded to nearest: a reciprocal within a unit, and one correction that makes it and a quotient right
+// to the last bit (every mantissa tried; quotients below 2^-126 do not count). The divisions in full are 25 instructions of some 100 for 8 values
+__device__ __forceinline__ float f8_scale(float most) {
+  constexpr float c = 1.0f / 448.0f;
+  const float q = most * c;
+  return fmaxf(__builtin_fmaf(__builtin_fmaf(-448.0f, q, most), c, q), 0x1p-126f);
+}
+__device__ __forceinline__ float f8_inverse(float s) {
+  const float r = __builtin_amdgcn_rcpf(s);
+  return __builtin_fmaf(__builtin_fmaf(-s, r, 1.0f), r, r);
+}
 // x * inv rounded to e4m3, ties to the even code; |x * inv| of a finite x is below 448.001 and so never past the largest
 __device__ __forceinline__ uint2 f8_codes(const float (&f)[8], float inv) {
   uint32_t w[2];

@@ -312,7 +312,9 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
         if (j == 0) to_half(wf[i & 1], wh);
         d[q & 3] = mfma_half(wh, xh[j]);
       } else {
+        __builtin_amdgcn_s_setprio(1);   // ahead of the other wave's fmas: 2% of the widest tile's time
         d[q & 3] = mfma_block(wf[i & 1], xf[j]);
+        __builtin_amdgcn_s_setprio(0);
       }
       asm volatile("" : "+v"(d[q & 3]));
       if (i == T::AN - 1) {
@@ -408,169 +410,20 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   tile_out<TYPE, T::AM, T::AN>(p, acc, m0 + wm * 16 * T::AM, n0 + wn * 16 * T::AN, lane);
 }
 
-// Many rows of many outputs: tiles of 256 outputs by 32 SX rows on one workgroup per CU, 8 waves of 64 outputs by 16 SX rows, the tiles of a
-// workgroup one after the other in one unbroken run of steps: the next tile's first block is on its way while the last one's last block is
-// multiplied, and its sums leave from registers.
-template <int SX_>
-struct Wide {
-  static constexpr int SX = SX_, WN = 4, WM = 2, AN = 4, Waves = 8, Threads = 512, BN = 256, BM = 32 * SX;
-  static constexpr int Loads = (BN + BM + 63) / 64, Codes = (BN + BM) * 128, Stage = Codes + BM * 4, Lds = 2 * Stage, Q = AN * SX;
-};
-struct F8WideP {
-  F8GemmP g;
-  int nbx, nby;      // tiles of N, of M
-};
-
-template <int TYPE, class T>
-__global__ __launch_bounds__(T::Threads, 2) void f8_wide_kernel(const F8WideP a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const F8GemmP& p = a.g;
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = wv % T::WN, wm = wv / T::WN, l16 = lane & 15, g = lane >> 4, nk = p.blocks;
-  // consecutive workgroups go to the 8 XCDs in turn: each XCD takes neighbours in the order of tiles, which goes down a band of 4 row
-  // tiles, then on to the next column tile: what an XCD works on at one time is 4 x 8 tiles
-  const int G = gridDim.x, tiles = a.nbx * a.nby;
-  const int xcd = blockIdx.x % 8, cu = blockIdx.x / 8, rounds = tiles / G, rest = tiles - rounds * G;
-  // tile of round r, or -1: a last round that is not full is spread over the XCDs too
-  auto tile_of = [&](int r) {
-    if (G % 8) return r * G + (int)blockIdx.x < tiles ? r * G + (int)blockIdx.x : -1;
-    if (r < rounds) return r * G + xcd * (G / 8) + cu;
-    const int first = rest * xcd / 8;
-    return r == rounds && first + cu < rest * (xcd + 1) / 8 ? r * G + first + cu : -1;
-  };
-  constexpr int kBand = 4;
-  const int per = a.nbx * kBand;
-
-  // ---- loads: a wave's load i fills rows (8 i + wv) 8 .. + 7 of a stage, weights first; rows past the last are it again
-  const uint32_t lbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  i32x4 rw, rx;
-  const int sbase = min((wv & 3) * 64, T::BM - 64);   // the 64 scales that a wave loads
-  int off[T::Loads], soff, m0 = 0, n0 = 0, lk = 0;    // where loads are aimed
-  auto aim = [&](int t) {
-    const int band = t / per, rows = min(kBand, a.nby - band * kBand), in = t - band * per;
-    m0 = (band * kBand + in % rows) * T::BM;
-    n0 = in / rows * T::BN;
-    rw = resource(p.w + (int64_t)n0 * p.ldw);
-    rx = resource(p.x + (int64_t)m0 * p.ldx);
-#pragma unroll
-    for (int i = 0; i < T::Loads; ++i) {
-      const int r = (i * T::Waves + wv) * 8 + (lane >> 3), c = ((lane & 7) ^ f8_key(r)) * 16;
-      off[i] = i < 4 ? min(r, p.N - 1 - n0) * (int)p.ldw + c : min(r - T::BN, p.M - 1 - m0) * (int)p.ldx + c;
-    }
-    soff = min(sbase + lane, p.M - 1 - m0) * 4;
-    lk = 0;
-  };
-  // the last load of BM = 224, 160 has work for half the waves: the others repeat the one before
-  constexpr int Rows = (T::BN + T::BM) / 8;
-  auto load = [&](int st, int i) {
-    const bool spare = (i + 1) * T::Waves > Rows && i * T::Waves + wv >= Rows;
-    dma16(lbase + st + ((spare ? i - 1 : i) * T::Waves + wv) * 1024, spare ? off[i - (i > 0)] : off[i], i < 4 ? rw : rx, lk * 128);
-  };
-  auto load_scales = [&](int st) {
-    dma4(lbase + st + T::Codes + sbase * 4, soff, resource(p.xs + m0 + (int64_t)lk * p.ldxs), 0);
-  };
-
-  f32x4 acc[T::SX][T::AN];
-  const int chunk = (g ^ f8_key(l16)) << 4, wrow = (wn * 16 * T::AN + l16) * 128, xrow = (T::BN + wm * 16 * T::SX + l16) * 128;
-  const int w0 = wrow + chunk, w1 = wrow + (chunk ^ 64), x0 = xrow + chunk, x1 = xrow + (chunk ^ 64);
-  const int srow = T::Codes + (wm * 16 * T::SX + l16) * 4;
-  float wsv = 0.0f, s = 0.0f, sf[3];
-  i32x8 wf[T::AN], xf[3];
-  f32x4 d[4];   // the last cells' products, on their way into acc
-  // the activations' fragments take turns; an odd number's last has a place of its own
-  constexpr auto turn = [](int j) { return (T::SX & 1) && j == T::SX - 1 ? 2 : j & 1; };
-  auto read_w = [&](const uint8_t* st, int i) { wf[i] = codes32(*(const i32x4*)(st + w0 + i * 2048), *(const i32x4*)(st + w1 + i * 2048)); };
-  auto read_x = [&](const uint8_t* st, int j) {
-    xf[turn(j)] = codes32(*(const i32x4*)(st + x0 + j * 2048), *(const i32x4*)(st + x1 + j * 2048));
-    sf[turn(j)] = *(const float*)(st + srow + j * 64);
-  };
-  auto fold = [&](int q) {
-    f32x4& v = acc[q / T::AN][q % T::AN];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(d[q & 3][e], s, v[e]);
-    asm volatile("" : "+v"(v));   // here and below: keeps the cell's order
-  };
-  // A step is a block of k: SX rows of 4 cells, a cell one block product: its matrix instruction, and the fmas of the product two cells
-  // before, which is done by then. One barrier, ahead of the last row: every wave then holds the rest of its step in registers.
-  auto step = [&](const uint8_t* st, const uint8_t* st_next, int st_load, float wk) {
-#pragma unroll
-    for (int q = 0; q < T::Q; ++q) {
-      const int j = q / T::AN, i = q % T::AN;
-      if (q == T::Q - T::AN) {
-        wait_dma<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        read_x(st_next, 0);
-      }
-      d[q & 3] = mfma_block(wf[i], xf[turn(j)]);
-      asm volatile("" : "+v"(d[q & 3]));
-      if (j == T::SX - 1) {
-        read_w(st_next, i);
-      } else {
-        if (i == 0) read_x(st, j + 1);
-        if (q < T::Loads) load(st_load, q);
-        if (q == T::Loads) load_scales(st_load);
-      }
-      fold((q + T::Q - 2) % T::Q);
-      if (i == 1) s = sf[turn(j)] * wk;
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-
-  int tile = tile_of(0);
-  if (tile < 0) return;   // whole workgroups
-  aim(tile);
-#pragma unroll
-  for (int i = 0; i < T::Loads; ++i) load(0, i);
-  load_scales(0);
-  wait_dma<0>();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < T::AN; ++i) read_w(lds, i);
-  read_x(lds, 0);
-  int at = 0, to = T::Stage;
-  for (int round = 0; tile >= 0;) {
-    const int m = m0 + wm * 16 * T::SX, n = n0 + wn * 16 * T::AN;
-    tile = tile_of(++round);
-    const float* ws = p.ws + (int64_t)(min(n, p.N - 1) >> 7) * p.ldws;   // of this wave's outputs: 64 steps' in a lane each
-#pragma unroll
-    for (int j = 0; j < T::SX; ++j)
-#pragma unroll
-      for (int i = 0; i < T::AN; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) d[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    s = 0.0f;
-    for (int kb = 0; kb < nk; ++kb) {
-      if ((kb & 63) == 0) {
-        wsv = ws[min(kb + lane, nk - 1)];
-        asm volatile("" : "+v"(wsv));   // waited for here: no other step has a wait of its own for it
-      }
-      if (kb + 1 < nk) ++lk;
-      else if (tile >= 0) aim(tile);   // else: the last block again, never read
-      step(lds + at, lds + to, to, __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wsv), kb & 63)));
-      const int x = at;
-      at = to;
-      to = x;
-    }
-    fold(T::Q - 2);
-    fold(T::Q - 1);
-    tile_out<TYPE, T::SX, T::AN>(p, acc, m, n, lane);
-  }
-  wait_dma<0>();   // loads that nothing reads must not land in another workgroup's LDS
-}
-
 using TileSmall = F8Tile<2, 2, 2, 2, 9>;   // 64 outputs of 64 rows, 4 waves of 32 x 32
 using TileLow = F8Tile<4, 1, 2, 4, 6>;     // 128 of 64, 4 waves of 32 x 64
 using TileHalf = F8Tile<2, 4, 4, 2, 4>;    // 128 of 128, 8 waves of 64 x 32
 using TileLong = F8Tile<2, 4, 4, 4, 3>;    // 128 of 256, 8 waves of 64 x 64
-using TileWide = Wide<8>;
+using TileWide = F8Tile<2, 4, 8, 4, 2>;    // 256 of 256, 8 waves of 128 x 64
 
 template <int W, int U, int MT, int NT> static void f8_thin_launch(F8GemmP p, int type, hipStream_t s) {
   p.nt = (p.N + 16 * NT - 1) / (16 * NT);
   auto k = type == P0_F32 ? f8_thin_kernel<P0_F32, W, U, MT, NT> : type == P0_F16 ? f8_thin_kernel<P0_F16, W, U, MT, NT> : f8_thin_kernel<P0_BF16, W, U, MT, NT>;
   hipLaunchKernelGGL(k, dim3((unsigned)(p.nt * ((p.M + 16 * MT - 1) / (16 * MT)))), dim3(64 * W), 0, s, p);
+}
+template <class T> static auto f8_tile_of(int type) {   // fp32 results hold more in registers: not in the widest tile's
+  constexpr int F = T::AN * T::AM < 32 ? P0_F32 : P0_BF16;
+  return type == P0_F32 ? f8_tile_kernel<F, T> : type == P0_F16 ? f8_tile_kernel<P0_F16, T> : f8_tile_kernel<P0_BF16, T>;
 }
 template <class T> static void f8_tile_launch(const F8GemmP& g, int type, int nks, hipStream_t s) {
   F8TileP a{g, (g.N + T::BN - 1) / T::BN, (g.M + T::BM - 1) / T::BM};
@@ -578,28 +431,19 @@ template <class T> static void f8_tile_launch(const F8GemmP& g, int type, int nk
   a.nks = (g.blocks + a.spk - 1) / a.spk;
   a.part = ctx().part;
   a.cnt = ctx().kv_counters;   // one per tile where there are slices: at most half as many as CUs
-  auto k = type == P0_F32 ? f8_tile_kernel<P0_F32, T> : type == P0_F16 ? f8_tile_kernel<P0_F16, T> : f8_tile_kernel<P0_BF16, T>;
-  hipLaunchKernelGGL(k, dim3((unsigned)(a.nbx * a.nby * a.nks)), dim3(T::Threads), T::Lds, s, a);
+  hipLaunchKernelGGL(f8_tile_of<T>(type), dim3((unsigned)(a.nbx * a.nby * a.nks)), dim3(T::Threads), T::Lds, s, a);
 }
 template <class T> static int f8_tile_init() {
-  const void* k[] = {(const void*)f8_tile_kernel<P0_F32, T>, (const void*)f8_tile_kernel<P0_F16, T>, (const void*)f8_tile_kernel<P0_BF16, T>};
-  for (const void* f : k) P0_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, T::Lds), "p0_open: f8_gemm");
+  for (int type : {P0_F32, P0_F16, P0_BF16})
+    P0_HIP(hipFuncSetAttribute((const void*)f8_tile_of<T>(type), hipFuncAttributeMaxDynamicSharedMemorySize, T::Lds), "p0_open: f8_gemm");
   return P0_OK;
-}
-template <class T> static void f8_wide_launch(const F8GemmP& g, int type, hipStream_t s) {
-  F8WideP a{g, (g.N + T::BN - 1) / T::BN, (g.M + T::BM - 1) / T::BM};
-  const int64_t tiles = (int64_t)a.nbx * a.nby, cus = ctx().cu_count;
-  auto k = type == P0_F16 ? f8_wide_kernel<P0_F16, T> : f8_wide_kernel<P0_BF16, T>;
-  hipLaunchKernelGGL(k, dim3((unsigned)(tiles < cus ? tiles : cus)), dim3(T::Threads), T::Lds, s, a);
 }
 int f8_gemm_init() {
   if (int r = f8_tile_init<TileSmall>()) return r;
   if (int r = f8_tile_init<TileLow>()) return r;
   if (int r = f8_tile_init<TileHalf>()) return r;
   if (int r = f8_tile_init<TileLong>()) return r;
-  for (const void* k : {(const void*)f8_wide_kernel<P0_F16, TileWide>, (const void*)f8_wide_kernel<P0_BF16, TileWide>})
-    P0_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, TileWide::Lds), "p0_open: f8_gemm");
-  return P0_OK;
+  return f8_tile_init<TileWide>();
 }
 
 // Which tile, and how many slices of K, by time: a round of workgroups takes its blocks of k, one after the other, and then its outputs; a
@@ -638,7 +482,7 @@ static void f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
   else if (kind == 1) f8_tile_launch<TileLow>(p, type, nks, s);
   else if (kind == 2) f8_tile_launch<TileHalf>(p, type, nks, s);
   else if (kind == 3) f8_tile_launch<TileLong>(p, type, nks, s);
-  else f8_wide_launch<TileWide>(p, type, s);
+  else f8_tile_launch<TileWide>(p, type, 1, s);
 }
 
 static int gemm_f8_call(const p0_f8_gemm_args_t* a) {

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const PackP p) {
   if (lane == 0) red[threadIdx.x >> 6] = most;
   __syncthreads();
   most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float s = f8_scale(most), inv = 1.0f / s;
+  const float s = f8_scale(most), inv = f8_inverse(s);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int64_t r = n0 + 16 * j;
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const PackP p) {
 __device__ __forceinline__ float gated(int glu, float g, float u) {
   // g * sigmoid(z), z = g, or 2 sqrt(2 / pi) (g + 0.044715 g^3) (= 0.5 g (1 + tanh(z / 2)))
   const float z = glu == P0_GLU_SILU ? g : 1.5957691216f * (g + 0.044715f * g * g * g);
-  return g / (1.0f + __expf(-z)) * u;
+  return g * __builtin_amdgcn_rcpf(1.0f + __expf(-z)) * u;
 }
 struct RowsF8P {
   const void* x;
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsF8P p) {
       for (int j = 0; j < 8; ++j) f[u][j] = gated(p.glu, f[u][j], g[u][j]);
     }
     const float s = f8_scale(f8_max16(f8_most(f[u])));
-    const uint2 w = f8_codes(f[u], 1.0f / s);
+    const uint2 w = f8_codes(f[u], f8_inverse(s));
     if (m >= p.M) continue;
     *(uint2*)(p.y + m * p.ldy + c) = w;
     if ((threadIdx.x & 15) == 0) p.s[(int64_t)(c >> 7) * p.lds + m] = s;
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void f8_norm_kernel(const No
       for (int j = 0; j < 8; ++j) f[i][j] = VEC || c + j < p.D ? f[i][j] * rstd * (g[j] + one) + b[j] : 0.0f;
     }
     const float s = f8_scale(f8_max16(f8_most(f[i])));
-    *(uint2*)(p.y + m * p.ldy + c) = f8_codes(f[i], 1.0f / s);
+    *(uint2*)(p.y + m * p.ldy + c) = f8_codes(f[i], f8_inverse(s));
     if ((lane & 15) == 0) p.s[(int64_t)(c >> 7) * p.lds + m] = s;
   }
 }
