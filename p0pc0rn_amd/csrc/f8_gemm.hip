@@ -29,7 +29,6 @@ struct F8GemmP {
   void* y;
   int64_t ldx, ldxs, ldw, ldws, ldy;
   int M, N, blocks;    // blocks of 128 k
-  int nt;              // tiles of N
   int yvec;            // 1: 4 consecutive outputs from a multiple of 4 on are aligned together; 2: rows are 16-byte aligned
 };
 
@@ -83,73 +82,57 @@ template <int TYPE> __device__ __forceinline__ void store4(const F8GemmP& p, int
   }
 }
 
-// Few rows: a workgroup takes 16 NT outputs of 16 MT rows, its W waves the blocks of k in turn, U at a time; their sums meet in LDS.
-template <int TYPE, int W, int U, int MT, int NT>
+// Few rows: a workgroup takes 16 NT outputs of 16 rows, its W waves the blocks of k in turn; their sums meet in LDS.
+// PAIR: 8 outputs of up to 8 rows, two blocks of k at a time: the matrix instruction's rows 8 - 15 are the same weights' next block, its columns 8 - 15 the
+// same rows', and of its four quarters the two that pair a block with itself are kept.
+template <int TYPE, int W, int NT, bool PAIR>
 __global__ __launch_bounds__(64 * W) void f8_thin_kernel(const F8GemmP p) {
-  __shared__ f32x4 part[W][MT * NT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
-  const int mt = blockIdx.x / (unsigned)p.nt, n0 = (blockIdx.x - mt * p.nt) * 16 * NT, m0 = mt * 16 * MT;
+  static_assert(!PAIR || NT == 1, "one tile of pairs");
+  __shared__ f32x4 part[W][NT][64];
+  constexpr int BN = PAIR ? 8 : 16 * NT, Step = PAIR ? 2 : 1;   // outputs of a workgroup, blocks of a wave's turn
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15, row = PAIR ? l16 & 7 : l16, own = PAIR ? l16 >> 3 : 0;
+  const int n0 = blockIdx.x * BN, m = min(row, p.M - 1);   // rows past the last: it again
   const uint8_t* w[NT];
-  const uint8_t* x[MT];
-  const float* xs[MT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) w[i] = p.w + min(n0 + 16 * i + l16, p.N - 1) * p.ldw + g * 16;   // rows past the last: it again
-#pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int m = min(m0 + 16 * j + l16, p.M - 1);
-    x[j] = p.x + m * p.ldx + g * 16;
-    xs[j] = p.xs + m;
-  }
+  for (int i = 0; i < NT; ++i) w[i] = p.w + min(n0 + 16 * i + row, p.N - 1) * p.ldw + g * 16;
+  const uint8_t* x = p.x + m * p.ldx + g * 16;
+  const float* xs = p.xs + m;
   const float* ws = p.ws + (int64_t)(n0 >> 7) * p.ldws;
-  f32x4 acc[MT][NT];
+  f32x4 acc[NT];
 #pragma unroll
-  for (int j = 0; j < MT; ++j)
+  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int kb = wave * Step; kb < p.blocks; kb += W * Step) {
+    const int k = min(kb + own, p.blocks - 1);   // past the last block: it again, times 0
+    const float s = kb + own < p.blocks ? xs[k * p.ldxs] * ws[k] : 0.0f;
+    const i32x8 b = codes32(*(const i32x4*)(x + (int64_t)k * 128), *(const i32x4*)(x + (int64_t)k * 128 + 64));
+    i32x8 a[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int kb = wave; kb < p.blocks; kb += U * W) {
-    i32x8 a[U][NT], b[U][MT];
-    float s[U][MT];
+    for (int i = 0; i < NT; ++i) a[i] = codes32(*(const i32x4*)(w[i] + (int64_t)k * 128), *(const i32x4*)(w[i] + (int64_t)k * 128 + 64));
+    half8v bh[4];
+    to_half(b, bh);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {   // past the last block: it again, times 0
-      const int k = min(kb + u * W, p.blocks - 1);
+    for (int i = 0; i < NT; ++i) {
+      half8v ah[4];
+      to_half(a[i], ah);
+      const f32x4 d = mfma_half(ah, bh);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) a[u][i] = codes32(*(const i32x4*)(w[i] + (int64_t)k * 128), *(const i32x4*)(w[i] + (int64_t)k * 128 + 64));
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        b[u][j] = codes32(*(const i32x4*)(x[j] + (int64_t)k * 128), *(const i32x4*)(x[j] + (int64_t)k * 128 + 64));
-        s[u][j] = kb + u * W < p.blocks ? xs[j][k * p.ldxs] * ws[k] : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      half8v ah[NT][4];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) to_half(a[u][i], ah[i]);
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        half8v bh[4];
-        to_half(b[u][j], bh);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          const f32x4 d = mfma_half(ah[i], bh);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][i][e] = __builtin_fmaf(d[e], s[u][j], acc[j][i][e]);
-        }
-      }
+      for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(d[e], s, acc[i][e]);
     }
   }
 #pragma unroll
-  for (int j = 0; j < MT; ++j)
-#pragma unroll
-    for (int i = 0; i < NT; ++i) part[wave][j * NT + i][lane] = acc[j][i];
+  for (int i = 0; i < NT; ++i) part[wave][i][lane] = acc[i];
   __syncthreads();
-  for (int c = wave; c < MT * NT; c += W) {
-    f32x4 v = part[0][c][lane];
+  if (wave >= NT) return;
+  f32x4 v = part[0][wave][lane];
 #pragma unroll
-    for (int k = 1; k < W; ++k) v += part[k][c][lane];
-    const int m = m0 + c / NT * 16 + l16, n = n0 + c % NT * 16 + 4 * g;
-    if (m < p.M && n < p.N) store4<TYPE>(p, m, n, v);
+  for (int k = 1; k < W; ++k) v += part[k][wave][lane];
+  const int n = n0 + wave * 16 + 4 * g;
+  if constexpr (PAIR) {   // the other block's sums: 32 lanes of outputs and 8 columns further on
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += __shfl(v[e], lane + 40, 64);
+    if (g >= 2 || l16 >= 8) return;
   }
+  if (l16 < p.M && n < p.N) store4<TYPE>(p, l16, n, v);
 }
 
 // The sums of a wave's 16 AM rows from row m on, of 16 AN outputs from output n on
@@ -416,10 +399,10 @@ using TileHalf = F8Tile<2, 4, 4, 2, 4>;    // 128 of 128, 8 waves of 64 x 32
 using TileLong = F8Tile<2, 4, 4, 4, 3>;    // 128 of 256, 8 waves of 64 x 64
 using TileWide = F8Tile<2, 4, 8, 4, 2>;    // 256 of 256, 8 waves of 128 x 64
 
-template <int W, int U, int MT, int NT> static void f8_thin_launch(F8GemmP p, int type, hipStream_t s) {
-  p.nt = (p.N + 16 * NT - 1) / (16 * NT);
-  auto k = type == P0_F32 ? f8_thin_kernel<P0_F32, W, U, MT, NT> : type == P0_F16 ? f8_thin_kernel<P0_F16, W, U, MT, NT> : f8_thin_kernel<P0_BF16, W, U, MT, NT>;
-  hipLaunchKernelGGL(k, dim3((unsigned)(p.nt * ((p.M + 16 * MT - 1) / (16 * MT)))), dim3(64 * W), 0, s, p);
+template <int W, int NT, bool PAIR> static void f8_thin_launch(const F8GemmP& p, int type, hipStream_t s) {
+  const int bn = PAIR ? 8 : 16 * NT;
+  auto k = type == P0_F32 ? f8_thin_kernel<P0_F32, W, NT, PAIR> : type == P0_F16 ? f8_thin_kernel<P0_F16, W, NT, PAIR> : f8_thin_kernel<P0_BF16, W, NT, PAIR>;
+  hipLaunchKernelGGL(k, dim3((unsigned)((p.N + bn - 1) / bn)), dim3(64 * W), 0, s, p);
 }
 template <class T> static auto f8_tile_of(int type) {   // fp32 results hold more in registers: not in the widest tile's
   constexpr int F = T::AN * T::AM < 32 ? P0_F32 : P0_BF16;
@@ -514,10 +497,13 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   const uintptr_t ya = (uintptr_t)a->y | (uintptr_t)(ldy * size);
   p.yvec = ya % 16 == 0 ? 2 : ya % (4 * size) == 0;
   if (M <= 16) {
-    // the blocks of k in turns over the waves, one block a wave and turn: 4 waves while that is at most 4 turns, more for longer k.
-    // Enough outputs for two workgroups a CU, and rows that are worth it: 32 outputs a workgroup, which halves its reads of the rows
-    if (N >= 16384 && M > 8) f8_thin_launch<4, 1, 1, 2>(p, a->type, ctx().cur);
-    else f8_thin_launch<8, 1, 1, 1>(p, a->type, ctx().cur);
+    // Measured (us; rows, outputs x k): pairs of blocks where 16 outputs a workgroup would leave CUs without one: 5, 2048 x 8192 6.6 / 7.6, 1, 1024 x
+    // 4096 4.0 / 4.6, but 1, 4096 x 8192 9.4 / 8.4. 32 outputs a workgroup, which halves its reads of the rows: 16, 16384 x 2048 8.4 / 10.1, but 16,
+    // 4096 x 2048 5.2 / 4.1 and 5, 16384 x 8192 29.4 / 24.9. 16 waves for long k: 1, 16384 x 4096 14.2 / 14.9 of 8; 1, 16384 x 2048 9.0 / 7.5
+    if (M <= 8 && N <= 8 * ctx().cu_count && blocks >= 16) f8_thin_launch<16, 1, true>(p, a->type, ctx().cur);
+    else if (M <= 8 && blocks >= 32) f8_thin_launch<16, 1, false>(p, a->type, ctx().cur);
+    else if (M > 8 && N >= 8192) f8_thin_launch<4, 2, false>(p, a->type, ctx().cur);
+    else f8_thin_launch<8, 1, false>(p, a->type, ctx().cur);
   } else {
     f8_tile_choice(p, a->type, ctx().cur);
   }

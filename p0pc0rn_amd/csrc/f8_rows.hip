@@ -120,24 +120,25 @@ __device__ __forceinline__ float sum64(float v) {
   v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
 }
-// W waves take a row (W = 1: a workgroup has four rows), a lane 8 channels of NC steps of 512 W. The row stays in registers.
+// A workgroup takes a row, its up to 16 waves 512 channels each of NC steps, a lane 8 of them. The row stays in registers; each sum is one
+// exchange through LDS.
 // VEC: every run of 8 channels is there whole or not at all, and 16-byte aligned everywhere.
-template <int XT, int TT, int W, int NC, bool VEC>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void f8_norm_kernel(const NormP p) {
-  __shared__ float red[3][W];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t m = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
-  if (m >= p.M) return;
-  const int c0 = ((W == 1 ? 0 : wave) * 64 + lane) * 8;
+// Bound: HBM at many rows (32760 rows of 2560 bf16 channels, modulated: 112 us for 588 MB, 5.2 TB/s; a copy 5.5), launch and round trips
+// at few (1 row of 2048 fp32 channels: 3.6 us). A wave with a row of its own, four in a workgroup, took 136 and 3.7: five loads a lane
+// at a time and their registers leave fewer waves to cover them.
+template <int XT, int TT, int NC, bool VEC>
+__global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
+  __shared__ float red[3][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = blockDim.x >> 6;
+  const int64_t m = blockIdx.x;
+  const int c0 = (wave * 64 + lane) * 8;
   auto total = [&](float v, int slot) {
     v = sum64(v);
-    if constexpr (W > 1) {
-      if (lane == 0) red[slot][wave] = v;
-      __syncthreads();
-      v = 0.0f;
-#pragma unroll
-      for (int i = 0; i < W; ++i) v += red[slot][i];
-    }
+    if (W == 1) return v;
+    if (lane == 0) red[slot][wave] = v;
+    __syncthreads();
+    v = red[slot][0];
+    for (int i = 1; i < W; ++i) v += red[slot][i];
     return v;
   };
   auto count = [&](int c) { return VEC ? 8 : p.D - c < 8 ? p.D - c : 8; };   // of the 8 channels from c < D on
@@ -301,11 +302,9 @@ static int rows_f8_call(const p0_f8_rows_args_t* a) {
 }
 
 typedef void (*NormKernel)(NormP);
-template <int XT, int TT> static NormKernel norm_kernel(bool vec, int W, int steps) {
-  if (!vec) return W == 4 ? f8_norm_kernel<XT, TT, 4, 4, false> : f8_norm_kernel<XT, TT, 16, 4, false>;
-  if (W == 1) return steps == 1 ? f8_norm_kernel<XT, TT, 1, 1, true> : steps == 2 ? f8_norm_kernel<XT, TT, 1, 2, true> : f8_norm_kernel<XT, TT, 1, 5, true>;
-  if (W == 4) return steps == 1 ? f8_norm_kernel<XT, TT, 4, 1, true> : steps == 2 ? f8_norm_kernel<XT, TT, 4, 2, true> : f8_norm_kernel<XT, TT, 4, 4, true>;
-  return steps <= 2 ? f8_norm_kernel<XT, TT, 16, 2, true> : f8_norm_kernel<XT, TT, 16, 4, true>;
+template <int XT, int TT> static NormKernel norm_kernel(bool vec, int NC) {
+  if (!vec) return NC == 1 ? f8_norm_kernel<XT, TT, 1, false> : f8_norm_kernel<XT, TT, 4, false>;
+  return NC == 1 ? f8_norm_kernel<XT, TT, 1, true> : NC == 2 ? f8_norm_kernel<XT, TT, 2, true> : f8_norm_kernel<XT, TT, 4, true>;
 }
 
 static int norm_call(const p0_f8_norm_args_t* a) {
@@ -343,15 +342,20 @@ static int norm_call(const p0_f8_norm_args_t* a) {
   const bool vec = D % 8 == 0 && ((uintptr_t)a->x | (uintptr_t)(ldx * xsize) | (uintptr_t)xo | (uintptr_t)(ldo * xsize) | (uintptr_t)a->t |
                                   (uintptr_t)(ldt * tsize) | (uintptr_t)a->tw | (uintptr_t)a->w | (uintptr_t)a->b) % 16 == 0;
   p.mode = a->mode; p.one = a->w_one ? 1 : 0; p.scale = scale; p.eps = a->eps != 0.0f ? a->eps : 1e-6f;
-  const int W = vec && D <= 2560 && M >= 256 ? 1 : D <= 8192 ? 4 : 16, steps = (int)((K8 + 512 * W - 1) / (512 * W));
+  // Waves of one step, but for two where rows are longer than 16 waves' one, and for 16-bit rows that fill the chip several times over (us,
+  // one step / two: 32760 rows of 2560 bf16 channels 129 / 112, 4608 of 4096 28.9 / 27.4; 1021 of 1536 5.0 / 5.8; 4608 of 2048 fp32 channels
+  // 23.9 / 25.7), and four for the longest
+  const int steps = (int)((K8 + 511) / 512);
+  const bool two = vec && (steps > 16 || (xsize == 2 && steps > 1 && M * steps >= 16384));
+  const int NC = steps > (vec ? 32 : 16) ? 4 : two ? 2 : 1, W = (steps + NC - 1) / NC;
   const int tt = a->t ? a->t_type : a->type;
   NormKernel k = nullptr;
-#define P0_NORM(XT, TT) if (a->type == XT && tt == TT) k = norm_kernel<XT, TT>(vec, W, steps)
+#define P0_NORM(XT, TT) if (a->type == XT && tt == TT) k = norm_kernel<XT, TT>(vec, NC)
   P0_NORM(P0_F32, P0_F32); P0_NORM(P0_F32, P0_F16); P0_NORM(P0_F32, P0_BF16);
   P0_NORM(P0_F16, P0_F32); P0_NORM(P0_F16, P0_F16); P0_NORM(P0_F16, P0_BF16);
   P0_NORM(P0_BF16, P0_F32); P0_NORM(P0_BF16, P0_F16); P0_NORM(P0_BF16, P0_BF16);
 #undef P0_NORM
-  hipLaunchKernelGGL(k, dim3((unsigned)(W == 1 ? (M + 3) / 4 : M)), dim3(W == 1 ? 256 : 64 * W), 0, ctx().cur, p);
+  hipLaunchKernelGGL(k, dim3((unsigned)M), dim3(64 * W), 0, ctx().cur, p);
   P0_LAUNCHED(op);
   return P0_OK;
 }

@@ -5,6 +5,8 @@
 // is many turns: it is held in 64 bits, in turns, and only the fraction of a turn goes on in 32.
 #include "f8_common.hpp"
 
+#include <cmath>
+
 namespace p0 {
 
 constexpr int kRopeThreads = 256, kRopePairs = 256, kRopeTable = 2048;   // pairs of a head at most; angles of a workgroup's rows
@@ -15,12 +17,11 @@ struct RopeP {
   const float* qw;
   const float* kw;
   int64_t ldr, ldh, yldr, yldh, pos_ld, rows;
-  double log2_theta;
+  double pow[4][8];           // an axis's frequency, in turns a position: pow[0] of its first pair's axis times the bits of the pair's number
   int heads, hq, dim, R;      // R: channels that turn
-  int first[4], size[4];      // an axis's first pair, its channels
-  int axes, shared, inter, vec;
+  int first[4];               // an axis's first pair
+  int axes, shared, inter;
   int rb, hb, hblocks;        // rows, heads of a workgroup, workgroups a row block
-  uint32_t magic;             // item / hb = item * magic >> 20
   int ls;                     // 1 << ls lanes take a head
   float eps;
 };
@@ -33,84 +34,61 @@ __device__ __forceinline__ float2 rope_turn(const RopeP& p, int64_t row, int i) 
   if (i >= p.R / 2) return float2{1.0f, 0.0f};
   int a = 0;
   for (int k = 1; k < p.axes; ++k) a = i >= p.first[k] ? k : a;
-  const double e = p.shared ? 2.0 * i / p.R : 2.0 * (i - p.first[a]) / p.size[a];
-  const double turns = (double)p.pos[a * p.pos_ld + row] * (exp2(-e * p.log2_theta) * 0.15915494309189535);
+  // theta^-e / 2 pi: pair j of its axis (of all, where the axes share one range) has the frequency of pair 1 to the power of j, by j's bits
+  const int j = p.shared ? i : i - p.first[a];
+  double f = 0.15915494309189535;
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const double t = f * p.pow[a][b];
+    f = j >> b & 1 ? t : f;
+  }
+  const double turns = (double)p.pos[a * p.pos_ld + row] * f;
   float s, c;
   sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
   return float2{c, s};
 }
 
-// V pairs a lane
-template <int TYPE, int V> __device__ __forceinline__ void rope_load(const RopeP& p, int64_t at, int i0, int n, float (&u)[V], float (&v)[V]) {
-  if constexpr (V > 1) {   // vec: whole runs, all of one kind of pair
-    if (p.inter) {
-      float f[2 * V];
-#pragma unroll
-      for (int h = 0; h < 2 * V; h += 8) {
-        float g[8];
-        f8_load8<TYPE>(p.x, at + 2 * i0 + h, true, 8, g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[h + j] = g[j];
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) { u[j] = f[2 * j]; v[j] = f[2 * j + 1]; }
-    } else {
-      f8_load8<TYPE>(p.x, at + i0, true, 8, u);
-      f8_load8<TYPE>(p.x, at + i0 + p.R / 2, true, 8, v);
-    }
-  } else {
+// KIND 0: a lane has one pair at a time, 16 lanes a head. Whole 16-byte runs of one kind of pair: 1: neighbours, 4 pairs of a lane, dim / 8 lanes a head
+// (rounded up to a power of two); 2: halves, 8 pairs of a lane, dim / 16 lanes
+template <int TYPE, int KIND> __device__ __forceinline__ void rope_pairs(const void* x, int64_t at, int i0, int half, float (&u)[8], float (&v)[8]) {
+  if constexpr (KIND == 1) {
     float g[8];
-    f8_load8<TYPE>(p.x, at + rope_first(p, i0), false, n, g);
-    u[0] = g[0];
-    f8_load8<TYPE>(p.x, at + rope_second(p, i0), false, n, g);
-    v[0] = g[0];
-  }
-}
-template <int TYPE, int V> __device__ __forceinline__ void rope_store(const RopeP& p, int64_t at, int i0, const float (&u)[V], const float (&v)[V]) {
-  if constexpr (V > 1) {
-    if (p.inter) {
+    f8_load8<TYPE>(x, at + 2 * i0, true, 8, g);
 #pragma unroll
-      for (int h = 0; h < V; h += 4) {
-        float g[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { g[2 * j] = u[h + j]; g[2 * j + 1] = v[h + j]; }
-        f8_store8<TYPE>(p.y, at + 2 * (i0 + h), true, 8, g);
-      }
-    } else {
-      f8_store8<TYPE>(p.y, at + i0, true, 8, u);
-      f8_store8<TYPE>(p.y, at + i0 + p.R / 2, true, 8, v);
-    }
+    for (int j = 0; j < 4; ++j) { u[j] = g[2 * j]; v[j] = g[2 * j + 1]; }
   } else {
-    const float a[8] = {u[0]}, b[8] = {v[0]};
-    f8_store8<TYPE>(p.y, at + rope_first(p, i0), false, 1, a);
-    f8_store8<TYPE>(p.y, at + rope_second(p, i0), false, 1, b);
+    f8_load8<TYPE>(x, at + i0, true, 8, u);
+    f8_load8<TYPE>(x, at + i0 + half, true, 8, v);
   }
 }
 
-// V = 8: 8 pairs a lane, dim / 16 lanes a head (rounded up to a power of two); V = 1: one pair a lane at a time, 16 lanes a head
-template <int TYPE, int V>
+template <int TYPE, int KIND>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeP p) {
-  __shared__ float2 turn[kRopeTable];
+  __shared__ __attribute__((aligned(16))) float2 turn[kRopeTable];
   const int64_t blk = blockIdx.x / (unsigned)p.hblocks, row0 = blk * p.rb;
   const int h0 = (int)(blockIdx.x - blk * p.hblocks) * p.hb, pairs = p.dim / 2;
   const int rows = (int)(p.rows - row0 < p.rb ? p.rows - row0 : p.rb), hb = p.heads - h0 < p.hb ? p.heads - h0 : p.hb;
-  for (int r = 0; r < rows; ++r)
-    for (int i = threadIdx.x; i < pairs; i += kRopeThreads) turn[r * pairs + i] = rope_turn(p, row0 + r, i);
+  for (int k = threadIdx.x; k < rows * pairs; k += kRopeThreads) {
+    const int r = k / pairs;
+    turn[k] = rope_turn(p, row0 + r, k - r * pairs);
+  }
   __syncthreads();
-  const int lane = threadIdx.x & ((1 << p.ls) - 1), items = rows * p.hb;
+  const int lane = threadIdx.x & ((1 << p.ls) - 1), items = rows * hb;
+  const uint32_t magic = (1u << 20) / (uint32_t)hb + 1;   // it / hb = it * magic >> 20: exact while it * hb < 2^20
   for (int it = threadIdx.x >> p.ls; it < items; it += kRopeThreads >> p.ls) {
-    const int r = (int)((uint32_t)it * p.magic >> 20), hl = it - r * p.hb, h = h0 + hl;
-    if (hl >= hb) continue;   // the last block of heads may be shorter (whole groups of lanes)
+    const int r = (int)((uint32_t)it * magic >> 20), h = h0 + it - r * hb;
     const int64_t from = (row0 + r) * p.ldr + h * p.ldh, to = (row0 + r) * p.yldr + h * p.yldh;
     const float* w = h < p.hq ? p.qw : p.kw;
-    if constexpr (V > 1) {
+    if constexpr (KIND > 0) {
+      constexpr int V = KIND == 1 ? 4 : 8;
       const int i0 = lane * V;
       const bool on = i0 < pairs;
-      float u[V], v[V];
-      if (on) rope_load<TYPE, V>(p, from, i0, 1, u, v);
+      float u[8], v[8];
+      if (on) rope_pairs<TYPE, KIND>(p.x, from, i0, p.R / 2, u, v);
       if (w) {
-        float ss = 0.0f;
+        float ss = 0.0f, wu[8], wv[8];
         if (on) {
+          rope_pairs<P0_F32, KIND>(w, 0, i0, p.R / 2, wu, wv);
 #pragma unroll
           for (int j = 0; j < V; ++j) ss += u[j] * u[j] + v[j] * v[j];
         }
@@ -118,43 +96,49 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeP p) {
         const float rstd = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
         if (on) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            u[j] = u[j] * rstd * w[rope_first(p, i0 + j)];
-            v[j] = v[j] * rstd * w[rope_second(p, i0 + j)];
-          }
+          for (int j = 0; j < V; ++j) { u[j] *= rstd * wu[j]; v[j] *= rstd * wv[j]; }
         }
       }
       if (on) {
+        float a[8], b[8];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float2 t = turn[r * pairs + i0 + j];
-          const float a = u[j] * t.x - v[j] * t.y, b = v[j] * t.x + u[j] * t.y;
-          u[j] = a;
-          v[j] = b;
+          a[j] = u[j] * t.x - v[j] * t.y;
+          b[j] = v[j] * t.x + u[j] * t.y;
         }
-        rope_store<TYPE, V>(p, to, i0, u, v);
+        if constexpr (KIND == 1) {
+          const float g[8] = {a[0], b[0], a[1], b[1], a[2], b[2], a[3], b[3]};
+          f8_store8<TYPE>(p.y, to + 2 * i0, true, 8, g);
+        } else {
+          f8_store8<TYPE>(p.y, to + i0, true, 8, a);
+          f8_store8<TYPE>(p.y, to + i0 + p.R / 2, true, 8, b);
+        }
       }
     } else {
+      auto load = [&](int c) {
+        float g[8];
+        f8_load8<TYPE>(p.x, from + c, false, 1, g);
+        return g[0];
+      };
       float rstd = 1.0f;
       if (w) {
-        float ss = 0.0f, u[1], v[1];
+        float ss = 0.0f;
         for (int i = lane; i < pairs; i += 16) {
-          rope_load<TYPE, 1>(p, from, i, 1, u, v);
-          ss += u[0] * u[0] + v[0] * v[0];
+          const float u = load(rope_first(p, i)), v = load(rope_second(p, i));
+          ss += u * u + v * v;
         }
         for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
         rstd = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
       }
       for (int i = lane; i < pairs; i += 16) {
-        float u[1], v[1];
-        rope_load<TYPE, 1>(p, from, i, 1, u, v);
-        if (w) {
-          u[0] = u[0] * rstd * w[rope_first(p, i)];
-          v[0] = v[0] * rstd * w[rope_second(p, i)];
-        }
+        const int cu = rope_first(p, i), cv = rope_second(p, i);
+        float u = load(cu), v = load(cv);
+        if (w) { u *= rstd * w[cu]; v *= rstd * w[cv]; }
         const float2 t = turn[r * pairs + i];
-        const float a[1] = {u[0] * t.x - v[0] * t.y}, b[1] = {v[0] * t.x + u[0] * t.y};
-        rope_store<TYPE, 1>(p, to, i, a, b);
+        const float a[8] = {u * t.x - v * t.y}, b[8] = {v * t.x + u * t.y};
+        f8_store8<TYPE>(p.y, to + cu, false, 1, a);
+        f8_store8<TYPE>(p.y, to + cv, false, 1, b);
       }
     }
   }
@@ -171,13 +155,14 @@ static int rope_call(const p0_rope_args_t* a) {
   const int64_t heads = (int64_t)a->hq + a->hk;
   if (a->hq < 0 || a->hk < 0 || heads < 1 || heads > 65535) { set_error("%s: %d and %d heads", op, (int)a->hq, (int)a->hk); return P0_EINVAL; }
   RopeP p{};
+  int size_of[4];
   p.axes = a->axes ? a->axes : 1;
   if (p.axes < 1 || p.axes > 4) { set_error("%s: %d axes", op, (int)a->axes); return P0_EINVAL; }
   for (int k = 0; k < p.axes; ++k) {
     const int d = a->axis_dim[k] || p.axes > 1 ? a->axis_dim[k] : a->dim;
     if (d < 2 || d % 2 || d > a->dim - p.R) { set_error("%s: axis %d of %d channels (heads of %d)", op, k, d, (int)a->dim); return P0_EINVAL; }
     p.first[k] = p.R / 2;
-    p.size[k] = d;
+    size_of[k] = d;
     p.R += d;
   }
   const double theta = a->theta != 0.0 ? a->theta : 10000.0;
@@ -205,14 +190,16 @@ static int rope_call(const p0_rope_args_t* a) {
   if (int r = refuse_in_chain(op)) return r;
   if (int r = require_open(op)) return r;
   p.x = a->x; p.y = a->y; p.pos = a->pos; p.qw = a->qw; p.kw = a->kw; p.rows = a->rows;
-  p.log2_theta = log2(theta);
   p.heads = (int)heads; p.hq = a->hq; p.dim = a->dim; p.shared = a->freq; p.inter = a->mode == P0_ROPE_INTER;
   p.eps = a->eps != 0.0f ? a->eps : 1e-6f;
-  // 8 pairs a lane where every lane's are whole 16-byte runs of one kind
+  for (int k = 0; k < p.axes; ++k) {
+    long double f = powl((long double)theta, -2.0L / (a->freq ? p.R : size_of[k]));   // squares of squares: in more bits than are kept
+    for (int b = 0; b < 8; ++b, f *= f) p.pow[k][b] = (double)f;
+  }
   const bool rows16 = ((uintptr_t)a->x | (uintptr_t)a->y | (uintptr_t)(p.ldr * size) | (uintptr_t)(p.ldh * size) | (uintptr_t)(p.yldr * size) |
-                       (uintptr_t)(p.yldh * size)) % 16 == 0;
-  p.vec = rows16 && a->dim % 16 == 0 && (p.inter || p.R == a->dim);
-  const int lanes = p.vec ? a->dim / 16 : 16;
+                       (uintptr_t)(p.yldh * size) | (uintptr_t)a->qw | (uintptr_t)a->kw) % 16 == 0;
+  const int kind = !rows16 ? 0 : p.inter ? (a->dim % 8 == 0 ? 1 : 0) : a->dim % 16 == 0 && p.R == a->dim ? 2 : 0;
+  const int lanes = kind == 1 ? a->dim / 8 : kind == 2 ? a->dim / 16 : 16;
   while (1 << p.ls < lanes) ++p.ls;
   const int side = kRopeThreads >> p.ls, pairs = a->dim / 2;
   // A workgroup's work is four rounds of its groups of lanes where that leaves work for every CU: several rows, or a part of a row's
@@ -222,10 +209,9 @@ static int rope_call(const p0_rope_args_t* a) {
   p.rb = side * rounds / p.hb;
   if (p.rb > kRopeTable / pairs) p.rb = kRopeTable / pairs;
   p.hblocks = (int)((heads + p.hb - 1) / p.hb);
-  p.magic = (1u << 20) / (uint32_t)p.hb + 1;   // exact below 2^20 / hb: items are at most side * rounds <= 256 * 4... of hb <= 1024
   const int64_t grid = (a->rows + p.rb - 1) / p.rb * p.hblocks;
   if (grid >= (1ll << 31)) { set_error("%s: %lld rows of %lld heads", op, (long long)a->rows, (long long)heads); return P0_EINVAL; }
-#define P0_ROPE(T) if (a->type == T) hipLaunchKernelGGL((p.vec ? rope_kernel<T, 8> : rope_kernel<T, 1>), dim3((unsigned)grid), dim3(kRopeThreads), 0, ctx().cur, p)
+#define P0_ROPE(T) if (a->type == T) hipLaunchKernelGGL((kind == 0 ? rope_kernel<T, 0> : kind == 1 ? rope_kernel<T, 1> : rope_kernel<T, 2>), dim3((unsigned)grid), dim3(kRopeThreads), 0, ctx().cur, p)
   P0_ROPE(P0_F32);
   P0_ROPE(P0_F16);
   P0_ROPE(P0_BF16);
