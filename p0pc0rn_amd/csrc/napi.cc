@@ -367,6 +367,66 @@ napi_value Beam(napi_env env, napi_callback_info info) {
   return undef(env);
 }
 
+// ---- 8-bit linears and the rotation of heads
+float f32(napi_env env, napi_value obj, const char* name) { return (float)field(env, obj, name); }
+napi_value F8Pack(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_f8_pack_args_t r{};
+  r.x = ptr<const void>(env, o, "x"); r.ldx = i64(env, o, "ldx"); r.type = i32(env, o, "type"); r.N = i64(env, o, "N"); r.K = i64(env, o, "K");
+  r.w = ptr<void>(env, o, "w"); r.ldw = i64(env, o, "ldw"); r.s = ptr<float>(env, o, "s"); r.lds = i64(env, o, "lds");
+  if (fail(env, p0_f8_pack(&r))) return nullptr;
+  return undef(env);
+}
+napi_value F8Norm(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_f8_norm_args_t r{};
+  r.x = ptr<void>(env, o, "x"); r.ldx = i64(env, o, "ldx"); r.type = i32(env, o, "type");
+  r.t = ptr<const void>(env, o, "t"); r.ldt = i64(env, o, "ldt"); r.t_type = i32(env, o, "t_type"); r.tw = ptr<const float>(env, o, "tw");
+  r.x_out = ptr<void>(env, o, "x_out"); r.ldo = i64(env, o, "ldo"); r.scale = f32(env, o, "scale"); r.eps = f32(env, o, "eps");
+  r.mode = i32(env, o, "mode"); r.w_one = i32(env, o, "w_one"); r.w = ptr<const float>(env, o, "w"); r.b = ptr<const float>(env, o, "b");
+  r.M = i64(env, o, "M"); r.D = i64(env, o, "D");
+  r.y = ptr<void>(env, o, "y"); r.ldy = i64(env, o, "ldy"); r.s = ptr<float>(env, o, "s"); r.lds = i64(env, o, "lds");
+  if (fail(env, p0_f8_norm(&r))) return nullptr;
+  return undef(env);
+}
+napi_value F8Rows(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_f8_rows_args_t r{};
+  r.x = ptr<const void>(env, o, "x"); r.ldx = i64(env, o, "ldx"); r.type = i32(env, o, "type"); r.up = i64(env, o, "up"); r.glu = i32(env, o, "glu");
+  r.M = i64(env, o, "M"); r.D = i64(env, o, "D");
+  r.y = ptr<void>(env, o, "y"); r.ldy = i64(env, o, "ldy"); r.s = ptr<float>(env, o, "s"); r.lds = i64(env, o, "lds");
+  if (fail(env, p0_f8_rows(&r))) return nullptr;
+  return undef(env);
+}
+napi_value F8Gemm(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_f8_gemm_args_t r{};
+  r.x = ptr<const void>(env, o, "x"); r.ldx = i64(env, o, "ldx"); r.xs = ptr<const float>(env, o, "xs"); r.ldxs = i64(env, o, "ldxs");
+  r.w = ptr<const void>(env, o, "w"); r.ldw = i64(env, o, "ldw"); r.ws = ptr<const float>(env, o, "ws"); r.ldws = i64(env, o, "ldws");
+  r.M = i64(env, o, "M"); r.N = i64(env, o, "N"); r.K = i64(env, o, "K"); r.type = i32(env, o, "type");
+  r.y = ptr<void>(env, o, "y"); r.ldy = i64(env, o, "ldy");
+  if (fail(env, p0_f8_gemm(&r))) return nullptr;
+  return undef(env);
+}
+napi_value Rope(napi_env env, napi_callback_info info) {
+  auto a = args(env, info, 1);
+  napi_value o = a[0];
+  p0_rope_args_t r{};
+  r.x = ptr<const void>(env, o, "x"); r.ldr = i64(env, o, "ldr"); r.ldh = i64(env, o, "ldh");
+  r.y = ptr<void>(env, o, "y"); r.y_ldr = i64(env, o, "y_ldr"); r.y_ldh = i64(env, o, "y_ldh");
+  r.type = i32(env, o, "type"); r.rows = i64(env, o, "rows"); r.hq = i32(env, o, "hq"); r.hk = i32(env, o, "hk"); r.dim = i32(env, o, "dim");
+  r.mode = i32(env, o, "mode"); r.axes = i32(env, o, "axes"); r.freq = i32(env, o, "freq");
+  r.axis_dim[0] = i32(env, o, "axis0"); r.axis_dim[1] = i32(env, o, "axis1"); r.axis_dim[2] = i32(env, o, "axis2"); r.axis_dim[3] = i32(env, o, "axis3");
+  r.pos = ptr<const int32_t>(env, o, "pos"); r.pos_ld = i64(env, o, "pos_ld"); r.theta = field(env, o, "theta");
+  r.qw = ptr<const float>(env, o, "qw"); r.kw = ptr<const float>(env, o, "kw"); r.eps = f32(env, o, "eps");
+  if (fail(env, p0_rope(&r))) return nullptr;
+  return undef(env);
+}
+
 napi_value UploadFile(napi_env env, napi_callback_info info) {   // uploadFile(path, offset, bytes, dst, dstOff)
   auto a = args(env, info, 5);
   size_t len = 0;
@@ -478,6 +538,7 @@ napi_value Init(napi_env env, napi_value exports) {
       {"rowstats", Rowstats}, {"normadd", Normadd}, {"argmaxM", ArgmaxM}, {"uploadFile", UploadFile},
       {"kvPageBytes", KvPageBytes}, {"kvPut", KvPut}, {"kvGet", KvGet}, {"kvAttn", KvAttn}, {"kvUpdate", KvUpdate},
       {"kvCompact", KvCompact}, {"beam", Beam},
+      {"f8Pack", F8Pack}, {"f8Norm", F8Norm}, {"f8Rows", F8Rows}, {"f8Gemm", F8Gemm}, {"rope", Rope},
   };
   for (auto& f : fns) {
     napi_value v;

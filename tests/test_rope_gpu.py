@@ -115,3 +115,27 @@ def test_a_head_of_zeros_or_nan(dev):
     assert (got[1] == 0).all() and np.isnan(got[2]).all() and np.isfinite(got[[0, 3]]).all()
     for r in (xr, pr, y, w):
         r.free()
+
+
+def test_recorded_rotation_replays(dev):
+    """a copy and a rotation in place, recorded; the program's own calls between the replays"""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((30, 256)).astype(np.float32)
+    src, buf, pr, y = capi.to_device(x), capi.Buffer(x.nbytes), capi.to_device(np.arange(30, dtype=np.int32)), capi.Buffer(x.nbytes)
+
+    def step():
+        capi.copy(src, 0, buf, 0, x.nbytes)
+        capi.rope(capi.rope_args(x=buf, y=buf, type=0, rows=30, hq=4, dim=64, mode=1, pos=pr))
+
+    rec = capi.record(step)
+    capi.rope(capi.rope_args(x=src, y=y, type=0, rows=30, hq=4, dim=64, mode=1, pos=pr))
+    want = y.read(np.uint8, x.nbytes)
+    for _ in range(4):
+        buf.fill_u32(0xA5A5A5A5)
+        rec.replay()
+        assert np.array_equal(buf.read(np.uint8, x.nbytes), want)
+        step()
+        assert np.array_equal(buf.read(np.uint8, x.nbytes), want)
+    rec.free()
+    for b in (src, buf, pr, y):
+        b.free()
