@@ -35,6 +35,15 @@ inline int f8_check(const char* op, const char* name, const Span& s, int align) 
   }
   return P0_OK;
 }
+// a launch of n workgroups: at most 2^32 threads lie along x, the rest goes along y (f8_group gives a workgroup's number; the last ones may
+// be past n)
+inline bool f8_grid(int64_t n, int threads, dim3* g) {
+  const int64_t x = (1ll << 31) / threads, y = (n + x - 1) / x;
+  if (y > 65535) return false;
+  *g = dim3((unsigned)(y > 1 ? x : n), (unsigned)y);
+  return true;
+}
+__device__ __forceinline__ int64_t f8_group() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 inline bool f8_type(int t) { return t >= P0_F32 && t <= P0_BF16; }
 inline int f8_size(int t) { return t == P0_F32 ? 4 : 2; }
 inline int64_t f8_blocks(int64_t n) { return (n + kF8Block - 1) / kF8Block; }
@@ -115,15 +124,23 @@ __device__ __forceinline__ float f8_max16(float v) {   // of the lane's 16: rota
   v = fmaxf(v, f8_dpp<0x122>(v));
   return fmaxf(v, f8_dpp<0x121>(v));
 }
-// the largest finite magnitude of 8 values
+// the largest magnitude of 8 values (NaN does not count), and the largest finite one
 __device__ __forceinline__ float f8_most(const float (&f)[8]) {
+  float most = fabsf(f[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) most = fmaxf(most, fabsf(f[j]));
+  return most;
+}
+__device__ __forceinline__ float f8_most_finite(const float (&f)[8]) {
   float most = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float a = fabsf(f[j]);
-    most = fmaxf(most, a < INFINITY ? a : 0.0f);
-  }
+  for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.0f);
   return most;
+}
+// the largest finite magnitude of a block, 8 values a lane of 16. A block of NaN alone has none (0), one with an infinity is looked through again
+__device__ __forceinline__ float f8_block_most(const float (&f)[8]) {
+  const float most = f8_max16(f8_most(f));
+  return most < INFINITY ? most : f8_max16(f8_most_finite(f));
 }
 // max(most / 448, 2^-126) and 1 / s, each rounded to nearest: a reciprocal within a unit, and one correction that makes it and a quotient right
 // to the last bit (every mantissa tried; quotients below 2^-126 do not count). The divisions in full are 25 instructions of some 100 for 8 values

@@ -434,6 +434,7 @@ int f8_gemm_init() {
 // blocks, each tile and slicing measured on its own: the fastest by them is on average within 1% of the fastest measured, 13%
 // at the worst (2048 rows, 2048 outputs, 64 blocks: 43.8 for 38.6). Measured (us; 16-bit results, small / low / half / long / wide):
 // 64 rows, 16384 x 2048: 11.0 / 12.9 / 14.1 / 20 / 30; 256 rows 34 / 23 / 16.1 / 22 / 38; 1021 rows - / 88 / 57 / 44 / 38.7.
+constexpr int64_t kF8Groups = (1 << 23) - 1;   // workgroups of 512 threads: less than 2^32 threads
 struct F8Shape {
   int bn, bm;
   float block, round;       // 16-bit results
@@ -444,7 +445,7 @@ constexpr F8Shape kF8Shapes[] = {{64, 64, 0.32f, 2.4f, 0.51f, 3.6f},       // Ti
                                  {128, 128, 0.61f, 2.4f, 0.94f, 7.1f},     // TileHalf
                                  {128, 256, 1.01f, 3.3f, 1.54f, 9.8f},     // TileLong
                                  {256, 256, 1.73f, 8.0f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
-static void f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
+static bool f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
   const bool f32 = type == P0_F32;
   const int cus = ctx().cu_count;
   float least = 0.0f;
@@ -455,17 +456,20 @@ static void f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
     for (int n = 1; n <= 16; n *= 2) {
       if (n > 1 && (k == 4 || p.blocks / n < 4 || tiles * n > cus || (size_t)tiles * n * c.bn * c.bm > ctx().part_floats)) break;
       const int64_t groups = tiles * n, rounds = (groups + cus - 1) / cus;
+      if (groups > kF8Groups) break;
       const float fill = groups < cus ? (float)groups / cus : 1.0f, alone = f32 ? 0.8f : 0.67f;   // a chip that is not full runs a little faster
       const float t = rounds * ((p.blocks + n - 1) / n * (f32 ? c.block32 : c.block) * (alone + (1.0f - alone) * fill) + (f32 ? c.round32 : c.round)) +
                       (n > 1 ? 1.5f + 0.265f * n * (c.bn * c.bm / 4096) : 0.0f);
       if (kind < 0 || t < least) { least = t; kind = k; nks = n; }
     }
   }
+  if (kind < 0) return false;
   if (kind == 0) f8_tile_launch<TileSmall>(p, type, nks, s);
   else if (kind == 1) f8_tile_launch<TileLow>(p, type, nks, s);
   else if (kind == 2) f8_tile_launch<TileHalf>(p, type, nks, s);
   else if (kind == 3) f8_tile_launch<TileLong>(p, type, nks, s);
   else f8_tile_launch<TileWide>(p, type, 1, s);
+  return true;
 }
 
 static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
@@ -473,7 +477,7 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   if (!a) { set_error("%s: no arguments", op); return P0_EINVAL; }
   if (!f8_type(a->type)) { set_error("%s: type %d", op, (int)a->type); return P0_EINVAL; }
   if (a->M < 0 || a->M > (1 << 30)) { set_error("%s: M %lld", op, (long long)a->M); return P0_EINVAL; }
-  if (a->N < 0 || a->N > (1 << 30)) { set_error("%s: N %lld", op, (long long)a->N); return P0_EINVAL; }
+  if (a->N < 0 || a->N > (1 << 26)) { set_error("%s: N %lld", op, (long long)a->N); return P0_EINVAL; }
   if (a->K < 128 || a->K % 128 || a->K > (1 << 20)) { set_error("%s: K %lld must be a multiple of 128", op, (long long)a->K); return P0_EINVAL; }
   if (a->M == 0 || a->N == 0) { if (int r = refuse_in_chain(op)) return r; return require_open(op); }
   const int size = f8_size(a->type);
@@ -489,8 +493,6 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   if (int r = f8_check(op, "ws", ws, 4)) return r;
   if (int r = f8_check(op, "y", y, size)) return r;
   if (overlap(x, y) || overlap(w, y) || overlap(xs, y) || overlap(ws, y)) { set_error("%s: y overlaps an input", op); return P0_EINVAL; }
-  const int64_t tiles = (N + 15) / 16 * ((M + 15) / 16);
-  if (tiles >= (1ll << 31)) { set_error("%s: %lld x %lld outputs", op, (long long)M, (long long)N); return P0_EINVAL; }
   if (int r = refuse_in_chain(op)) return r;
   if (int r = require_open(op)) return r;
   F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks};
@@ -504,8 +506,9 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
     else if (M <= 8 && blocks >= 32) f8_thin_launch<16, 1, false>(p, a->type, ctx().cur);
     else if (M > 8 && N >= 8192) f8_thin_launch<4, 2, false>(p, a->type, ctx().cur);
     else f8_thin_launch<8, 1, false>(p, a->type, ctx().cur);
-  } else {
-    f8_tile_choice(p, a->type, ctx().cur);
+  } else if (!f8_tile_choice(p, a->type, ctx().cur)) {
+    set_error("%s: %lld x %lld outputs", op, (long long)M, (long long)N);
+    return P0_EINVAL;
   }
   P0_LAUNCHED(op);
   return P0_OK;

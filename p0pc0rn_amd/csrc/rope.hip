@@ -65,8 +65,9 @@ template <int TYPE, int KIND> __device__ __forceinline__ void rope_pairs(const v
 template <int TYPE, int KIND>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeP p) {
   __shared__ __attribute__((aligned(16))) float2 turn[kRopeTable];
-  const int64_t blk = blockIdx.x / (unsigned)p.hblocks, row0 = blk * p.rb;
-  const int h0 = (int)(blockIdx.x - blk * p.hblocks) * p.hb, pairs = p.dim / 2;
+  const int64_t group = f8_group(), blk = group / p.hblocks, row0 = blk * p.rb;
+  const int h0 = (int)(group - blk * p.hblocks) * p.hb, pairs = p.dim / 2;
+  if (row0 >= p.rows) return;
   const int rows = (int)(p.rows - row0 < p.rb ? p.rows - row0 : p.rb), hb = p.heads - h0 < p.hb ? p.heads - h0 : p.hb;
   for (int k = threadIdx.x; k < rows * pairs; k += kRopeThreads) {
     const int r = k / pairs;
@@ -209,9 +210,9 @@ static int rope_call(const p0_rope_args_t* a) {
   p.rb = side * rounds / p.hb;
   if (p.rb > kRopeTable / pairs) p.rb = kRopeTable / pairs;
   p.hblocks = (int)((heads + p.hb - 1) / p.hb);
-  const int64_t grid = (a->rows + p.rb - 1) / p.rb * p.hblocks;
-  if (grid >= (1ll << 31)) { set_error("%s: %lld rows of %lld heads", op, (long long)a->rows, (long long)heads); return P0_EINVAL; }
-#define P0_ROPE(T) if (a->type == T) hipLaunchKernelGGL((kind == 0 ? rope_kernel<T, 0> : kind == 1 ? rope_kernel<T, 1> : rope_kernel<T, 2>), dim3((unsigned)grid), dim3(kRopeThreads), 0, ctx().cur, p)
+  dim3 grid;
+  if (!f8_grid((a->rows + p.rb - 1) / p.rb * p.hblocks, kRopeThreads, &grid)) { set_error("%s: %lld rows of %lld heads", op, (long long)a->rows, (long long)heads); return P0_EINVAL; }
+#define P0_ROPE(T) if (a->type == T) hipLaunchKernelGGL((kind == 0 ? rope_kernel<T, 0> : kind == 1 ? rope_kernel<T, 1> : rope_kernel<T, 2>), grid, dim3(kRopeThreads), 0, ctx().cur, p)
   P0_ROPE(P0_F32);
   P0_ROPE(P0_F16);
   P0_ROPE(P0_BF16);

@@ -348,7 +348,8 @@ def test_gemm_of_one_code_finds_every_place(dev, M, N, K, type_):
         xc[np.arange(M), at] = f8.encode(1.0)
         xs[:] = (1 + np.arange(K // 128) % 4)[:, None]
         rng = np.random.default_rng(M)
-        wc = f8.encode(rng.integers(-15, 16, (N, K)).astype(np.float64))
+        wc = rng.integers(0, 254, (N, K)).astype(np.uint8)                # any code, the least ones among them
+        wc[(wc & 127) == 127] = 1
         ws = (2.0 ** rng.integers(-3, 4, (f8.blocks(N), K // 128))).astype(np.float32)
         x, w, xsr, wsr = Rows(np.uint8, M, K, raw=xc), Rows(np.uint8, N, K, raw=wc), Rows(np.float32, K // 128, M, raw=xs), Rows(np.float32, f8.blocks(N), K // 128, raw=ws)
         y = Rows(RAW[type_], M, N)
@@ -415,3 +416,38 @@ def test_calls_refused_in_a_chain(dev):
         capi.lib().p0_chain_end(ctypes.byref(h))
         if h.value:
             capi.lib().p0_chain_free(h)
+
+
+def test_rows_far_apart(dev):
+    """rows 2 GiB apart: offsets past 32 bits in what each operator reads and writes"""
+    ld, rows = (1 << 30) + 64, 3
+    rng = np.random.default_rng(3)
+    far = capi.Buffer(2 * (2 * ld + 1024))
+    x = to_type(rng.standard_normal((rows, 256)).astype(np.float32), "bf16")
+    put = lambda: [far.upload(x[0][i], 2 * i * ld) for i in range(rows)]  # noqa: E731
+    get = lambda n: np.stack([far.read(np.uint16, n, 2 * i * ld) for i in range(rows)])  # noqa: E731
+    put()
+    y, s = Rows(np.uint8, rows, 256), Rows(np.float32, 2, rows)
+    capi.f8_rows(capi.f8_rows_args(x=far, ldx=ld, type=2, M=rows, D=256, y=y.ptr, s=s.ptr))
+    wc, ws = f8.quantise(x[1].astype(np.float32))
+    assert np.array_equal(y.read(), wc) and np.array_equal(s.read(), ws)
+    capi.f8_pack(capi.f8_pack_args(x=far, ldx=ld, type=2, N=rows, K=256, w=y.ptr, s=s.ptr, lds=2))
+    assert np.array_equal(y.read(), f8.pack(x[1].astype(np.float32))[0])
+    capi.f8_norm(capi.f8_norm_args(x=far, ldx=ld, type=2, t=far, t_type=2, ldt=ld, x_out=far.ptr + 512, ldo=ld, M=rows, D=256, y=y.ptr, s=s.ptr))
+    assert np.array_equal(np.stack([far.read(np.uint16, 256, 2 * i * ld + 512) for i in range(rows)]), to_type((2 * x[1]).astype(np.float32), "bf16")[0])
+    put()
+    pos = capi.to_device(np.zeros(rows, np.int32))
+    capi.rope(capi.rope_args(x=far, ldr=ld, y=far, y_ldr=ld, type=2, rows=rows, hq=4, dim=64, pos=pos))
+    assert np.array_equal(get(256), x[0])
+    for M in (rows, 20):   # a product whose rows are far apart: the kernel for few rows, and one of tiles into columns of one buffer
+        n = 24
+        ops = operands(rng, M, n, 128)
+        dv = [capi.to_device(o) for o in ops]
+        out = capi.Buffer(4 * ((M - 1) * (1 << 28) + n)) if M == rows else capi.Buffer(4 * M * (1 << 26))
+        ldy = (1 << 28) if M == rows else (1 << 26)
+        capi.f8_gemm(capi.f8_gemm_args(x=dv[0], xs=dv[1], w=dv[2], ws=dv[3], M=M, N=n, K=128, type=0, y=out, ldy=ldy))
+        product_near(np.stack([out.read(np.float32, n, 4 * i * ldy) for i in range(M)]).astype(np.float64), "f32", *ops, 128)
+        for b in dv + [out]:
+            b.free()
+    for b in (far, y, s, pos):
+        b.free()

@@ -116,6 +116,7 @@ ROPE = dict(x=P, y=P + BIG, type=1, rows=4, hq=2, hk=1, dim=64, pos=P + 2 * BIG)
     (GEMM, "f8_gemm", dict(K=0), "f8_gemm: K 0 must be a multiple of 128"),
     (GEMM, "f8_gemm", dict(K=192), "f8_gemm: K 192 must be a multiple of 128"),
     (GEMM, "f8_gemm", dict(M=-1), "f8_gemm: M -1"),
+    (GEMM, "f8_gemm", dict(N=(1 << 26) + 1), "f8_gemm: N 67108865"),
     (GEMM, "f8_gemm", dict(type=4), "f8_gemm: type 4"),
     (GEMM, "f8_gemm", dict(ldx=1 << 23), "f8_gemm: rows 8388608 and 256 B apart"),
     (GEMM, "f8_gemm", dict(ldw=264), "f8_gemm: w must be 16-byte aligned, its rows too"),
