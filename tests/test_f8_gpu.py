@@ -306,6 +306,37 @@ def test_gemm_sizes(dev, M, N, K):
     product_near(got, "f32", *ops, K)
 
 
+# rows, outputs and k that take each tile, in one and in more slices of k, ragged at both ends
+@pytest.mark.parametrize("M,N,K,type_", [(23, 4327, 2560, "f16"), (27, 33, 2048, "bf16"), (94, 21, 5120, "f32"), (17, 6123, 2048, "f32"),
+                                         (77, 8820, 128, "f32"), (17, 8431, 5120, "bf16"), (17, 4191, 5120, "f32"),
+                                         (195, 8757, 128, "f16"), (195, 8757, 128, "f32"), (69, 8194, 5120, "bf16"), (65, 4395, 8192, "f32"),
+                                         (390, 8346, 128, "bf16"), (522, 7318, 128, "f32"), (387, 8171, 8192, "f16"), (200, 8694, 8192, "f32"),
+                                         (1025, 7295, 384, "f16"), (1025, 7295, 384, "bf16"), (1021, 16383, 2048, "bf16"), (1537, 9217, 1280, "f16")])
+def test_gemm_tiles(dev, M, N, K, type_):
+    """a sample of the rows and outputs, the first and the last among them (the whole product is the GPU's work)"""
+    rng = np.random.default_rng(M)
+    xc, wc = rng.integers(0, 254, (M, K)).astype(np.uint8), rng.integers(0, 254, (N, K)).astype(np.uint8)
+    xc[(xc & 127) == 127], wc[(wc & 127) == 127] = 0, 0
+    xs, ws = np.exp(rng.standard_normal((K // 128, M))).astype(np.float32) * 1e-3, np.exp(rng.standard_normal((f8.blocks(N), K // 128))).astype(np.float32) * 1e-4
+    x, w, xsr, wsr = (Rows(a.dtype, a.shape[0], a.shape[1], raw=a) for a in (xc, wc, xs, ws))
+    y = Rows(RAW[type_], M, N)
+    capi.f8_gemm(capi.f8_gemm_args(x=x.ptr, xs=xsr.ptr, w=w.ptr, ws=wsr.ptr, M=M, N=N, K=K, type=capi.TYPE[type_], y=y.ptr))
+    got = from_type(y.read(), type_).reshape(M, N)
+    m = np.unique(np.r_[0, M - 1, rng.integers(0, M, 40)])
+    n = np.unique(np.r_[0, N - 1, np.arange(0, N, 128), rng.integers(0, N, 60)])
+    full = f8.weight(wc, ws)[n]
+    a = f8.values(xc[m], np.ascontiguousarray(xs[:, m]))
+    want, total = a @ full.T, np.abs(a) @ np.abs(full).T
+    bound = (128 + 2 * K / 128) * 2.0 ** -23 * total
+    if type_ != "f32":
+        for k in range(0, K, 8):
+            bound += 7 * 2.0 ** -13 * (np.abs(a[:, None, k:k + 8]) * np.abs(full[None, :, k:k + 8])).max(2)
+    err = np.abs(got[np.ix_(m, n)] - want)
+    assert (err <= bound + HALF[type_] * (np.abs(want) + bound) + TINY[type_]).all(), (err / np.maximum(bound, 1e-30)).max()
+    for r in (x, w, xsr, wsr, y):
+        r.free()
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 100, 512), (13, 500, 640), (70, 390, 256), (300, 770, 384), (600, 2050, 640)])
 @pytest.mark.parametrize("type_", ["f16", "bf16"])
 def test_gemm_types(dev, M, N, K, type_):
