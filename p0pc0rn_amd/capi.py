@@ -582,11 +582,14 @@ def f8_gemm(args):
     check(lib().p0_f8_gemm(C.byref(args)))
 
 
+_Axes = i32 * 4
+
+
 def rope_args(**kw):
     """axis_dim is a sequence of 1 .. 4 channel counts, one per axis"""
     dims = kw.get("axis_dim")
     if dims is not None:
-        kw["axis_dim"] = (i32 * 4)(*dims)
+        kw["axis_dim"] = _Axes(*dims)
         kw.setdefault("axes", len(dims))
     return _fields(RopeArgs, kw)
 
