@@ -539,7 +539,7 @@ int p0_f8_gemm(const p0_f8_gemm_args_t* a);
  * one that holds channel 2 i when the axes lie one after the other, its angle pos[a][row] theta^-e with e = 2 j / axis_dim[a], j
  * the pair's place within its axis (freq 0), or e = 2 i / R (freq 1): (u, v) -> (u cos - v sin, v cos + u sin). Positions are
  * int32, pos[a * pos_ld + row] (pos_ld 0 = rows); angles are held in 64 bits, so far positions lose nothing. axes 0 counts as
- * 1, an axis_dim[0] of 0 with one axis as dim, theta 0 as 10000. */
+ * 1, an axis_dim[0] of 0 with one axis as dim, theta 0 as 10000; theta is at least 1: no pair turns by more than 1 rad a position. */
 typedef struct {
   const void* x; int64_t ldr, ldh;
   void* y; int64_t y_ldr, y_ldh;

@@ -82,7 +82,10 @@ template <int TYPE> __device__ __forceinline__ void store4(const F8GemmP& p, int
   }
 }
 
-// Few rows: a workgroup takes 16 NT outputs of 16 rows, its W waves the blocks of k in turn; their sums meet in LDS.
+// Few rows: a workgroup takes 16 NT outputs of 16 rows, its W waves the blocks of k in turn; their sums meet in LDS. A wave's loads are
+// all on their way before its first product; no LDS in between, as no two waves want the same byte of the weight.
+// Bound: the weight's bytes, and below some 30 MB of them launch and round trips: 1 row, 16384 outputs x 2048 k 7.4 us (33.6 MB, 4.5 TB/s), 5 rows,
+// 2048 x 8192 6.5 us (16.9 MB, 2.6 TB/s).
 // PAIR: 8 outputs of up to 8 rows, two blocks of k at a time: the matrix instruction's rows 8 - 15 are the same weights' next block, its columns 8 - 15 the
 // same rows', and of its four quarters the two that pair a block with itself are kept.
 template <int TYPE, int W, int NT, bool PAIR>
@@ -172,6 +175,11 @@ __device__ __forceinline__ void tile_out(const F8GemmP& p, const f32x4 (&acc)[AM
 // (and g ^ 4) of rows 0 .. 15 for the lane groups g = 0 .. 3, and LDS serves lanes 0-3, 12-15 of one group with 4-11 of the next; under key = r & 6 those
 // 16 lie in 16 different (row parity, position) pairs, so no bank conflicts (the counter reads 0; a key that suits 16 lanes of one
 // group each, (r ^ r / 8) & 7, read 48%).
+// Bound: the matrix instructions at the clock that they leave. 4608 rows, 9216 outputs x 9216 k, fp16 results: 352-357 us, 2.2 PFLOP/s (a
+// library's product with a scale per row 327; of 8192 each way 2.36). On random codes the 16 x 16 x 128 instruction by itself reaches 3.75 PFLOP/s, with an fma a
+// value beside it 3.38, on zeros 4.88: the clock goes down under them. Tried on the widest tile, us: 32 x 32 x 64 instructions the same; two groups of waves
+// half a step apart the same; the next stage's lines into L2 ahead 9% more; workgroups that stay and take tile after tile 359; the tiles' blocks of
+// k dealt out evenly 402 (neighbours no longer share lines in L2); bands of 2 or 8 row tiles slower.
 // One barrier a step, ahead of the step's last matrix instructions: every wave then holds the rest of its step in registers, the
 // next step's first fragments are read while those run, and the stage just left is free for loads.
 __device__ __forceinline__ int f8_key(int r) { return r & 6; }
@@ -431,9 +439,10 @@ int f8_gemm_init() {
 
 // Which tile, and how many slices of K, by time: a round of workgroups takes its blocks of k, one after the other, and then its outputs; a
 // slice's sums go through memory. The figures (us a block and a round) are fitted to 67 shapes of 17 to 2048 rows, 512 to 16384 outputs, 16 to 72
-// blocks, each tile and slicing measured on its own: the fastest by them is on average within 1% of the fastest measured, 13%
-// at the worst (2048 rows, 2048 outputs, 64 blocks: 43.8 for 38.6). Measured (us; 16-bit results, small / low / half / long / wide):
-// 64 rows, 16384 x 2048: 11.0 / 12.9 / 14.1 / 20 / 30; 256 rows 34 / 23 / 16.1 / 22 / 38; 1021 rows - / 88 / 57 / 44 / 38.7.
+// blocks, each tile and slicing measured on its own: the fastest by them is on average within 1% of the fastest measured, 12%
+// at the worst (2048 rows, 2048 outputs, 64 blocks: 44.9 for 40.2). Measured (us; 16384 outputs x 2048 k, small / low / half / long / wide): bf16 results,
+// 64 rows 11.1 / 12.7 / 13.2 / 17.4 / 28.9; 256 rows 36 / 23 / 18.1 / 21.5 / 33; 1021 rows 137 / 89 / 57 / 46 / 37.8; fp32, 1021 rows 199 / 134 /
+// 95 / 75. Slices (256 rows, 2048 outputs x 8192 k): low in 1 / 2 / 4 27.9 / 19.4 / 16.0, half in 8 20.8.
 constexpr int64_t kF8Groups = (1 << 23) - 1;   // workgroups of 512 threads: less than 2^32 threads
 struct F8Shape {
   int bn, bm;

@@ -17,7 +17,9 @@ struct PackP {
   int blocks;   // of 128 channels in a row
   int vec;
 };
-// A workgroup takes a block of 128 x 128, a thread 8 rows of 8 channels.
+// A workgroup takes a block of 128 x 128, a thread 8 rows of 8 channels: 8 loads of 16 bytes on their way at once.
+// Bound: HBM (18432 x 9216 bf16 values: 99.8 us for 510 MB, 5.1 TB/s; a copy of as many bytes 95); launch and round trips for small ones (1536 x
+// 2048 f16 values, 192 workgroups: 4.9 us).
 template <int TYPE>
 __global__ __launch_bounds__(256) void f8_pack_kernel(const PackP p) {
   __shared__ float red[4];
@@ -72,7 +74,8 @@ struct RowsF8P {
   int vec, glu;
 };
 // A workgroup takes a strip of 256 >> ls rows.
-// Bound: HBM (4608 rows of 9216 f16 channels: 24 us for 128 MB, 5.3 TB/s), gated ones nearly as much the arithmetic: 45 us for 212 MB, 4.7 TB/s.
+// Bound: HBM (4608 rows of 9216 f16 channels: 24 us for 128 MB, 5.3 TB/s), gated ones nearly as much the arithmetic: 45-48 us for 214 MB, 4.6 TB/s (a copy of as
+// many bytes 41). Few rows are a launch (5 of 8192 fp32 channels, gated: 4.9 us).
 // With two rows a thread 47.6, four 51.6: the other waves cover a wave's loads better than its own.
 template <int TYPE, bool GLU>
 __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsF8P p) {
@@ -121,8 +124,8 @@ __device__ __forceinline__ float sum64(float v) {
 // A workgroup takes a row, its up to 16 waves 512 channels each of NC steps, a lane 8 of them. The row stays in registers; each sum is one
 // exchange through LDS.
 // VEC: every run of 8 channels is there whole or not at all, and 16-byte aligned everywhere.
-// Bound: HBM at many rows (32760 rows of 2560 bf16 channels, modulated: 112 us for 588 MB, 5.2 TB/s; a copy 5.5), launch and round trips
-// at few (1 row of 2048 fp32 channels: 3.6 us). A wave with a row of its own, four in a workgroup, took 136 and 3.7: five loads a lane
+// Bound: HBM at many rows (32760 rows of 2560 bf16 channels, modulated: 112-122 us for 590 MB, 4.9-5.3 TB/s; a copy of as many bytes 114),
+// launch and round trips at few (1 row of 2048 fp32 channels: 3.9-4.2 us back to back, 5.5 with the host's part). A wave with a row of its own, four in a workgroup, took 136 and 3.7: five loads a lane
 // at a time and their registers leave fewer waves to cover them.
 template <int XT, int TT, int NC, bool VEC>
 __global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
@@ -341,8 +344,8 @@ static int norm_call(const p0_f8_norm_args_t* a) {
                                   (uintptr_t)(ldt * tsize) | (uintptr_t)a->tw | (uintptr_t)a->w | (uintptr_t)a->b) % 16 == 0;
   p.mode = a->mode; p.one = a->w_one ? 1 : 0; p.scale = scale; p.eps = a->eps != 0.0f ? a->eps : 1e-6f;
   // Waves of one step, but for two where rows are longer than 16 waves' one, and for 16-bit rows that fill the chip several times over (us,
-  // one step / two: 32760 rows of 2560 bf16 channels 129 / 112, 4608 of 4096 28.9 / 27.4; 1021 of 1536 5.0 / 5.8; 4608 of 2048 fp32 channels
-  // 23.9 / 25.7), and four for the longest
+  // one step / two: 32760 rows of 2560 bf16 channels 128 / 112, 4608 of 4096 28.9 / 27.4; 1021 of 1536 5.0 / 5.8; 4608 of 2048 fp32 channels
+  // 23.8 / 25.6), and four for the longest
   const int steps = (int)((K8 + 511) / 512);
   const bool two = vec && (steps > 16 || (xsize == 2 && steps > 1 && M * steps >= 16384));
   const int NC = steps > (vec ? 32 : 16) ? 4 : two ? 2 : 1, W = (steps + NC - 1) / NC;

@@ -135,6 +135,9 @@ ROPE = dict(x=P, y=P + BIG, type=1, rows=4, hq=2, hk=1, dim=64, pos=P + 2 * BIG)
     (ROPE, "rope", dict(axis_dim=[32, 15]), "rope: axis 1 of 15 channels (heads of 64)"),
     (ROPE, "rope", dict(axis_dim=[32, 0]), "rope: axis 1 of 0 channels (heads of 64)"),
     (ROPE, "rope", dict(theta=-1.0), "rope: theta -1"),
+    (ROPE, "rope", dict(theta=0.5), "rope: theta 0.5"),
+    (ROPE, "rope", dict(theta=float("nan")), "rope: theta nan"),
+    (ROPE, "rope", dict(theta=float("inf")), "rope: theta inf"),
     (ROPE, "rope", dict(ldh=62), "rope: heads 62 and 64 apart"),
     (ROPE, "rope", dict(ldr=128), "rope: x has rows of 384 B, 256 B apart"),
     (ROPE, "rope", dict(pos=None), "rope: missing pos buffer"),
