@@ -16,6 +16,8 @@
 #include "dma.hpp"
 #include "f8_common.hpp"
 
+#include <type_traits>
+
 namespace p0 {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -189,7 +191,9 @@ struct F8Tile {
   static constexpr int WN = WN_, WM = WM_, AN = AN_, AM = AM_, S = S_;
   static constexpr int Waves = WN * WM, Threads = 64 * Waves, BN = 16 * AN * WN, BM = 16 * AM * WM;
   static constexpr int Rows = BN + BM, Loads = Rows / 8 / Waves;   // loads of 8 rows, per wave
-  static constexpr int Codes = Rows * 128, Stage = Codes + 4 * (BM < 64 ? 64 : BM), Lds = S * Stage;
+  static constexpr int Codes = Rows * 128, Stage = Codes + 4 * (BM < 64 ? 64 : BM), Ring = S * Stage;
+  static constexpr int Lds = Ring + 512 * Waves;   // behind the stages: a wave's weight scales, of 64 steps and of the next 64
+  static constexpr bool Slices = AN * AM < 32;   // the widest tile is for outputs that fill the chip without
   static_assert(Rows % (8 * Waves) == 0 && 128 % (16 * AN) == 0 && BM <= 64 * Waves, "tile");
 };
 
@@ -250,9 +254,12 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   const int chunk = (g ^ f8_key(l16)) << 4, wrow = (wn * 16 * T::AN + l16) * 128, xrow = (T::BN + wm * 16 * T::AM + l16) * 128;
   const int w0 = wrow + chunk, w1 = wrow + (chunk ^ 64), x0 = xrow + chunk, x1 = xrow + (chunk ^ 64);
   const int srow = T::Codes + (wm * 16 * T::AM + l16) * 4;
-  // the weight's scales of this wave's rows: 64 steps' in a lane each
-  const float* ws = p.ws + (int64_t)(min(n0 + wn * 16 * T::AN, p.N - 1) >> 7) * p.ldws;
-  float wsv = 0.0f;
+  // the weight's scales of this wave's rows: 64 steps' at a time, 64 steps ahead
+  const i32x4 rws = resource(p.ws + (int64_t)(min(n0 + wn * 16 * T::AN, p.N - 1) >> 7) * p.ldws);
+  const int wsat = T::Ring + wv * 512;
+  auto load_ws = [&](int kb) { dma4(lbase + wsat + ((kb - kb0) & 64) * 4, min(kb + lane, nk - 1) * 4, rws, 0); };
+  float w;
+  auto read_ws = [&](int kb) { w = *(const float*)(lds + wsat + ((kb - kb0) & 127) * 4); };
 
   i32x8 wf[2], xf[T::AM];
   half8v xh[Exact ? T::AM : 1][4], wh[4];
@@ -279,11 +286,7 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
     asm volatile("" : "+v"(v));   // here and below: keeps the cell's order
   };
   auto step = [&](int kb, const uint8_t* st, const uint8_t* st_next, int st_load) {
-    if (((kb - kb0) & 63) == 0) {
-      wsv = ws[min(kb + lane, nk - 1)];
-      asm volatile("" : "+v"(wsv));   // waited for here: no other step has a wait of its own for it
-    }
-    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wsv), (kb - kb0) & 63));
+    if (((kb - kb0) & 63) == 0 && kb + 64 < nk) load_ws(kb + 64);   // (one load more than the count below knows of: that waits for more, not less)
     if constexpr (Exact) {
 #pragma unroll
       for (int j = 0; j < T::AM; ++j) to_half(xf[j], xh[j]);
@@ -321,24 +324,27 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
 #pragma unroll
         for (int k = 0; k < T::AM; ++k) s[k] = sf[k] * w;
       }
+      if (q == Q - 1) read_ws(kb + 1);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  load_ws(kb0);
 #pragma unroll
   for (int kb = 0; kb < T::S - 1; ++kb) {
 #pragma unroll
     for (int l = 0; l < T::Loads; ++l) load(kb0 + kb, kb * T::Stage, l);
     load_scales(kb0 + kb, kb * T::Stage);
   }
-  wait_dma<0>();
+  wait_dma<(T::S - 2) * (T::Loads + 1)>();   // the first stage has come
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int j = 0; j < T::AM; ++j) read_x(lds, j);
   read_w(lds, 0);
+  read_ws(kb0);
   int at = 0, to = (T::S - 1) * T::Stage;
   for (int kb = kb0; kb < nk; ++kb) {
-    const int next = at + T::Stage == T::Lds ? 0 : at + T::Stage;
+    const int next = at + T::Stage == T::Ring ? 0 : at + T::Stage;
     step(kb, lds + at, lds + next, to);
     to = at;
     at = next;
@@ -347,7 +353,7 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   fold(Q - 1);
   wait_dma<0>();   // loads that nothing reads must not land in another workgroup's LDS
 
-  if (a.nks > 1) {
+  if (T::Slices && a.nks > 1) {
     // The slices' sums meet in the workspace: it is uncached, a store is in memory once acknowledged and device-scope loads read memory,
     // so the arrival count needs no fence. The last workgroup to arrive adds the slices in order and leaves the count at zero.
     typedef unsigned long long u64;
@@ -378,21 +384,30 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
       f32x4 v[QB];
 #pragma unroll
       for (int q = 0; q < QB; ++q) v[q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      for (int k = 0; k < a.nks; ++k) {
-        u64 w[QB][2];
+      auto add = [&](auto count, int k0) {   // `count` slices' words on their way together
+        constexpr int KB = decltype(count)::value;
+        u64 w[KB][QB][2];
 #pragma unroll
-        for (int q = 0; q < QB; ++q)
+        for (int k = 0; k < KB; ++k)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            w[q][h] = __hip_atomic_load(all + k * slice + ((q0 + q) * 2 + h) * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          for (int q = 0; q < QB; ++q)
 #pragma unroll
-        for (int q = 0; q < QB; ++q)
+            for (int h = 0; h < 2; ++h)
+              w[k][q][h] = __hip_atomic_load(all + (k0 + k) * slice + ((q0 + q) * 2 + h) * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            v[q][2 * h] += __uint_as_float((uint32_t)w[q][h]);
-            v[q][2 * h + 1] += __uint_as_float((uint32_t)(w[q][h] >> 32));
-          }
-      }
+        for (int k = 0; k < KB; ++k)
+#pragma unroll
+          for (int q = 0; q < QB; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              v[q][2 * h] += __uint_as_float((uint32_t)w[k][q][h]);
+              v[q][2 * h + 1] += __uint_as_float((uint32_t)(w[k][q][h] >> 32));
+            }
+      };
+      int k = 0;
+      for (; k + 4 <= a.nks; k += 4) add(std::integral_constant<int, 4>{}, k);
+      for (; k + 2 <= a.nks; k += 2) add(std::integral_constant<int, 2>{}, k);
+      if (k < a.nks) add(std::integral_constant<int, 1>{}, k);
 #pragma unroll
       for (int q = 0; q < QB; ++q) acc[(q0 + q) % T::AM][(q0 + q) / T::AM] = v[q];
     }
@@ -438,22 +453,22 @@ int f8_gemm_init() {
 }
 
 // Which tile, and how many slices of K, by time: a round of workgroups takes its blocks of k, one after the other, and then its outputs; a
-// slice's sums go through memory. The figures (us a block and a round) are fitted to 67 shapes of 17 to 2048 rows, 512 to 16384 outputs, 16 to 72
-// blocks, each tile and slicing measured on its own: the fastest by them is on average within 1% of the fastest measured, 12%
-// at the worst (2048 rows, 2048 outputs, 64 blocks: 44.9 for 40.2). Measured (us; 16384 outputs x 2048 k, small / low / half / long / wide): bf16 results,
-// 64 rows 11.1 / 12.7 / 13.2 / 17.4 / 28.9; 256 rows 36 / 23 / 18.1 / 21.5 / 33; 1021 rows 137 / 89 / 57 / 46 / 37.8; fp32, 1021 rows 199 / 134 /
-// 95 / 75. Slices (256 rows, 2048 outputs x 8192 k): low in 1 / 2 / 4 27.9 / 19.4 / 16.0, half in 8 20.8.
+// slice's sums go through memory. The figures (us a block and a round) are fitted to 122 shapes of 17 to 4489 rows, 65 to 18334 outputs, 1 to
+// 122 blocks, each tile and slicing measured on its own: the fastest by them is on average within 0.5% of the fastest measured, 12% at the
+// worst (83 rows, 158 outputs, 11 blocks, fp32: 8.7 for 7.8). Measured (us; 16384 outputs x 2048 k, small / low / half / long / wide): bf16
+// results, 64 rows 11.0 / 12.3 / 13.5 / 17.4 / 28.9; 256 rows 36 / 22.1 / 17.1 / 21.3 / 33; 1021 rows 137 / 89 / 55 / 45 / 37.8; fp32, 1021 rows
+// 199 / 134 / 91 / 75. Slices (256 rows, 2048 outputs x 8192 k): low in 1 / 2 / 4 27.9 / 19.1 / 15.7, half in 8 21.3.
 constexpr int64_t kF8Groups = (1 << 23) - 1;   // workgroups of 512 threads: less than 2^32 threads
 struct F8Shape {
   int bn, bm;
   float block, round;       // 16-bit results
   float block32, round32;   // fp32 results: half the matrix rate, conversions
 };
-constexpr F8Shape kF8Shapes[] = {{64, 64, 0.32f, 2.4f, 0.51f, 3.6f},       // TileSmall
-                                 {128, 64, 0.47f, 2.2f, 0.72f, 4.5f},      // TileLow
-                                 {128, 128, 0.61f, 2.4f, 0.94f, 7.1f},     // TileHalf
-                                 {128, 256, 1.01f, 3.3f, 1.54f, 9.8f},     // TileLong
-                                 {256, 256, 1.73f, 8.0f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
+constexpr F8Shape kF8Shapes[] = {{64, 64, 0.326f, 1.7f, 0.60f, 2.1f},      // TileSmall
+                                 {128, 64, 0.46f, 2.1f, 0.80f, 4.0f},      // TileLow
+                                 {128, 128, 0.613f, 2.55f, 1.02f, 7.2f},   // TileHalf
+                                 {128, 256, 1.036f, 4.3f, 1.49f, 15.7f},   // TileLong
+                                 {256, 256, 1.65f, 8.9f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
 static bool f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
   const bool f32 = type == P0_F32;
   const int cus = ctx().cu_count;
@@ -466,9 +481,9 @@ static bool f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
       if (n > 1 && (k == 4 || p.blocks / n < 4 || tiles * n > cus || (size_t)tiles * n * c.bn * c.bm > ctx().part_floats)) break;
       const int64_t groups = tiles * n, rounds = (groups + cus - 1) / cus;
       if (groups > kF8Groups) break;
-      const float fill = groups < cus ? (float)groups / cus : 1.0f, alone = f32 ? 0.8f : 0.67f;   // a chip that is not full runs a little faster
+      const float fill = groups < cus ? (float)groups / cus : 1.0f, alone = f32 ? 0.65f : 0.72f;   // a chip that is not full runs a little faster
       const float t = rounds * ((p.blocks + n - 1) / n * (f32 ? c.block32 : c.block) * (alone + (1.0f - alone) * fill) + (f32 ? c.round32 : c.round)) +
-                      (n > 1 ? 1.5f + 0.265f * n * (c.bn * c.bm / 4096) : 0.0f);
+                      (n > 1 ? 1.2f + (f32 ? 0.26f : 0.3f) * n * (c.bn * c.bm / 4096) : 0.0f);
       if (kind < 0 || t < least) { least = t; kind = k; nks = n; }
     }
   }

@@ -311,7 +311,13 @@ def test_gemm_sizes(dev, M, N, K):
                                          (77, 8820, 128, "f32"), (17, 8431, 5120, "bf16"), (17, 4191, 5120, "f32"),
                                          (195, 8757, 128, "f16"), (195, 8757, 128, "f32"), (69, 8194, 5120, "bf16"), (65, 4395, 8192, "f32"),
                                          (390, 8346, 128, "bf16"), (522, 7318, 128, "f32"), (387, 8171, 8192, "f16"), (200, 8694, 8192, "f32"),
-                                         (1025, 7295, 384, "f16"), (1025, 7295, 384, "bf16"), (1021, 16383, 2048, "bf16"), (1537, 9217, 1280, "f16")])
+                                         (1025, 7295, 384, "f16"), (1025, 7295, 384, "bf16"), (1021, 16383, 2048, "bf16"), (1537, 9217, 1280, "f16"),
+                                         # the same again for the figures of each tile as they are now; over 64 blocks of k in one go; 7 slices
+                                         (1537, 1282, 9216, "f16"), (1025, 906, 16640, "f32"), (259, 6531, 128, "f32"), (2050, 905, 128, "bf16"),
+                                         (1025, 975, 5120, "bf16"), (1537, 2435, 9216, "f16"), (1537, 2435, 9216, "f32"), (1537, 2561, 128, "bf16"),
+                                         (1537, 2562, 640, "f32"), (1537, 1281, 16640, "bf16"), (1537, 1292, 8192, "f32"), (1537, 1155, 9216, "f16"),
+                                         (1537, 1155, 9216, "f32"), (65, 8197, 128, "f32"), (700, 710, 5120, "f16"), (2050, 130, 16640, "f32"),
+                                         (2050, 3849, 9216, "f16"), (1537, 4993, 640, "bf16"), (130, 70, 4224, "f32"), (130, 70, 4224, "f16")])
 def test_gemm_tiles(dev, M, N, K, type_):
     """a sample of the rows and outputs, the first and the last among them (the whole product is the GPU's work)"""
     rng = np.random.default_rng(M)
