@@ -17,6 +17,7 @@
 #include "f8_common.hpp"
 
 #include <type_traits>
+#include <utility>
 
 namespace p0 {
 
@@ -31,6 +32,7 @@ struct F8GemmP {
   void* y;
   int64_t ldx, ldxs, ldw, ldws, ldy;
   int M, N, blocks;    // blocks of 128 k
+  int turned;          // few rows: workgroups go over the rows first
   int yvec;            // 1: 4 consecutive outputs from a multiple of 4 on are aligned together; 2: rows are 16-byte aligned
 };
 
@@ -82,6 +84,136 @@ template <int TYPE> __device__ __forceinline__ void store4(const F8GemmP& p, int
       for (int i = 0; i < 4; ++i)
         if (n + i < p.N) y[i] = (uint16_t)h[i];
   }
+}
+
+// A row's 16-byte chunk c of a block lies in LDS at position c ^ key(row): a fragment's read takes chunk g (and g ^ 4) of rows 0 .. 15 for the lane
+// groups g = 0 .. 3, and LDS serves lanes 0-3, 12-15 of one group with 4-11 of the next; under key = r & 6 those 16 lie in 16 different (row
+// parity, position) pairs, so no bank conflicts (the counter reads 0; a key that suits 16 lanes of one group each, (r ^ r / 8) & 7, read 48%).
+__device__ __forceinline__ int f8_key(int r) { return r & 6; }
+
+// Few rows: a workgroup takes 16 NT outputs (weight rows) of 8 XD rows, its W waves the blocks of k in turn; their sums meet in LDS. A wave
+// keeps S of its turns' blocks in LDS of its own, filled by loads that go straight there, 8 whole rows of 128 codes each: no barrier before the end.
+// Lanes that load their own fragments from global memory ask 64 times an instruction, 16 rows side by side, where these ask 16 times: 16 rows, 2048 x 8192
+// 9.4 us that way, 6.0 this.
+// PAIR: 8 outputs of up to 8 rows, two blocks of k at a time: the matrix instruction's rows 8 - 15 are the same weights' next block, its columns 8 - 15 the
+// same rows', and of its four quarters the two that pair a block with itself are kept.
+// Bound: the weight's bytes, and below some 30 MB of them launch and round trips: 1 row, 16384 outputs x 2048 k 7.6 us (33.6 MB, 4.4 TB/s), 9216 x 14720 24.8 us
+// (5.5 TB/s); 5 rows, 2048 x 8192 5.1 us (16.9 MB, 3.3 TB/s).
+template <int W_, int NT_, int XD_, bool PAIR_, int S_>
+struct F8Few {
+  static constexpr int W = W_, NT = NT_, XD = XD_, S = S_, MT = (XD + 1) / 2;
+  static constexpr bool PAIR = PAIR_;
+  static constexpr int BN = PAIR ? 8 : 16 * NT, BM = 8 * XD, Step = PAIR ? 2 : 1;   // outputs and rows of a workgroup, blocks of a wave's turn
+  static constexpr int XL = PAIR ? 2 : XD, Loads = 2 * NT + XL + Step;              // loads of x rows, all of a turn's
+  static constexpr int Codes = (2 * NT + XL) * 1024, Stage = Codes + 256 * Step, Mine = S * Stage + 512, Lds = W * Mine;
+  static_assert(!PAIR || (NT == 1 && XD == 1), "one tile of pairs");
+  static_assert(NT * MT <= W && NT * MT * 1024 <= Mine && BM <= 64, "tile");
+};
+
+template <int TYPE, class T>
+__global__ __launch_bounds__(64 * T::W) void f8_few_kernel(const F8GemmP p) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr int NT = T::NT, MT = T::MT, W = T::W, S = T::S, Step = T::Step;
+  constexpr bool Exact = TYPE == P0_F32 || T::BM <= 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, l16 = lane & 15;
+  const int n0 = (p.turned ? blockIdx.y : blockIdx.x) * T::BN, m0 = (p.turned ? blockIdx.x : blockIdx.y) * T::BM;
+  if (n0 >= p.N || m0 >= p.M) return;
+  const int own = T::PAIR ? l16 >> 3 : 0;
+  uint8_t* mine = lds + wave * T::Mine;
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
+  const i32x4 rw = resource(p.w + (int64_t)n0 * p.ldw), rx = resource(p.x + (int64_t)m0 * p.ldx), rws = resource(p.ws + (int64_t)(n0 >> 7) * p.ldws);
+  const int last = p.blocks - 1, r8 = lane >> 3, c8 = ((lane & 7) ^ f8_key(r8)) * 16;
+  int wo[2 * NT], xo[T::XL];   // rows past the last: it again
+#pragma unroll
+  for (int i = 0; i < 2 * NT; ++i) wo[i] = min(T::PAIR ? r8 : 8 * i + r8, p.N - 1 - n0) * (int)p.ldw + c8;
+#pragma unroll
+  for (int i = 0; i < T::XL; ++i) xo[i] = min(T::PAIR ? r8 : 8 * i + r8, p.M - 1 - m0) * (int)p.ldx + c8;
+  const int so = min(lane % T::BM, p.M - 1 - m0) * 4;
+  const int turns = (p.blocks - wave * Step + W * Step - 1) / (W * Step);   // this wave's
+  auto load = [&](int t, int st) {   // turn t's blocks into the stage at LDS offset st; past the last block: it again
+    const int kb = (t * W + wave) * Step;
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) dma16(base + st + i * 1024, wo[i], rw, (T::PAIR ? min(kb + i, last) : kb) * 128);
+#pragma unroll
+    for (int i = 0; i < T::XL; ++i) dma16(base + st + (2 * NT + i) * 1024, xo[i], rx, (T::PAIR ? min(kb + i, last) : kb) * 128);
+#pragma unroll
+    for (int i = 0; i < Step; ++i) dma4(base + st + T::Codes + i * 256, so, resource(p.xs + m0 + (int64_t)min(kb + i, last) * p.ldxs), 0);
+  };
+  // the weight's scales of 64 / Step turns, and of the next
+  auto load_ws = [&](int t) {
+    const int u = t + lane / Step;
+    dma4(base + S * T::Stage + (t / (64 / Step) & 1) * 256, min((u * W + wave) * Step + lane % Step, last) * 4, rws, 0);
+  };
+  const int chunk = (g ^ f8_key(l16)) << 4;
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (turns > 0) load_ws(0);
+#pragma unroll
+  for (int t = 0; t < S; ++t)
+    if (t < turns) load(t, t * T::Stage);
+  int at = 0;
+  for (int t = 0; t < turns; ++t) {
+    if (t % (64 / Step) == 0 && t + 64 / Step < turns) load_ws(t + 64 / Step);   // (one load more than counted: the wait is for more, not less)
+    if (t + S <= turns) wait_dma<(S - 1) * T::Loads>();
+    else wait_dma<0>();
+    const uint8_t* st = mine + at;
+    auto frag = [&](int row) { return codes32(*(const i32x4*)(st + row * 128 + chunk), *(const i32x4*)(st + row * 128 + (chunk ^ 64))); };
+    i32x8 a[NT], b[MT];
+    float s[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) a[i] = frag(16 * i + l16);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const int row = T::XL == 1 ? l16 & 7 : 16 * j + l16;
+      b[j] = frag(16 * NT + row);
+      s[j] = *(const float*)(st + T::Codes + own * 256 + (T::PAIR ? l16 & 7 : row) * 4);
+    }
+    const float sw = *(const float*)(mine + S * T::Stage + (t / (64 / Step) & 1) * 256 + (t % (64 / Step) * Step + own) * 4);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t + S < turns) load(t + S, at);
+    at = at + T::Stage == S * T::Stage ? 0 : at + T::Stage;
+    const float w = !T::PAIR || (t * W + wave) * Step + own <= last ? sw : 0.0f;   // past the last block: times 0
+    half8v ah[Exact ? NT : 1][4];
+    if constexpr (Exact) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) to_half(a[i], ah[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      half8v bh[4];
+      if constexpr (Exact) to_half(b[j], bh);
+      const float f = s[j] * w;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        f32x4 d;
+        if constexpr (Exact) d = mfma_half(ah[i], bh);
+        else d = mfma_block(a[i], b[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][i][e] = __builtin_fmaf(d[e], f, acc[j][i][e]);
+      }
+    }
+  }
+  wait_dma<0>();
+#pragma unroll
+  for (int j = 0; j < MT; ++j)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) ((f32x4*)mine)[(j * NT + i) * 64 + lane] = acc[j][i];
+  __syncthreads();
+  if (wave >= NT * MT) return;
+  auto part = [&](int k) { return ((const f32x4*)(lds + k * T::Mine))[wave * 64 + lane]; };
+  f32x4 v = part(0);
+#pragma unroll
+  for (int k = 1; k < W; ++k) v += part(k);
+  const int n = n0 + wave % NT * 16 + 4 * g, m = m0 + wave / NT * 16 + l16;
+  if constexpr (T::PAIR) {   // the other block's sums: 32 lanes of outputs and 8 columns further on
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += __shfl(v[e], lane + 40, 64);
+    if (g >= 2 || l16 >= 8) return;
+  }
+  if (l16 < T::BM && m < p.M && n < p.N) store4<TYPE>(p, m, n, v);
 }
 
 // Few rows: a workgroup takes 16 NT outputs of 16 rows, its W waves the blocks of k in turn; their sums meet in LDS. A wave's loads are
@@ -173,10 +305,7 @@ __device__ __forceinline__ void tile_out(const F8GemmP& p, const f32x4 (&acc)[AM
 
 // Many rows: a workgroup takes BN outputs (weight rows) of BM activation rows, its WN x WM waves 16 AN x 16 AM of them each. A stage in LDS is
 // a block of k of every row: BN + BM rows of 128 codes and BM scales, S stages in all, filled by loads that go straight to LDS,
-// S - 1 steps ahead and dealt out over a step. The 16-byte chunk c of row r lies at position c ^ key(r): a fragment's read takes chunk g
-// (and g ^ 4) of rows 0 .. 15 for the lane groups g = 0 .. 3, and LDS serves lanes 0-3, 12-15 of one group with 4-11 of the next; under key = r & 6 those
-// 16 lie in 16 different (row parity, position) pairs, so no bank conflicts (the counter reads 0; a key that suits 16 lanes of one
-// group each, (r ^ r / 8) & 7, read 48%).
+// S - 1 steps ahead and dealt out over a step; chunks lie as above.
 // Bound: the matrix instructions at the clock that they leave. 4608 rows, 9216 outputs x 9216 k, fp16 results: 352-357 us, 2.2 PFLOP/s (a
 // library's product with a scale per row 327; of 8192 each way 2.36). On random codes the 16 x 16 x 128 instruction by itself reaches 3.75 PFLOP/s, with an fma a
 // value beside it 3.38, on zeros 4.88: the clock goes down under them. Tried on the widest tile, us: 32 x 32 x 64 instructions the same; two groups of waves
@@ -184,8 +313,6 @@ __device__ __forceinline__ void tile_out(const F8GemmP& p, const f32x4 (&acc)[AM
 // k dealt out evenly 402 (neighbours no longer share lines in L2); bands of 2 or 8 row tiles slower.
 // One barrier a step, ahead of the step's last matrix instructions: every wave then holds the rest of its step in registers, the
 // next step's first fragments are read while those run, and the stage just left is free for loads.
-__device__ __forceinline__ int f8_key(int r) { return r & 6; }
-
 template <int WN_, int WM_, int AN_, int AM_, int S_>
 struct F8Tile {
   static constexpr int WN = WN_, WM = WM_, AN = AN_, AM = AM_, S = S_;
@@ -416,16 +543,38 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   tile_out<TYPE, T::AM, T::AN>(p, acc, m0 + wm * 16 * T::AM, n0 + wn * 16 * T::AN, lane);
 }
 
+using FewPairs = F8Few<8, 1, 1, true, 2>;    // 8 outputs of 8 rows, 8 waves of two blocks a turn
+using FewPairs4 = F8Few<4, 1, 1, true, 2>;   // the same, 4 waves
+using Few8 = F8Few<4, 1, 1, false, 2>;       // 16 outputs of 8 rows, 4 waves
+using Few16 = F8Few<8, 1, 2, false, 2>;      // 16 of 16, 8 waves
+using Few16b = F8Few<4, 1, 2, false, 2>;     // the same, 4 waves
+using Few32 = F8Few<8, 1, 4, false, 2>;      // 16 of 32, 8 waves
+using Few32w = F8Few<8, 2, 4, false, 1>;     // 32 of 32, 8 waves
 using TileSmall = F8Tile<2, 2, 2, 2, 9>;   // 64 outputs of 64 rows, 4 waves of 32 x 32
 using TileLow = F8Tile<4, 1, 2, 4, 6>;     // 128 of 64, 4 waves of 32 x 64
 using TileHalf = F8Tile<2, 4, 4, 2, 4>;    // 128 of 128, 8 waves of 64 x 32
 using TileLong = F8Tile<2, 4, 4, 4, 3>;    // 128 of 256, 8 waves of 64 x 64
 using TileWide = F8Tile<2, 4, 8, 4, 2>;    // 256 of 256, 8 waves of 128 x 64
 
-template <int W, int NT, bool PAIR> static void f8_thin_launch(const F8GemmP& p, int type, hipStream_t s) {
-  const int bn = PAIR ? 8 : 16 * NT;
-  auto k = type == P0_F32 ? f8_thin_kernel<P0_F32, W, NT, PAIR> : type == P0_F16 ? f8_thin_kernel<P0_F16, W, NT, PAIR> : f8_thin_kernel<P0_BF16, W, NT, PAIR>;
-  hipLaunchKernelGGL(k, dim3((unsigned)((p.N + bn - 1) / bn)), dim3(64 * W), 0, s, p);
+template <class T> static auto f8_few_of(int type) {
+  return type == P0_F32 ? f8_few_kernel<P0_F32, T> : type == P0_F16 ? f8_few_kernel<P0_F16, T> : f8_few_kernel<P0_BF16, T>;
+}
+template <class T> static void f8_few_launch(const F8GemmP& g, int type, hipStream_t s) {
+  F8GemmP p = g;
+  unsigned nx = (unsigned)((p.N + T::BN - 1) / T::BN), ny = (unsigned)((p.M + T::BM - 1) / T::BM);
+  if (ny > 1) {
+    // The operand with more rows goes along x, in a multiple of 8: consecutive workgroups go to the 8 XCDs in turn, so each L2 holds an eighth of it
+    // (us, weights along x / rows: 1021 rows, 130 outputs x 8192 k 12.3 / 7.9; 128 rows, 4096 x 2048 5.7 / 6.5)
+    p.turned = p.M > p.N;
+    if (p.turned) std::swap(nx, ny);
+    nx = (nx + 7) / 8 * 8;
+  }
+  hipLaunchKernelGGL(f8_few_of<T>(type), dim3(nx, ny), dim3(64 * T::W), T::Lds, s, p);
+}
+template <class T> static int f8_few_init() {
+  for (int type : {P0_F32, P0_F16, P0_BF16})
+    P0_HIP(hipFuncSetAttribute((const void*)f8_few_of<T>(type), hipFuncAttributeMaxDynamicSharedMemorySize, T::Lds), "p0_open: f8_gemm");
+  return P0_OK;
 }
 template <class T> static auto f8_tile_of(int type) {   // fp32 results hold more in registers: not in the widest tile's
   constexpr int F = T::AN * T::AM < 32 ? P0_F32 : P0_BF16;
@@ -445,6 +594,13 @@ template <class T> static int f8_tile_init() {
   return P0_OK;
 }
 int f8_gemm_init() {
+  if (int r = f8_few_init<FewPairs>()) return r;
+  if (int r = f8_few_init<FewPairs4>()) return r;
+  if (int r = f8_few_init<Few8>()) return r;
+  if (int r = f8_few_init<Few16>()) return r;
+  if (int r = f8_few_init<Few16b>()) return r;
+  if (int r = f8_few_init<Few32>()) return r;
+  if (int r = f8_few_init<Few32w>()) return r;
   if (int r = f8_tile_init<TileSmall>()) return r;
   if (int r = f8_tile_init<TileLow>()) return r;
   if (int r = f8_tile_init<TileHalf>()) return r;
@@ -469,7 +625,20 @@ constexpr F8Shape kF8Shapes[] = {{64, 64, 0.326f, 1.7f, 0.60f, 2.1f},      // Ti
                                  {128, 128, 0.613f, 2.55f, 1.02f, 7.2f},   // TileHalf
                                  {128, 256, 1.036f, 4.3f, 1.49f, 15.7f},   // TileLong
                                  {256, 256, 1.65f, 8.9f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
-static bool f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
+// Up to a few times as many workgroups as CUs the kernel for few rows is ahead of the tiles, whose steps wait for each other: a round, then the longer of
+// a wave's turns and of what a CU's workgroups ask for in all. Fitted to 255 shapes of 17 to 3330 rows; the choice among these two and the tiles is
+// on average within 1% of the fastest measured, 10% at the worst (512 rows, 1536 outputs x 1024 k). Measured (us; few in 16 x 32 / in 32 x 32 / tile): 64
+// rows, 2048 x 8192 k 7.2 / 8.4 / 11.5; 64, 2048 x 2048 3.9 / 4.0 / 7.4; 256, 512 x 2048 3.7 / 4.0 / 7.3; 128, 4096 x 2048 9.9 / 5.7 / 8.7;
+// 1021, 2048 x 2048 36.6 / 16.6 / 11.1. Past 4 groups a CU (6 where results are fp32) the tiles
+// are ahead whatever the rest says (256, 4096 x 2048: - / 9.4 / 8.7); weights past 64 MB stream better into them (64, 9216 x 9216 40 / 32 / 26).
+struct F8FewShape {
+  int bn, bm, waves, per_cu;
+  float round, turn, block, group;           // us: a round of workgroups, a turn of a wave, a block and a workgroup of each CU
+  float round32, turn32, block32, group32;   // fp32 results
+};
+constexpr F8FewShape kF8FewShapes[] = {{16, 32, 8, 1, 0.41f, 0.486f, 0.060f, 0.09f, 0.53f, 0.62f, 0.05f, 0.0f},     // Few32
+                                       {32, 32, 8, 2, 0.0f, 0.60f, 0.085f, 0.41f, 0.0f, 0.665f, 0.10f, 0.55f}};   // Few32w
+static bool f8_choice(const F8GemmP& p, int type, hipStream_t s) {
   const bool f32 = type == P0_F32;
   const int cus = ctx().cu_count;
   float least = 0.0f;
@@ -487,8 +656,20 @@ static bool f8_tile_choice(const F8GemmP& p, int type, hipStream_t s) {
       if (kind < 0 || t < least) { least = t; kind = k; nks = n; }
     }
   }
+  for (int k = 0; k < 2; ++k) {
+    const F8FewShape& c = kF8FewShapes[k];
+    const int64_t groups = ((int64_t)p.N + c.bn - 1) / c.bn * (((int64_t)p.M + c.bm - 1) / c.bm);
+    if (groups > (f32 ? 6 : 4) * cus || (int64_t)p.N * p.blocks > 1 << 19) continue;
+    const int rounds = (int)((groups + (int64_t)cus * c.per_cu - 1) / ((int64_t)cus * c.per_cu)), turns = (p.blocks + c.waves - 1) / c.waves;
+    const float each = groups > cus ? (float)groups / cus : 1.0f, wait = rounds * turns * (f32 ? c.turn32 : c.turn),
+                ask = each * p.blocks * (f32 ? c.block32 : c.block);
+    const float t = rounds * (f32 ? c.round32 : c.round) + (wait > ask ? wait : ask) + each * (f32 ? c.group32 : c.group);
+    if (kind < 0 || t < least) { least = t; kind = 5 + k; }
+  }
   if (kind < 0) return false;
-  if (kind == 0) f8_tile_launch<TileSmall>(p, type, nks, s);
+  if (kind == 5) f8_few_launch<Few32>(p, type, s);
+  else if (kind == 6) f8_few_launch<Few32w>(p, type, s);
+  else if (kind == 0) f8_tile_launch<TileSmall>(p, type, nks, s);
   else if (kind == 1) f8_tile_launch<TileLow>(p, type, nks, s);
   else if (kind == 2) f8_tile_launch<TileHalf>(p, type, nks, s);
   else if (kind == 3) f8_tile_launch<TileLong>(p, type, nks, s);
@@ -519,18 +700,20 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   if (overlap(x, y) || overlap(w, y) || overlap(xs, y) || overlap(ws, y)) { set_error("%s: y overlaps an input", op); return P0_EINVAL; }
   if (int r = refuse_in_chain(op)) return r;
   if (int r = require_open(op)) return r;
-  F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks};
+  F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks, 0};
   const uintptr_t ya = (uintptr_t)a->y | (uintptr_t)(ldy * size);
   p.yvec = ya % 16 == 0 ? 2 : ya % (4 * size) == 0;
   if (M <= 16) {
-    // Measured (us; rows, outputs x k): pairs of blocks where 16 outputs a workgroup would leave CUs without one: 5, 2048 x 8192 6.6 / 7.6, 1, 1024 x
-    // 4096 4.0 / 4.6, but 1, 4096 x 8192 9.4 / 8.4. 32 outputs a workgroup, which halves its reads of the rows: 16, 16384 x 2048 8.4 / 10.1, but 16,
-    // 4096 x 2048 5.2 / 4.1 and 5, 16384 x 8192 29.4 / 24.9. 16 waves for long k: 1, 16384 x 4096 14.2 / 14.9 of 8; 1, 16384 x 2048 9.0 / 7.5
-    if (M <= 8 && N <= 8 * ctx().cu_count && blocks >= 16) f8_thin_launch<16, 1, true>(p, a->type, ctx().cur);
-    else if (M <= 8 && blocks >= 32) f8_thin_launch<16, 1, false>(p, a->type, ctx().cur);
-    else if (M > 8 && N >= 8192) f8_thin_launch<4, 2, false>(p, a->type, ctx().cur);
-    else f8_thin_launch<8, 1, false>(p, a->type, ctx().cur);
-  } else if (!f8_tile_choice(p, a->type, ctx().cur)) {
+    // Measured (us; rows, outputs x k). Up to 8 rows, pairs of 8 waves / of 4 / 16 outputs: 5, 2048 x 8192 5.1 / 5.6 / 7.3; 1, 9216 x 2048 6.9 / 6.0 / 5.5,
+    // x 4096 10.2 / 9.1 / 10.2, x 8192 14.9 / 15.8 / 16.4; 1, 16384 x 2048 11.3 / 8.4 / 7.7, x 4096 15.5 / 12.7 / 14.8. Up to 16, 8 waves / 4: 16, 2048 x 8192
+    // 6.0 / 7.6; 16, 9216 x 14720 33.3 / 33.8; 16, 16384 x 2048 9.2 / 8.1. Up to 16 blocks both are alike where there are few outputs
+    const bool many = N > 18 * ctx().cu_count;   // workgroups of 8 outputs: more than two a CU
+    if (M > 8 && blocks <= 16) f8_few_launch<Few16b>(p, a->type, ctx().cur);
+    else if (M > 8) f8_few_launch<Few16>(p, a->type, ctx().cur);
+    else if (blocks <= 16) f8_few_launch<Few8>(p, a->type, ctx().cur);
+    else if (many && (blocks < 64 || N > 1 << 25)) f8_few_launch<FewPairs4>(p, a->type, ctx().cur);   // (8 waves of 2^26 outputs: 2^32 threads)
+    else f8_few_launch<FewPairs>(p, a->type, ctx().cur);
+  } else if (!f8_choice(p, a->type, ctx().cur)) {
     set_error("%s: %lld x %lld outputs", op, (long long)M, (long long)N);
     return P0_EINVAL;
   }

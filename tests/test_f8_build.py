@@ -20,7 +20,7 @@ def test_the_kernels_spill_no_registers():
             notes = subprocess.run([READELF, "--notes", f], capture_output=True, text=True, check=True).stdout
             for name, n in re.findall(r"\.name: +(_ZN2p0\d+(?:f8_|rope_)\S+).*?\.vgpr_spill_count: +(\d+)", notes, re.S):
                 spills[name] = int(n)
-    assert len(spills) == 3 + 6 + 45 + 12 + 14 + 9 and not any(spills.values()), {k: v for k, v in spills.items() if v}
+    assert len(spills) == 3 + 6 + 45 + 21 + 14 + 9 and not any(spills.values()), {k: v for k, v in spills.items() if v}
 
 
 def test_slices_are_joined_over_device_scope_accesses():
@@ -28,6 +28,9 @@ def test_slices_are_joined_over_device_scope_accesses():
     kernels = _code("f8_tile_kernel")
     assert len(kernels) == 14
     for name, code in kernels.items():
+        if "F8TileILi2ELi4ELi8ELi4ELi2E" in name:   # the widest tile takes no slices
+            assert not any(" sc1" in x for x in code), name
+            continue
         loads = [x for x in code if re.match(r"(global|flat)_load_dwordx2 ", x)]
         stores = [x for x in code if re.match(r"(global|flat)_store_dwordx2 ", x) and " sc1" in x]
         assert len(loads) >= 8 and all(" sc1" in x for x in loads) and len(stores) >= 8, (name, len(loads), len(stores))
