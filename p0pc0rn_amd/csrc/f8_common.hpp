@@ -52,32 +52,75 @@ inline int64_t f8_blocks(int64_t n) { return (n + kF8Block - 1) / kF8Block; }
 template <int TYPE> __device__ __forceinline__ float f8_value(uint32_t h) {   // a 16-bit value's low half
   return TYPE == P0_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
 }
-// n of 8 consecutive elements from element i on (vec: all 8, 16-byte aligned); the others are 0
-template <int TYPE> __device__ __forceinline__ void f8_load8(const void* x, int64_t i, bool vec, int n, float (&f)[8]) {
-  if constexpr (TYPE == P0_F32) {
-    const float* a = (const float*)x + i;
-    if (vec) {
-      const float4 u = *(const float4*)a, v = *(const float4*)(a + 4);
-      f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
-    } else {
+// 16 bytes at any element's address: one access, as global memory takes them unaligned
+struct __attribute__((packed, aligned(2))) F8Any16 { uint32_t w[4]; };
+__device__ __forceinline__ uint4 f8_load16(const void* a) {
+  const F8Any16 v = *(const F8Any16*)a;
+  return uint4{v.w[0], v.w[1], v.w[2], v.w[3]};
+}
+__device__ __forceinline__ void f8_store16(void* a, const uint4& v) { *(F8Any16*)a = F8Any16{{v.x, v.y, v.z, v.w}}; }
+// n of 8 consecutive elements (n >= 1) from element i on, of a row that has `before` elements ahead of it and n or more (`room`) from it on; the others
+// are 0. f8_fetch8 asks for them, f8_take8 makes them values: of several, all are asked for first. One or two 16-byte accesses: of the row's last 8
+// elements, moved down, where there are fewer than 8 from i on (one by one only in rows shorter than 8). What is read beside the n is not used: it may
+// change meanwhile.
+template <int TYPE> struct F8Raw { uint32_t w[TYPE == P0_F32 ? 8 : 4]; };
+template <int TYPE> __device__ __forceinline__ void f8_fetch8(const void* x, int64_t i, int before, int room, F8Raw<TYPE>& f) {
+  constexpr int W = TYPE == P0_F32 ? 8 : 4;
+  const int back = room < 8 ? 8 - room : 0;
+  if (back == 0 || back <= before) {
+    const char* a = (const char*)x + (i - back) * (TYPE == P0_F32 ? 4 : 2);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = j < n ? a[j] : 0.0f;
-    }
-  } else {
-    const uint16_t* a = (const uint16_t*)x + i;
-    if (vec) {
-      const uint4 u = *(const uint4*)a;
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        f[2 * j] = f8_value<TYPE>(w[j] & 0xFFFFu);
-        f[2 * j + 1] = TYPE == P0_F16 ? f8_value<TYPE>(w[j] >> 16) : __uint_as_float(w[j] & 0xFFFF0000u);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = j < n ? f8_value<TYPE>(a[j]) : 0.0f;
+    for (int k = 0; k < W / 4; ++k) {
+      const uint4 u = f8_load16(a + 16 * k);
+      f.w[4 * k] = u.x; f.w[4 * k + 1] = u.y; f.w[4 * k + 2] = u.z; f.w[4 * k + 3] = u.w;
     }
   }
+}
+template <int TYPE> __device__ __forceinline__ void f8_take8(const F8Raw<TYPE>& raw, const void* x, int64_t i, int n, int before, int room, float (&f)[8]) {
+  constexpr int W = TYPE == P0_F32 ? 8 : 4;
+  uint32_t w[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) w[k] = raw.w[k];
+  const int back = room < 8 ? 8 - room : 0;
+  if (back > before) {
+    if constexpr (TYPE == P0_F32) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = ((const uint32_t*)x)[i + min(k, n - 1)];
+    } else {
+      const uint16_t* a = (const uint16_t*)x + i;
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = a[min(2 * k, n - 1)] | (uint32_t)a[min(2 * k + 1, n - 1)] << 16;
+    }
+  } else if (back) {   // down by `back` elements
+#pragma unroll
+    for (int b = W / 2; b > 0; b /= 2) {
+      const bool on = back & (TYPE == P0_F32 ? b : 2 * b);
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = on ? (k + b < W ? w[k + b] : 0u) : w[k];
+    }
+    if constexpr (TYPE != P0_F32) {
+      const bool on = back & 1;
+#pragma unroll
+      for (int k = 0; k < W; ++k) w[k] = on ? w[k] >> 16 | (k + 1 < W ? w[k + 1] << 16 : 0u) : w[k];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    if constexpr (TYPE == P0_F32) f[k] = __uint_as_float(w[k]);
+    else {
+      f[2 * k] = f8_value<TYPE>(w[k] & 0xFFFFu);
+      f[2 * k + 1] = TYPE == P0_F16 ? f8_value<TYPE>(w[k] >> 16) : __uint_as_float(w[k] & 0xFFFF0000u);
+    }
+  }
+  if (n < 8) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) f[k] = k < n ? f[k] : 0.0f;
+  }
+}
+template <int TYPE> __device__ __forceinline__ void f8_load8(const void* x, int64_t i, int n, int before, int room, float (&f)[8]) {
+  F8Raw<TYPE> raw;
+  f8_fetch8<TYPE>(x, i, before, room, raw);
+  f8_take8<TYPE>(raw, x, i, n, before, room, f);
 }
 // to the nearest value of a 16-bit type, ties to the even one
 template <int TYPE> __device__ __forceinline__ uint32_t f8_half(float v) {
@@ -88,12 +131,12 @@ template <int TYPE> __device__ __forceinline__ float f8_rounded(float v) {
   if constexpr (TYPE == P0_F32) return v;
   else return f8_value<TYPE>(f8_half<TYPE>(v));
 }
-template <int TYPE> __device__ __forceinline__ void f8_store8(void* x, int64_t i, bool vec, int n, const float (&f)[8]) {
+template <int TYPE> __device__ __forceinline__ void f8_store8(void* x, int64_t i, bool all, int n, const float (&f)[8]) {
   if constexpr (TYPE == P0_F32) {
     float* a = (float*)x + i;
-    if (vec) {
-      *(float4*)a = float4{f[0], f[1], f[2], f[3]};
-      *(float4*)(a + 4) = float4{f[4], f[5], f[6], f[7]};
+    if (all) {
+      f8_store16(a, uint4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])});
+      f8_store16(a + 4, uint4{__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])});
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -101,11 +144,11 @@ template <int TYPE> __device__ __forceinline__ void f8_store8(void* x, int64_t i
     }
   } else {
     uint16_t* a = (uint16_t*)x + i;
-    if (vec) {
+    if (all) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = f8_half<TYPE>(f[2 * j]) | f8_half<TYPE>(f[2 * j + 1]) << 16;
-      *(uint4*)a = uint4{w[0], w[1], w[2], w[3]};
+      f8_store16(a, uint4{w[0], w[1], w[2], w[3]});
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)

@@ -15,7 +15,6 @@ struct PackP {
   int64_t ldx, ldw, lds;
   int64_t N, K;
   int blocks;   // of 128 channels in a row
-  int vec;
 };
 // A workgroup takes a block of 128 x 128, a thread 8 rows of 8 channels: 8 loads of 16 bytes on their way at once.
 // Bound: HBM (18432 x 9216 bf16 values: 99.8 us for 510 MB, 5.1 TB/s; a copy of as many bytes 95); launch and round trips for small ones (1536 x
@@ -28,11 +27,17 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const PackP p) {
   const int kb = (int)(blk - nb * p.blocks), c = kb * 128 + (threadIdx.x & 15) * 8, lane = threadIdx.x & 63;
   const int64_t n0 = nb * 128 + (threadIdx.x >> 4);
   const int n = (int)(p.K - c < 8 ? (p.K - c < 0 ? 0 : p.K - c) : 8);
+  F8Raw<TYPE> raw[8];
   float f[8][8], most = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int64_t r = n0 + 16 * j;
-    if (r < p.N) f8_load8<TYPE>(p.x, r * p.ldx + c, p.vec && n == 8, n, f[j]);
+    if (r < p.N && n > 0) f8_fetch8<TYPE>(p.x, r * p.ldx + c, c, n, raw[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int64_t r = n0 + 16 * j;
+    if (r < p.N && n > 0) f8_take8<TYPE>(raw[j], p.x, r * p.ldx + c, n, c, n, f[j]);
     else
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[j][i] = 0.0f;
@@ -71,7 +76,7 @@ struct RowsF8P {
   int64_t ldx, up, ldy, lds;
   int64_t M, D;
   int strips, ls;   // 1 << ls lanes side by side take a strip of 8 << ls channels of a row
-  int vec, glu;
+  int glu;
 };
 // A workgroup takes a strip of 256 >> ls rows.
 // Bound: HBM (4608 rows of 9216 f16 channels: 24 us for 128 MB, 5.3 TB/s), gated ones nearly as much the arithmetic: 45-48 us for 214 MB, 4.6 TB/s (a copy of as
@@ -84,14 +89,18 @@ __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsF8P p) {
   const int64_t m = rblk * side + (threadIdx.x >> p.ls);
   if (c >= (int)((p.D + 127) / 128 * 128) || m >= p.M) return;   // whole blocks of lanes
   const int n = (int)(p.D - c < 8 ? (p.D - c < 0 ? 0 : p.D - c) : 8);
-  const bool vec = p.vec && n == 8;
-  float f[8];
-  f8_load8<TYPE>(p.x, m * p.ldx + c, vec, n, f);
-  if constexpr (GLU) {
-    float u[8];
-    f8_load8<TYPE>(p.x, m * p.ldx + p.up + c, vec, n, u);
+  float f[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  if (n > 0) {
+    F8Raw<TYPE> gate, up;
+    f8_fetch8<TYPE>(p.x, m * p.ldx + c, c, n, gate);
+    if constexpr (GLU) f8_fetch8<TYPE>(p.x, m * p.ldx + p.up + c, c, n, up);
+    f8_take8<TYPE>(gate, p.x, m * p.ldx + c, n, c, n, f);
+    if constexpr (GLU) {
+      float u[8];
+      f8_take8<TYPE>(up, p.x, m * p.ldx + p.up + c, n, c, n, u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = gated(p.glu, f[j], u[j]);
+      for (int j = 0; j < 8; ++j) f[j] = gated(p.glu, f[j], u[j]);
+    }
   }
   const float s = f8_scale(f8_block_most(f));
   *(uint2*)(p.y + m * p.ldy + c) = f8_codes(f, f8_inverse(s));
@@ -123,9 +132,10 @@ __device__ __forceinline__ float sum64(float v) {
 }
 // A workgroup takes a row, its up to 16 waves 512 channels each of NC steps, a lane 8 of them. The row stays in registers; each sum is one
 // exchange through LDS.
-// VEC: every run of 8 channels is there whole or not at all, and 16-byte aligned everywhere.
-// Bound: HBM at many rows (32760 rows of 2560 bf16 channels, modulated: 112-122 us for 590 MB, 4.9-5.3 TB/s; a copy of as many bytes 114),
-// launch and round trips at few (1 row of 2048 fp32 channels: 3.9-4.2 us back to back, 5.5 with the host's part). A wave with a row of its own, four in a workgroup, took 136 and 3.7: five loads a lane
+// VEC: every run of 8 channels is there whole or not at all.
+// Bound: HBM at many rows (32760 rows of 2560 bf16 channels, modulated: 109-120 us for 590 MB, 4.9-5.4 TB/s; a copy of as many bytes 114),
+// launch and round trips at few (1 row of 2048 fp32 channels: 3.6-4.2 us back to back, 5.5 with the host's part). Rows whose last run of 8 is not whole
+// cost little more (644 rows of 14425 bf16 channels: 30 us for 66 MB; in single channels 84). A wave with a row of its own, four in a workgroup, took 136 and 3.7: five loads a lane
 // at a time and their registers leave fewer waves to cover them.
 template <int XT, int TT, int NC, bool VEC>
 __global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
@@ -149,12 +159,20 @@ __global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
     for (int j = 0; j < 8; ++j) v[j] = x;
   };
   float f[NC][8];
+  F8Raw<XT> xr[NC];
+  F8Raw<TT> tr[NC];
   const float over = 1.0f / (float)p.D;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = c0 + i * 512 * W;
+    if (c < p.D) f8_fetch8<XT>(p.x, m * p.ldx + c, c, count(c), xr[i]);
+    if (p.t && c < p.D) f8_fetch8<TT>(p.t, m * p.ldt + c, c, count(c), tr[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = c0 + i * 512 * W;
     fill(f[i], 0.0f);
-    if (c < p.D) f8_load8<XT>(p.x, m * p.ldx + c, VEC, count(c), f[i]);
+    if (c < p.D) f8_take8<XT>(xr[i], p.x, m * p.ldx + c, count(c), c, count(c), f[i]);
   }
   if (p.t) {
     float t[NC][8], ss = 0.0f;
@@ -162,7 +180,7 @@ __global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
     for (int i = 0; i < NC; ++i) {
       const int c = c0 + i * 512 * W;
       fill(t[i], 0.0f);
-      if (c < p.D) f8_load8<TT>(p.t, m * p.ldt + c, VEC, count(c), t[i]);
+      if (c < p.D) f8_take8<TT>(tr[i], p.t, m * p.ldt + c, count(c), c, count(c), t[i]);
     }
     if (p.tw) {
 #pragma unroll
@@ -175,7 +193,7 @@ __global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
         const int c = c0 + i * 512 * W;
         if (c >= p.D) continue;
         float g[8];
-        f8_load8<P0_F32>(p.tw, c, VEC, count(c), g);
+        f8_load8<P0_F32>(p.tw, c, count(c), c, count(c), g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) t[i][j] *= r * g[j];
       }
@@ -194,7 +212,7 @@ __global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
       sum += f[i][j];
     }
     const int c = c0 + i * 512 * W;
-    if (p.xo && c < p.D) f8_store8<XT>(p.xo, m * p.ldo + c, VEC, count(c), f[i]);
+    if (p.xo && c < p.D) f8_store8<XT>(p.xo, m * p.ldo + c, VEC || count(c) == 8, count(c), f[i]);
   }
   const float mean = p.mode == 0 ? total(sum, 1) * over : 0.0f;
 #pragma unroll
@@ -213,9 +231,9 @@ __global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
     if (c >= (p.D + 127) / 128 * 128) break;   // whole blocks of lanes
     if (c < p.D) {
       float g[8], b[8];
-      if (p.w) f8_load8<P0_F32>(p.w, c, VEC, count(c), g);
+      if (p.w) f8_load8<P0_F32>(p.w, c, count(c), c, count(c), g);
       else fill(g, p.one ? 0.0f : 1.0f);
-      if (p.b) f8_load8<P0_F32>(p.b, c, VEC, count(c), b);
+      if (p.b) f8_load8<P0_F32>(p.b, c, count(c), c, count(c), b);
       else fill(b, 0.0f);
       const float one = p.one ? 1.0f : 0.0f;
 #pragma unroll
@@ -255,7 +273,7 @@ static int pack_call(const p0_f8_pack_args_t* a) {
   dim3 grid;
   if (!f8_grid(f8_blocks(a->N) * blocks, 256, &grid)) { set_error("%s: %lld x %lld values", op, (long long)a->N, (long long)a->K); return P0_EINVAL; }
   if (int r = refuse(op)) return r;
-  PackP p{a->x, (uint8_t*)a->w, a->s, ldx, ldw, lds, a->N, a->K, (int)blocks, ((uintptr_t)a->x | (uintptr_t)(ldx * size)) % 16 == 0};
+  PackP p{a->x, (uint8_t*)a->w, a->s, ldx, ldw, lds, a->N, a->K, (int)blocks};
   auto k = a->type == P0_F32 ? f8_pack_kernel<P0_F32> : a->type == P0_F16 ? f8_pack_kernel<P0_F16> : f8_pack_kernel<P0_BF16>;
   hipLaunchKernelGGL(k, grid, dim3(256), 0, ctx().cur, p);
   P0_LAUNCHED(op);
@@ -288,8 +306,7 @@ static int rows_f8_call(const p0_f8_rows_args_t* a) {
   if (int r = f8_check(op, "s", s, 4)) return r;
   if (overlap(x, y) || overlap(x, s) || overlap(y, s)) { set_error("%s: outputs overlap", op); return P0_EINVAL; }
   if (int r = refuse(op)) return r;
-  RowsF8P p{a->x, (uint8_t*)a->y, a->s, ldx, up, ldy, lds, a->M, a->D, 0, 7, 0, a->glu};
-  p.vec = ((uintptr_t)a->x | (uintptr_t)(ldx * size) | (uintptr_t)(up * size)) % 16 == 0;
+  RowsF8P p{a->x, (uint8_t*)a->y, a->s, ldx, up, ldy, lds, a->M, a->D, 0, 7, a->glu};
   // strips of up to 128 lanes that leave no more than an eighth idle (20000 rows of 520 gated channels: 18.9 us in strips of 16 lanes, 21.8 of 128;
   // 4608 of 9216: 52.3 and 45.4)
   const int64_t chunks = K8 / 8;
@@ -304,7 +321,7 @@ static int rows_f8_call(const p0_f8_rows_args_t* a) {
 
 typedef void (*NormKernel)(NormP);
 template <int XT, int TT> static NormKernel norm_kernel(bool vec, int NC) {
-  if (!vec) return NC == 1 ? f8_norm_kernel<XT, TT, 1, false> : f8_norm_kernel<XT, TT, 4, false>;
+  if (!vec) return NC == 1 ? f8_norm_kernel<XT, TT, 1, false> : NC == 2 ? f8_norm_kernel<XT, TT, 2, false> : f8_norm_kernel<XT, TT, 4, false>;
   return NC == 1 ? f8_norm_kernel<XT, TT, 1, true> : NC == 2 ? f8_norm_kernel<XT, TT, 2, true> : f8_norm_kernel<XT, TT, 4, true>;
 }
 
@@ -340,15 +357,14 @@ static int norm_call(const p0_f8_norm_args_t* a) {
   NormP p{};
   p.x = a->x; p.t = a->t; p.xo = xo; p.tw = a->tw; p.w = a->w; p.b = a->b; p.y = (uint8_t*)a->y; p.s = a->s;
   p.ldx = ldx; p.ldt = ldt; p.ldo = ldo; p.ldy = ldy; p.lds = lds; p.M = M; p.D = (int)D;
-  const bool vec = D % 8 == 0 && ((uintptr_t)a->x | (uintptr_t)(ldx * xsize) | (uintptr_t)xo | (uintptr_t)(ldo * xsize) | (uintptr_t)a->t |
-                                  (uintptr_t)(ldt * tsize) | (uintptr_t)a->tw | (uintptr_t)a->w | (uintptr_t)a->b) % 16 == 0;
+  const bool vec = D % 8 == 0;
   p.mode = a->mode; p.one = a->w_one ? 1 : 0; p.scale = scale; p.eps = a->eps != 0.0f ? a->eps : 1e-6f;
   // Waves of one step, but for two where rows are longer than 16 waves' one, and for 16-bit rows that fill the chip several times over (us,
   // one step / two: 32760 rows of 2560 bf16 channels 128 / 112, 4608 of 4096 28.9 / 27.4; 1021 of 1536 5.0 / 5.8; 4608 of 2048 fp32 channels
   // 23.8 / 25.6), and four for the longest
   const int steps = (int)((K8 + 511) / 512);
-  const bool two = vec && (steps > 16 || (xsize == 2 && steps > 1 && M * steps >= 16384));
-  const int NC = steps > (vec ? 32 : 16) ? 4 : two ? 2 : 1, W = (steps + NC - 1) / NC;
+  const bool two = steps > 16 || (xsize == 2 && steps > 1 && M * steps >= 16384);
+  const int NC = steps > 32 ? 4 : two ? 2 : 1, W = (steps + NC - 1) / NC;
   const int tt = a->t ? a->t_type : a->type;
   NormKernel k = nullptr;
 #define P0_NORM(XT, TT) if (a->type == XT && tt == TT) k = norm_kernel<XT, TT>(vec, NC)

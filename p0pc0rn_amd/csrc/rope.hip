@@ -25,13 +25,9 @@ struct RopeP {
   int first[4];               // an axis's first pair
   int axes, shared, inter;
   int rb, hb, hblocks;        // rows, heads of a workgroup, workgroups a row block
-  int ls;                     // 1 << ls lanes take a head
+  int ls, nl;                 // 1 << ls lanes take a head; halves: the first nl of them what turns
   float eps;
 };
-
-// the two channels of pair i; past the turning ones neighbours go together, unturned
-__device__ __forceinline__ int rope_first(const RopeP& p, int i) { return p.inter || i >= p.R / 2 ? 2 * i : i; }
-__device__ __forceinline__ int rope_second(const RopeP& p, int i) { return p.inter || i >= p.R / 2 ? 2 * i + 1 : i + p.R / 2; }
 
 __device__ __forceinline__ float2 rope_turn(const RopeP& p, int64_t row, int i) {
   if (i >= p.R / 2) return float2{1.0f, 0.0f};
@@ -51,23 +47,13 @@ __device__ __forceinline__ float2 rope_turn(const RopeP& p, int64_t row, int i) 
   return float2{c, s};
 }
 
-// KIND 0: a lane has one pair at a time, 16 lanes a head. Whole 16-byte runs of one kind of pair: 1: neighbours, 4 pairs of a lane, dim / 8 lanes a head
-// (rounded up to a power of two); 2: halves, 8 pairs of a lane, dim / 16 lanes
-template <int TYPE, int KIND> __device__ __forceinline__ void rope_pairs(const void* x, int64_t at, int i0, int half, float (&u)[8], float (&v)[8]) {
-  if constexpr (KIND == 1) {
-    float g[8];
-    f8_load8<TYPE>(x, at + 2 * i0, true, 8, g);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { u[j] = g[2 * j]; v[j] = g[2 * j + 1]; }
-  } else {
-    f8_load8<TYPE>(x, at + i0, true, 8, u);
-    f8_load8<TYPE>(x, at + i0 + half, true, 8, v);
-  }
-}
-
-template <int TYPE, int KIND>
+// A lane has the same up to 8 pairs (halves: 8 first channels and their 8 partners) or 4 (neighbours: a run of 8 channels) of its head throughout; channels
+// that do not turn go to further lanes, 16 each (halves), or with their neighbours. Runs of 8 are whole 16-byte accesses at any alignment (9 rows of 24
+// heads of 512 fp32 channels, of which 384 turn by halves: 4.7 us, where single channels took 6.1).
+// WHOLE: every lane has all of its pairs, so no counts are looked at: 32760 rows of 40 heads of 128 bf16 channels, by halves and normalised, 132 us, with them 203.
+template <int TYPE, bool HALF, bool WHOLE>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeP p) {
-  __shared__ __attribute__((aligned(16))) float2 turn[kRopeTable];
+  __shared__ __attribute__((aligned(16))) float2 turn[kRopeTable + 8];   // (a last lane may read past its pairs)
   const int64_t group = f8_group(), blk = group / p.hblocks, row0 = blk * p.rb;
   const int h0 = (int)(group - blk * p.hblocks) * p.hb, pairs = p.dim / 2;
   if (row0 >= p.rows) return;
@@ -79,72 +65,53 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(const RopeP p) {
   __syncthreads();
   const int lane = threadIdx.x & ((1 << p.ls) - 1), items = rows * hb;
   const uint32_t magic = (1u << 20) / (uint32_t)hb + 1;   // it / hb = it * magic >> 20: exact while it * hb < 2^20
+  // the lane's channels: nu from cu on and, halves, nv from cv on
+  constexpr int V = HALF ? 8 : 4;
+  const bool turns = WHOLE || !HALF || lane < p.nl;
+  const int i0 = lane * V, rest = p.R + (lane - p.nl) * 16, cu = HALF ? (turns ? i0 : rest) : 2 * i0, cv = turns ? p.R / 2 + i0 : rest + 8;
+  const int end = (HALF && turns ? p.R / 2 : p.dim) - cu, nu = WHOLE ? (end > 0 ? 8 : 0) : min(8, end),
+            nv = !HALF ? 0 : WHOLE ? nu : min(8, (turns ? p.R : p.dim) - cv);
   for (int it = threadIdx.x >> p.ls; it < items; it += kRopeThreads >> p.ls) {
     const int r = (int)((uint32_t)it * magic >> 20), h = h0 + it - r * hb;
     const int64_t from = (row0 + r) * p.ldr + h * p.ldh, to = (row0 + r) * p.yldr + h * p.yldh;
     const float* w = h < p.hq ? p.qw : p.kw;
-    if constexpr (KIND > 0) {
-      constexpr int V = KIND == 1 ? 4 : 8;
-      const int i0 = lane * V;
-      const bool on = i0 < pairs;
-      float u[8], v[8];
-      if (on) rope_pairs<TYPE, KIND>(p.x, from, i0, p.R / 2, u, v);
-      if (w) {
-        float ss = 0.0f, wu[8], wv[8];
-        if (on) {
-          rope_pairs<P0_F32, KIND>(w, 0, i0, p.R / 2, wu, wv);
+    float a[8], b[8];
+    const int n8 = WHOLE ? 8 : nu, v8 = WHOLE ? 8 : nv, ru = WHOLE ? 8 : p.dim - cu, rv = WHOLE ? 8 : p.dim - cv;
+    {
+      F8Raw<TYPE> u, v;
+      if (nu > 0) f8_fetch8<TYPE>(p.x, from + cu, cu, ru, u);
+      if (nv > 0) f8_fetch8<TYPE>(p.x, from + cv, cv, rv, v);
+      if (nu > 0) f8_take8<TYPE>(u, p.x, from + cu, n8, cu, ru, a);
+      if (nv > 0) f8_take8<TYPE>(v, p.x, from + cv, v8, cv, rv, b);
+    }
+    if (w) {
+      float ss = 0.0f, g[8];
 #pragma unroll
-          for (int j = 0; j < V; ++j) ss += u[j] * u[j] + v[j] * v[j];
-        }
-        for (int o = 1 << p.ls >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        const float rstd = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
-        if (on) {
+      for (int j = 0; j < 8; ++j) ss += (nu > 0 ? a[j] * a[j] : 0.0f) + (nv > 0 ? b[j] * b[j] : 0.0f);
+      for (int o = 1 << p.ls >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+      const float rstd = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
+      if (nu > 0) {
+        f8_load8<P0_F32>(w, cu, n8, cu, ru, g);
 #pragma unroll
-          for (int j = 0; j < V; ++j) { u[j] *= rstd * wu[j]; v[j] *= rstd * wv[j]; }
-        }
+        for (int j = 0; j < 8; ++j) a[j] *= rstd * g[j];
       }
-      if (on) {
-        float a[8], b[8];
+      if (nv > 0) {
+        f8_load8<P0_F32>(w, cv, v8, cv, rv, g);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float2 t = turn[r * pairs + i0 + j];
-          a[j] = u[j] * t.x - v[j] * t.y;
-          b[j] = v[j] * t.x + u[j] * t.y;
-        }
-        if constexpr (KIND == 1) {
-          const float g[8] = {a[0], b[0], a[1], b[1], a[2], b[2], a[3], b[3]};
-          f8_store8<TYPE>(p.y, to + 2 * i0, true, 8, g);
-        } else {
-          f8_store8<TYPE>(p.y, to + i0, true, 8, a);
-          f8_store8<TYPE>(p.y, to + i0 + p.R / 2, true, 8, b);
-        }
-      }
-    } else {
-      auto load = [&](int c) {
-        float g[8];
-        f8_load8<TYPE>(p.x, from + c, false, 1, g);
-        return g[0];
-      };
-      float rstd = 1.0f;
-      if (w) {
-        float ss = 0.0f;
-        for (int i = lane; i < pairs; i += 16) {
-          const float u = load(rope_first(p, i)), v = load(rope_second(p, i));
-          ss += u * u + v * v;
-        }
-        for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        rstd = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
-      }
-      for (int i = lane; i < pairs; i += 16) {
-        const int cu = rope_first(p, i), cv = rope_second(p, i);
-        float u = load(cu), v = load(cv);
-        if (w) { u *= rstd * w[cu]; v *= rstd * w[cv]; }
-        const float2 t = turn[r * pairs + i];
-        const float a[8] = {u * t.x - v * t.y}, b[8] = {v * t.x + u * t.y};
-        f8_store8<TYPE>(p.y, to + cu, false, 1, a);
-        f8_store8<TYPE>(p.y, to + cv, false, 1, b);
+        for (int j = 0; j < 8; ++j) b[j] *= rstd * g[j];
       }
     }
+    if (nu > 0 && turns) {
+      const float2* t = turn + r * pairs + i0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float u = HALF ? a[j] : a[2 * j], v = HALF ? b[j] : a[2 * j + 1], x = u * t[j].x - v * t[j].y, y = v * t[j].x + u * t[j].y;
+        if constexpr (HALF) { a[j] = x; b[j] = y; }
+        else if (i0 + j < p.R / 2) { a[2 * j] = x; a[2 * j + 1] = y; }   // (an infinity beside a channel that does not turn stays off it)
+      }
+    }
+    if (nu > 0) f8_store8<TYPE>(p.y, to + cu, n8 == 8, n8, a);
+    if (nv > 0) f8_store8<TYPE>(p.y, to + cv, v8 == 8, v8, b);
   }
 }
 
@@ -200,10 +167,9 @@ static int rope_call(const p0_rope_args_t* a) {
     long double f = powl((long double)theta, -2.0L / (a->freq ? p.R : size_of[k]));   // squares of squares: in more bits than are kept
     for (int b = 0; b < 8; ++b, f *= f) p.pow[k][b] = (double)f;
   }
-  const bool rows16 = ((uintptr_t)a->x | (uintptr_t)a->y | (uintptr_t)(p.ldr * size) | (uintptr_t)(p.ldh * size) | (uintptr_t)(p.yldr * size) |
-                       (uintptr_t)(p.yldh * size) | (uintptr_t)a->qw | (uintptr_t)a->kw) % 16 == 0;
-  const int kind = !rows16 ? 0 : p.inter ? (a->dim % 8 == 0 ? 1 : 0) : a->dim % 16 == 0 && p.R == a->dim ? 2 : 0;
-  const int lanes = kind == 1 ? a->dim / 8 : kind == 2 ? a->dim / 16 : 16;
+  const bool half = !p.inter, whole = half ? p.R == a->dim && a->dim % 16 == 0 : a->dim % 8 == 0;   // every lane has 8 pairs, or 4
+  p.nl = (p.R / 2 + 7) / 8;
+  const int lanes = half ? p.nl + (a->dim - p.R + 15) / 16 : (a->dim + 7) / 8;   // at most 64
   while (1 << p.ls < lanes) ++p.ls;
   const int side = kRopeThreads >> p.ls, pairs = a->dim / 2;
   // A workgroup's work is four rounds of its groups of lanes where that leaves work for every CU: several rows, or a part of a row's
@@ -216,7 +182,7 @@ static int rope_call(const p0_rope_args_t* a) {
   p.hblocks = (int)((heads + p.hb - 1) / p.hb);
   dim3 grid;
   if (!f8_grid((a->rows + p.rb - 1) / p.rb * p.hblocks, kRopeThreads, &grid)) { set_error("%s: %lld rows of %lld heads", op, (long long)a->rows, (long long)heads); return P0_EINVAL; }
-#define P0_ROPE(T) if (a->type == T) hipLaunchKernelGGL((kind == 0 ? rope_kernel<T, 0> : kind == 1 ? rope_kernel<T, 1> : rope_kernel<T, 2>), grid, dim3(kRopeThreads), 0, ctx().cur, p)
+#define P0_ROPE(T) if (a->type == T) hipLaunchKernelGGL((half ? (whole ? rope_kernel<T, true, true> : rope_kernel<T, true, false>) : whole ? rope_kernel<T, false, true> : rope_kernel<T, false, false>), grid, dim3(kRopeThreads), 0, ctx().cur, p)
   P0_ROPE(P0_F32);
   P0_ROPE(P0_F16);
   P0_ROPE(P0_BF16);

@@ -8,7 +8,7 @@ import pytest
 from oracle import f8
 from p0pc0rn_amd import capi
 from tests.test_f8_gpu import RAW, Rows, activations, codes_near, operands, product, product_near, values_in
-from tests.test_kv_gpu import from_type
+from tests.test_kv_gpu import from_type, to_type
 
 pytestmark = pytest.mark.gpu
 
@@ -166,4 +166,54 @@ def test_first_and_last_positions(dev, mode):
     bound = (1e-6 + 2.4e-6) * (np.abs(u) + np.abs(v))
     assert (np.abs(ga - a) <= bound).all() and (np.abs(gb - b) <= bound).all()
     for r in (xb, yb, pb):
+        r.free()
+
+
+@pytest.mark.parametrize("mode", ["inter", "half"])
+@pytest.mark.parametrize("type_", ["f32", "bf16"])
+def test_channels_that_do_not_turn_beside_infinities(dev, mode, type_):
+    """what lies past the turning channels keeps its bits, beside infinities and NaN too"""
+    raw, v = to_type(np.random.default_rng(1).standard_normal((6, 2, 80)).astype(np.float32), type_)
+    inf, nan = (np.uint16(0x7F80), np.uint16(0x7FC0)) if type_ == "bf16" else (np.float32(np.inf), np.float32(np.nan))
+    raw = raw.copy()
+    raw[0, 0, 61], raw[1, 1, 60], raw[2, 0, 79], raw[3, 1, 62:70] = inf, inf, nan, inf
+    raw[4, 0, 60:] = 0
+    raw[4, 0, 61::2] = np.uint16(0x8000) if type_ == "bf16" else -0.0
+    xb, yb, pb = capi.to_device(raw), capi.Buffer(raw.nbytes), capi.to_device(np.arange(6, dtype=np.int32))
+    capi.rope(capi.rope_args(x=xb, y=yb, type=capi.TYPE[type_], rows=6, hq=1, hk=1, dim=80, mode=capi.ROPE[mode], axis_dim=[60], pos=pb))
+    bits = np.uint16 if type_ == "bf16" else np.uint32
+    got = yb.read(bits, raw.size).reshape(raw.shape)
+    assert np.array_equal(got[..., 60:], raw.view(bits)[..., 60:])
+    assert np.isfinite(from_type(got[..., :60].view(RAW[type_]), type_)).all()
+    for b in (xb, yb, pb):
+        b.free()
+
+
+@pytest.mark.parametrize("shift", [1, 3, 5])
+@pytest.mark.parametrize("D", [1001, 2056, 4099])
+def test_rows_at_any_alignment(dev, D, shift):
+    """rows of 16-bit values that begin at any element: the norm's, the gated rows' and the weight's inputs and the stream's output"""
+    M, ld = 9, D + shift
+    rng = np.random.default_rng(D)
+    xr, v = values_in("bf16", activations(rng, M, D), ld, 64 + 2 * shift)
+    tr, t = values_in("f16", activations(rng, M, D), ld + 2, 64 + 2 * shift)
+    out = Rows(np.uint16, M, D, ld, lead=64 + 2 * shift)
+    gr, gv = values_in("bf16", activations(rng, M, 2 * D), 2 * D + shift, 64 + 2 * shift)
+    wv = (1 + 0.3 * rng.standard_normal(D)).astype(np.float32)
+    w = Rows(np.float32, 1, D, raw=wv[None], lead=64 + 4 * shift)
+    y, s = Rows(np.uint8, M, 128 * f8.blocks(D)), Rows(np.float32, f8.blocks(D), M)
+    capi.f8_norm(capi.f8_norm_args(x=xr.ptr, ldx=ld, type=2, t=tr.ptr, t_type=1, ldt=ld + 2, x_out=out.ptr, ldo=ld, w=w.ptr, mode=1, M=M, D=D, y=y.ptr, s=s.ptr))
+    stream = to_type((v.astype(np.float32) + t.astype(np.float32)), "bf16")
+    assert np.array_equal(out.read(), stream[0])
+    want = stream[1] / np.sqrt((stream[1] ** 2).mean(1, keepdims=True) + 1e-6) * wv
+    codes_near(y.read(), s.read(), want, 2.0 ** -17 * (np.abs(want) + np.abs(want).mean(1, keepdims=True)))
+    capi.f8_rows(capi.f8_rows_args(x=gr.ptr, ldx=gr.ld, type=2, glu=1, M=M, D=D, y=y.ptr, s=s.ptr))
+    g, u = gv[:, :D].astype(np.float64), gv[:, D:].astype(np.float64)
+    value = g / (1 + np.exp(-g)) * u
+    codes_near(y.read(), s.read(), value, 2.0 ** -16 * np.abs(value))
+    pw, ps = Rows(np.uint8, M, 128 * f8.blocks(D)), Rows(np.float32, 1, f8.blocks(D))
+    capi.f8_pack(capi.f8_pack_args(x=xr.ptr, ldx=ld, type=2, N=M, K=D, w=pw.ptr, s=ps.ptr))
+    codes, scales = f8.pack(v.astype(np.float32))
+    assert np.array_equal(pw.read(), codes) and np.array_equal(ps.read(), scales)
+    for r in (xr, tr, out, gr, w, y, s, pw, ps):
         r.free()
