@@ -97,7 +97,7 @@ __device__ __forceinline__ int f8_key(int r) { return r & 6; }
 // 9.4 us that way, 6.0 this.
 // PAIR: 8 outputs of up to 8 rows, two blocks of k at a time: the matrix instruction's rows 8 - 15 are the same weights' next block, its columns 8 - 15 the
 // same rows', and of its four quarters the two that pair a block with itself are kept.
-// Bound: the weight's bytes, and below some 30 MB of them launch and round trips: 1 row, 16384 outputs x 2048 k 7.6 us (33.6 MB, 4.4 TB/s), 9216 x 14720 24.8 us
+// Bound: the weight's bytes, and below some 30 MB of them launch and round trips: 1 row, 16384 outputs x 2048 k 7.4 us (33.6 MB, 4.5 TB/s), 9216 x 14720 24.8 us
 // (5.5 TB/s); 5 rows, 2048 x 8192 5.1 us (16.9 MB, 3.3 TB/s).
 template <int W_, int NT_, int XD_, bool PAIR_, int S_>
 struct F8Few {
@@ -216,62 +216,6 @@ __global__ __launch_bounds__(64 * T::W) void f8_few_kernel(const F8GemmP p) {
   if (l16 < T::BM && m < p.M && n < p.N) store4<TYPE>(p, m, n, v);
 }
 
-// Few rows: a workgroup takes 16 NT outputs of 16 rows, its W waves the blocks of k in turn; their sums meet in LDS. A wave's loads are
-// all on their way before its first product; no LDS in between, as no two waves want the same byte of the weight.
-// Bound: the weight's bytes, and below some 30 MB of them launch and round trips: 1 row, 16384 outputs x 2048 k 7.4 us (33.6 MB, 4.5 TB/s), 5 rows,
-// 2048 x 8192 6.5 us (16.9 MB, 2.6 TB/s).
-// PAIR: 8 outputs of up to 8 rows, two blocks of k at a time: the matrix instruction's rows 8 - 15 are the same weights' next block, its columns 8 - 15 the
-// same rows', and of its four quarters the two that pair a block with itself are kept.
-template <int TYPE, int W, int NT, bool PAIR>
-__global__ __launch_bounds__(64 * W) void f8_thin_kernel(const F8GemmP p) {
-  static_assert(!PAIR || NT == 1, "one tile of pairs");
-  __shared__ f32x4 part[W][NT][64];
-  constexpr int BN = PAIR ? 8 : 16 * NT, Step = PAIR ? 2 : 1;   // outputs of a workgroup, blocks of a wave's turn
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15, row = PAIR ? l16 & 7 : l16, own = PAIR ? l16 >> 3 : 0;
-  const int n0 = blockIdx.x * BN, m = min(row, p.M - 1);   // rows past the last: it again
-  const uint8_t* w[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) w[i] = p.w + min(n0 + 16 * i + row, p.N - 1) * p.ldw + g * 16;
-  const uint8_t* x = p.x + m * p.ldx + g * 16;
-  const float* xs = p.xs + m;
-  const float* ws = p.ws + (int64_t)(n0 >> 7) * p.ldws;
-  f32x4 acc[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int kb = wave * Step; kb < p.blocks; kb += W * Step) {
-    const int k = min(kb + own, p.blocks - 1);   // past the last block: it again, times 0
-    const float s = kb + own < p.blocks ? xs[k * p.ldxs] * ws[k] : 0.0f;
-    const i32x8 b = codes32(*(const i32x4*)(x + (int64_t)k * 128), *(const i32x4*)(x + (int64_t)k * 128 + 64));
-    i32x8 a[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) a[i] = codes32(*(const i32x4*)(w[i] + (int64_t)k * 128), *(const i32x4*)(w[i] + (int64_t)k * 128 + 64));
-    half8v bh[4];
-    to_half(b, bh);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      half8v ah[4];
-      to_half(a[i], ah);
-      const f32x4 d = mfma_half(ah, bh);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][e] = __builtin_fmaf(d[e], s, acc[i][e]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NT; ++i) part[wave][i][lane] = acc[i];
-  __syncthreads();
-  if (wave >= NT) return;
-  f32x4 v = part[0][wave][lane];
-#pragma unroll
-  for (int k = 1; k < W; ++k) v += part[k][wave][lane];
-  const int n = n0 + wave * 16 + 4 * g;
-  if constexpr (PAIR) {   // the other block's sums: 32 lanes of outputs and 8 columns further on
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += __shfl(v[e], lane + 40, 64);
-    if (g >= 2 || l16 >= 8) return;
-  }
-  if (l16 < p.M && n < p.N) store4<TYPE>(p, l16, n, v);
-}
-
 // The sums of a wave's 16 AM rows from row m on, of 16 AN outputs from output n on
 template <int TYPE, int AM, int AN>
 __device__ __forceinline__ void tile_out(const F8GemmP& p, const f32x4 (&acc)[AM][AN], int m, int n, int lane) {
@@ -306,7 +250,7 @@ __device__ __forceinline__ void tile_out(const F8GemmP& p, const f32x4 (&acc)[AM
 // Many rows: a workgroup takes BN outputs (weight rows) of BM activation rows, its WN x WM waves 16 AN x 16 AM of them each. A stage in LDS is
 // a block of k of every row: BN + BM rows of 128 codes and BM scales, S stages in all, filled by loads that go straight to LDS,
 // S - 1 steps ahead and dealt out over a step; chunks lie as above.
-// Bound: the matrix instructions at the clock that they leave. 4608 rows, 9216 outputs x 9216 k, fp16 results: 352-357 us, 2.2 PFLOP/s (a
+// Bound: the matrix instructions at the clock that they leave. 4608 rows, 9216 outputs x 9216 k, fp16 results: 350-372 us box to box, 2.1-2.2 PFLOP/s (a
 // library's product with a scale per row 327; of 8192 each way 2.36). On random codes the 16 x 16 x 128 instruction by itself reaches 3.75 PFLOP/s, with an fma a
 // value beside it 3.38, on zeros 4.88: the clock goes down under them. Tried on the widest tile, us: 32 x 32 x 64 instructions the same; two groups of waves
 // half a step apart the same; the next stage's lines into L2 ahead 9% more; workgroups that stay and take tile after tile 359; the tiles' blocks of

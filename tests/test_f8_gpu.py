@@ -317,7 +317,10 @@ def test_gemm_sizes(dev, M, N, K):
                                          (1025, 975, 5120, "bf16"), (1537, 2435, 9216, "f16"), (1537, 2435, 9216, "f32"), (1537, 2561, 128, "bf16"),
                                          (1537, 2562, 640, "f32"), (1537, 1281, 16640, "bf16"), (1537, 1292, 8192, "f32"), (1537, 1155, 9216, "f16"),
                                          (1537, 1155, 9216, "f32"), (65, 8197, 128, "f32"), (700, 710, 5120, "f16"), (2050, 130, 16640, "f32"),
-                                         (2050, 3849, 9216, "f16"), (1537, 4993, 640, "bf16"), (130, 70, 4224, "f32"), (130, 70, 4224, "f16")])
+                                         (2050, 3849, 9216, "f16"), (1537, 4993, 640, "bf16"), (130, 70, 4224, "f32"), (130, 70, 4224, "f16"),
+                                         (1025, 996, 5120, "bf16"), (1025, 867, 5120, "f16"), (130, 4097, 16640, "f32"), (1025, 1282, 16640, "f32"),
+                                         (17, 24, 25600, "f32"), (17, 24, 26880, "bf16"), (387, 1249, 128, "bf16"), (1025, 938, 9216, "f16"),
+                                         (1537, 2306, 9216, "f32"), (387, 307, 9216, "bf16"), (17, 20, 9216, "f16"), (195, 577, 128, "f32")])
 def test_gemm_tiles(dev, M, N, K, type_):
     """a sample of the rows and outputs, the first and the last among them (the whole product is the GPU's work)"""
     rng = np.random.default_rng(M)
