@@ -58,6 +58,8 @@ __device__ __forceinline__ uint4 f8_load16(const void* a) {
   const F8Any16 v = *(const F8Any16*)a;
   return uint4{v.w[0], v.w[1], v.w[2], v.w[3]};
 }
+struct __attribute__((packed, aligned(2))) F8Any8 { uint32_t w[2]; };
+__device__ __forceinline__ void f8_store8(void* a, const uint2& v) { *(F8Any8*)a = F8Any8{{v.x, v.y}}; }
 __device__ __forceinline__ void f8_store16(void* a, const uint4& v) { *(F8Any16*)a = F8Any16{{v.x, v.y, v.z, v.w}}; }
 // n of 8 consecutive elements (n >= 1) from element i on, of a row that has `before` elements ahead of it and n or more (`room`) from it on; the others
 // are 0. f8_fetch8 asks for them, f8_take8 makes them values: of several, all are asked for first. One or two 16-byte accesses: of the row's last 8

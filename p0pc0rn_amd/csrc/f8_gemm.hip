@@ -24,6 +24,12 @@ namespace p0 {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// Consecutive workgroups go to the 8 XCDs in turn: of n in a line XCD i has the i-th of 8 runs
+__device__ __forceinline__ int f8_run(int b, int n) {
+  const int xcd = b & 7;
+  return xcd * (n >> 3) + min(xcd, n & 7) + (b >> 3);
+}
+
 struct F8GemmP {
   const uint8_t* x;
   const float* xs;
@@ -32,8 +38,7 @@ struct F8GemmP {
   void* y;
   int64_t ldx, ldxs, ldw, ldws, ldy;
   int M, N, blocks;    // blocks of 128 k
-  int turned;          // few rows: workgroups go over the rows first
-  int yvec;            // 1: 4 consecutive outputs from a multiple of 4 on are aligned together; 2: rows are 16-byte aligned
+  int turned, run;     // few rows: rows lie along the grid's x; run: the grid is a line, workgroups of `run` along y for each along x
 };
 
 // a lane's 32 codes of a block: 16 bytes from two places
@@ -68,7 +73,7 @@ template <int TYPE> __device__ __forceinline__ void store4(const F8GemmP& p, int
   const int64_t o = (int64_t)m * p.ldy + n;
   if constexpr (TYPE == P0_F32) {
     float* y = (float*)p.y + o;
-    if (p.yvec && n + 4 <= p.N) *(float4*)y = float4{v[0], v[1], v[2], v[3]};
+    if (n + 4 <= p.N) f8_store16(y, uint4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])});
     else
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -78,7 +83,7 @@ template <int TYPE> __device__ __forceinline__ void store4(const F8GemmP& p, int
     uint32_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = f8_half<TYPE>(v[i]);
-    if (p.yvec && n + 4 <= p.N) *(uint2*)y = uint2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+    if (n + 4 <= p.N) f8_store8(y, uint2{h[0] | h[1] << 16, h[2] | h[3] << 16});
     else
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -107,7 +112,7 @@ struct F8Few {
   static constexpr int XL = PAIR ? 2 : XD, Loads = 2 * NT + XL + Step;              // loads of x rows, all of a turn's
   static constexpr int Codes = (2 * NT + XL) * 1024, Stage = Codes + 256 * Step, Mine = S * Stage + 512, Lds = W * Mine;
   static_assert(!PAIR || (NT == 1 && XD == 1), "one tile of pairs");
-  static_assert(NT * MT <= W && NT * MT * 1024 <= Mine && BM <= 64, "tile");
+  static_assert(NT * MT * 1024 <= Mine && BM <= 64, "tile");
 };
 
 template <int TYPE, class T>
@@ -116,8 +121,13 @@ __global__ __launch_bounds__(64 * T::W) void f8_few_kernel(const F8GemmP p) {
   constexpr int NT = T::NT, MT = T::MT, W = T::W, S = T::S, Step = T::Step;
   constexpr bool Exact = TYPE == P0_F32 || T::BM <= 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, l16 = lane & 15;
-  const int n0 = (p.turned ? blockIdx.y : blockIdx.x) * T::BN, m0 = (p.turned ? blockIdx.x : blockIdx.y) * T::BM;
-  if (n0 >= p.N || m0 >= p.M) return;
+  int bx = blockIdx.x, by = blockIdx.y;
+  if (p.run) {
+    const int at = f8_run(bx, gridDim.x);
+    bx = at / p.run;
+    by = at - bx * p.run;
+  }
+  const int n0 = (p.turned ? by : bx) * T::BN, m0 = (p.turned ? bx : by) * T::BM;
   const int own = T::PAIR ? l16 >> 3 : 0;
   uint8_t* mine = lds + wave * T::Mine;
   const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
@@ -202,25 +212,29 @@ __global__ __launch_bounds__(64 * T::W) void f8_few_kernel(const F8GemmP p) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) ((f32x4*)mine)[(j * NT + i) * 64 + lane] = acc[j][i];
   __syncthreads();
-  if (wave >= NT * MT) return;
-  auto part = [&](int k) { return ((const f32x4*)(lds + k * T::Mine))[wave * 64 + lane]; };
-  f32x4 v = part(0);
 #pragma unroll
-  for (int k = 1; k < W; ++k) v += part(k);
-  const int n = n0 + wave % NT * 16 + 4 * g, m = m0 + wave / NT * 16 + l16;
-  if constexpr (T::PAIR) {   // the other block's sums: 32 lanes of outputs and 8 columns further on
+  for (int c = 0; c < NT * MT; c += W) {
+    const int cell = c + wave;
+    if (cell >= NT * MT) return;
+    auto part = [&](int k) { return ((const f32x4*)(lds + k * T::Mine))[cell * 64 + lane]; };
+    f32x4 v = part(0);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += __shfl(v[e], lane + 40, 64);
-    if (g >= 2 || l16 >= 8) return;
+    for (int k = 1; k < W; ++k) v += part(k);
+    const int n = n0 + cell % NT * 16 + 4 * g, m = m0 + cell / NT * 16 + l16;
+    if constexpr (T::PAIR) {   // the other block's sums: 32 lanes of outputs and 8 columns further on
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += __shfl(v[e], lane + 40, 64);
+      if (g >= 2 || l16 >= 8) return;
+    }
+    if (l16 < T::BM && m < p.M && n < p.N) store4<TYPE>(p, m, n, v);
   }
-  if (l16 < T::BM && m < p.M && n < p.N) store4<TYPE>(p, m, n, v);
 }
 
 // The sums of a wave's 16 AM rows from row m on, of 16 AN outputs from output n on
 template <int TYPE, int AM, int AN>
 __device__ __forceinline__ void tile_out(const F8GemmP& p, const f32x4 (&acc)[AM][AN], int m, int n, int lane) {
   const int l16 = lane & 15, g = lane >> 4;
-  const bool whole = m + 16 * AM <= p.M && n + 16 * AN <= p.N && p.yvec > 1;
+  const bool whole = m + 16 * AM <= p.M && n + 16 * AN <= p.N;
 #pragma unroll
   for (int j = 0; j < AM; ++j) {
     const int mr = m + 16 * j + l16;
@@ -236,7 +250,7 @@ __device__ __forceinline__ void tile_out(const F8GemmP& p, const f32x4 (&acc)[AM
           a[h] = x[0];
           b[h] = x[1];
         }
-        *(uint4*)((uint16_t*)p.y + (int64_t)mr * p.ldy + n + 16 * (i + (g & 1)) + 8 * (g >> 1)) = uint4{a[0], a[1], b[0], b[1]};
+        f8_store16((uint16_t*)p.y + (int64_t)mr * p.ldy + n + 16 * (i + (g & 1)) + 8 * (g >> 1), uint4{a[0], a[1], b[0], b[1]});
       }
     } else if (mr < p.M) {
 #pragma unroll
@@ -284,12 +298,9 @@ __global__ __launch_bounds__(T::Threads, 2) void f8_tile_kernel(const F8TileP a)
   const F8GemmP& p = a.g;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = wv % T::WN, wm = wv / T::WN, l16 = lane & 15, g = lane >> 4;
-  // consecutive workgroups go to the 8 XCDs in turn: each XCD takes a contiguous run of tiles, which goes down a band of 4 row tiles, then
-  // on to the next column tile
+  // each XCD takes a contiguous run of tiles, which goes down a band of 4 row tiles, then on to the next column tile
   constexpr int kBand = 4;
-  const int groups = a.nbx * a.nby * a.nks;
-  int t = blockIdx.x;
-  if (groups % 8 == 0) t = (blockIdx.x % 8) * (groups / 8) + blockIdx.x / 8;
+  const int t = f8_run(blockIdx.x, a.nbx * a.nby * a.nks);
   const int per = a.nbx * a.nks * kBand, band = t / per, brows = min(kBand, a.nby - band * kBand), in = t - band * per;
   const int mb = band * kBand + in % brows, cs = in / brows, ks = cs % a.nks, nb = cs / a.nks;
   const int m0 = mb * T::BM, n0 = nb * T::BN;
@@ -494,6 +505,8 @@ using Few16 = F8Few<8, 1, 2, false, 2>;      // 16 of 16, 8 waves
 using Few16b = F8Few<4, 1, 2, false, 2>;     // the same, 4 waves
 using Few32 = F8Few<8, 1, 4, false, 2>;      // 16 of 32, 8 waves
 using Few32w = F8Few<8, 2, 4, false, 1>;     // 32 of 32, 8 waves
+using Few32x = F8Few<8, 4, 4, false, 1>;     // 64 of 32, 8 waves
+using Few64 = F8Few<8, 4, 8, false, 1>;      // 64 of 64, 8 waves
 using TileSmall = F8Tile<2, 2, 2, 2, 9>;   // 64 outputs of 64 rows, 4 waves of 32 x 32
 using TileLow = F8Tile<4, 1, 2, 4, 6>;     // 128 of 64, 4 waves of 32 x 64
 using TileHalf = F8Tile<2, 4, 4, 2, 4>;    // 128 of 128, 8 waves of 64 x 32
@@ -507,11 +520,16 @@ template <class T> static void f8_few_launch(const F8GemmP& g, int type, hipStre
   F8GemmP p = g;
   unsigned nx = (unsigned)((p.N + T::BN - 1) / T::BN), ny = (unsigned)((p.M + T::BM - 1) / T::BM);
   if (ny > 1) {
-    // The operand with more rows goes along x, in a multiple of 8: consecutive workgroups go to the 8 XCDs in turn, so each L2 holds an eighth of it
-    // (us, weights along x / rows: 1021 rows, 130 outputs x 8192 k 12.3 / 7.9; 128 rows, 4096 x 2048 5.7 / 6.5)
+    // The operand with more rows goes along x: consecutive workgroups go to the 8 XCDs in turn, so each L2 holds an eighth of it (us, weights along x /
+    // rows: 1021 rows, 130 outputs x 8192 k 12.3 / 7.9). Where x is no multiple of 8 the XCDs take runs of a line of all workgroups, so that none has more than
+    // another (1737 rows, 563 x 3968 in 28 x 9 tiles 11.6, x filled up to 32 19.4)
     p.turned = p.M > p.N;
     if (p.turned) std::swap(nx, ny);
-    nx = (nx + 7) / 8 * 8;
+    if (nx % 8) {
+      p.run = (int)ny;
+      nx *= ny;
+      ny = 1;
+    }
   }
   hipLaunchKernelGGL(f8_few_of<T>(type), dim3(nx, ny), dim3(64 * T::W), T::Lds, s, p);
 }
@@ -545,6 +563,8 @@ int f8_gemm_init() {
   if (int r = f8_few_init<Few16b>()) return r;
   if (int r = f8_few_init<Few32>()) return r;
   if (int r = f8_few_init<Few32w>()) return r;
+  if (int r = f8_few_init<Few32x>()) return r;
+  if (int r = f8_few_init<Few64>()) return r;
   if (int r = f8_tile_init<TileSmall>()) return r;
   if (int r = f8_tile_init<TileLow>()) return r;
   if (int r = f8_tile_init<TileHalf>()) return r;
@@ -570,10 +590,12 @@ constexpr F8Shape kF8Shapes[] = {{64, 64, 0.326f, 1.7f, 0.60f, 2.1f},      // Ti
                                  {128, 256, 1.036f, 4.3f, 1.49f, 15.7f},   // TileLong
                                  {256, 256, 1.65f, 8.9f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
 // Up to a few times as many workgroups as CUs the kernel for few rows is ahead of the tiles, whose steps wait for each other: a round, then the longer of
-// a wave's turns and of what a CU's workgroups ask for in all. Fitted to 255 shapes of 17 to 3330 rows; the choice among these two and the tiles is
+// a wave's turns and of what a CU's workgroups ask for in all. Fitted to 255 shapes of 17 to 3330 rows; the choice among the first two and the tiles is
 // on average within 1% of the fastest measured, 10% at the worst (512 rows, 1536 outputs x 1024 k). Measured (us; few in 16 x 32 / in 32 x 32 / tile): 64
 // rows, 2048 x 8192 k 7.2 / 8.4 / 11.5; 64, 2048 x 2048 3.9 / 4.0 / 7.4; 256, 512 x 2048 3.7 / 4.0 / 7.3; 128, 4096 x 2048 9.9 / 5.7 / 8.7;
-// 1021, 2048 x 2048 36.6 / 16.6 / 11.1. Past 4 groups a CU (6 where results are fp32) the tiles
+// 1021, 2048 x 2048 36.6 / 16.6 / 11.1. In 64 x 32 and 64 x 64, long k of as many workgroups as CUs: 256 rows, 2048 x 8192 11.7 / 15.4 (tile 14.8); 512,
+// 2048 x 8192 20.8 / 17.3 (21.1), fp32 25.5 / 21.6 (27.8); 1021, 1024 x 4096 14.4 / 11.5 (14.1). Past one group a CU those two are far behind
+// (1187 rows, 1541 x 9600 51.6 in 64 x 64, tile 35.9). Past 4 groups a CU (6 where results are fp32) the tiles
 // are ahead whatever the rest says (256, 4096 x 2048: - / 9.4 / 8.7); weights past 64 MB stream better into them (64, 9216 x 9216 40 / 32 / 26).
 struct F8FewShape {
   int bn, bm, waves, per_cu;
@@ -581,7 +603,9 @@ struct F8FewShape {
   float round32, turn32, block32, group32;   // fp32 results
 };
 constexpr F8FewShape kF8FewShapes[] = {{16, 32, 8, 1, 0.41f, 0.486f, 0.060f, 0.09f, 0.53f, 0.62f, 0.05f, 0.0f},     // Few32
-                                       {32, 32, 8, 2, 0.0f, 0.60f, 0.085f, 0.41f, 0.0f, 0.665f, 0.10f, 0.55f}};   // Few32w
+                                       {32, 32, 8, 2, 0.0f, 0.60f, 0.085f, 0.41f, 0.0f, 0.665f, 0.10f, 0.55f},    // Few32w
+                                      {64, 32, 8, 1, 0.95f, 1.02f, 0.0f, 0.0f, 1.05f, 1.30f, 0.0f, 0.0f},        // Few32x
+                                      {64, 64, 8, 1, 3.0f, 1.45f, 0.0f, 0.0f, 3.5f, 1.94f, 0.0f, 0.0f}};         // Few64
 static bool f8_choice(const F8GemmP& p, int type, hipStream_t s) {
   const bool f32 = type == P0_F32;
   const int cus = ctx().cu_count;
@@ -600,10 +624,10 @@ static bool f8_choice(const F8GemmP& p, int type, hipStream_t s) {
       if (kind < 0 || t < least) { least = t; kind = k; nks = n; }
     }
   }
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < 4; ++k) {
     const F8FewShape& c = kF8FewShapes[k];
     const int64_t groups = ((int64_t)p.N + c.bn - 1) / c.bn * (((int64_t)p.M + c.bm - 1) / c.bm);
-    if (groups > (f32 ? 6 : 4) * cus || (int64_t)p.N * p.blocks > 1 << 19) continue;
+    if (groups > (k > 1 ? 1 : f32 ? 6 : 4) * cus || (int64_t)p.N * p.blocks > 1 << 19) continue;
     const int rounds = (int)((groups + (int64_t)cus * c.per_cu - 1) / ((int64_t)cus * c.per_cu)), turns = (p.blocks + c.waves - 1) / c.waves;
     const float each = groups > cus ? (float)groups / cus : 1.0f, wait = rounds * turns * (f32 ? c.turn32 : c.turn),
                 ask = each * p.blocks * (f32 ? c.block32 : c.block);
@@ -613,6 +637,8 @@ static bool f8_choice(const F8GemmP& p, int type, hipStream_t s) {
   if (kind < 0) return false;
   if (kind == 5) f8_few_launch<Few32>(p, type, s);
   else if (kind == 6) f8_few_launch<Few32w>(p, type, s);
+  else if (kind == 7) f8_few_launch<Few32x>(p, type, s);
+  else if (kind == 8) f8_few_launch<Few64>(p, type, s);
   else if (kind == 0) f8_tile_launch<TileSmall>(p, type, nks, s);
   else if (kind == 1) f8_tile_launch<TileLow>(p, type, nks, s);
   else if (kind == 2) f8_tile_launch<TileHalf>(p, type, nks, s);
@@ -644,9 +670,7 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   if (overlap(x, y) || overlap(w, y) || overlap(xs, y) || overlap(ws, y)) { set_error("%s: y overlaps an input", op); return P0_EINVAL; }
   if (int r = refuse_in_chain(op)) return r;
   if (int r = require_open(op)) return r;
-  F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks, 0};
-  const uintptr_t ya = (uintptr_t)a->y | (uintptr_t)(ldy * size);
-  p.yvec = ya % 16 == 0 ? 2 : ya % (4 * size) == 0;
+  F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks, 0, 0};
   if (M <= 16) {
     // Measured (us; rows, outputs x k). Up to 8 rows, pairs of 8 waves / of 4 / 16 outputs: 5, 2048 x 8192 5.1 / 5.6 / 7.3; 1, 9216 x 2048 6.9 / 6.0 / 5.5,
     // x 4096 10.2 / 9.1 / 10.2, x 8192 14.9 / 15.8 / 16.4; 1, 16384 x 2048 11.3 / 8.4 / 7.7, x 4096 15.5 / 12.7 / 14.8. Up to 16, 8 waves / 4: 16, 2048 x 8192
