@@ -573,9 +573,9 @@ int f8_gemm_init() {
 }
 
 // Which tile, and how many slices of K, by time: a round of workgroups takes its blocks of k, one after the other, and then its outputs; a
-// slice's sums go through memory. The figures (us a block and a round) are fitted to 122 shapes of 17 to 4489 rows, 65 to 18334 outputs, 1 to
-// 122 blocks, each tile and slicing measured on its own: the fastest by them is on average within 0.5% of the fastest measured, 12% at the
-// worst (83 rows, 158 outputs, 11 blocks, fp32: 8.7 for 7.8). Measured (us; 16384 outputs x 2048 k, small / low / half / long / wide): bf16
+// slice's sums go through memory. The figures (us a block and a round) are fitted to 129 shapes of 17 to 4571 rows, 131 to 18216 outputs, 1 to
+// 127 blocks, each tile and slicing measured on its own: the fastest by them is on average within 0.2% of the fastest measured, 5% at
+// the worst (689 rows, 15753 outputs, 27 blocks, fp32: 97.8 for 93.1). Measured (us; 16384 outputs x 2048 k, small / low / half / long / wide): bf16
 // results, 64 rows 11.0 / 12.3 / 13.5 / 17.4 / 28.9; 256 rows 36 / 22.1 / 17.1 / 21.3 / 33; 1021 rows 137 / 89 / 55 / 45 / 37.8; fp32, 1021 rows
 // 199 / 134 / 91 / 75. Slices (256 rows, 2048 outputs x 8192 k): low in 1 / 2 / 4 27.9 / 19.1 / 15.7, half in 8 21.3.
 constexpr int64_t kF8Groups = (1 << 23) - 1;   // workgroups of 512 threads: less than 2^32 threads
@@ -584,11 +584,11 @@ struct F8Shape {
   float block, round;       // 16-bit results
   float block32, round32;   // fp32 results: half the matrix rate, conversions
 };
-constexpr F8Shape kF8Shapes[] = {{64, 64, 0.326f, 1.7f, 0.60f, 2.1f},      // TileSmall
-                                 {128, 64, 0.46f, 2.1f, 0.80f, 4.0f},      // TileLow
-                                 {128, 128, 0.613f, 2.55f, 1.02f, 7.2f},   // TileHalf
-                                 {128, 256, 1.036f, 4.3f, 1.49f, 15.7f},   // TileLong
-                                 {256, 256, 1.65f, 8.9f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
+constexpr F8Shape kF8Shapes[] = {{64, 64, 0.318f, 2.0f, 0.51f, 2.35f},     // TileSmall
+                                 {128, 64, 0.441f, 2.3f, 0.70f, 2.9f},     // TileLow
+                                 {128, 128, 0.613f, 2.65f, 0.97f, 3.6f},   // TileHalf
+                                 {128, 256, 1.032f, 3.9f, 1.50f, 6.0f},    // TileLong
+                                 {256, 256, 1.72f, 7.5f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
 // Up to a few times as many workgroups as CUs the kernel for few rows is ahead of the tiles, whose steps wait for each other: a round, then the longer of
 // a wave's turns and of what a CU's workgroups ask for in all. Fitted to 255 shapes of 17 to 3330 rows; the choice among the first two and the tiles is
 // on average within 1% of the fastest measured, 10% at the worst (512 rows, 1536 outputs x 1024 k). Measured (us; few in 16 x 32 / in 32 x 32 / tile): 64
@@ -596,7 +596,8 @@ constexpr F8Shape kF8Shapes[] = {{64, 64, 0.326f, 1.7f, 0.60f, 2.1f},      // Ti
 // 1021, 2048 x 2048 36.6 / 16.6 / 11.1. In 64 x 32 and 64 x 64, long k of as many workgroups as CUs: 256 rows, 2048 x 8192 11.7 / 15.4 (tile 14.8); 512,
 // 2048 x 8192 20.8 / 17.3 (21.1), fp32 25.5 / 21.6 (27.8); 1021, 1024 x 4096 14.4 / 11.5 (14.1). Past one group a CU those two are far behind
 // (1187 rows, 1541 x 9600 51.6 in 64 x 64, tile 35.9). Past 4 groups a CU (6 where results are fp32) the tiles
-// are ahead whatever the rest says (256, 4096 x 2048: - / 9.4 / 8.7); weights past 64 MB stream better into them (64, 9216 x 9216 40 / 32 / 26).
+// are ahead whatever the rest says (256, 4096 x 2048: - / 9.4 / 8.7); weights past 64 MB stream better
+// into them, but for fp32 (64, 9216 x 9216 40 / 32 / 26; 17, 9216 x 9216 fp32 24 / - / 34).
 struct F8FewShape {
   int bn, bm, waves, per_cu;
   float round, turn, block, group;           // us: a round of workgroups, a turn of a wave, a block and a workgroup of each CU
@@ -618,16 +619,16 @@ static bool f8_choice(const F8GemmP& p, int type, hipStream_t s) {
       if (n > 1 && (k == 4 || p.blocks / n < 4 || tiles * n > cus || (size_t)tiles * n * c.bn * c.bm > ctx().part_floats)) break;
       const int64_t groups = tiles * n, rounds = (groups + cus - 1) / cus;
       if (groups > kF8Groups) break;
-      const float fill = groups < cus ? (float)groups / cus : 1.0f, alone = f32 ? 0.65f : 0.72f;   // a chip that is not full runs a little faster
+      const float fill = groups < cus ? (float)groups / cus : 1.0f, alone = f32 ? 0.8f : 0.7f;   // a chip that is not full runs a little faster
       const float t = rounds * ((p.blocks + n - 1) / n * (f32 ? c.block32 : c.block) * (alone + (1.0f - alone) * fill) + (f32 ? c.round32 : c.round)) +
-                      (n > 1 ? 1.2f + (f32 ? 0.26f : 0.3f) * n * (c.bn * c.bm / 4096) : 0.0f);
+                      (n > 1 ? 3.0f + (f32 ? 0.26f : 0.23f) * n * (c.bn * c.bm / 4096) : 0.0f);
       if (kind < 0 || t < least) { least = t; kind = k; nks = n; }
     }
   }
   for (int k = 0; k < 4; ++k) {
     const F8FewShape& c = kF8FewShapes[k];
     const int64_t groups = ((int64_t)p.N + c.bn - 1) / c.bn * (((int64_t)p.M + c.bm - 1) / c.bm);
-    if (groups > (k > 1 ? 1 : f32 ? 6 : 4) * cus || (int64_t)p.N * p.blocks > 1 << 19) continue;
+    if (groups > (k > 1 ? 1 : f32 ? 6 : 4) * cus || (!f32 && (int64_t)p.N * p.blocks > 1 << 19)) continue;
     const int rounds = (int)((groups + (int64_t)cus * c.per_cu - 1) / ((int64_t)cus * c.per_cu)), turns = (p.blocks + c.waves - 1) / c.waves;
     const float each = groups > cus ? (float)groups / cus : 1.0f, wait = rounds * turns * (f32 ? c.turn32 : c.turn),
                 ask = each * p.blocks * (f32 ? c.block32 : c.block);

@@ -320,7 +320,10 @@ def test_gemm_sizes(dev, M, N, K):
                                          (2050, 3849, 9216, "f16"), (1537, 4993, 640, "bf16"), (130, 70, 4224, "f32"), (130, 70, 4224, "f16"),
                                          (1025, 996, 5120, "bf16"), (1025, 867, 5120, "f16"), (130, 4097, 16640, "f32"), (1025, 1282, 16640, "f32"),
                                          (17, 24, 25600, "f32"), (17, 24, 26880, "bf16"), (387, 1249, 128, "bf16"), (1025, 938, 9216, "f16"),
-                                         (1537, 2306, 9216, "f32"), (387, 307, 9216, "bf16"), (17, 20, 9216, "f16"), (195, 577, 128, "f32")])
+                                         (1537, 2306, 9216, "f32"), (387, 307, 9216, "bf16"), (17, 20, 9216, "f16"), (195, 577, 128, "f32"),
+                                         (522, 875, 1024, "bf16"), (522, 835, 1024, "f32"), (1025, 801, 2048, "f16"), (1025, 839, 2048, "f32"),
+                                         (1021, 1793, 5120, "bf16"), (1025, 1474, 5120, "f32"), (387, 306, 53760, "f16"), (130, 321, 53760, "f32"),
+                                         (1025, 642, 128, "bf16"), (387, 1699, 128, "f32"), (1537, 642, 128, "f32"), (387, 2306, 128, "f16")])
 def test_gemm_tiles(dev, M, N, K, type_):
     """a sample of the rows and outputs, the first and the last among them (the whole product is the GPU's work)"""
     rng = np.random.default_rng(M)
