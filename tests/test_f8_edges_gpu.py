@@ -83,7 +83,7 @@ class Product:
 
 def test_recordings_that_share_the_slices_workspace(dev):
     """products in slices of K, each in a recording of its own, replayed in turn and beside an eager one"""
-    many = [Product(17, 24, 25600, "bf16", 1), Product(18, 24, 26880, "f32", 2), Product(20, 30, 30720, "f16", 3)]
+    many = [Product(17, 24, 25600, "bf16", 1), Product(18, 24, 26880, "f32", 2), Product(20, 30, 28160, "f16", 3)]
     want = []
     for p in many:
         p.call()
