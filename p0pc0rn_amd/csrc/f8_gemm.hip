@@ -185,7 +185,7 @@ __global__ __launch_bounds__(64 * T::W) void f8_few_kernel(const F8GemmP p) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (t + S < turns) load(t + S, at);
     at = at + T::Stage == S * T::Stage ? 0 : at + T::Stage;
-    const float w = !T::PAIR || (t * W + wave) * Step + own <= last ? sw : 0.0f;   // past the last block: times 0
+    const bool in = !T::PAIR || (t * W + wave) * Step + own <= last;   // past the last block: times 0
     half8v ah[Exact ? NT : 1][4];
     if constexpr (Exact) {
 #pragma unroll
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(64 * T::W) void f8_few_kernel(const F8GemmP p) {
     for (int j = 0; j < MT; ++j) {
       half8v bh[4];
       if constexpr (Exact) to_half(b[j], bh);
-      const float f = s[j] * w;
+      const float f = in ? s[j] * sw : 0.0f;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         f32x4 d;

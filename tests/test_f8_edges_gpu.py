@@ -217,3 +217,24 @@ def test_rows_at_any_alignment(dev, D, shift):
     assert np.array_equal(pw.read(), codes) and np.array_equal(ps.read(), scales)
     for r in (xr, tr, out, gr, w, y, s, pw, ps):
         r.free()
+
+
+@pytest.mark.parametrize("M", [1, 3, 8, 9, 16, 17, 40])
+@pytest.mark.parametrize("blocks", [1, 3, 17, 31, 65])
+def test_scales_that_are_infinite(dev, M, blocks):
+    """an infinite scale of the last block makes that row infinite, not NaN, and no other: nothing is added twice with it"""
+    N, K = 20, 128 * blocks
+    codes = lambda n: np.full((n, K), 0x38, np.uint8)  # noqa: E731  (1.0)
+    xs, ws = np.full((blocks, M), 0.5, np.float32), np.full((1, blocks), 0.25, np.float32)
+    xs[-1, M // 2] = np.inf
+    x, w, s, r = Rows(np.uint8, M, K, raw=codes(M)), Rows(np.uint8, N, K, raw=codes(N)), Rows(np.float32, blocks, M, raw=xs), Rows(np.float32, 1, blocks, raw=ws)
+    for type_ in ("f32", "bf16"):
+        y = Rows(RAW[type_], M, N)
+        capi.f8_gemm(capi.f8_gemm_args(x=x.ptr, xs=s.ptr, w=w.ptr, ws=r.ptr, M=M, N=N, K=K, type=capi.TYPE[type_], y=y.ptr))
+        got = from_type(y.read(), type_).reshape(M, N)
+        want = np.full((M, N), 16.0 * blocks)
+        want[M // 2] = np.inf
+        assert np.array_equal(got, want if type_ == "f32" else to_type(want, "bf16")[1])
+        y.free()
+    for b in (x, w, s, r):
+        b.free()
