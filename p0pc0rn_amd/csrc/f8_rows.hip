@@ -60,14 +60,29 @@ __global__ __launch_bounds__(256) void f8_pack_kernel(const PackP p) {
 }
 
 // ------------------------------------------------------------------------------------------------ activations
-// g u sigmoid(z), z = g, or 2 sqrt(2 / pi) (g + 0.044715 g^3) (= 0.5 g (1 + tanh(z / 2))), to 3 units: what the product z log2 e and the reciprocal
-// round off is put back. Past |z| = 200 the sigmoid is 0 or 1; a NaN gate is one in g.
-__device__ __forceinline__ float gated(int glu, float g, float u) {
-  constexpr float L = 1.4426950409f, Ln = 0.69314718056f;
-  const float z = fminf(fmaxf(glu == P0_GLU_SILU ? g : 1.5957691216f * (g + 0.044715f * g * g * g), -200.0f), 200.0f);
-  const float t = -z * L, d = 1.0f + __builtin_amdgcn_exp2f(t) * __builtin_fmaf(__builtin_fmaf(-z, L, -t), Ln, 1.0f);
+// g u sigmoid(z), z = g (silu), or 2 sqrt(2 / pi) (g + 0.044715 g^3) (gelu: 0.5 g (1 + tanh(z / 2))), within 8 units of 2^-24. An error of z is one of exp(-z) z times
+// as large, so what its products and constants round off is kept (c) and put back: without, 9 units at z = -20 and 21 at -80 (silu), 46 at g = -5 and 129 at -8 (gelu).
+// A sigmoid below the least normal value (z < -87.3) is 0. A NaN gate is one in g.
+template <int TYPE> __device__ __forceinline__ float gated(int glu, float g, float u) {
+#pragma clang fp contract(off)
+  constexpr float Ln = 0.69314718056f;
+  float t, c;   // |z| log2 e = t + c
+  if (glu == P0_GLU_SILU) {
+    constexpr float L = 1.4426950409f, Ll = 1.925963e-8f;   // log2 e = L + Ll
+    const float z = fminf(fabsf(g), 200.0f);
+    t = z * L;
+    c = __builtin_fmaf(z, Ll, __builtin_fmaf(z, L, -t));
+  } else {
+    constexpr float L = 2.3022082f, Ll = 1.2948402e-8f, K = 0.044715f, Kl = 1.5461444e-9f;   // 2 sqrt(2 / pi) log2 e = L + Ll, 0.044715 = K + Kl
+    const float x = fminf(fabsf(g), 16.0f), xx = x * x, p = __builtin_fmaf(xx, K, 1.0f), z = x * p;   // times 2 sqrt(2 / pi): |z|
+    float pe = __builtin_fmaf(xx, Kl, __builtin_fmaf(xx, K, 1.0f - p));
+    if constexpr (TYPE == P0_F32) pe = __builtin_fmaf(__builtin_fmaf(x, x, -xx), K, pe);   // squares of 16-bit values are exact
+    t = z * L;
+    c = __builtin_fmaf(__builtin_fmaf(x, pe, __builtin_fmaf(x, p, -z)), L, __builtin_fmaf(z, Ll, __builtin_fmaf(z, L, -t)));
+  }
+  const float e = __builtin_amdgcn_exp2f(-t), E = __builtin_fmaf(e, c * -Ln, e), d = 1.0f + E;   // exp(-|z|)
   const float r = __builtin_amdgcn_rcpf(d), q = __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r);
-  return g * (d < 1e37f ? q : r) * u;
+  return g * (g < 0.0f ? E : 1.0f) * q * u;
 }
 struct RowsF8P {
   const void* x;
@@ -79,7 +94,7 @@ struct RowsF8P {
   int glu;
 };
 // A workgroup takes a strip of 256 >> ls rows.
-// Bound: HBM (4608 rows of 9216 f16 channels: 24 us for 128 MB, 5.3 TB/s), gated ones nearly as much the arithmetic: 45-48 us for 214 MB, 4.6 TB/s (a copy of as
+// Bound: HBM (4608 rows of 9216 f16 channels: 24 us for 128 MB, 5.3 TB/s), gated ones nearly as much the arithmetic: silu 42-43 us, gelu 46-47 for 214 MB, 4.6-5 TB/s (a copy of as
 // many bytes 41). Few rows are a launch (5 of 8192 fp32 channels, gated: 4.9 us).
 // With two rows a thread 47.6, four 51.6: the other waves cover a wave's loads better than its own.
 template <int TYPE, bool GLU>
@@ -99,7 +114,7 @@ __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsF8P p) {
       float u[8];
       f8_take8<TYPE>(up, p.x, m * p.ldx + p.up + c, n, c, n, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = gated(p.glu, f[j], u[j]);
+      for (int j = 0; j < 8; ++j) f[j] = gated<TYPE>(p.glu, f[j], u[j]);
     }
   }
   const float s = f8_scale(f8_block_most(f));
