@@ -43,6 +43,38 @@ console.log(JSON.stringify([res, P.f8Width(1), P.f8Width(256)]));
         "rope: mode third"]
 
 
+def test_what_is_missing_is_named(tmp_path):
+    """an operand, its scales or an output left out: the library's message, not an error of the language"""
+    out = run_node(tmp_path, r"""
+const g = {}, B = { ptr: 4096 }, C = { ptr: 1 << 20 }, D = { ptr: 1 << 21 }, E = { ptr: 1 << 22 }, F = { ptr: 1 << 23 }, res = [];
+const codes = (b, s) => ({ buf: b, s: s && { buf: s } });
+const t = (f) => { try { f(); res.push('no error'); } catch (e) { res.push(e.message); } };
+t(() => P.f8Pack(g, { N: 4, K: 4, w: codes(C, D) }));
+t(() => P.f8Pack(g, { x: { buf: B }, N: 4, K: 4 }));
+t(() => P.f8Pack(g, { x: { buf: B }, N: 4, K: 4, w: { buf: C } }));
+t(() => P.f8Norm(g, { M: 2, D: 40, y: codes(C, D) }));
+t(() => P.f8Norm(g, { x: { buf: B }, M: 2, D: 40 }));
+t(() => P.f8Norm(g, { x: { buf: B }, M: 2, D: 40, y: { buf: C } }));
+t(() => P.f8Rows(g, { M: 2, D: 4, y: codes(C, D) }));
+t(() => P.f8Rows(g, { x: { buf: B }, M: 2, D: 4 }));
+t(() => P.f8Rows(g, { x: { buf: B }, M: 2, D: 4, y: codes(C) }));
+t(() => P.f8Gemm(g, { w: codes(D, E), M: 2, N: 4, K: 128, y: { buf: F } }));
+t(() => P.f8Gemm(g, { x: codes(B), w: codes(D, E), M: 2, N: 4, K: 128, y: { buf: F } }));
+t(() => P.f8Gemm(g, { x: codes(B, C), M: 2, N: 4, K: 128, y: { buf: F } }));
+t(() => P.f8Gemm(g, { x: codes(B, C), w: codes(D), M: 2, N: 4, K: 128, y: { buf: F } }));
+t(() => P.f8Gemm(g, { x: codes(B, C), w: codes(D, E), M: 2, N: 4, K: 128 }));
+t(() => P.rope(g, { y: { buf: C }, rows: 2, hq: 1, dim: 64, pos: { buf: D } }));
+t(() => P.rope(g, { x: { buf: B }, rows: 2, hq: 1, dim: 64 }));
+console.log(JSON.stringify(res));
+""")
+    assert json.loads(out.strip().splitlines()[-1]) == [
+        "f8_pack: missing x buffer", "f8_pack: missing w buffer", "f8_pack: missing s buffer",
+        "f8_norm: missing x buffer", "f8_norm: missing y buffer", "f8_norm: missing s buffer",
+        "f8_rows: missing x buffer", "f8_rows: missing y buffer", "f8_rows: missing s buffer",
+        "f8_gemm: missing x buffer", "f8_gemm: missing xs buffer", "f8_gemm: missing w buffer", "f8_gemm: missing ws buffer", "f8_gemm: missing y buffer",
+        "rope: missing x buffer", "rope: missing pos buffer"]
+
+
 @pytest.mark.gpu
 def test_a_layers_front(tmp_path):
     """norm, product, rotation in place, a gate: against the CPU restatement, product and rotation within 2^-15 of the row's largest"""
