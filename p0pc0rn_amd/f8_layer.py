@@ -46,6 +46,8 @@ class Decoder:
     """`layers` layers of random weights: hidden `K`, `heads` query heads on `kv_heads` key heads of `dim`, FFN `mlp`."""
 
     def __init__(self, layers=2, K=512, heads=8, kv_heads=2, dim=64, mlp=1024, axis_dim=None, theta=10000.0, mode="half", seed=1):
+        if layers < 1:
+            raise ValueError("f8_layer: %d layers" % layers)
         self.layers, self.K, self.heads, self.kv_heads, self.dim, self.mlp = layers, K, heads, kv_heads, dim, mlp
         self.axis_dim, self.theta, self.mode = axis_dim or [dim], theta, mode
         self.width = (heads + 2 * kv_heads) * dim
@@ -124,7 +126,11 @@ class Run:
 
     def step(self, rows, pos):
         """rows [B, M, K] (fp32) at positions [axes, B, M]: the sequences' next tokens -> the stream after the layers, [B, M, K]"""
-        B, M, K = rows.shape
+        rows, pos = np.asarray(rows), np.asarray(pos)
+        M = rows.shape[1] if rows.ndim == 3 else 0
+        if M < 1 or rows.shape != (self.B, M, self.m.K) or pos.shape != (len(self.m.axis_dim), self.B, M):
+            raise ValueError("f8_layer: rows %s, positions %s of %d sequences of %d channels, %d axes"
+                             % (rows.shape, pos.shape, self.B, self.m.K, len(self.m.axis_dim)))
         self.sequences(M)
         self.x.upload(np.ascontiguousarray(rows, np.float32))
         self.pos.upload(np.ascontiguousarray(pos, np.int32))
@@ -137,9 +143,11 @@ def main():
     ap.add_argument("--prompt", type=int, default=512)
     ap.add_argument("--tokens", type=int, default=16)
     a = ap.parse_args()
+    if a.prompt < 1 or a.tokens < 0:
+        ap.error("a prompt has at least one row")
     capi.open_device(0)
     m = Decoder()
-    run = Run(m, 1, a.prompt + a.tokens, max(a.prompt, 1))
+    run = Run(m, 1, a.prompt + a.tokens, a.prompt)
     x = np.random.default_rng(2).standard_normal((1, a.prompt + a.tokens, m.K)).astype(np.float32)
     at = np.arange(x.shape[1])[None, None]
     y = run.step(x[:, :a.prompt], at[:, :, :a.prompt])
