@@ -14,6 +14,7 @@
 // Both operands' k may come in any order that is the same for both: lane group g (16 lanes) holds bytes [16 g, 16 g + 16) and
 // [64 + 16 g, 80 + 16 g) of a block.
 #include "dma.hpp"
+#include "f8_choice.hpp"
 #include "f8_common.hpp"
 
 #include <type_traits>
@@ -572,79 +573,26 @@ int f8_gemm_init() {
   return f8_tile_init<TileWide>();
 }
 
-// Which tile, and how many slices of K, by time: a round of workgroups takes its blocks of k, one after the other, and then its outputs; a
-// slice's sums go through memory. The figures (us a block and a round) are fitted to 129 shapes of 17 to 4571 rows, 131 to 18216 outputs, 1 to
-// 127 blocks, each tile and slicing measured on its own: the fastest by them is on average within 0.2% of the fastest measured, 5% at
-// the worst (689 rows, 15753 outputs, 27 blocks, fp32: 97.8 for 93.1). Measured (us; 16384 outputs x 2048 k, small / low / half / long / wide): bf16
-// results, 64 rows 11.0 / 12.3 / 13.5 / 17.4 / 28.9; 256 rows 36 / 22.1 / 17.1 / 21.3 / 33; 1021 rows 137 / 89 / 55 / 45 / 37.8; fp32, 1021 rows
-// 199 / 134 / 91 / 75. Slices (256 rows, 2048 outputs x 8192 k): low in 1 / 2 / 4 27.9 / 19.1 / 15.7, half in 8 21.3.
-constexpr int64_t kF8Groups = (1 << 23) - 1;   // workgroups of 512 threads: less than 2^32 threads
-struct F8Shape {
-  int bn, bm;
-  float block, round;       // 16-bit results
-  float block32, round32;   // fp32 results: half the matrix rate, conversions
-};
-constexpr F8Shape kF8Shapes[] = {{64, 64, 0.318f, 2.0f, 0.51f, 2.35f},     // TileSmall
-                                 {128, 64, 0.441f, 2.3f, 0.70f, 2.9f},     // TileLow
-                                 {128, 128, 0.613f, 2.65f, 0.97f, 3.6f},   // TileHalf
-                                 {128, 256, 1.032f, 3.9f, 1.50f, 6.0f},    // TileLong
-                                 {256, 256, 1.72f, 7.5f, 0.0f, 0.0f}};     // TileWide: 16-bit results, no slices
-// Up to a few times as many workgroups as CUs the kernel for few rows is ahead of the tiles, whose steps wait for each other: a round, then the longer of
-// a wave's turns and of what a CU's workgroups ask for in all. Fitted to 255 shapes of 17 to 3330 rows; the choice among the first two and the tiles is
-// on average within 1% of the fastest measured, 10% at the worst (512 rows, 1536 outputs x 1024 k). Measured (us; few in 16 x 32 / in 32 x 32 / tile): 64
-// rows, 2048 x 8192 k 7.2 / 8.4 / 11.5; 64, 2048 x 2048 3.9 / 4.0 / 7.4; 256, 512 x 2048 3.7 / 4.0 / 7.3; 128, 4096 x 2048 9.9 / 5.7 / 8.7;
-// 1021, 2048 x 2048 36.6 / 16.6 / 11.1. In 64 x 32 and 64 x 64, long k of as many workgroups as CUs: 256 rows, 2048 x 8192 11.7 / 15.4 (tile 14.8); 512,
-// 2048 x 8192 20.8 / 17.3 (21.1), fp32 25.5 / 21.6 (27.8); 1021, 1024 x 4096 14.4 / 11.5 (14.1). Past one group a CU those two are far behind
-// (1187 rows, 1541 x 9600 51.6 in 64 x 64, tile 35.9). Past 4 groups a CU (6 where results are fp32) the tiles
-// are ahead whatever the rest says (256, 4096 x 2048: - / 9.4 / 8.7); weights past 64 MB stream better
-// into them, but for fp32 (64, 9216 x 9216 40 / 32 / 26; 17, 9216 x 9216 fp32 24 / - / 34).
-struct F8FewShape {
-  int bn, bm, waves, per_cu;
-  float round, turn, block, group;           // us: a round of workgroups, a turn of a wave, a block and a workgroup of each CU
-  float round32, turn32, block32, group32;   // fp32 results
-};
-constexpr F8FewShape kF8FewShapes[] = {{16, 32, 8, 1, 0.41f, 0.486f, 0.060f, 0.09f, 0.53f, 0.62f, 0.05f, 0.0f},     // Few32
-                                       {32, 32, 8, 2, 0.0f, 0.60f, 0.085f, 0.41f, 0.0f, 0.665f, 0.10f, 0.55f},    // Few32w
-                                      {64, 32, 8, 1, 0.95f, 1.02f, 0.0f, 0.0f, 1.05f, 1.30f, 0.0f, 0.0f},        // Few32x
-                                      {64, 64, 8, 1, 3.0f, 1.45f, 0.0f, 0.0f, 3.5f, 1.94f, 0.0f, 0.0f}};         // Few64
-static bool f8_choice(const F8GemmP& p, int type, hipStream_t s) {
-  const bool f32 = type == P0_F32;
-  const int cus = ctx().cu_count;
-  float least = 0.0f;
-  int kind = -1, nks = 1;
-  for (int k = 0; k < (f32 ? 4 : 5); ++k) {
-    const F8Shape& c = kF8Shapes[k];
-    const int64_t tiles = ((int64_t)p.N + c.bn - 1) / c.bn * (((int64_t)p.M + c.bm - 1) / c.bm);
-    for (int n = 1; n <= 16; n *= 2) {
-      if (n > 1 && (k == 4 || p.blocks / n < 4 || tiles * n > cus || (size_t)tiles * n * c.bn * c.bm > ctx().part_floats)) break;
-      const int64_t groups = tiles * n, rounds = (groups + cus - 1) / cus;
-      if (groups > kF8Groups) break;
-      const float fill = groups < cus ? (float)groups / cus : 1.0f, alone = f32 ? 0.8f : 0.7f;   // a chip that is not full runs a little faster
-      const float t = rounds * ((p.blocks + n - 1) / n * (f32 ? c.block32 : c.block) * (alone + (1.0f - alone) * fill) + (f32 ? c.round32 : c.round)) +
-                      (n > 1 ? 3.0f + (f32 ? 0.26f : 0.23f) * n * (c.bn * c.bm / 4096) : 0.0f);
-      if (kind < 0 || t < least) { least = t; kind = k; nks = n; }
-    }
+// false: more outputs than a launch takes
+static bool f8_launch(const F8GemmP& p, int type, hipStream_t s) {
+  const F8Choice c = f8_choice(p.M, p.N, p.blocks, type == P0_F32, ctx().cu_count, ctx().part_floats);
+  switch (c.form) {
+    case kF8TileSmall: f8_tile_launch<TileSmall>(p, type, c.slices, s); break;
+    case kF8TileLow: f8_tile_launch<TileLow>(p, type, c.slices, s); break;
+    case kF8TileHalf: f8_tile_launch<TileHalf>(p, type, c.slices, s); break;
+    case kF8TileLong: f8_tile_launch<TileLong>(p, type, c.slices, s); break;
+    case kF8TileWide: f8_tile_launch<TileWide>(p, type, 1, s); break;
+    case kF8Few32: f8_few_launch<Few32>(p, type, s); break;
+    case kF8Few32w: f8_few_launch<Few32w>(p, type, s); break;
+    case kF8Few32x: f8_few_launch<Few32x>(p, type, s); break;
+    case kF8Few64: f8_few_launch<Few64>(p, type, s); break;
+    case kF8Few8: f8_few_launch<Few8>(p, type, s); break;
+    case kF8Pairs4: f8_few_launch<FewPairs4>(p, type, s); break;
+    case kF8Pairs: f8_few_launch<FewPairs>(p, type, s); break;
+    case kF8Few16b: f8_few_launch<Few16b>(p, type, s); break;
+    case kF8Few16: f8_few_launch<Few16>(p, type, s); break;
+    default: return false;
   }
-  for (int k = 0; k < 4; ++k) {
-    const F8FewShape& c = kF8FewShapes[k];
-    const int64_t groups = ((int64_t)p.N + c.bn - 1) / c.bn * (((int64_t)p.M + c.bm - 1) / c.bm);
-    if (groups > (k > 1 ? 1 : f32 ? 6 : 4) * cus || (!f32 && (int64_t)p.N * p.blocks > 1 << 19)) continue;
-    const int rounds = (int)((groups + (int64_t)cus * c.per_cu - 1) / ((int64_t)cus * c.per_cu)), turns = (p.blocks + c.waves - 1) / c.waves;
-    const float each = groups > cus ? (float)groups / cus : 1.0f, wait = rounds * turns * (f32 ? c.turn32 : c.turn),
-                ask = each * p.blocks * (f32 ? c.block32 : c.block);
-    const float t = rounds * (f32 ? c.round32 : c.round) + (wait > ask ? wait : ask) + each * (f32 ? c.group32 : c.group);
-    if (kind < 0 || t < least) { least = t; kind = 5 + k; }
-  }
-  if (kind < 0) return false;
-  if (kind == 5) f8_few_launch<Few32>(p, type, s);
-  else if (kind == 6) f8_few_launch<Few32w>(p, type, s);
-  else if (kind == 7) f8_few_launch<Few32x>(p, type, s);
-  else if (kind == 8) f8_few_launch<Few64>(p, type, s);
-  else if (kind == 0) f8_tile_launch<TileSmall>(p, type, nks, s);
-  else if (kind == 1) f8_tile_launch<TileLow>(p, type, nks, s);
-  else if (kind == 2) f8_tile_launch<TileHalf>(p, type, nks, s);
-  else if (kind == 3) f8_tile_launch<TileLong>(p, type, nks, s);
-  else f8_tile_launch<TileWide>(p, type, 1, s);
   return true;
 }
 
@@ -672,20 +620,7 @@ static int gemm_f8_call(const p0_f8_gemm_args_t* a) {
   if (int r = refuse_in_chain(op)) return r;
   if (int r = require_open(op)) return r;
   F8GemmP p{(const uint8_t*)a->x, a->xs, (const uint8_t*)a->w, a->ws, a->y, ldx, ldxs, ldw, ldws, ldy, (int)M, (int)N, (int)blocks, 0, 0};
-  if (M <= 16) {
-    // Measured (us; rows, outputs x k). Up to 8 rows, pairs of 8 waves / of 4 / 16 outputs: 5, 2048 x 8192 5.1 / 5.6 / 7.3; 1, 9216 x 2048 6.9 / 6.0 / 5.5,
-    // x 4096 10.2 / 9.1 / 10.2, x 8192 14.9 / 15.8 / 16.4; 1, 16384 x 2048 11.3 / 8.4 / 7.7, x 4096 15.5 / 12.7 / 14.8. Up to 16, 8 waves / 4: 16, 2048 x 8192
-    // 6.0 / 7.6; 16, 9216 x 14720 33.3 / 33.8; 16, 16384 x 2048 9.2 / 8.1. Up to 16 blocks both are alike where there are few outputs
-    const bool many = N > 18 * ctx().cu_count;   // workgroups of 8 outputs: more than two a CU
-    if (M > 8 && blocks <= 16) f8_few_launch<Few16b>(p, a->type, ctx().cur);
-    else if (M > 8) f8_few_launch<Few16>(p, a->type, ctx().cur);
-    else if (blocks <= 16) f8_few_launch<Few8>(p, a->type, ctx().cur);
-    else if (many && (blocks < 64 || N > 1 << 25)) f8_few_launch<FewPairs4>(p, a->type, ctx().cur);   // (8 waves of 2^26 outputs: 2^32 threads)
-    else f8_few_launch<FewPairs>(p, a->type, ctx().cur);
-  } else if (!f8_choice(p, a->type, ctx().cur)) {
-    set_error("%s: %lld x %lld outputs", op, (long long)M, (long long)N);
-    return P0_EINVAL;
-  }
+  if (!f8_launch(p, a->type, ctx().cur)) { set_error("%s: %lld x %lld outputs", op, (long long)M, (long long)N); return P0_EINVAL; }
   P0_LAUNCHED(op);
   return P0_OK;
 }
