@@ -149,3 +149,26 @@ def test_form(dev, form, slices, shape, type_):
     rng = np.random.default_rng(M + N)
     ops = operands(rng, M, N, 128 * blocks)
     sample_near(product(ops, N, type_), ops, type_, sample(rng, M, 64), sample(rng, N, 64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,slices,shape,type_", [(f, n, s, t) for f, n, s, types in LISTED for t in types if t != "f16" or f == "wide"])
+def test_values_that_are_not_finite(dev, form, slices, shape, type_):
+    """a NaN code makes its row of the results NaN, one of the weight its column, in the first, a middle and the last block of k and at the lowest and the highest
+    place of 8; no other value changes, though the matrix instructions take 16 rows and columns, and 8 k, together"""
+    M, N, blocks = shape
+    K = 128 * blocks
+    rng = np.random.default_rng(M + N)
+    ops = operands(rng, M, N, K)
+    clean = product(ops, N, type_)
+    at = [0, 7, (blocks // 2) * 128 + 63, (blocks - 1) * 128, K - 1]
+    rows, cols = np.unique(rng.integers(0, M, 5))[:max(1, M // 2)], np.unique(rng.integers(0, N, 5))[:max(1, N // 2)]
+    for i, r in enumerate(rows):
+        ops[0][r, at[i]] = (0x7F, 0xFF)[i % 2]
+    for i, r in enumerate(cols):
+        ops[2][r, at[4 - i]] = (0xFF, 0x7F)[i % 2]
+    got = product(ops, N, type_)
+    nan = np.zeros((M, N), bool)
+    nan[rows], nan[:, cols] = True, True
+    assert np.array_equal(np.isnan(got), nan) and np.isfinite(clean).all()
+    assert np.array_equal(got[~nan], clean[~nan])
