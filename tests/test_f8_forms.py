@@ -172,3 +172,29 @@ def test_values_that_are_not_finite(dev, form, slices, shape, type_):
     nan[rows], nan[:, cols] = True, True
     assert np.array_equal(np.isnan(got), nan) and np.isfinite(clean).all()
     assert np.array_equal(got[~nan], clean[~nan])
+
+
+CUT = [("few32", (29, 133, 9)), ("few32w", (33, 2111, 1)), ("few64", (1149, 737, 16)), ("small", (135, 331, 241)), ("low", (129, 5921, 1)), ("half", (199, 8249, 1)),
+       ("long", (1735, 1159, 100)), ("wide", (1021, 16383, 16))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,shape", CUT)
+@pytest.mark.parametrize("cancel", [False, True])
+def test_outliers_beside_small_values(dev, form, shape, cancel):
+    """one large product and seven small ones in each 8 consecutive k, the large ones of two neighbouring 8s the same with opposite signs (cancel) or not. 16-bit
+    results lose at most 7 * 2^-13 of the largest of each 8 (sample_near's bound), where that is more than a share of the result; fp32 results lose none"""
+    M, N, blocks = shape
+    K = 128 * blocks
+    rng = np.random.default_rng(M)
+    small = rng.choice([15.0, 13.0, 0.9375, 7.5, 2.0], (M, K))
+    x = small.copy()
+    x[:, 0::8] = rng.choice([448.0, 256.0, 240.0], (M, K // 16)).repeat(2, 1)
+    w = np.ones((N, K))
+    w[:, 0::8] = rng.choice([448.0, 256.0], (N, K // 16)).repeat(2, 1)
+    if cancel:
+        w[:, 8::16] *= -1
+    ops = f8.encode(x), np.full((blocks, M), 2.0 ** -10, np.float32), f8.encode(w), np.full((f8.blocks(N), blocks), 2.0 ** -10, np.float32)
+    m, n = sample(rng, M, 64), sample(rng, N, 64)
+    for type_ in ("f16", "bf16", "f32"):
+        sample_near(product(ops, N, type_), ops, type_, m, n)
