@@ -17,12 +17,18 @@ struct F8Choice {
   int slices;   // of K
 };
 
-// Which tile, and how many slices of K, by time: a round of workgroups takes its blocks of k, one after the other, and then its outputs; a
-// slice's sums go through memory. The figures (us a block and a round) are fitted to 129 shapes of 17 to 4571 rows, 131 to 18216 outputs, 1 to
-// 127 blocks, each tile and slicing measured on its own: the fastest by them is on average within 0.2% of the fastest measured, 5% at
-// the worst (689 rows, 15753 outputs, 27 blocks, fp32: 97.8 for 93.1). Measured (us; 16384 outputs x 2048 k, small / low / half / long / wide): bf16
-// results, 64 rows 11.0 / 12.3 / 13.5 / 17.4 / 28.9; 256 rows 36 / 22.1 / 17.1 / 21.3 / 33; 1021 rows 137 / 89 / 55 / 45 / 37.8; fp32, 1021 rows
-// 199 / 134 / 91 / 75. Slices (256 rows, 2048 outputs x 8192 k): low in 1 / 2 / 4 27.9 / 19.1 / 15.7, half in 8 21.3.
+// The rule past 16 rows: the form, and for a tile the slices of K (a power of two, as long as the slices' workgroups are no more than the CUs),
+// with the least time by the figures below. The rule up to 16 rows is in f8_choice.
+//
+// Tiles: a round of workgroups takes its blocks of k, one after the other, and then its outputs; a slice's sums go through memory. The figures (us
+// a block and a round) are fitted to 129 shapes of 17 to 4571 rows, 131 to 18216 outputs, 1 to 127 blocks, each tile and slicing measured on its
+// own: the fastest by them is on average within 0.2% of the fastest measured, 5% at the worst (689 rows, 15753 outputs, 27 blocks, fp32: 97.8 for 93.1).
+//   us, 16384 outputs x 2048 k   small   low   half   long   wide
+//   64 rows, bf16                11.0    12.3  13.5   17.4   28.9
+//   256 rows, bf16               36      22.1  17.1   21.3   33
+//   1021 rows, bf16              137     89    55     45     37.8
+//   1021 rows, fp32              199     134   91     75     -
+//   slices (256 rows, 2048 outputs x 8192 k): low in 1 / 2 / 4 27.9 / 19.1 / 15.7, half in 8 21.3
 constexpr int64_t kF8Groups = (1 << 23) - 1;   // workgroups of 512 threads: less than 2^32 threads
 struct F8Shape {
   int bn, bm;
@@ -34,15 +40,21 @@ constexpr F8Shape kF8Shapes[] = {{64, 64, 0.318f, 2.0f, 0.51f, 2.35f},     // kF
                                  {128, 128, 0.613f, 2.65f, 0.97f, 3.6f},   // kF8TileHalf
                                  {128, 256, 1.032f, 3.9f, 1.50f, 6.0f},    // kF8TileLong
                                  {256, 256, 1.72f, 7.5f, 0.0f, 0.0f}};     // kF8TileWide: 16-bit results, no slices
-// Up to a few times as many workgroups as CUs the kernel for few rows is ahead of the tiles, whose steps wait for each other: a round, then the longer of
+// The kernel for few rows, ahead of the tiles, whose steps wait for each other, up to a few times as many workgroups as CUs: a round, then the longer of
 // a wave's turns and of what a CU's workgroups ask for in all. Fitted to 255 shapes of 17 to 3330 rows; the choice among the first two and the tiles is
-// on average within 1% of the fastest measured, 10% at the worst (512 rows, 1536 outputs x 1024 k). Measured (us; few in 16 x 32 / in 32 x 32 / tile): 64
-// rows, 2048 x 8192 k 7.2 / 8.4 / 11.5; 64, 2048 x 2048 3.9 / 4.0 / 7.4; 256, 512 x 2048 3.7 / 4.0 / 7.3; 128, 4096 x 2048 9.9 / 5.7 / 8.7;
-// 1021, 2048 x 2048 36.6 / 16.6 / 11.1. In 64 x 32 and 64 x 64, long k of as many workgroups as CUs: 256 rows, 2048 x 8192 11.7 / 15.4 (tile 14.8); 512,
-// 2048 x 8192 20.8 / 17.3 (21.1), fp32 25.5 / 21.6 (27.8); 1021, 1024 x 4096 14.4 / 11.5 (14.1). Past one group a CU those two are far behind
-// (1187 rows, 1541 x 9600 51.6 in 64 x 64, tile 35.9). Past 4 groups a CU (6 where results are fp32) the tiles
-// are ahead whatever the rest says (256, 4096 x 2048: - / 9.4 / 8.7); weights past 64 MB stream better
-// into them, but for fp32 (64, 9216 x 9216 40 / 32 / 26; 17, 9216 x 9216 fp32 24 / - / 34).
+// on average within 1% of the fastest measured, 10% at the worst (512 rows, 1536 outputs x 1024 k). It is left out past 4 workgroups a CU (6 where results
+// are fp32; 256 rows, 4096 x 2048: 32 x 32 9.4 us, tile 8.7), past one for 64 x 32 and 64 x 64 (1187 rows, 1541 x 9600: 51.6 in 64 x 64, tile 35.9), and,
+// but for fp32, at weights past 64 MB, which stream better into tiles (64 rows, 9216 x 9216: 16 x 32 40, 32 x 32 32, tile 26; 17, fp32: 16 x 32 24, tile 34).
+//   us: rows, outputs x k   16 x 32   32 x 32   64 x 32   64 x 64   tile
+//   64, 2048 x 8192         7.2       8.4       -         -         11.5
+//   64, 2048 x 2048         3.9       4.0       -         -         7.4
+//   256, 512 x 2048         3.7       4.0       -         -         7.3
+//   128, 4096 x 2048        9.9       5.7       -         -         8.7
+//   1021, 2048 x 2048       36.6      16.6      -         -         11.1
+//   256, 2048 x 8192        -         -         11.7      15.4      14.8
+//   512, 2048 x 8192        -         -         20.8      17.3      21.1
+//   the same, fp32          -         -         25.5      21.6      27.8
+//   1021, 1024 x 4096       -         -         14.4      11.5      14.1
 struct F8FewShape {
   int bn, bm, waves, per_cu;
   float round, turn, block, group;           // us: a round of workgroups, a turn of a wave, a block and a workgroup of each CU

@@ -17,7 +17,7 @@ struct PackP {
   int blocks;   // of 128 channels in a row
 };
 // A workgroup takes a block of 128 x 128, a thread 8 rows of 8 channels: 8 loads of 16 bytes on their way at once.
-// Bound: HBM (18432 x 9216 bf16 values: 99.8 us for 510 MB, 5.1 TB/s; a copy of as many bytes 95); launch and round trips for small ones (1536 x
+// Bound: HBM (18432 x 9216 bf16 values: 94.4 us for 510 MB, 5.4 TB/s; a copy of as many bytes 95); launch and round trips for small ones (1536 x
 // 2048 f16 values, 192 workgroups: 4.9 us).
 template <int TYPE>
 __global__ __launch_bounds__(256) void f8_pack_kernel(const PackP p) {
@@ -148,10 +148,11 @@ __device__ __forceinline__ float sum64(float v) {
 // A workgroup takes a row, its up to 16 waves 512 channels each of NC steps, a lane 8 of them. The row stays in registers; each sum is one
 // exchange through LDS.
 // VEC: every run of 8 channels is there whole or not at all.
-// Bound: HBM at many rows (32760 rows of 2560 bf16 channels, modulated: 109-120 us for 590 MB, 4.9-5.4 TB/s; a copy of as many bytes 114),
-// launch and round trips at few (1 row of 2048 fp32 channels: 3.6-4.2 us back to back, 5.5 with the host's part). Rows whose last run of 8 is not whole
-// cost little more (644 rows of 14425 bf16 channels: 30 us for 66 MB; in single channels 84). A wave with a row of its own, four in a workgroup, took 136 and 3.7: five loads a lane
-// at a time and their registers leave fewer waves to cover them.
+// Bound: HBM at many rows (32760 rows of 2560 bf16 channels, modulated: 117-120 us for 590 MB, 4.9-5.0 TB/s; a copy of as many bytes 114),
+// launch and round trips at few (1 row of 2048 fp32 channels: 2.9 us, 5.5 with the host's part). Rows whose last run of 8 is not whole take a third more: every
+// wave carries the counts and the moves of the odd end (us, 644 rows of 14425 bf16 channels 21.0, of 14424 15.4; 908 of 13303 with the norm of t 33.7, of 13304
+// 25.6; in single channels 644 of 14425 took 84). A wave with a row of its own, four in a workgroup, took 136 and 3.7: five loads a lane at a time and their
+// registers leave fewer waves to cover them.
 template <int XT, int TT, int NC, bool VEC>
 __global__ __launch_bounds__(1024) void f8_norm_kernel(const NormP p) {
   __shared__ float red[3][16];

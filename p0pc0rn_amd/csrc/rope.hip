@@ -5,7 +5,9 @@
 // is many turns: it is held in 64 bits, in turns, and only the fraction of a turn goes on in 32.
 //
 // Bound: HBM (32760 rows of 40 heads of 128 bf16 channels on three axes: 123 us for 671 MB, 5.4 TB/s; a copy of as many bytes 125), launch and
-// round trips at few rows (1 row of 10 heads of 256 fp32 channels, normalised: 5.6 us, of the kernel 3.8).
+// round trips at few rows (1 row of 10 heads of 256 fp32 channels, normalised: 5.4-5.7 us, of the kernel 4.4). Halves whose pairs are no multiple
+// of 8 take up to twice as long as whole ones, for runs that begin off any 32 bytes and single stores at their ends (us, 8000 rows of 10 bf16 heads: 126
+// of 128 channels turn 21.2, all 10.6; 100 of 100 15.3, 96 of 96 9.7).
 #include "f8_common.hpp"
 
 #include <cmath>
