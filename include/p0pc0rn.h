@@ -488,7 +488,7 @@ int p0_f8_pack(const p0_f8_pack_args_t* a);
  *   x_out = r (NULL: x itself, in place; not written where there is neither t nor a scale nor x_out)
  *   mode 1: y = r / sqrt(mean(r^2) + eps) * g + b;  mode 0: y = (r - mean(r)) / sqrt(var(r) + eps) * g + b
  *   g = w, or 1 + w with w_one (an lnmod's scale), or 1 without w; b 0 without b
- * Sums and statistics are fp32. eps 0 = 1e-6. ldx, ldt, ldo 0 = D, ldy 0 = D rounded up, lds 0 = M. x_out has x's type. */
+ * Sums and statistics are fp32, which a row's sum of squares has to fit (values up to 1e17). eps 0 = 1e-6. ldx, ldt, ldo 0 = D, ldy 0 = D rounded up, lds 0 = M. x_out has x's type. */
 typedef struct {
   void* x; int64_t ldx; int32_t type;
   const void* t; int64_t ldt; int32_t t_type;
@@ -505,7 +505,7 @@ typedef struct {
 int p0_f8_norm(const p0_f8_norm_args_t* a);
 
 /* M rows of D activations into codes: x[m][c], or act(x[m][c]) * x[m][up + c] (up 0 = D; gelu: 0.5 g (1 + tanh(sqrt(2 / pi) (g +
- * 0.044715 g^3)))). ldx 0 = D, with a glu up + D; ldy 0 = D rounded up, lds 0 = M. */
+ * 0.044715 g^3)))), in fp32 to 8 units of 2^-24; where the gate is so far below zero that exp of it is less than 2^-126, 0. ldx 0 = D, with a glu up + D; ldy 0 = D rounded up, lds 0 = M. */
 typedef struct {
   const void* x; int64_t ldx; int32_t type;
   int64_t up; int32_t glu;
