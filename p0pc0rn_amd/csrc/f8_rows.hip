@@ -96,7 +96,7 @@ struct RowsF8P {
 // A workgroup takes a strip of 256 >> ls rows.
 // Bound: HBM (4608 rows of 9216 f16 channels: 24 us for 128 MB, 5.3 TB/s), gated ones nearly as much the arithmetic: silu 42-43 us, gelu 46-47 for 214 MB, 4.6-5 TB/s (a copy of as
 // many bytes 41). Few rows are a launch (5 of 8192 fp32 channels, gated: 4.9 us).
-// With two rows a thread 47.6, four 51.6: the other waves cover a wave's loads better than its own.
+// Two rows a thread took 4% longer, four 13%: the other waves cover a wave's loads better than its own.
 template <int TYPE, bool GLU>
 __global__ __launch_bounds__(256) void f8_rows_kernel(const RowsF8P p) {
   const int64_t blk = f8_group(), rblk = blk / p.strips;
@@ -323,8 +323,8 @@ static int rows_f8_call(const p0_f8_rows_args_t* a) {
   if (overlap(x, y) || overlap(x, s) || overlap(y, s)) { set_error("%s: outputs overlap", op); return P0_EINVAL; }
   if (int r = refuse(op)) return r;
   RowsF8P p{a->x, (uint8_t*)a->y, a->s, ldx, up, ldy, lds, a->M, a->D, 0, 7, a->glu};
-  // strips of up to 128 lanes that leave no more than an eighth idle (20000 rows of 520 gated channels: 18.9 us in strips of 16 lanes, 21.8 of 128;
-  // 4608 of 9216: 52.3 and 45.4)
+  // strips of up to 128 lanes that leave no more than an eighth idle (us, strips of 16 lanes / of 128, f16: 20000 rows of 520 channels 8.9 / 9.6, gated by
+  // silu 14.1 / 17.9; 4608 of 9216 26.9 / 26.3, gated 41.2 / 42.7)
   const int64_t chunks = K8 / 8;
   while (p.ls > 4 && ((chunks + (1 << p.ls) - 1) >> p.ls << p.ls) - chunks > chunks / 8) --p.ls;
   p.strips = (int)((chunks + (1 << p.ls) - 1) >> p.ls);
