@@ -10,7 +10,6 @@ enum F8Form {
   kF8TileSmall, kF8TileLow, kF8TileHalf, kF8TileLong, kF8TileWide,   // f8_tile_kernel, as kF8Shapes
   kF8Few32, kF8Few32w, kF8Few32x, kF8Few64,                          // f8_few_kernel past 16 rows, as kF8FewShapes
   kF8Few8, kF8Pairs4, kF8Pairs, kF8Few16b, kF8Few16,                 // up to 16
-  kF8Forms
 };
 struct F8Choice {
   int form;     // -1: none takes as many outputs

@@ -94,7 +94,7 @@ struct RowsF8P {
   int glu;
 };
 // A workgroup takes a strip of 256 >> ls rows.
-// Bound: HBM (4608 rows of 9216 f16 channels: 24 us for 128 MB, 5.3 TB/s), gated ones nearly as much the arithmetic: silu 42-43 us, gelu 46-47 for 214 MB, 4.6-5 TB/s (a copy of as
+// Bound: HBM (4608 rows of 9216 f16 channels: 24 us for 128 MB, 5.3 TB/s), gated ones nearly as much the arithmetic: silu 42-43 us, gelu 46-48 for 214 MB, 4.5-5 TB/s (a copy of as
 // many bytes 41). Few rows are a launch (5 of 8192 fp32 channels, gated: 4.9 us).
 // Two rows a thread took 4% longer, four 13%: the other waves cover a wave's loads better than its own.
 template <int TYPE, bool GLU>
