@@ -541,7 +541,8 @@ int p0_f8_gemm(const p0_f8_gemm_args_t* a);
  * on are not rotated): pair i < R / 2 is channels (2 i, 2 i + 1) (P0_ROPE_INTER) or (i, i + R / 2) (P0_ROPE_HALF), its axis the
  * one that holds channel 2 i when the axes lie one after the other, its angle pos[a][row] theta^-e with e = 2 j / axis_dim[a], j
  * the pair's place within its axis (freq 0), or e = 2 i / R (freq 1): (u, v) -> (u cos - v sin, v cos + u sin). Positions are
- * int32, pos[a * pos_ld + row] (pos_ld 0 = rows); angles are held in 64 bits, so far positions lose nothing. axes 0 counts as
+ * int32, pos[a * pos_ld + row] (pos_ld 0 = rows); angles are held in 64 bits, so positions up to 2^20 lose nothing (at 2^31 an angle is
+ * off by up to 2.4e-6 rad). axes 0 counts as
  * 1, an axis_dim[0] of 0 with one axis as dim, theta 0 as 10000; theta is at least 1: no pair turns by more than 1 rad a position. */
 typedef struct {
   const void* x; int64_t ldr, ldh;
